@@ -1,7 +1,8 @@
 """roaster_amd -- Python access to libroaster_moe.so, the MI355X MoE-FFN hot path.
 
-The product is the C ABI declared in include/kernels.h (the reference's kernel API)
-and include/roaster_moe.h (expert table, whole-layer decode / prefill).  This module
+The product is the C ABI declared in include/kernels.h (the reference's kernel API),
+include/roaster_moe.h (expert table, whole-layer decode / prefill) and
+include/roaster_attn.h (attention over a paged key/value cache).  This module
 only loads that library with ctypes and declares its signatures, so that tests and
 the benchmark can call the same entry points a C caller would.  It fails loudly
 when the library has not been built: there is no Python or CPU fallback.
@@ -21,6 +22,7 @@ Q6K_BYTES = 210
 OK, EINVAL, EDEVICE, EROUTE, ENOMEM = 0, -1, -2, -3, -4
 GATE, UP, DOWN = 0, 1, 2
 PREC_F16, PREC_SPLIT, PREC_BF16 = 0, 1, 2
+KV_F32, KV_F16 = 0, 1
 
 
 class KernelMatvecJob(C.Structure):
@@ -69,6 +71,35 @@ class RoasterPrefillOpts(C.Structure):
     _fields_ = [("precision", C.c_int), ("logits_in", C.c_void_p), ("logit_bias", C.c_void_p),
                 ("logits_out", C.c_void_p), ("ids_out", C.c_void_p), ("w_out", C.c_void_p),
                 ("counts_out", C.c_void_p)]
+
+
+class RoasterKvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class RoasterKvPlan(C.Structure):
+    _fields_ = [("n_req", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int),
+                ("max_rows", C.c_int), ("len", C.c_void_p), ("add", C.c_void_p), ("len_out", C.c_void_p),
+                ("table", C.c_void_p), ("ring", C.c_void_p), ("ctl", C.c_void_p), ("ctl_out", C.c_void_p),
+                ("first", C.c_void_p), ("row_req", C.c_void_p), ("row_pos", C.c_void_p), ("row_slot", C.c_void_p)]
+
+
+class RoasterQkRope(C.Structure):
+    _fields_ = [("rows", C.c_int), ("q_heads", C.c_int),
+                ("q", C.c_void_p), ("q_row", C.c_size_t), ("q_head", C.c_size_t),
+                ("k", C.c_void_p), ("k_row", C.c_size_t), ("k_head", C.c_size_t),
+                ("v", C.c_void_p), ("v_row", C.c_size_t), ("v_head", C.c_size_t),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("rot_dim", C.c_int),
+                ("pair_adjacent", C.c_int), ("theta", C.c_double), ("row_pos", C.c_void_p), ("row_slot", C.c_void_p),
+                ("q_out", C.c_void_p)]
+
+
+class RoasterAttnPaged(C.Structure):
+    _fields_ = [("rows", C.c_int), ("q_heads", C.c_int), ("q", C.c_void_p), ("row_req", C.c_void_p),
+                ("row_pos", C.c_void_p), ("table", C.c_void_p), ("n_req", C.c_int), ("max_pages", C.c_int),
+                ("scale", C.c_float), ("gate", C.c_void_p), ("gate_row", C.c_size_t), ("gate_head", C.c_size_t),
+                ("out", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
 _P = C.c_void_p
@@ -143,6 +174,11 @@ _SIG = {
     "roaster_prefill_balanced_down": (C.c_int, [C.c_int]),
     "roaster_prefill_persistent_gate_up": (C.c_int, [C.c_int]),
     "roaster_prefill_fused_gemm": (C.c_int, [C.c_int]),
+    # roaster_attn.h
+    "roaster_kv_plan": (C.c_int, [C.POINTER(RoasterKvPlan)]),
+    "roaster_qk_rope_store": (C.c_int, [C.POINTER(RoasterQkRope), C.POINTER(RoasterKvCache)]),
+    "roaster_attn_ws_bytes": (C.c_size_t, [C.c_int, C.c_int, C.POINTER(RoasterKvCache)]),
+    "roaster_attn_paged": (C.c_int, [C.POINTER(RoasterAttnPaged), C.POINTER(RoasterKvCache)]),
 }
 
 _lib = None

@@ -75,6 +75,7 @@ int rt_take_err();           /* sync the stream, report and clear kernel error b
 void rt_err_words(int *(&w)[2]);   /* the device error words it would read, or NULL */
 void rt_set_aux_err(int *dev_word);   /* a second device error word rt_take_err reports and clears */
 void rt_aux_err_used();      /* a launch that may set it was queued */
+int *rt_attn_err();          /* the attention operators' device error word (attn.h), reported by roaster_sync; NULL: failed */
 int noalloc_setup(int dev);  /* api.hip: device address of the allocation-free scratch array */
 
 void dec_release();          /* decode.hip: frees the decode exchange buffer */

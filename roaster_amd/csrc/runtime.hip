@@ -8,7 +8,7 @@
  * backend is one HIP stream on the current device; weight bytes live in HBM and
  * host addresses are translated to their HBM copy, uploaded once.
  */
-#include "internal.h"
+#include "attn.h"
 
 #include <algorithm>
 
@@ -69,6 +69,8 @@ int rt_init_locked()
     /* device address of the allocation-free entry point's scratch array; a
      * failure is reported by that entry point and leaves the others working */
     (void)noalloc_setup(dev);
+    /* the control words, so that no later call allocates them under a capture */
+    (void)rt_ctrl();
     /* workgroup placement of the one-launch decode stack (a failure leaves
      * its exchanges going through memory) */
     (void)dec_probe_placement();
@@ -90,7 +92,8 @@ extern "C" void *roaster_stream(void)
 
 /* Control words of the decode and prefill kernels: [32] counts the
  * one-launch stack's workgroups (never reset) and [48] the prefill token
- * kernel's (0 between calls); [16] sticky error bits (1 = routing
+ * kernel's (0 between calls); [20] the attention operators' error bits
+ * (attn.h); [16] sticky error bits (1 = routing
  * found fewer than 8 finite logits, 2 = an exchange wait of the one-launch
  * stack gave up, 4 = a workgroup of it read an XCC_ID out of range), cleared
  * when reported; 4 also sends later launches' exchanges through memory. */
@@ -117,6 +120,28 @@ void rt_err_words(int *(&w)[2])
     w[1] = g_aux_used ? g_aux_err : NULL;
 }
 
+/* The attention operators' word: read once one of them has run (a captured
+ * graph may run them again at any time, so the flag stays). */
+static bool g_attn_used;
+
+int *rt_attn_err()
+{
+    unsigned *c = rt_ctrl();
+    if (!c) return NULL;
+    g_attn_used = true;
+    return (int *)(c + 20);
+}
+
+static int err_pin()
+{
+    if (!g_err_pin &&
+        rt_check(hipHostMalloc((void **)&g_err_pin, 64, hipHostMallocDefault), "error word hipHostMalloc")) {
+        g_err_pin = NULL;
+        return ROASTER_EDEVICE;
+    }
+    return 0;
+}
+
 int rt_take_err()
 {
     /* the error words come back with the stream's last work: copies queued
@@ -125,11 +150,7 @@ int rt_take_err()
     int *words[2];
     rt_err_words(words);
     g_aux_used = false;
-    if (!g_err_pin && (words[0] || words[1]) &&
-        rt_check(hipHostMalloc((void **)&g_err_pin, 64, hipHostMallocDefault), "error word hipHostMalloc")) {
-        g_err_pin = NULL;
-        return ROASTER_EDEVICE;
-    }
+    if ((words[0] || words[1]) && err_pin()) return ROASTER_EDEVICE;
     for (int i = 0; i < 2; i++) {
         if (!words[i]) continue;
         g_err_pin[i] = 0;
@@ -157,7 +178,22 @@ extern "C" int roaster_sync(void)
 {
     std::lock_guard<std::recursive_mutex> g(g_lock);
     if (rt_init_locked()) return ROASTER_EDEVICE;
-    return rt_take_err();
+    int *word = g_attn_used ? rt_attn_err() : NULL;
+    if (!word) return rt_take_err();
+    /* the attention operators' word comes back behind the stream's work, with
+     * the others; after another error it waits for the next call */
+    if (err_pin()) return ROASTER_EDEVICE;
+    g_err_pin[2] = 0;
+    if (rt_check(hipMemcpyAsync(g_err_pin + 2, word, sizeof(int), hipMemcpyDeviceToHost, g_rt.stream),
+                 "error word readback"))
+        return ROASTER_EDEVICE;
+    const int rc = rt_take_err(), e = g_err_pin[2];
+    if (rc || !e) return rc;
+    if (rt_check(hipMemset(word, 0, sizeof(int)), "error word reset")) return ROASTER_EDEVICE;
+    if (e & ATTN_ERR_PAGES) return rt_fail(ROASTER_ENOMEM, "roaster_kv_plan: too few free pages; the step was not planned");
+    if (e & ATTN_ERR_PLAN)
+        return rt_fail(ROASTER_EINVAL, "roaster_kv_plan: a length, the row count or the page ring out of range; the step was not planned");
+    return rt_fail(ROASTER_EINVAL, "attention: a request, position, page or slot out of range");
 }
 
 extern "C" int roaster_device_info(int *n_cu, int *n_xcd, size_t *hbm)
@@ -682,6 +718,7 @@ extern "C" void kernel_vk_shutdown(void)
     if (g_ctrl) {
         (void)hipFree(g_ctrl);
         g_ctrl = NULL;
+        g_attn_used = false;
     }
     if (g_err_pin) {
         (void)hipHostFree(g_err_pin);

@@ -1,0 +1,240 @@
+"""roaster_attn_paged against softmax attention in 64 bits, the error bound derived
+in attn_util.attn_bound.  What a row must not use -- tokens behind its position,
+pages of nobody, table entries past its last page -- holds NaN, infinities and
+wild numbers throughout."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import roaster_amd as R
+from attn_util import Attn, Cache, attn_oracle, check_attn, sync
+from gpu_util import Dev, log
+
+pytestmark = pytest.mark.gpu
+
+
+def make(rng, lens, KV, D, page, f16, spare=3):
+    """A cache with `lens` tokens of each request in shuffled pages, poison elsewhere."""
+    used = [-(-l // page) for l in lens]
+    n_pages = sum(used) + spare
+    ids = rng.permutation(n_pages).astype(np.int32)
+    width = max(1, max(used)) + 2
+    table = rng.choice(np.array([-5, 2 ** 30, n_pages, -2 ** 31], np.int32), (len(lens), width)).astype(np.int32)
+    dt = np.float16 if f16 else np.float32
+    kc, vc = (rng.choice(np.array([np.nan, np.inf, -np.inf], dt), (n_pages, KV, page, D)) for _ in range(2))
+    at = 0
+    for r, (l, u) in enumerate(zip(lens, used)):
+        table[r, :u] = ids[at:at + u]
+        for j in range(u):
+            m = min(page, l - j * page)
+            kc[ids[at + j], :, :m] = rng.standard_normal((KV, m, D)).astype(dt)
+            vc[ids[at + j], :, :m] = (rng.standard_normal((KV, m, D)) + 0.2).astype(dt)
+        at += u
+    return kc, vc, table
+
+
+def run_case(lens, rows, H, KV, D, page, f16, gate=False, peak=1.0, seed=0, scale=None):
+    """rows: (request, position) of each row."""
+    rng = np.random.default_rng(seed + 17 * len(lens) + D + page)
+    kc, vc, table = make(rng, lens, KV, D, page, f16)
+    rows = np.array(rows, np.int32).reshape(-1, 2)
+    T = len(rows)
+    q = (peak * rng.standard_normal((T, H, D))).astype(np.float32)
+    g = rng.standard_normal((T, H, 2, D)).astype(np.float32) if gate else None
+    scale = D ** -0.5 if scale is None else scale
+    c = Cache(kc, vc)
+    a = Attn(c, q, rows[:, 0].copy(), rows[:, 1].copy(), table, scale, g)
+    R.check(a.call(), "attn")
+    sync()
+    got = a.out.get()
+    want, mass, reach = attn_oracle(q, kc, vc, table, rows[:, 0], rows[:, 1], np.float64(np.float32(scale)),
+                                    g[:, :, 1] if gate else None)
+    skip = rows[:, 0] == -1
+    assert np.all(got[skip] == 77)
+    assert not got[(rows[:, 1] == -1) & ~skip].any()
+    rel = check_attn(got[~skip], want[~skip], mass[~skip], reach[~skip], int(rows[:, 1].max()) + 1, D)
+    # again on the same buffers: the same bits
+    R.check(a.call(), "attn")
+    sync()
+    assert np.array_equal(a.out.get().view(np.uint32), got.view(np.uint32))
+    return rel
+
+
+EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 127, 128, 129, 255, 256, 257, 500, 1025]
+HEADS = [(16, 2, 256), (4, 4, 256), (32, 8, 128), (7, 1, 128), (20, 4, 64), (16, 1, 64), (24, 2, 128), (2, 1, 256)]
+
+
+@pytest.mark.parametrize("H,KV,D", HEADS)
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("page", [16, 64])
+def test_one_row_a_request_of_every_length(H, KV, D, f16, page):
+    log(f"attn H={H} KV={KV} D={D} f16={f16} page={page}")
+    rel = run_case(EDGES, [(r, l - 1) for r, l in enumerate(EDGES)], H, KV, D, page, f16, gate=True)
+    log(f"  rel {rel:.2e}")
+
+
+@pytest.mark.parametrize("length", [1, 33, 300, 4097])
+@pytest.mark.parametrize("f16", [True, False])
+def test_one_request(length, f16):
+    for H, KV, D in HEADS[:1] + HEADS[3:5]:
+        log(f"attn one request length={length} H={H} KV={KV} D={D} f16={f16}")
+        run_case([length], [(0, length - 1)], H, KV, D, 256, f16, gate=length == 300)
+
+
+@pytest.mark.parametrize("page", [32, 4096])
+def test_long_rows_next_to_short_ones(page):
+    lens = [20000, 1, 0, 7, 3000, 40]
+    run_case(lens, [(r, l - 1) for r, l in enumerate(lens)], 16, 2, 256, page, True, gate=True)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_peaked_softmax(f16):
+    """Scores of +-60 and more: one position takes nearly all."""
+    for H, KV, D in HEADS[:1] + HEADS[2:3]:
+        run_case([700, 90], [(0, 699), (1, 89)], H, KV, D, 16, f16, peak=20.0)
+
+
+def test_scales():
+    for s in (0.0, -0.3, 1e-20, 1.0):
+        run_case([200], [(0, 199)], 16, 2, 256, 16, True, scale=s)
+
+
+CHUNKS = [
+    ([300], [(0, p) for p in range(300)]),                                            # a prompt from its first token
+    ([900], [(0, p) for p in range(644, 900)]),                                       # a chunk behind a context
+    ([70, 200, 33], [(0, p) for p in range(60, 70)] + [(1, p) for p in range(100, 200)] + [(2, p) for p in range(33)]),
+    ([40, 50], [(0, 39), (1, 49), (0, 38), (1, 3), (-1, -1), (0, 5), (0, 5), (1, -1), (0, 39)]),      # no order at all
+    ([120, 64], [(0, p) for p in range(100, 120)] + [(-1, -1)] * 5 + [(1, p) for p in range(60, 64)] + [(-1, -1)] * 40),
+]
+
+
+@pytest.mark.parametrize("i", range(len(CHUNKS)))
+@pytest.mark.parametrize("H,KV,D", [HEADS[0], HEADS[2], HEADS[3], HEADS[4], HEADS[5]])
+@pytest.mark.parametrize("f16", [True, False])
+def test_several_rows_a_request(i, H, KV, D, f16):
+    lens, rows = CHUNKS[i]
+    log(f"attn chunk {i} H={H} KV={KV} D={D} f16={f16}")
+    run_case(lens, rows, H, KV, D, 32, f16, gate=True)
+
+
+def test_many_rows_of_many_requests():
+    """More rows than a launch has workgroups."""
+    rng = np.random.default_rng(4)
+    lens = rng.integers(1, 40, 700).tolist()
+    run_case(lens, [(r, l - 1) for r, l in enumerate(lens)], 4, 2, 64, 16, True)
+
+
+def test_pages_shared_by_requests():
+    """Two requests with the same first pages, as a shared prompt has."""
+    rng = np.random.default_rng(8)
+    kc, vc, table = make(rng, [64, 20], 2, 128, 16, True)
+    table = np.stack([table[0], table[0]])
+    table[1, 3] = table[0, 0]
+    q = rng.standard_normal((2, 8, 128)).astype(np.float32)
+    req, pos = np.array([0, 1], np.int32), np.array([63, 55], np.int32)
+    a = Attn(Cache(kc, vc), q, req, pos, table, 0.1)
+    R.check(a.call(), "attn")
+    sync()
+    check_attn(a.out.get(), *attn_oracle(q, kc, vc, table, req, pos, np.float64(np.float32(0.1))), 64, 128)
+
+
+def test_infinite_and_nan_values_in_use():
+    """An infinite value reaches the heads that weigh it and no others' dims; a NaN key makes its rows NaN."""
+    rng = np.random.default_rng(2)
+    for f16 in (True, False):
+        kc, vc, table = make(rng, [50, 50], 2, 128, 16, f16)
+        vc[table[0, 3], 0, 1, 5] = np.inf              # the last token, in a tile's tail
+        kc[table[1, 0], 1, 2, 7] = np.nan
+        q = rng.standard_normal((2, 4, 128)).astype(np.float32)
+        req, pos = np.array([0, 1], np.int32), np.array([49, 49], np.int32)
+        a = Attn(Cache(kc, vc), q, req, pos, table, 0.1)
+        R.check(a.call(), "attn")
+        sync()
+        got = a.out.get()
+        assert np.all(np.isposinf(got[0, :2, 5])) and np.all(np.isnan(got[1, 2:]))
+        assert np.isfinite(np.delete(got[0, :2], 5, axis=1)).all() and np.isfinite(got[0, 2:]).all()
+        assert np.isfinite(got[1, :2]).all()
+
+
+@pytest.mark.parametrize("size", [1e-12, 1e-3, 1e4, 1e15])
+def test_queries_of_any_size(size):
+    """Queries far from 1, the scale making up for it: the fp16 parts go by the row's own size."""
+    rng = np.random.default_rng(6)
+    kc, vc, table = make(rng, [130], 2, 256, 16, True)
+    q = (size * rng.standard_normal((1, 16, 256))).astype(np.float32)
+    q[0, 3] = 0
+    req, pos = np.zeros(1, np.int32), np.array([129], np.int32)
+    scale = np.float32(1 / (16 * size))
+    a = Attn(Cache(kc, vc), q, req, pos, table, float(scale))
+    R.check(a.call(), "attn")
+    sync()
+    check_attn(a.out.get(), *attn_oracle(q, kc, vc, table, req, pos, np.float64(scale)), 130, 256)
+
+
+def test_rows_behind_the_count_stay():
+    rng = np.random.default_rng(3)
+    kc, vc, table = make(rng, [40], 2, 64, 16, True)
+    q = rng.standard_normal((5, 4, 64)).astype(np.float32)
+    req, pos = np.zeros(5, np.int32), np.full(5, 39, np.int32)
+    a = Attn(Cache(kc, vc), q, req, pos, table, 0.125, rows=3)
+    R.check(a.call(), "attn")
+    sync()
+    got = a.out.get()
+    assert np.all(got[3:] == 77) and not np.any(got[:3] == 77)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_bad_rows_are_nan_and_reported(f16):
+    """Requests, positions and pages out of range: NaN in those rows, the others right."""
+    rng = np.random.default_rng(7)
+    lens = [50, 60, 40, 3000]
+    kc, vc, table = make(rng, lens, 2, 128, 16, f16)
+    n_pages, width = kc.shape[0], table.shape[1]
+    bad = table.copy()
+    bad[1, 2], bad[2, 0] = n_pages, -1
+    rows = [(0, 49), (1, 59), (1, 31), (2, 39), (4, 3), (-2, 3), (0, -2), (0, 16 * width), (3, 2999), (0, 2 ** 31 - 1),
+            (0, -2 ** 31)] + [(0, 20)] * 30
+    rows = np.array(rows, np.int32)
+    q = rng.standard_normal((len(rows), 8, 128)).astype(np.float32)
+    a = Attn(Cache(kc, vc), q, rows[:, 0].copy(), rows[:, 1].copy(), bad, 0.1)
+    R.check(a.call(), "attn")
+    assert R.lib().roaster_sync() == R.EINVAL
+    sync()
+    got = a.out.get()
+    good = np.array([i for i in range(len(rows)) if i in (0, 2, 8) or i > 10])
+    assert all(np.isnan(got[i]).all() for i in range(len(rows)) if i not in good)
+    want = attn_oracle(q[good], kc, vc, table, rows[good, 0], rows[good, 1], np.float64(np.float32(0.1)))
+    check_attn(got[good], *want, 3000, 128)
+
+
+def test_cache_past_32_bit_offsets():
+    """Pages beyond 2^32 elements of a cache of 9 GB for the keys and as much for the values."""
+    L = R.lib()
+    KV, D, page, n_pages = 2, 256, 64, 140000
+    size = KV * page * D * 2
+    rng = np.random.default_rng(12)
+    lens = [64 * 5 + 9]
+    kc, vc, table = make(rng, lens, KV, D, page, True, spare=0)
+    ids = np.array([n_pages - 1 - 2 * i for i in range(6)], np.int32)
+    assert (int(ids.min()) * size) // 2 > 2 ** 32
+    k, v = (L.roaster_dev_alloc(n_pages * size) for _ in range(2))
+    assert k and v, R.last_error()
+    try:
+        for i in range(6):
+            for base, c in ((k, kc), (v, vc)):
+                part = np.ascontiguousarray(c[table[0, i]])
+                R.check(L.roaster_h2d(base + int(ids[i]) * size, part.ctypes.data, size), "h2d")
+        far = table.copy()
+        far[0, :6] = ids
+        q = rng.standard_normal((1, 16, D)).astype(np.float32)
+        req, pos = np.zeros(1, np.int32), np.array([lens[0] - 1], np.int32)
+        c = Cache(kc, vc)
+        a = Attn(c, q, req, pos, far, 0.0625)
+        c.c.k, c.c.v, c.c.n_pages = k, v, n_pages
+        R.check(a.call(), "attn")
+        sync()
+        check_attn(a.out.get(), *attn_oracle(q, kc, vc, table, req, pos, 0.0625), lens[0], D)
+    finally:
+        L.roaster_dev_free(k)
+        L.roaster_dev_free(v)
