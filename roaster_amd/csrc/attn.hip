@@ -1,77 +1,472 @@
 /*
  * attn.hip -- softmax attention of new rows over a paged key/value cache
  * (roaster_attn_paged; model.c:755-863, 1536-1602).
+ *
+ * A unit of work is one row and up to HPB query heads of one key/value head; it
+ * goes over the row's positions in tiles of TT tokens.  Every workgroup sums
+ * the rows' tiles by itself and takes an even share of all units' tiles laid
+ * end to end, whatever the rows' lengths; its waves take a unit's tiles in turn,
+ * each with its own running maximum and sums, and join them in LDS.  A unit that
+ * lies within one share is finished there.  Of one that a share's end cuts, the
+ * parts go to the workspace and attn_join_kernel joins them.
+ *
+ * Both products are MFMAs whose sixteen columns are the heads, and whose operands
+ * come from global memory straight into registers:
+ *   S^T = K Q^T   rows: 16 tokens, a lane holds 16 bytes of its token's key;
+ *   O^T = V^T P^T rows: 16 elements, a lane holds 16 bytes of each of its tokens'
+ *                 values, transposed among its own registers; a lane's scores
+ *                 are the very probabilities that its operand needs, so P
+ *                 never moves between lanes.
+ * fp16 cache: a query row is scaled by a power of two and split into two fp16
+ * parts, the probabilities likewise, and the parts are the columns h and h + 8:
+ * the eight heads fill the sixteen columns, and products are exact up to 2^-22
+ * of an operand.  f32 cache: f32 MFMAs, columns 8..15 unused.
  */
 #include "attn.h"
 #include "qdot.h"
 
 #define ATT_T 256
+#define ATT_W (ATT_T / 64)
+#define ATT_G 512             /* workgroups: two per CU */
+#define ATT_MIN 4             /* tiles of a share at least: one a wave */
+#define HPB 8                 /* query heads of a unit */
+#define P_UP 7.0f             /* probabilities are kept times 2^7 (relative to the running maximum, which they
+                                 may pass by 2^8): the low fp16 part of one of 2^-10 is still normal */
+#define M_LATE 8.0f           /* the running maximum moves only when a score passes it by this much */
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttArgs {
     RoasterAttnPaged a;
-    const void *kc, *vc;
+    const char *kc, *vc;
     KvShape s;
+    int group, blocks;        /* query heads of a key/value head, and their blocks of HPB */
+    int by_unit;              /* the join's table goes by unit (else by the share that began the unit) */
+    int2 *cut;                /* [.] first share and number of shares of a unit to join; 0 shares: none */
+    float *pm, *pl, *po;      /* parts [2 ATT_G][HPB], [..][HPB], [..][HPB][D]: slot 2g + 1 the unit that share g
+                                 began and did not finish, 2g the one that it found begun */
 };
 
-template <bool F16>
-__device__ __forceinline__ float att_at(const void *c, size_t i)
+template <int D, bool F16>
+struct AttCfg {
+    static constexpr int TT = F16 ? 32 : 16, SUB = TT / 16, SZ = F16 ? 2 : 4;
+    static constexpr int VE = F16 ? (D >= 128 ? 8 : 4) : 4;       /* elements of a value load */
+    static constexpr int NB = D / (16 * VE);                        /* value loads of a token */
+    static constexpr int KS = F16 ? D / 32 : D / 16;                 /* 16-byte key loads of a token */
+    static constexpr int VT = F16 ? 8 : 4;                           /* tokens of a lane's value operand */
+    static constexpr int LD = D + 4;                                 /* LDS row */
+};
+
+__device__ __forceinline__ float max_g(float v)       /* over the four lanes of a column */
 {
-    return F16 ? (float)((const _Float16 *)c)[i] : ((const float *)c)[i];
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum_g(float v)
+{
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+/* One wave's state of a unit: lane (c = lane % 16, g = lane / 16) holds column c. */
+template <int D, bool F16>
+struct AttWave {
+    using C = AttCfg<D, F16>;
+    f16x8 qh[F16 ? C::KS : 1];
+    f32x4 qf[F16 ? 1 : C::KS];
+    float fac;                      /* log2 score of a product */
+    float m, l;
+    f32x4 o[C::NB * C::VE];
+    gu32x4 k[C::SUB][C::KS];
+    gu32x4 v[C::VT][C::NB];
+
+    __device__ void begin(const float *q, int c, int g, int nh, float scale)
+    {
+        const bool on = (c & 7) < nh && (F16 || c < HPB);
+        const float *p = q + (size_t)(c & 7) * D;
+        float x[F16 ? 8 * C::KS : 4 * C::KS], top = 0;
+        constexpr int E = F16 ? 8 : 4;
+        for (int s = 0; s < C::KS; s++)
+            for (int j = 0; j < E; j += 4) {
+                const float4 y = on ? *(const float4 *)(p + 4 * E * s + E * g + j) : make_float4(0, 0, 0, 0);
+                x[E * s + j] = y.x; x[E * s + j + 1] = y.y; x[E * s + j + 2] = y.z; x[E * s + j + 3] = y.w;
+            }
+        if (F16) {
+            for (int i = 0; i < 8 * C::KS; i++) top = fmaxf(top, fabsf(x[i]));
+            top = max_g(top);
+            /* 2^e times the row's largest element lies in [2^13, 2^14) */
+            int e = top > 0 && top < INFINITY ? 14 - (ilogbf(top) + 1) : 0;
+            e = min(e, 120);
+            const float up = ldexpf(1.0f, e);
+            for (int s = 0; s < C::KS; s++)
+                for (int j = 0; j < 8; j++) {
+                    const float y = x[8 * s + j] * up;
+                    const _Float16 hi = (_Float16)y;
+                    qh[s][j] = c < 8 ? hi : (_Float16)(y - (float)hi);
+                }
+            fac = ldexpf(scale * 1.44269504088896341f, -e);
+        } else {
+            for (int s = 0; s < C::KS; s++)
+                for (int j = 0; j < 4; j++) qf[s][j] = x[4 * s + j];
+            fac = scale * 1.44269504088896341f;
+        }
+        m = -INFINITY;
+        l = 0;
+        for (int i = 0; i < C::NB * C::VE; i++) o[i] = (f32x4){};
+    }
+    /* Keys of the tile whose 16-token parts begin at at[] (bytes, uniform). */
+    __device__ void load_k(const char *kc, const size_t *at, int c, int g)
+    {
+        for (int u = 0; u < C::SUB; u++) {
+            const char *b = kc + at[u];
+            const unsigned off = c * D * C::SZ + g * 16;
+            for (int s = 0; s < C::KS; s++) k[u][s] = *(const GAS gu32x4 *)(b + off + 64 * s);
+        }
+    }
+    __device__ void load_v(const char *vc, const size_t *at, int c, int g)
+    {
+        for (int j = 0; j < C::VT; j++) {
+            const char *b = vc + at[j / 4];
+            const unsigned off = ((4 * g + (j & 3)) * D + C::VE * c) * C::SZ;
+            for (int n = 0; n < C::NB; n++) {
+                const GAS char *p = (const GAS char *)(b + off + 16 * C::VE * C::SZ * n);
+                if (C::VE * C::SZ == 16) v[j][n] = *(const GAS gu32x4 *)p;
+                else {
+                    const gu32x2 h = *(const GAS gu32x2 *)p;
+                    v[j][n] = (gu32x4){ h.x, h.y, 0, 0 };
+                }
+            }
+        }
+    }
+    /* Scores of the tile in k: a lane gets VT tokens of its column, those at 4g + j % 4 of part j / 4. */
+    __device__ void scores(float *s)
+    {
+        for (int u = 0; u < C::SUB; u++) {
+            f32x4 a = {};
+            if (F16)
+                for (int i = 0; i < C::KS; i++)
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[u][i]), qh[i], a, 0, 0, 0);
+            else
+                for (int i = 0; i < C::KS; i++) {
+                    const f32x4 x = __builtin_bit_cast(f32x4, k[u][i]);
+                    for (int j = 0; j < 4; j++) a = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], qf[i][j], a, 0, 0, 0);
+                }
+            for (int j = 0; j < 4; j++) s[4 * u + j] = F16 ? a[j] + dpp_f<0x128>(a[j]) : a[j];     /* row_ror:8: the other part's column */
+        }
+    }
+    /* The tile's softmax terms, p in place of the scores; `left` tokens of the tile count. */
+    __device__ void soften(float *s, int left, int g)
+    {
+        float mx = -INFINITY;
+        for (int j = 0; j < C::VT; j++) s[j] *= fac;
+        if (left < C::TT)
+            for (int j = 0; j < C::VT; j++)
+                if (16 * (j / 4) + 4 * g + (j & 3) >= left) s[j] = -INFINITY;
+        for (int j = 0; j < C::VT; j++) mx = fmaxf(mx, s[j]);
+        mx = max_g(mx);
+        if (__any(mx > m + M_LATE)) {
+            const float mn = fmaxf(m, mx), w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= w;
+            for (int i = 0; i < C::NB * C::VE; i++) o[i] *= w;
+            m = mn;
+        }
+        const float base = m - P_UP;
+        for (int j = 0; j < C::VT; j++) {
+            s[j] = __builtin_amdgcn_exp2f(s[j] - base);
+            l += s[j];
+        }
+    }
+    __device__ void values(const float *p, int left, int c, int g)
+    {
+        if (left < C::TT)                              /* what lies behind the row may be anything: 0 * NaN is NaN */
+            for (int j = 0; j < C::VT; j++)
+                if (16 * (j / 4) + 4 * g + (j & 3) >= left)
+                    for (int n = 0; n < C::NB; n++) v[j][n] = (gu32x4){};
+        if (F16) {
+            f16x8 b;
+            const float low = c < 8 ? 0.0f : 1.0f;
+            for (int j = 0; j < 8; j += 2) {
+                typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+                const h2 hi = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
+                const h2 r = __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)hi.x, low, p[j]), fmaf(-(float)hi.y, low, p[j + 1]));
+                b[j] = (_Float16)r.x;
+                b[j + 1] = (_Float16)r.y;
+            }
+            for (int n = 0; n < C::NB; n++)
+                for (int e = 0; e < C::VE; e++) {
+                    gu32x4 a;
+                    for (int j = 0; j < 4; j++)
+                        a[j] = __builtin_amdgcn_perm(v[2 * j + 1][n][e / 2], v[2 * j][n][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+                    o[n * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b,
+                                                                              o[n * C::VE + e], 0, 0, 0);
+                }
+        } else {
+            for (int n = 0; n < C::NB; n++)
+                for (int e = 0; e < 4; e++)
+                    for (int j = 0; j < 4; j++)
+                        o[n * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, v[j][n])[e], p[j],
+                                                                            o[n * 4 + e], 0, 0, 0);
+        }
+    }
+};
+
+/* Inclusive sums over the workgroup of 64-bit values; `tot` gets the whole. */
+__device__ __forceinline__ long long att_scan(long long v, long long *s_wave, long long &tot)
+{
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    _Pragma("unroll")
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long u = __shfl_up(v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 63) s_wave[w] = v;
+    __syncthreads();
+    long long before = 0, all = 0;
+    for (int i = 0; i < ATT_W; i++) {
+        if (i == w) before = all;
+        all += s_wave[i];
+    }
+    tot = all;
+    return v + before;
 }
 
-/* One workgroup per row and query head; its waves take the row's positions in
- * turn, each with its own running maximum and sum, and join them at the end. */
-template <int D, bool F16>
-__global__ __launch_bounds__(ATT_T) void attn_kernel(AttArgs A, int *err)
+/* Tiles of a row: at least one for a row that has an output to write. */
+template <int TT>
+__device__ __forceinline__ int att_tiles(const KvTable &T, int req, int pos, int shift)
 {
-    constexpr int N = D / 64, W = ATT_T / 64;
-    __shared__ float s_m[W], s_l[W], s_o[W][D];
-    __shared__ bool s_bad[W];
+    if (req == -1) return 0;
+    const int n = T.tokens(req, pos, shift);
+    return n <= TT ? 1 : (int)(((long long)n + TT - 1) / TT);
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_kernel(AttArgs A, int *err)
+{
+    using C = AttCfg<D, F16>;
+    __shared__ float s_o[ATT_W][HPB][C::LD], s_m[ATT_W][HPB], s_l[ATT_W][HPB];
+    __shared__ long long s_wave[ATT_W], s_at;
+    __shared__ int s_row;
     const RoasterAttnPaged &a = A.a;
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int r = a.row_req[t];
-    if (r == -1) return;
     const KvTable T = { a.n_req, a.max_pages };
-    const int n = T.tokens(r, a.row_pos[t], A.s.shift), kh = h / (a.q_heads / A.s.kv);
-    bool bad = n < 0;
-    const float *q = a.q + ((size_t)t * a.q_heads + h) * D + lane * N;
-    float qv[N], o[N] = {}, m = -INFINITY, sum = 0;
-    for (int i = 0; i < N; i++) qv[i] = q[i] * a.scale;
-    for (int j = w; j < n; j += W) {
-        const int p = a.table[T.entry(r, j, A.s.shift)];
-        if (!A.s.page_ok(p)) { bad = true; break; }
-        const size_t at = A.s.at(p, kh, j & ((1 << A.s.shift) - 1)) + lane * N;
-        float s = 0;
-        for (int i = 0; i < N; i++) s = fmaf(qv[i], att_at<F16>(A.kc, at + i), s);
-        s = group_sum<64>(s);
-        const float mn = s == s ? fmaxf(m, s) : s;             /* a NaN score stays one */
-        const float c = mn == -INFINITY ? 1.0f : expf(m - mn), e = mn == -INFINITY ? 0.0f : expf(s - mn);
-        sum = sum * c + e;
-        for (int i = 0; i < N; i++) o[i] = fmaf(e, att_at<F16>(A.vc, at + i), o[i] * c);
-        m = mn;
+    const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
+    const int per_row = A.s.kv * A.blocks, rows = a.rows;
+
+    /* this share: where it begins in all units' tiles laid end to end */
+    const int each = (rows + ATT_T - 1) / ATT_T;
+    long long mine = 0, tot;
+    for (int i = 0; i < each; i++) {
+        const int t = tid * each + i;
+        if (t < rows) mine += att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift);
     }
-    if (lane == 0) { s_m[w] = m; s_l[w] = sum; s_bad[w] = bad; }
-    for (int i = 0; i < N; i++) s_o[w][lane * N + i] = o[i];
+    const long long upto = att_scan(mine, s_wave, tot);
+    const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
+    long long at = blockIdx.x * share;
+    const long long end = min(all, at + share);
+    if (at >= end) {
+        if (!A.by_unit && tid == 0) A.cut[blockIdx.x] = make_int2(0, 0);
+        return;
+    }
+    if (at < upto * per_row && at >= (upto - mine) * per_row) {        /* one thread's rows hold it */
+        long long b = (upto - mine) * per_row;
+        int t = tid * each, n;
+        while (at >= b + (n = att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift)) * (long long)per_row) {
+            b += n * (long long)per_row;
+            t++;
+        }
+        s_row = t;
+        s_at = b;
+    }
     __syncthreads();
-    float mx = -INFINITY, l = 0;
-    bool any = false;                                       /* some wave met an index out of range */
-    for (int i = 0; i < W; i++) any |= s_bad[i];
-    for (int i = 0; i < W; i++) mx = fmaxf(mx, s_m[i]);
-    for (int i = 0; i < W; i++) l += s_m[i] == -INFINITY ? 0.0f : s_l[i] * expf(s_m[i] - mx);
-    if (any && threadIdx.x == 0) atomicOr(err, ATTN_ERR_INDEX);
-    for (int d = threadIdx.x; d < D; d += ATT_T) {
-        float y = 0;
-        for (int i = 0; i < W; i++) y += s_m[i] == -INFINITY ? 0.0f : s_o[i][d] * expf(s_m[i] - mx);
-        y = any ? NAN : l == 0 ? 0.0f : y / l;
-        if (a.gate) y /= 1.0f + expf(-a.gate[t * a.gate_row + h * a.gate_head + d]);
-        a.out[((size_t)t * a.q_heads + h) * D + d] = y;
+    int t = uni(s_row), req = uni(a.row_req[t]), pos = uni(a.row_pos[t]);
+    const long long row_at = s_at;
+    int tiles = att_tiles<C::TT>(T, req, pos, shift);
+    int hb = uni((int)((at - row_at) / tiles)), first = uni((int)((at - row_at) % tiles));
+
+    AttWave<D, F16> wv;
+    while (at < end) {
+        const int last = uni((int)min((long long)tiles, first + (end - at)));       /* tiles [first, last) of unit (t, hb) */
+        const int kh = hb / A.blocks, bk = hb % A.blocks, nh = min(HPB, A.group - bk * HPB);
+        const int h0 = kh * A.group + bk * HPB, n = T.tokens(req, pos, shift);
+        bool bad = n < 0;
+        wv.begin(a.q + ((size_t)t * a.q_heads + h0) * D, c, g, nh, a.scale);
+        /* the bytes at which tile i's 16-token parts begin; a part past the row's end repeats the first */
+        auto where = [&](int i, size_t *b) {
+            for (int u = 0; u < C::SUB; u++) {
+                const int tok = i * C::TT + 16 * u;
+                if (u && tok >= n) { b[u] = b[0]; continue; }
+                int p = uni(a.table[T.entry(req, tok, shift)]);
+                if (!A.s.page_ok(p)) { bad = true; p = 0; }
+                b[u] = A.s.at(p, kh, tok & ((1 << shift) - 1)) * C::SZ;
+            }
+        };
+        if (n > 0) {
+            size_t b[C::SUB];
+            int i = first + w;
+            if (i < last) {
+                where(i, b);
+                wv.load_k(A.kc, b, c, g);
+                wv.load_v(A.vc, b, c, g);
+            }
+            while (i < last) {
+                const int left = n - i * C::TT, next = i + ATT_W;
+                float s[C::VT];
+                wv.scores(s);
+                if (next < last) {
+                    where(next, b);
+                    wv.load_k(A.kc, b, c, g);
+                }
+                wv.soften(s, left, g);
+                wv.values(s, left, c, g);
+                if (next < last) wv.load_v(A.vc, b, c, g);
+                i = next;
+            }
+        }
+        /* the waves' parts into LDS; an infinite or NaN high part (an infinite value) stands for itself */
+        const float l = sum_g(wv.l);
+        if (g == 0 && c < HPB) { s_m[w][c] = wv.m; s_l[w][c] = l; }
+        for (int b = 0; b < C::NB; b++)
+            for (int i = 0; i < 4; i++) {
+                float y[C::VE];
+                for (int e = 0; e < C::VE; e++) {
+                    const float hi = wv.o[b * C::VE + e][i];
+                    y[e] = hi;
+                    if (F16) {
+                        const float lo = dpp_f<0x128>(hi);
+                        y[e] = fabsf(hi) < INFINITY ? hi + lo : hi;
+                    }
+                }
+                if (c < HPB)
+                    for (int e = 0; e < C::VE; e += 4)
+                        *(float4 *)&s_o[w][c][16 * C::VE * b + C::VE * (4 * g + i) + e] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+            }
+        const bool any = __syncthreads_or(bad);
+        if (any && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
+        const bool whole = first == 0 && last == tiles;
+        const int slot = 2 * blockIdx.x + (first == 0);
+        for (int idx = tid * 4; idx < nh * D; idx += ATT_T * 4) {
+            const int h = idx / D, d = idx % D;
+            float mx = -INFINITY, sum = 0;
+            f32x4 y = {};
+            for (int i = 0; i < ATT_W; i++) mx = fmaxf(mx, s_m[i][h]);
+            for (int i = 0; i < ATT_W; i++) {
+                const float f = s_m[i][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i][h] - mx);
+                sum += s_l[i][h] * f;
+                y += *(const f32x4 *)&s_o[i][h][d] * f;
+            }
+            if (any) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
+            if (whole) {
+                const size_t hh = h0 + h;
+                y *= n == 0 ? 0.0f : 1.0f / sum;
+                if (a.gate) {
+                    const float4 gt = *(const float4 *)(a.gate + t * a.gate_row + hh * a.gate_head + d);
+                    y[0] /= 1.0f + expf(-gt.x); y[1] /= 1.0f + expf(-gt.y); y[2] /= 1.0f + expf(-gt.z); y[3] /= 1.0f + expf(-gt.w);
+                }
+                *(f32x4 *)(a.out + ((size_t)t * a.q_heads + hh) * D + d) = y;
+            } else {
+                *(f32x4 *)(A.po + ((size_t)slot * HPB + h) * D + d) = y;
+                if (d == 0) {
+                    A.pm[slot * HPB + h] = mx;
+                    A.pl[slot * HPB + h] = sum;
+                }
+            }
+        }
+        if (!A.by_unit && first && at + last - first == end && tid == 0) A.cut[blockIdx.x] = make_int2(0, 0);
+        if (first == 0 && tid == 0) {                  /* for the join: the shares of this unit, 0 where it ends here */
+            const long long u1 = at + tiles - 1;
+            const int k = whole ? 0 : (int)(u1 / share) - (int)blockIdx.x + 1;
+            if (A.by_unit) A.cut[t * per_row + hb] = make_int2(blockIdx.x, k);
+            else if (at + last == end) A.cut[blockIdx.x] = make_int2(t * per_row + hb, k);
+        }
+        at += last - first;
+        first = 0;
+        if (++hb == per_row && at < end) {
+            hb = 0;
+            do {
+                t++;
+                req = uni(a.row_req[t]);
+            } while (req == -1);
+            pos = uni(a.row_pos[t]);
+            tiles = att_tiles<C::TT>(T, req, pos, shift);
+        }
+        __syncthreads();
     }
 }
+
+#define JOIN_T 512
+
+/* The parts of one cut unit's head: weights exp2(m_k - max), sums of the parts
+ * and of their l.  A workgroup reads one head's parts, D/4 lanes to a part. */
+template <int D>
+__global__ __launch_bounds__(JOIN_T) void attn_join_kernel(AttArgs A)
+{
+    constexpr int L = D / 4, N = JOIN_T / L;
+    __shared__ float s_w[ATT_G], s_red[JOIN_T / 64], s_l[JOIN_T / 64];
+    __shared__ f32x4 s_o[N][L];
+    const RoasterAttnPaged &a = A.a;
+    const int tid = threadIdx.x, h = blockIdx.y, per_row = A.s.kv * A.blocks;
+    int unit = blockIdx.x;
+    if (A.by_unit && a.row_req[unit / per_row] == -1) return;
+    const int2 e = A.cut[blockIdx.x];
+    const int n = e.y, g0 = A.by_unit ? e.x : (int)blockIdx.x;
+    if (n == 0) return;
+    if (!A.by_unit) unit = e.x;
+    const int t = unit / per_row, hb = unit % per_row, kh = hb / A.blocks, bk = hb % A.blocks;
+    if (h >= A.group - bk * HPB) return;
+    auto slot = [&](int k) { return (size_t)(k ? 2 * (g0 + k) : 2 * g0 + 1) * HPB + h; };
+    float m = -INFINITY, l = 0;
+    if (tid < n) {
+        m = A.pm[slot(tid)];
+        l = A.pl[slot(tid)];
+    }
+    float mx = m;
+    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    if ((tid & 63) == 0) s_red[tid >> 6] = mx;
+    __syncthreads();
+    for (int i = 0; i < JOIN_T / 64; i++) mx = fmaxf(mx, s_red[i]);
+    const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+    l *= w;
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    if ((tid & 63) == 0) s_l[tid >> 6] = l;
+    if (tid < n) s_w[tid] = w;
+    __syncthreads();
+    f32x4 y = {};
+    const int sub = tid / L, d = tid % L * 4;
+#pragma unroll 4
+    for (int k = sub; k < n; k += N) y += *(const f32x4 *)(A.po + slot(k) * D + d) * s_w[k];
+    s_o[sub][tid % L] = y;
+    __syncthreads();
+    if (tid >= L) return;
+    y = s_o[0][tid];
+    float sum = 0;
+    for (int i = 1; i < N; i++) y += s_o[i][tid];
+    for (int i = 0; i < JOIN_T / 64; i++) sum += s_l[i];
+    const size_t hh = kh * A.group + bk * HPB + h;
+    y *= 1.0f / sum;
+    if (a.gate) {
+        const float4 gt = *(const float4 *)(a.gate + t * a.gate_row + hh * a.gate_head + d);
+        y[0] /= 1.0f + expf(-gt.x); y[1] /= 1.0f + expf(-gt.y); y[2] /= 1.0f + expf(-gt.z); y[3] /= 1.0f + expf(-gt.w);
+    }
+    *(f32x4 *)(a.out + ((size_t)t * a.q_heads + hh) * D + d) = y;
+}
+
+/* Workspace: the cut table, then m and l of the parts, then the parts. */
+static const size_t ATT_CUT = (size_t)ATT_G * sizeof(int2), ATT_ML = (size_t)2 * ATT_G * HPB * 4;
 
 extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCache *c)
 {
     if (!attn_cache_ok(c) || rows < 0 || rows > (1 << 20) || q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads) return 0;
-    return 256;
+    return ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * HPB * c->head_dim * 4;
+}
+
+template <int D, bool F16>
+static void att_launch(const AttArgs &A, int *err)
+{
+    const long long units = (long long)A.a.rows * A.s.kv * A.blocks;
+    hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(ATT_G), dim3(ATT_T), 0, rt().stream, A, err);
+    hipLaunchKernelGGL((attn_join_kernel<D>), dim3(units < ATT_G ? (int)units : ATT_G, A.group < HPB ? A.group : HPB),
+                       dim3(JOIN_T), 0, rt().stream, A);
 }
 
 extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCache *c)
@@ -104,18 +499,21 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     const AttnDevice dev;
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
-    const AttArgs A = { *p, c->k, c->v, attn_shape(c) };
-    const dim3 gd(p->rows, p->q_heads), bd(ATT_T);
-#define ATT(DD, H) hipLaunchKernelGGL((attn_kernel<DD, H>), gd, bd, 0, rt().stream, A, err)
-    if (c->type == ROASTER_KV_F16) {
-        if (D == 256) ATT(256, true);
-        else if (D == 128) ATT(128, true);
-        else ATT(64, true);
-    } else {
-        if (D == 256) ATT(256, false);
-        else if (D == 128) ATT(128, false);
-        else ATT(64, false);
-    }
-#undef ATT
+    AttArgs A;
+    A.a = *p;
+    A.kc = (const char *)c->k;
+    A.vc = (const char *)c->v;
+    A.s = attn_shape(c);
+    A.group = p->q_heads / c->kv_heads;
+    A.blocks = (A.group + HPB - 1) / HPB;
+    A.by_unit = (long long)p->rows * c->kv_heads * A.blocks <= ATT_G;
+    A.cut = (int2 *)p->ws;
+    A.pm = (float *)((char *)p->ws + ATT_CUT);
+    A.pl = (float *)((char *)p->ws + ATT_CUT + ATT_ML);
+    A.po = (float *)((char *)p->ws + ATT_CUT + 2 * ATT_ML);
+    const bool f16 = c->type == ROASTER_KV_F16;
+    if (D == 256) f16 ? att_launch<256, true>(A, err) : att_launch<256, false>(A, err);
+    else if (D == 128) f16 ? att_launch<128, true>(A, err) : att_launch<128, false>(A, err);
+    else f16 ? att_launch<64, true>(A, err) : att_launch<64, false>(A, err);
     return rt_check(hipGetLastError(), "attention launch") ? ROASTER_EDEVICE : 0;
 }
