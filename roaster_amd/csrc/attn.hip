@@ -43,9 +43,10 @@ struct AttArgs {
     KvShape s;
     int group, blocks;        /* query heads of a key/value head, and their blocks of HPB */
     int by_unit;              /* the join's table goes by unit (else by the share that began the unit) */
+    int few;                  /* attn_few_kernel's parts: one a workgroup */
     int2 *cut;                /* [.] first share and number of shares of a unit to join; 0 shares: none */
-    float *pm, *pl, *po;      /* parts [2 ATT_G][HPB], [..][HPB], [..][HPB][D]: slot 2g + 1 the unit that share g
-                                 began and did not finish, 2g the one that it found begun */
+    float *pm, *pl, *po;      /* parts [2 ATT_G][HPB], [..][HPB], [..][HPB][D]: slot g with `few`, else 2g + 1 the unit
+                                 that share g began and did not finish, 2g the one that it found begun */
 };
 
 template <int D, bool F16>
@@ -82,39 +83,57 @@ struct AttWave {
     gu32x4 k[C::SUB][C::KS];
     gu32x4 v[C::VT][C::NB];
 
-    __device__ void begin(const float *q, int c, int g, int nh, float scale)
+    /* The unit's queries as they lie: column c's head, zeros where there is none. */
+    static constexpr int QE = F16 ? 8 : 4;          /* elements of a product operand */
+    struct Raw {
+        float4 x[QE * C::KS / 4];
+    };
+    __device__ static void load_q(Raw &r, const float *q, int c, int g, int nh)
+    {
+        const float *p = q + ((c & 7) < nh ? (c & 7) : 0) * D + QE * g;
+#pragma unroll
+        for (int s = 0; s < C::KS; s++)
+#pragma unroll
+            for (int j = 0; j < QE / 4; j++) r.x[QE / 4 * s + j] = *(const float4 *)(p + 4 * QE * s + 4 * j);
+    }
+    __device__ void clear()
+    {
+        m = -INFINITY;
+        l = 0;
+#pragma unroll
+        for (int i = 0; i < C::NB * C::VE; i++) o[i] = (f32x4){};
+    }
+    __device__ void begin(const Raw &r, int c, int nh, float scale)
     {
         const bool on = (c & 7) < nh && (F16 || c < HPB);
-        const float *p = q + (size_t)(c & 7) * D;
-        float x[F16 ? 8 * C::KS : 4 * C::KS], top = 0;
-        constexpr int E = F16 ? 8 : 4;
-        for (int s = 0; s < C::KS; s++)
-            for (int j = 0; j < E; j += 4) {
-                const float4 y = on ? *(const float4 *)(p + 4 * E * s + E * g + j) : make_float4(0, 0, 0, 0);
-                x[E * s + j] = y.x; x[E * s + j + 1] = y.y; x[E * s + j + 2] = y.z; x[E * s + j + 3] = y.w;
-            }
+        float x[QE * C::KS], top = 0;
+#pragma unroll
+        for (int s = 0; s < QE * C::KS / 4; s++) {
+            x[4 * s] = on ? r.x[s].x : 0.0f; x[4 * s + 1] = on ? r.x[s].y : 0.0f;
+            x[4 * s + 2] = on ? r.x[s].z : 0.0f; x[4 * s + 3] = on ? r.x[s].w : 0.0f;
+        }
         if (F16) {
-            for (int i = 0; i < 8 * C::KS; i++) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+            for (int i = 0; i < QE * C::KS; i++) top = fmaxf(top, fabsf(x[i]));
             top = max_g(top);
-            /* 2^e times the row's largest element lies in [2^13, 2^14) */
-            int e = top > 0 && top < INFINITY ? 14 - (ilogbf(top) + 1) : 0;
-            e = min(e, 120);
-            const float up = ldexpf(1.0f, e);
+            /* 2^e times the row's largest element lies in [2^13, 2^14); e within what a float's exponent holds */
+            const int b = (__builtin_bit_cast(int, top) >> 23) & 255, e = b == 255 ? 0 : min(13 + 127 - b, 120);
+            const float up = __builtin_bit_cast(float, (127 + e) << 23);
+#pragma unroll
             for (int s = 0; s < C::KS; s++)
+#pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float y = x[8 * s + j] * up;
                     const _Float16 hi = (_Float16)y;
                     qh[s][j] = c < 8 ? hi : (_Float16)(y - (float)hi);
                 }
-            fac = ldexpf(scale * 1.44269504088896341f, -e);
+            fac = scale * 1.44269504088896341f * __builtin_bit_cast(float, (127 - e) << 23);
         } else {
+#pragma unroll
             for (int s = 0; s < C::KS; s++)
                 for (int j = 0; j < 4; j++) qf[s][j] = x[4 * s + j];
             fac = scale * 1.44269504088896341f;
         }
-        m = -INFINITY;
-        l = 0;
-        for (int i = 0; i < C::NB * C::VE; i++) o[i] = (f32x4){};
     }
     /* Keys of the tile whose 16-token parts begin at at[] (bytes, uniform). */
     __device__ void load_k(const char *kc, const size_t *at, int c, int g)
@@ -241,17 +260,189 @@ __device__ __forceinline__ int att_tiles(const KvTable &T, int req, int pos, int
     return n <= TT ? 1 : (int)(((long long)n + TT - 1) / TT);
 }
 
+template <int D>
+struct AttLds {
+    float o[ATT_W][HPB][D + 4], m[ATT_W][HPB], l[ATT_W][HPB];
+};
+
+/* out of one row's head from the sums y and l, four elements at d. */
+__device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int t, int h, int d, f32x4 y, float l)
+{
+    y *= 1.0f / l;
+    if (a.gate) {
+        const float4 gt = *(const float4 *)(a.gate + t * a.gate_row + h * a.gate_head + d);
+        y[0] /= 1.0f + expf(-gt.x); y[1] /= 1.0f + expf(-gt.y); y[2] /= 1.0f + expf(-gt.z); y[3] /= 1.0f + expf(-gt.w);
+    }
+    *(f32x4 *)(a.out + ((size_t)t * a.q_heads + h) * D + d) = y;
+}
+
+/* Tiles [first, last) of unit (t, hb) by one workgroup: to out if that is all of
+ * them, else to part `slot`. */
+template <int D, bool F16>
+__device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *err, int t, int req, int pos, int hb, int first,
+                                         int last, bool whole, int slot)
+{
+    using C = AttCfg<D, F16>;
+    const RoasterAttnPaged &a = A.a;
+    const KvTable T = { a.n_req, a.max_pages };
+    const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
+    const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(HPB, A.group - bk * HPB);
+    const int h0 = kh * A.group + bk * HPB, n = T.tokens(req, pos, shift);
+    bool bad = n < 0;
+    AttWave<D, F16> wv;
+    typename AttWave<D, F16>::Raw raw;
+    /* page numbers of tile i's 16-token parts (a part past the row's end repeats the
+     * first), then the bytes at which the parts begin */
+    auto pages = [&](int i, int *p) {
+#pragma unroll
+        for (int u = 0; u < C::SUB; u++) {
+            const int tok = i * C::TT + 16 * u;
+            p[u] = u && tok >= n ? p[0] : a.table[T.entry(req, tok, shift)];
+        }
+    };
+    auto where = [&](int i, const int *p, size_t *b) {
+#pragma unroll
+        for (int u = 0; u < C::SUB; u++) {
+            const int tok = i * C::TT + 16 * u;
+            int pg = uni(p[u]);
+            if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
+            b[u] = A.s.at(pg, kh, (u && tok >= n ? i * C::TT : tok) & ((1 << shift) - 1)) * C::SZ;
+        }
+    };
+    wv.clear();
+    int i = first + w;
+    if (n > 0 && i < last) {
+        int p[C::SUB], i2 = i + ATT_W;
+        size_t b[C::SUB];
+        pages(i, p);
+        wv.load_q(raw, a.q + ((size_t)t * a.q_heads + h0) * D, c, g, nh);
+        where(i, p, b);
+        wv.load_k(A.kc, b, c, g);
+        if (i2 < last) pages(i2, p);
+        wv.load_v(A.vc, b, c, g);
+        wv.begin(raw, c, nh, a.scale);
+        while (1) {
+            const int left = n - i * C::TT;
+            const bool more = i2 < last;
+            float s[C::VT];
+            wv.scores(s);
+            if (more) {
+                where(i2, p, b);
+                wv.load_k(A.kc, b, c, g);
+                if (i2 + ATT_W < last) pages(i2 + ATT_W, p);
+            }
+            wv.soften(s, left, g);
+            wv.values(s, left, c, g);
+            if (!more) break;
+            wv.load_v(A.vc, b, c, g);
+            i = i2;
+            i2 += ATT_W;
+        }
+    }
+    /* the waves' parts into LDS; an infinite or NaN high part (an infinite value) stands for itself */
+    const float l = sum_g(wv.l);
+    if (g == 0 && c < HPB) { S.m[w][c] = wv.m; S.l[w][c] = l; }
+#pragma unroll
+    for (int b = 0; b < C::NB; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float y[C::VE];
+#pragma unroll
+            for (int e = 0; e < C::VE; e++) {
+                const float hi = wv.o[b * C::VE + e][i];
+                y[e] = hi;
+                if (F16) {
+                    const float lo = dpp_f<0x128>(hi);
+                    y[e] = fabsf(hi) < INFINITY ? hi + lo : hi;
+                }
+            }
+            if (c < HPB)
+#pragma unroll
+                for (int e = 0; e < C::VE; e += 4)
+                    *(float4 *)&S.o[w][c][16 * C::VE * b + C::VE * (4 * g + i) + e] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+        }
+    const bool any = __syncthreads_or(bad);
+    if (any && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
+    for (int idx = tid * 4; idx < nh * D; idx += ATT_T * 4) {
+        const int h = idx / D, d = idx % D;
+        float mx = -INFINITY, sum = 0;
+        f32x4 y = {};
+#pragma unroll
+        for (int i = 0; i < ATT_W; i++) mx = fmaxf(mx, S.m[i][h]);
+#pragma unroll
+        for (int i = 0; i < ATT_W; i++) {
+            const float f = S.m[i][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(S.m[i][h] - mx);
+            sum += S.l[i][h] * f;
+            y += *(const f32x4 *)&S.o[i][h][d] * f;
+        }
+        if (any) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
+        if (whole) att_store(a, D, t, h0 + h, d, y, n == 0 ? 1.0f : sum);      /* without positions: y is 0 */
+        else {
+            *(f32x4 *)(A.po + ((size_t)slot * HPB + h) * D + d) = y;
+            if (d == 0) {
+                A.pm[slot * HPB + h] = mx;
+                A.pl[slot * HPB + h] = sum;
+            }
+        }
+    }
+}
+
+/* Few units (at most ATT_G / 4, of at most 128 rows): every workgroup takes one
+ * unit's part.  All tiles over (ATT_G - units) is a part's size S that gives at
+ * most ATT_G parts, since a unit of n tiles has ceil(n / S); a unit's parts are
+ * equal.  Each wave finds its part from the rows by itself, without a barrier. */
+template <int D, bool F16>
+__global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_few_kernel(AttArgs A, int *err)
+{
+    using C = AttCfg<D, F16>;
+    __shared__ AttLds<D> S;
+    const RoasterAttnPaged &a = A.a;
+    const KvTable T = { a.n_req, a.max_pages };
+    const int lane = threadIdx.x & 63, shift = A.s.shift, rows = a.rows, per_row = A.s.kv * A.blocks;
+    int req[2], pos[2], tl[2] = { 0, 0 };
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int t = min(lane + 64 * k, rows - 1);
+        req[k] = a.row_req[t];
+        pos[k] = a.row_pos[t];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        if (lane + 64 * k < rows) tl[k] = att_tiles<C::TT>(T, req[k], pos[k], shift);
+    /* the sum in f32, a little too large if anything */
+    const float all = group_sum<64>((float)tl[0] + (float)tl[1]) * per_row;
+    const int size = max(ATT_MIN, (int)(all * (1.0001f / (ATT_G - rows * per_row))) + 1);
+    int ch[2], in[2];
+    ch[0] = in[0] = (tl[0] + size - 1) / size;
+    ch[1] = in[1] = (tl[1] + size - 1) / size;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u0 = __shfl_up(in[0], o), u1 = rows > 64 ? __shfl_up(in[1], o) : 0;
+        if (lane >= o) { in[0] += u0; in[1] += u1; }
+    }
+    in[1] += __builtin_amdgcn_readlane(in[0], 63);
+    const int me = blockIdx.x, r0 = __popcll(__ballot(in[0] * per_row <= me)),
+              r1 = r0 < 64 ? 0 : __popcll(__ballot(in[1] * per_row <= me)), t = r0 + r1;
+    if (t >= rows) return;
+    const int src = t & 63;
+    auto pick = [&](const int *v) { return t < 64 ? __builtin_amdgcn_readlane(v[0], src) : __builtin_amdgcn_readlane(v[1], src); };
+    const int chunks = pick(ch), tiles = pick(tl), at = me - (pick(in) - chunks) * per_row;
+    const int hb = uni(at / chunks), k = at - hb * chunks, base = uni(tiles / chunks), rem = tiles - base * chunks;
+    const int first = k * base + min(k, rem), last = first + base + (k < rem);
+    att_part<D, F16>(A, S, err, t, pick(req), pick(pos), hb, first, last, chunks == 1, me);
+    if (k == 0 && threadIdx.x == 0) A.cut[t * per_row + hb] = make_int2(me, chunks == 1 ? 0 : chunks);
+}
+
 template <int D, bool F16>
 __global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_kernel(AttArgs A, int *err)
 {
     using C = AttCfg<D, F16>;
-    __shared__ float s_o[ATT_W][HPB][C::LD], s_m[ATT_W][HPB], s_l[ATT_W][HPB];
+    __shared__ AttLds<D> S;
     __shared__ long long s_wave[ATT_W], s_at;
     __shared__ int s_row;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
-    const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
-    const int per_row = A.s.kv * A.blocks, rows = a.rows;
+    const int tid = threadIdx.x, shift = A.s.shift, per_row = A.s.kv * A.blocks, rows = a.rows;
 
     /* this share: where it begins in all units' tiles laid end to end */
     const int each = (rows + ATT_T - 1) / ATT_T;
@@ -280,108 +471,21 @@ __global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_kern
     }
     __syncthreads();
     int t = uni(s_row), req = uni(a.row_req[t]), pos = uni(a.row_pos[t]);
-    const long long row_at = s_at;
     int tiles = att_tiles<C::TT>(T, req, pos, shift);
-    int hb = uni((int)((at - row_at) / tiles)), first = uni((int)((at - row_at) % tiles));
-
-    AttWave<D, F16> wv;
-    while (at < end) {
+    int hb = uni((int)((at - s_at) / tiles)), first = uni((int)((at - s_at) % tiles));
+    while (1) {
         const int last = uni((int)min((long long)tiles, first + (end - at)));       /* tiles [first, last) of unit (t, hb) */
-        const int kh = hb / A.blocks, bk = hb % A.blocks, nh = min(HPB, A.group - bk * HPB);
-        const int h0 = kh * A.group + bk * HPB, n = T.tokens(req, pos, shift);
-        bool bad = n < 0;
-        wv.begin(a.q + ((size_t)t * a.q_heads + h0) * D, c, g, nh, a.scale);
-        /* the bytes at which tile i's 16-token parts begin; a part past the row's end repeats the first */
-        auto where = [&](int i, size_t *b) {
-            for (int u = 0; u < C::SUB; u++) {
-                const int tok = i * C::TT + 16 * u;
-                if (u && tok >= n) { b[u] = b[0]; continue; }
-                int p = uni(a.table[T.entry(req, tok, shift)]);
-                if (!A.s.page_ok(p)) { bad = true; p = 0; }
-                b[u] = A.s.at(p, kh, tok & ((1 << shift) - 1)) * C::SZ;
-            }
-        };
-        if (n > 0) {
-            size_t b[C::SUB];
-            int i = first + w;
-            if (i < last) {
-                where(i, b);
-                wv.load_k(A.kc, b, c, g);
-                wv.load_v(A.vc, b, c, g);
-            }
-            while (i < last) {
-                const int left = n - i * C::TT, next = i + ATT_W;
-                float s[C::VT];
-                wv.scores(s);
-                if (next < last) {
-                    where(next, b);
-                    wv.load_k(A.kc, b, c, g);
-                }
-                wv.soften(s, left, g);
-                wv.values(s, left, c, g);
-                if (next < last) wv.load_v(A.vc, b, c, g);
-                i = next;
-            }
-        }
-        /* the waves' parts into LDS; an infinite or NaN high part (an infinite value) stands for itself */
-        const float l = sum_g(wv.l);
-        if (g == 0 && c < HPB) { s_m[w][c] = wv.m; s_l[w][c] = l; }
-        for (int b = 0; b < C::NB; b++)
-            for (int i = 0; i < 4; i++) {
-                float y[C::VE];
-                for (int e = 0; e < C::VE; e++) {
-                    const float hi = wv.o[b * C::VE + e][i];
-                    y[e] = hi;
-                    if (F16) {
-                        const float lo = dpp_f<0x128>(hi);
-                        y[e] = fabsf(hi) < INFINITY ? hi + lo : hi;
-                    }
-                }
-                if (c < HPB)
-                    for (int e = 0; e < C::VE; e += 4)
-                        *(float4 *)&s_o[w][c][16 * C::VE * b + C::VE * (4 * g + i) + e] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-            }
-        const bool any = __syncthreads_or(bad);
-        if (any && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
-        const bool whole = first == 0 && last == tiles;
-        const int slot = 2 * blockIdx.x + (first == 0);
-        for (int idx = tid * 4; idx < nh * D; idx += ATT_T * 4) {
-            const int h = idx / D, d = idx % D;
-            float mx = -INFINITY, sum = 0;
-            f32x4 y = {};
-            for (int i = 0; i < ATT_W; i++) mx = fmaxf(mx, s_m[i][h]);
-            for (int i = 0; i < ATT_W; i++) {
-                const float f = s_m[i][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i][h] - mx);
-                sum += s_l[i][h] * f;
-                y += *(const f32x4 *)&s_o[i][h][d] * f;
-            }
-            if (any) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
-            if (whole) {
-                const size_t hh = h0 + h;
-                y *= n == 0 ? 0.0f : 1.0f / sum;
-                if (a.gate) {
-                    const float4 gt = *(const float4 *)(a.gate + t * a.gate_row + hh * a.gate_head + d);
-                    y[0] /= 1.0f + expf(-gt.x); y[1] /= 1.0f + expf(-gt.y); y[2] /= 1.0f + expf(-gt.z); y[3] /= 1.0f + expf(-gt.w);
-                }
-                *(f32x4 *)(a.out + ((size_t)t * a.q_heads + hh) * D + d) = y;
-            } else {
-                *(f32x4 *)(A.po + ((size_t)slot * HPB + h) * D + d) = y;
-                if (d == 0) {
-                    A.pm[slot * HPB + h] = mx;
-                    A.pl[slot * HPB + h] = sum;
-                }
-            }
-        }
-        if (!A.by_unit && first && at + last - first == end && tid == 0) A.cut[blockIdx.x] = make_int2(0, 0);
-        if (first == 0 && tid == 0) {                  /* for the join: the shares of this unit, 0 where it ends here */
-            const long long u1 = at + tiles - 1;
-            const int k = whole ? 0 : (int)(u1 / share) - (int)blockIdx.x + 1;
-            if (A.by_unit) A.cut[t * per_row + hb] = make_int2(blockIdx.x, k);
-            else if (at + last == end) A.cut[blockIdx.x] = make_int2(t * per_row + hb, k);
+        const bool whole = first == 0 && last == tiles, cuts = first == 0 && !whole;
+        att_part<D, F16>(A, S, err, t, req, pos, hb, first, last, whole, 2 * blockIdx.x + (first == 0));
+        if (tid == 0) {                                /* for the join: the shares of a unit begun and cut here */
+            const int k = cuts ? (int)((at + tiles - 1) / share) - (int)blockIdx.x + 1 : 0;
+            if (A.by_unit && first == 0) A.cut[t * per_row + hb] = make_int2(blockIdx.x, k);
+            if (!A.by_unit && at + (last - first) == end) A.cut[blockIdx.x] = make_int2(t * per_row + hb, k);
         }
         at += last - first;
+        if (at >= end) break;
         first = 0;
-        if (++hb == per_row && at < end) {
+        if (++hb == per_row) {
             hb = 0;
             do {
                 t++;
@@ -390,65 +494,72 @@ __global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_kern
             pos = uni(a.row_pos[t]);
             tiles = att_tiles<C::TT>(T, req, pos, shift);
         }
-        __syncthreads();
+        __syncthreads();                               /* S is free again */
     }
 }
 
 #define JOIN_T 512
 
-/* The parts of one cut unit's head: weights exp2(m_k - max), sums of the parts
- * and of their l.  A workgroup reads one head's parts, D/4 lanes to a part. */
+/* The parts of one cut unit's head, D/4 lanes to a part: each group of lanes
+ * joins its parts as a running softmax does, the groups join in LDS. */
 template <int D>
 __global__ __launch_bounds__(JOIN_T) void attn_join_kernel(AttArgs A)
 {
     constexpr int L = D / 4, N = JOIN_T / L;
-    __shared__ float s_w[ATT_G], s_red[JOIN_T / 64], s_l[JOIN_T / 64];
+    __shared__ float s_m[N], s_l[N];
     __shared__ f32x4 s_o[N][L];
     const RoasterAttnPaged &a = A.a;
     const int tid = threadIdx.x, h = blockIdx.y, per_row = A.s.kv * A.blocks;
     int unit = blockIdx.x;
+    const int2 e = A.cut[unit];
     if (A.by_unit && a.row_req[unit / per_row] == -1) return;
-    const int2 e = A.cut[blockIdx.x];
-    const int n = e.y, g0 = A.by_unit ? e.x : (int)blockIdx.x;
+    const int n = e.y, g0 = A.by_unit ? e.x : unit;
     if (n == 0) return;
     if (!A.by_unit) unit = e.x;
     const int t = unit / per_row, hb = unit % per_row, kh = hb / A.blocks, bk = hb % A.blocks;
     if (h >= A.group - bk * HPB) return;
-    auto slot = [&](int k) { return (size_t)(k ? 2 * (g0 + k) : 2 * g0 + 1) * HPB + h; };
-    float m = -INFINITY, l = 0;
-    if (tid < n) {
-        m = A.pm[slot(tid)];
-        l = A.pl[slot(tid)];
-    }
-    float mx = m;
-    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    if ((tid & 63) == 0) s_red[tid >> 6] = mx;
-    __syncthreads();
-    for (int i = 0; i < JOIN_T / 64; i++) mx = fmaxf(mx, s_red[i]);
-    const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
-    l *= w;
-    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
-    if ((tid & 63) == 0) s_l[tid >> 6] = l;
-    if (tid < n) s_w[tid] = w;
-    __syncthreads();
-    f32x4 y = {};
     const int sub = tid / L, d = tid % L * 4;
-#pragma unroll 4
-    for (int k = sub; k < n; k += N) y += *(const f32x4 *)(A.po + slot(k) * D + d) * s_w[k];
+    float m = -INFINITY, l = 0;
+    f32x4 y = {};
+    for (int k0 = sub; k0 < n; k0 += 4 * N) {
+        float pm[4], pl[4];
+        f32x4 po[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int k = k0 + j * N, q = k < n ? k : k0;
+            const size_t at = (size_t)(A.few ? g0 + q : q ? 2 * (g0 + q) : 2 * g0 + 1) * HPB + h;
+            pm[j] = k < n ? A.pm[at] : -INFINITY;
+            pl[j] = A.pl[at];
+            po[j] = *(const f32x4 *)(A.po + at * D + d);
+        }
+        float mn = m;
+#pragma unroll
+        for (int j = 0; j < 4; j++) mn = fmaxf(mn, pm[j]);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        y *= f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (k0 + j * N >= n) continue;
+            const float w = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
+            l += pl[j] * w;
+            y += po[j] * w;
+        }
+        m = mn;
+    }
+    if (d == 0) { s_m[sub] = m; s_l[sub] = l; }
     s_o[sub][tid % L] = y;
     __syncthreads();
     if (tid >= L) return;
-    y = s_o[0][tid];
-    float sum = 0;
-    for (int i = 1; i < N; i++) y += s_o[i][tid];
-    for (int i = 0; i < JOIN_T / 64; i++) sum += s_l[i];
-    const size_t hh = kh * A.group + bk * HPB + h;
-    y *= 1.0f / sum;
-    if (a.gate) {
-        const float4 gt = *(const float4 *)(a.gate + t * a.gate_row + hh * a.gate_head + d);
-        y[0] /= 1.0f + expf(-gt.x); y[1] /= 1.0f + expf(-gt.y); y[2] /= 1.0f + expf(-gt.z); y[3] /= 1.0f + expf(-gt.w);
+    float mx = -INFINITY, sum = 0;
+    y = (f32x4){};
+    for (int i = 0; i < N; i++) mx = fmaxf(mx, s_m[i]);
+    for (int i = 0; i < N; i++) {
+        const float w = s_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - mx);
+        sum += s_l[i] * w;
+        y += s_o[i][tid] * w;
     }
-    *(f32x4 *)(a.out + ((size_t)t * a.q_heads + hh) * D + d) = y;
+    att_store(a, D, t, kh * A.group + bk * HPB + h, 4 * tid, y, sum);
 }
 
 /* Workspace: the cut table, then m and l of the parts, then the parts. */
@@ -464,7 +575,8 @@ template <int D, bool F16>
 static void att_launch(const AttArgs &A, int *err)
 {
     const long long units = (long long)A.a.rows * A.s.kv * A.blocks;
-    hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(ATT_G), dim3(ATT_T), 0, rt().stream, A, err);
+    if (A.few) hipLaunchKernelGGL((attn_few_kernel<D, F16>), dim3(ATT_G), dim3(ATT_T), 0, rt().stream, A, err);
+    else hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(ATT_G), dim3(ATT_T), 0, rt().stream, A, err);
     hipLaunchKernelGGL((attn_join_kernel<D>), dim3(units < ATT_G ? (int)units : ATT_G, A.group < HPB ? A.group : HPB),
                        dim3(JOIN_T), 0, rt().stream, A);
 }
@@ -506,7 +618,9 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     A.s = attn_shape(c);
     A.group = p->q_heads / c->kv_heads;
     A.blocks = (A.group + HPB - 1) / HPB;
-    A.by_unit = (long long)p->rows * c->kv_heads * A.blocks <= ATT_G;
+    const long long units = (long long)p->rows * c->kv_heads * A.blocks;
+    A.by_unit = units <= ATT_G;
+    A.few = units <= ATT_G / 4 && p->rows <= 128;
     A.cut = (int2 *)p->ws;
     A.pm = (float *)((char *)p->ws + ATT_CUT);
     A.pl = (float *)((char *)p->ws + ATT_CUT + ATT_ML);
