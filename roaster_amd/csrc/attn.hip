@@ -27,7 +27,7 @@
 
 #define ATT_T 256
 #define ATT_W (ATT_T / 64)
-#define ATT_G 512             /* workgroups: two per CU */
+#define ATT_G 512             /* workgroups at most: two per CU */
 #define ATT_MIN 4             /* tiles of a share at least: one a wave */
 #define HPB 8                 /* query heads of a unit */
 #define P_UP 7.0f             /* probabilities are kept times 2^7 (relative to the running maximum, which they
@@ -35,6 +35,7 @@
 #define M_LATE 8.0f           /* the running maximum moves only when a score passes it by this much */
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttArgs {
@@ -43,6 +44,7 @@ struct AttArgs {
     KvShape s;
     int group, blocks;        /* query heads of a key/value head, and their blocks of HPB */
     int by_unit;              /* the join's table goes by unit (else by the share that began the unit) */
+    int grid;                 /* workgroups */
     int few;                  /* attn_few_kernel's parts: one a workgroup */
     int2 *cut;                /* [.] first share and number of shares of a unit to join; 0 shares: none */
     float *pm, *pl, *po;      /* parts [2 ATT_G][HPB], [..][HPB], [..][HPB][D]: slot g with `few`, else 2g + 1 the unit
@@ -51,11 +53,11 @@ struct AttArgs {
 
 template <int D, bool F16>
 struct AttCfg {
-    static constexpr int TT = F16 ? 32 : 16, SUB = TT / 16, SZ = F16 ? 2 : 4;
+    static constexpr int TT = 16, SUB = 1, SZ = F16 ? 2 : 4;
     static constexpr int VE = F16 ? (D >= 128 ? 8 : 4) : 4;       /* elements of a value load */
     static constexpr int NB = D / (16 * VE);                        /* value loads of a token */
     static constexpr int KS = F16 ? D / 32 : D / 16;                 /* 16-byte key loads of a token */
-    static constexpr int VT = F16 ? 8 : 4;                           /* tokens of a lane's value operand */
+    static constexpr int VT = 4;                                     /* tokens of a lane's value operand */
     static constexpr int LD = D + 4;                                 /* LDS row */
 };
 
@@ -70,6 +72,31 @@ __device__ __forceinline__ float sum_g(float v)
     return v + __shfl_xor(v, 32);
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+/* N elements of a query column (a lane's quarter of them, or zeros) as hi + lo fp16
+ * parts of 2^e times themselves (or, without BOTH, the one that `low` says in hi);
+ * gives back 2^-e.  2^e times the column's largest
+ * element lies in [2^13, 2^14), e within what a float's exponent holds. */
+template <int N, bool BOTH>
+__device__ __forceinline__ float split_q(const float4 *x, bool on, f16x8 *hi, f16x8 *lo, bool low = false)
+{
+    float top = 0;
+#pragma unroll
+    for (int i = 0; i < N / 4; i++)
+        top = fmaxf(fmaxf(fmaxf(top, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
+    top = max_g(on ? top : 0.0f);
+    const int b = (__builtin_bit_cast(int, top) >> 23) & 255, e = b == 255 ? 0 : min(13 + 127 - b, 120);
+    const float up = __builtin_bit_cast(float, (127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float4 f = x[i / 4];
+        const float y = on ? (i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w) * up : 0.0f;
+        const _Float16 h = (_Float16)y, r = (_Float16)(y - (float)h);
+        hi[i / 8][i % 8] = !BOTH && low ? r : h;
+        if constexpr (BOTH) lo[i / 8][i % 8] = r;
+    }
+    return __builtin_bit_cast(float, (127 - e) << 23);
+}
 
 /* One wave's state of a unit: lane (c = lane % 16, g = lane / 16) holds column c. */
 template <int D, bool F16>
@@ -106,33 +133,12 @@ struct AttWave {
     __device__ void begin(const Raw &r, int c, int nh, float scale)
     {
         const bool on = (c & 7) < nh && (F16 || c < HPB);
-        float x[QE * C::KS], top = 0;
-#pragma unroll
-        for (int s = 0; s < QE * C::KS / 4; s++) {
-            x[4 * s] = on ? r.x[s].x : 0.0f; x[4 * s + 1] = on ? r.x[s].y : 0.0f;
-            x[4 * s + 2] = on ? r.x[s].z : 0.0f; x[4 * s + 3] = on ? r.x[s].w : 0.0f;
-        }
-        if (F16) {
-#pragma unroll
-            for (int i = 0; i < QE * C::KS; i++) top = fmaxf(top, fabsf(x[i]));
-            top = max_g(top);
-            /* 2^e times the row's largest element lies in [2^13, 2^14); e within what a float's exponent holds */
-            const int b = (__builtin_bit_cast(int, top) >> 23) & 255, e = b == 255 ? 0 : min(13 + 127 - b, 120);
-            const float up = __builtin_bit_cast(float, (127 + e) << 23);
-#pragma unroll
-            for (int s = 0; s < C::KS; s++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float y = x[8 * s + j] * up;
-                    const _Float16 hi = (_Float16)y;
-                    qh[s][j] = c < 8 ? hi : (_Float16)(y - (float)hi);
-                }
-            fac = scale * 1.44269504088896341f * __builtin_bit_cast(float, (127 - e) << 23);
+        fac = scale * 1.44269504088896341f;
+        if constexpr (F16) {
+            fac *= split_q<8 * C::KS, false>(r.x, on, qh, qh, c >= 8);
         } else {
 #pragma unroll
-            for (int s = 0; s < C::KS; s++)
-                for (int j = 0; j < 4; j++) qf[s][j] = x[4 * s + j];
-            fac = scale * 1.44269504088896341f;
+            for (int s = 0; s < C::KS; s++) qf[s] = on ? (f32x4){ r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w } : (f32x4){};
         }
     }
     /* Keys of the tile whose 16-token parts begin at at[] (bytes, uniform). */
@@ -182,11 +188,10 @@ struct AttWave {
         for (int j = 0; j < C::VT; j++) s[j] *= fac;
         if (left < C::TT)
             for (int j = 0; j < C::VT; j++)
-                if (16 * (j / 4) + 4 * g + (j & 3) >= left) s[j] = -INFINITY;
+                if (4 * g + j >= left) s[j] = -INFINITY;
         for (int j = 0; j < C::VT; j++) mx = fmaxf(mx, s[j]);
-        mx = max_g(mx);
         if (__any(mx > m + M_LATE)) {
-            const float mn = fmaxf(m, mx), w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float mn = fmaxf(m, max_g(mx)), w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             l *= w;
             for (int i = 0; i < C::NB * C::VE; i++) o[i] *= w;
             m = mn;
@@ -201,25 +206,29 @@ struct AttWave {
     {
         if (left < C::TT)                              /* what lies behind the row may be anything: 0 * NaN is NaN */
             for (int j = 0; j < C::VT; j++)
-                if (16 * (j / 4) + 4 * g + (j & 3) >= left)
+                if (4 * g + j >= left)
                     for (int n = 0; n < C::NB; n++) v[j][n] = (gu32x4){};
         if (F16) {
-            f16x8 b;
+            f16x4 b;
             const float low = c < 8 ? 0.0f : 1.0f;
-            for (int j = 0; j < 8; j += 2) {
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
                 typedef __fp16 h2 __attribute__((ext_vector_type(2)));
                 const h2 hi = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
                 const h2 r = __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)hi.x, low, p[j]), fmaf(-(float)hi.y, low, p[j + 1]));
                 b[j] = (_Float16)r.x;
                 b[j + 1] = (_Float16)r.y;
             }
+#pragma unroll
             for (int n = 0; n < C::NB; n++)
+#pragma unroll
                 for (int e = 0; e < C::VE; e++) {
-                    gu32x4 a;
-                    for (int j = 0; j < 4; j++)
+                    gu32x2 a;
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
                         a[j] = __builtin_amdgcn_perm(v[2 * j + 1][n][e / 2], v[2 * j][n][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-                    o[n * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b,
-                                                                              o[n * C::VE + e], 0, 0, 0);
+                    o[n * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), b,
+                                                                             o[n * C::VE + e], 0, 0, 0);
                 }
         } else {
             for (int n = 0; n < C::NB; n++)
@@ -392,7 +401,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *er
  * most ATT_G parts, since a unit of n tiles has ceil(n / S); a unit's parts are
  * equal.  Each wave finds its part from the rows by itself, without a barrier. */
 template <int D, bool F16>
-__global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_few_kernel(AttArgs A, int *err)
+__global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kernel(AttArgs A, int *err)
 {
     using C = AttCfg<D, F16>;
     __shared__ AttLds<D> S;
@@ -411,7 +420,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_few_
         if (lane + 64 * k < rows) tl[k] = att_tiles<C::TT>(T, req[k], pos[k], shift);
     /* the sum in f32, a little too large if anything */
     const float all = group_sum<64>((float)tl[0] + (float)tl[1]) * per_row;
-    const int size = max(ATT_MIN, (int)(all * (1.0001f / (ATT_G - rows * per_row))) + 1);
+    const int size = max(ATT_MIN, (int)(all * (1.0001f / ((int)gridDim.x - rows * per_row))) + 1);
     int ch[2], in[2];
     ch[0] = in[0] = (tl[0] + size - 1) / size;
     ch[1] = in[1] = (tl[1] + size - 1) / size;
@@ -434,7 +443,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_few_
 }
 
 template <int D, bool F16>
-__global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_kernel(AttArgs A, int *err)
+__global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(AttArgs A, int *err)
 {
     using C = AttCfg<D, F16>;
     __shared__ AttLds<D> S;
@@ -496,6 +505,360 @@ __global__ __launch_bounds__(ATT_T, D == 256 ? (F16 ? 2 : 1) : 2) void attn_kern
         }
         __syncthreads();                               /* S is free again */
     }
+}
+
+/* ---- several rows of a request together (fp16 cache) ------------------------
+ * A run is up to R rows of one request, one behind the other with positions that
+ * do not fall: a prompt's chunk.  The workgroup brings each tile of the run's
+ * keys and values into LDS once; a wave has two groups of 16 columns (row, head)
+ * and multiplies every operand it reads by both groups' high and low parts, so
+ * that the scores come out whole and no two lanes compute the same.  Shares,
+ * cuts and the join go as in attn_kernel, a unit being a run and a block of
+ * heads.  Four waves of up to 512 registers: queries (two parts) and sums of
+ * two groups take 256 of them at dim 256. */
+#define ROWS_G 256            /* workgroups: one per CU */
+#define ROWS_COLS 128         /* columns of a unit: 4 waves of 2 groups of 16 */
+
+struct RowsCut {
+    int row, n, hb, k;        /* first row, rows and head block of a unit, and its number of shares (0: not to be joined) */
+};
+
+struct RowsArgs {
+    RoasterAttnPaged a;
+    const char *kc, *vc;
+    KvShape s;
+    int group, blocks, hpb;   /* query heads of a key/value head, their blocks, heads of a block */
+    int rpg, R;               /* rows of a column group, of a run */
+    RowsCut *cut;             /* [ROWS_G] by the share that began a unit and did not finish it */
+    float *pm, *pl, *po;      /* parts [2 ROWS_G][ROWS_COLS] and [..][D], slots as in AttArgs */
+};
+
+/* Tokens of row t; where they are, the row goes on with the run of row t - 1. */
+struct RowsAt {
+    int req, n;
+    bool joined;
+};
+__device__ __forceinline__ RowsAt rows_at(const RowsArgs &A, const KvTable &T, int t)
+{
+    RowsAt x;
+    x.req = A.a.row_req[t];
+    x.n = x.req == -1 ? -1 : T.tokens(x.req, A.a.row_pos[t], A.s.shift);
+    x.joined = false;
+    if (t % A.R && x.n >= 0) {
+        const int r = A.a.row_req[t - 1];
+        if (r == x.req) {
+            const int n = T.tokens(r, A.a.row_pos[t - 1], A.s.shift);
+            x.joined = n >= 0 && n <= x.n;
+        }
+    }
+    return x;
+}
+/* Tiles of the run that ends with row t, 0 if none does. */
+__device__ __forceinline__ int rows_tiles(const RowsArgs &A, const KvTable &T, int t)
+{
+    const RowsAt x = rows_at(A, T, t);
+    if (x.req == -1 || (t + 1 < A.a.rows && rows_at(A, T, t + 1).joined)) return 0;
+    return x.n <= 32 ? 1 : (int)(((long long)x.n + 31) / 32);
+}
+
+template <int D>
+__global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *err)
+{
+    using C = AttCfg<D, true>;
+    constexpr int CH = D / 8, PT = CH / 8, NO = C::NB * C::VE;         /* 16-byte pieces of a token, of a thread; sums of a lane */
+    __shared__ gu32x4 s_k[2][32 * CH], s_v[2][32 * CH];
+    __shared__ long long s_wave[ATT_W], s_at;
+    __shared__ int s_row;
+    const RoasterAttnPaged &a = A.a;
+    const KvTable T = { a.n_req, a.max_pages };
+    const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
+    const int per_row = A.s.kv * A.blocks, rows = a.rows;
+
+    const int each = (rows + ATT_T - 1) / ATT_T;
+    long long mine = 0, tot;
+    for (int i = 0; i < each; i++) {
+        const int t = tid * each + i;
+        if (t < rows) mine += rows_tiles(A, T, t);
+    }
+    const long long upto = att_scan(mine, s_wave, tot);
+    const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
+    long long at = blockIdx.x * share;
+    const long long end = min(all, at + share);
+    if (at >= end) {
+        if (tid == 0) A.cut[blockIdx.x].k = 0;
+        return;
+    }
+    if (at < upto * per_row && at >= (upto - mine) * per_row) {
+        long long b = (upto - mine) * per_row;
+        int t = tid * each, n;
+        while (at >= b + (n = rows_tiles(A, T, t)) * (long long)per_row) {
+            b += n * (long long)per_row;
+            t++;
+        }
+        s_row = t;
+        s_at = b;
+    }
+    __syncthreads();
+    int t1 = uni(s_row), tiles = uni(rows_tiles(A, T, t1));
+    int hb = uni((int)((at - s_at) / tiles)), first = uni((int)((at - s_at) % tiles));
+    const int cr = c / A.hpb, ch = c - cr * A.hpb;                      /* this lane's column: its row and head within the group */
+    while (1) {
+        const int last = uni((int)min((long long)tiles, first + (end - at)));
+        const bool whole = first == 0 && last == tiles, cuts = first == 0 && !whole;
+        int t0 = t1;
+        while (t0 % A.R && uni(rows_at(A, T, t0).joined)) t0--;
+        const int nr = t1 - t0 + 1, req = uni(a.row_req[t1]), n = uni(T.tokens(req, a.row_pos[t1], shift));
+        const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(A.hpb, A.group - bk * A.hpb);
+        const int h0 = kh * A.group + bk * A.hpb;
+        bool bad = n < 0;
+
+        /* the tile's bytes, 16-token part by part, as in att_part */
+        auto where = [&](int i, size_t *b) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int tok = i * 32 + 16 * u;
+                if (u && tok >= n) { b[1] = b[0]; continue; }
+                int pg = uni(a.table[T.entry(req, tok, shift)]);
+                if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
+                b[u] = A.s.at(pg, kh, tok & ((1 << shift) - 1)) * 2;
+            }
+        };
+        gu32x4 sk[PT], sv[PT];
+        auto fetch = [&](const size_t *b) {
+#pragma unroll
+            for (int i = 0; i < PT; i++) {
+                const int x = tid + ATT_T * i, row = x / CH;
+                const size_t off = (row < 16 ? b[0] : b[1]) + (size_t)((row & 15) * CH + x % CH) * 16;
+                sk[i] = *(const GAS gu32x4 *)(A.kc + off);
+                sv[i] = *(const GAS gu32x4 *)(A.vc + off);
+            }
+        };
+        /* piece x of a token's row lies at x ^ (row & 7): the 16 rows that an operand read takes fall on different banks */
+        auto put = [&](int buf) {
+#pragma unroll
+            for (int i = 0; i < PT; i++) {
+                const int x = tid + ATT_T * i, row = x / CH, at = row * CH + ((x % CH) ^ (row & 7));
+                s_k[buf][at] = sk[i];
+                s_v[buf][at] = sv[i];
+            }
+        };
+        size_t b[2];
+        if (n > 0) {
+            where(first, b);
+            fetch(b);
+        }
+        f16x8 qh[2][C::KS], ql[2][C::KS];
+        f32x4 o[2][NO];
+        float m[2], l[2], fac[2];
+        int nc[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int i = (2 * w + j) * A.rpg + cr;
+            const bool on = cr < A.rpg && i < nr && ch < nh;
+            const float *q = a.q + ((size_t)(t0 + (on ? i : 0)) * a.q_heads + h0 + (on ? ch : 0)) * D + 8 * g;
+            float4 x[2 * C::KS];
+#pragma unroll
+            for (int s = 0; s < 2 * C::KS; s++) x[s] = *(const float4 *)(q + 32 * (s / 2) + 4 * (s % 2));
+            nc[j] = on ? T.tokens(req, a.row_pos[t0 + i], shift) : 0;
+            fac[j] = split_q<8 * C::KS, true>(x, on, qh[j], ql[j]) * (a.scale * 1.44269504088896341f);
+            m[j] = -INFINITY;
+            l[j] = 0;
+#pragma unroll
+            for (int k = 0; k < NO; k++) o[j][k] = (f32x4){};
+        }
+        if (n > 0) {
+            int most = max(nc[0], nc[1]), least = INT32_MAX;            /* over the wave's columns in use */
+#pragma unroll
+            for (int j = 0; j < 2; j++) least = min(least, nc[j] > 0 ? nc[j] : INT32_MAX);
+            for (int x = 32; x; x >>= 1) {
+                most = max(most, __shfl_xor(most, x));
+                least = min(least, __shfl_xor(least, x));
+            }
+            most = uni(most);
+            least = uni(least);
+            put(0);
+            __syncthreads();
+            /* this wave's own rows may end before the run does: then it only brings tiles */
+            const int mine = min(last, (int)(((long long)most + 31) / 32));
+            int i = first;
+            for (; i < mine; i++) {
+                const int buf = (i - first) & 1;
+                if (i + 1 < last) {
+                    where(i + 1, b);
+                    fetch(b);
+                }
+                {
+                    f32x4 acc[2][2] = {};
+#pragma unroll
+                    for (int s = 0; s < C::KS; s++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const int row = 16 * u + c;
+                            const f16x8 kf = __builtin_bit_cast(f16x8, s_k[buf][row * CH + ((4 * s + g) ^ (row & 7))]);
+#pragma unroll
+                            for (int j = 0; j < 2; j++) acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[j][s], acc[j][u], 0, 0, 0);
+#pragma unroll
+                            for (int j = 0; j < 2; j++) acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[j][s], acc[j][u], 0, 0, 0);
+                        }
+                    f16x8 ph[2], pl[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        float p[8], mx = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) p[k] = acc[j][k / 4][k & 3] * fac[j];
+                        if ((i + 1) * 32 > least) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if (i * 32 + 16 * (k / 4) + 4 * g + (k & 3) >= nc[j]) p[k] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; k++) mx = fmaxf(mx, p[k]);
+                        if (__any(mx > m[j] + M_LATE)) {
+                            const float mn = fmaxf(m[j], max_g(mx)), f = m[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[j] - mn);
+                            l[j] *= f;
+#pragma unroll
+                            for (int k = 0; k < NO; k++) o[j][k] *= f;
+                            m[j] = mn;
+                        }
+                        /* a column that has met no position yet keeps its terms 0 */
+                        const float base = m[j] == -INFINITY ? 0.0f : m[j] - P_UP;
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2) {
+                            typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+                            const float x = __builtin_amdgcn_exp2f(p[k] - base), y = __builtin_amdgcn_exp2f(p[k + 1] - base);
+                            l[j] += x;
+                            l[j] += y;
+                            const h2 hi = __builtin_amdgcn_cvt_pkrtz(x, y), lo = __builtin_amdgcn_cvt_pkrtz(x - (float)hi.x, y - (float)hi.y);
+                            ph[j][k] = (_Float16)hi.x; ph[j][k + 1] = (_Float16)hi.y;
+                            pl[j][k] = (_Float16)lo.x; pl[j][k + 1] = (_Float16)lo.y;
+                        }
+                    }
+                    const int left = n - i * 32;
+#pragma unroll
+                    for (int nb = 0; nb < C::NB; nb++) {
+                        gu32x4 v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int row = 4 * g + (k & 3) + 16 * (k / 4);
+                            if constexpr (C::VE == 8) v[k] = s_v[buf][row * CH + ((16 * nb + c) ^ (row & 7))];
+                            else {
+                                const gu32x2 h = ((const gu32x2 *)&s_v[buf][row * CH + ((c >> 1) ^ (row & 7))])[c & 1];
+                                v[k] = (gu32x4){ h.x, h.y, 0, 0 };
+                            }
+                            if (left < 32 && row >= left) v[k] = (gu32x4){};     /* behind the run: may be anything */
+                        }
+#pragma unroll
+                        for (int e = 0; e < C::VE; e++) {
+                            gu32x4 x;
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                x[k] = __builtin_amdgcn_perm(v[2 * k + 1][e / 2], v[2 * k][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+                            const f16x8 vf = __builtin_bit_cast(f16x8, x);
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+                                o[j][nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[j], o[j][nb * C::VE + e], 0, 0, 0);
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+                                o[j][nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[j], o[j][nb * C::VE + e], 0, 0, 0);
+                        }
+                    }
+                }
+                if (i + 1 < last) put(buf ^ 1);
+                __syncthreads();
+            }
+            for (; i < last; i++) {
+                if (i + 1 < last) {
+                    where(i + 1, b);
+                    fetch(b);
+                    put((i - first + 1) & 1);
+                }
+                __syncthreads();
+            }
+        }
+        if (bad && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
+        const int slot = 2 * blockIdx.x + (first == 0);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int i = (2 * w + j) * A.rpg + cr;
+            if (!(cr < A.rpg && i < nr && ch < nh)) continue;
+            float sum = sum_g(l[j]);
+            if (bad) sum = NAN;
+            const int col = i * A.hpb + ch;
+            if (!whole && g == 0) {
+                A.pm[slot * ROWS_COLS + col] = m[j];
+                A.pl[slot * ROWS_COLS + col] = sum;
+            }
+#pragma unroll
+            for (int nb = 0; nb < C::NB; nb++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int e = 0; e < C::VE; e += 4) {
+                        f32x4 y;
+#pragma unroll
+                        for (int z = 0; z < 4; z++) y[z] = o[j][nb * C::VE + e + z][k];
+                        const int d = 16 * C::VE * nb + C::VE * (4 * g + k) + e;
+                        if (whole) att_store(a, D, t0 + i, h0 + ch, d, y, nc[j] == 0 ? 1.0f : sum);
+                        else *(f32x4 *)(A.po + ((size_t)slot * ROWS_COLS + col) * D + d) = y;
+                    }
+        }
+        at += last - first;
+        if (tid == 0 && at == end) {
+            const RowsCut x = { t0, nr, hb, cuts ? (int)((at - last + tiles - 1) / share) - (int)blockIdx.x + 1 : 0 };
+            A.cut[blockIdx.x] = x;
+        }
+        if (at >= end) break;
+        first = 0;
+        if (++hb == per_row) {
+            hb = 0;
+            do {
+                t1++;
+                tiles = uni(rows_tiles(A, T, t1));
+            } while (tiles == 0);
+        }
+    }
+}
+
+/* The parts of a cut run's columns, D/4 lanes to a column. */
+template <int D>
+__global__ __launch_bounds__(ATT_T) void attn_rows_join_kernel(RowsArgs A)
+{
+    constexpr int L = D / 4;
+    const RowsCut x = A.cut[blockIdx.x];
+    const int col = blockIdx.y * (ATT_T / L) + threadIdx.x / L, d = threadIdx.x % L * 4, g0 = blockIdx.x;
+    const int i = col / A.hpb, ch = col - i * A.hpb;
+    const int kh = x.hb / A.blocks, bk = x.hb - kh * A.blocks;
+    if (x.k == 0 || i >= x.n || ch >= A.group - bk * A.hpb) return;
+    float m = -INFINITY, l = 0;
+    f32x4 y = {};
+    for (int k0 = 0; k0 < x.k; k0 += 4) {
+        float pm[4], pl[4];
+        f32x4 po[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int k = min(k0 + j, x.k - 1);
+            const size_t at = (size_t)(k ? 2 * (g0 + k) : 2 * g0 + 1) * ROWS_COLS + col;
+            pm[j] = k0 + j < x.k ? A.pm[at] : -INFINITY;
+            pl[j] = A.pl[at];
+            po[j] = *(const f32x4 *)(A.po + at * D + d);
+        }
+        float mn = m;
+#pragma unroll
+        for (int j = 0; j < 4; j++) mn = fmaxf(mn, pm[j]);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        y *= f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (k0 + j >= x.k) continue;
+            const float w = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
+            l += pl[j] * w;
+            y += po[j] * w;
+        }
+        m = mn;
+    }
+    const int t = x.row + i;
+    att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, d, y, A.a.row_pos[t] == -1 ? 1.0f : l);
 }
 
 #define JOIN_T 512
@@ -565,19 +928,34 @@ __global__ __launch_bounds__(JOIN_T) void attn_join_kernel(AttArgs A)
 /* Workspace: the cut table, then m and l of the parts, then the parts. */
 static const size_t ATT_CUT = (size_t)ATT_G * sizeof(int2), ATT_ML = (size_t)2 * ATT_G * HPB * 4;
 
+/* The same of attn_rows_kernel. */
+static const size_t ROWS_CUT = (size_t)ROWS_G * sizeof(RowsCut), ROWS_ML = (size_t)2 * ROWS_G * ROWS_COLS * 4;
+
+/* Calls that may go by runs of rows: with fewer rows there is little to share. */
+static bool rows_may(int rows, int type) { return type == ROASTER_KV_F16 && rows >= 16; }
+
 extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCache *c)
 {
     if (!attn_cache_ok(c) || rows < 0 || rows > (1 << 20) || q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads) return 0;
-    return ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * HPB * c->head_dim * 4;
+    const size_t one = ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * HPB * c->head_dim * 4,
+                 run = ROWS_CUT + 2 * ROWS_ML + (size_t)2 * ROWS_G * ROWS_COLS * c->head_dim * 4;
+    return rows_may(rows, c->type) && run > one ? run : one;
+}
+
+template <int D>
+static void rows_launch(const RowsArgs &A, int *err)
+{
+    hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ATT_T), 0, rt().stream, A, err);
+    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_G, ROWS_COLS * D / 4 / ATT_T), dim3(ATT_T), 0, rt().stream, A);
 }
 
 template <int D, bool F16>
 static void att_launch(const AttArgs &A, int *err)
 {
     const long long units = (long long)A.a.rows * A.s.kv * A.blocks;
-    if (A.few) hipLaunchKernelGGL((attn_few_kernel<D, F16>), dim3(ATT_G), dim3(ATT_T), 0, rt().stream, A, err);
-    else hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(ATT_G), dim3(ATT_T), 0, rt().stream, A, err);
-    hipLaunchKernelGGL((attn_join_kernel<D>), dim3(units < ATT_G ? (int)units : ATT_G, A.group < HPB ? A.group : HPB),
+    if (A.few) hipLaunchKernelGGL((attn_few_kernel<D, F16>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
+    else hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
+    hipLaunchKernelGGL((attn_join_kernel<D>), dim3(A.by_unit ? (int)units : A.grid, A.group < HPB ? A.group : HPB),
                        dim3(JOIN_T), 0, rt().stream, A);
 }
 
@@ -611,6 +989,28 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     const AttnDevice dev;
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
+    /* Runs of rows pay where requests have several rows each, which the two counts
+     * tell on average (a call of other rows is right as well, only slower). */
+    if (rows_may(p->rows, c->type) && p->rows >= 4 * (long long)p->n_req) {
+        RowsArgs A;
+        A.a = *p;
+        A.kc = (const char *)c->k;
+        A.vc = (const char *)c->v;
+        A.s = attn_shape(c);
+        A.group = p->q_heads / c->kv_heads;
+        A.hpb = A.group < 16 ? A.group : 16;
+        A.blocks = (A.group + A.hpb - 1) / A.hpb;
+        A.rpg = 16 / A.hpb;
+        A.R = 2 * ATT_W * A.rpg;
+        A.cut = (RowsCut *)p->ws;
+        A.pm = (float *)((char *)p->ws + ROWS_CUT);
+        A.pl = (float *)((char *)p->ws + ROWS_CUT + ROWS_ML);
+        A.po = (float *)((char *)p->ws + ROWS_CUT + 2 * ROWS_ML);
+        if (D == 256) rows_launch<256>(A, err);
+        else if (D == 128) rows_launch<128>(A, err);
+        else rows_launch<64>(A, err);
+        return rt_check(hipGetLastError(), "attention launch") ? ROASTER_EDEVICE : 0;
+    }
     AttArgs A;
     A.a = *p;
     A.kc = (const char *)c->k;
@@ -619,8 +1019,9 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     A.group = p->q_heads / c->kv_heads;
     A.blocks = (A.group + HPB - 1) / HPB;
     const long long units = (long long)p->rows * c->kv_heads * A.blocks;
-    A.by_unit = units <= ATT_G;
-    A.few = units <= ATT_G / 4 && p->rows <= 128;
+    A.grid = D == 256 && c->type == ROASTER_KV_F32 ? ATT_G / 2 : ATT_G;
+    A.by_unit = units <= A.grid;
+    A.few = units <= A.grid / 8 && p->rows <= 128;
     A.cut = (int2 *)p->ws;
     A.pm = (float *)((char *)p->ws + ATT_CUT);
     A.pl = (float *)((char *)p->ws + ATT_CUT + ATT_ML);
