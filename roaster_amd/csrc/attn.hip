@@ -36,6 +36,8 @@
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttArgs {
@@ -73,27 +75,43 @@ __device__ __forceinline__ float sum_g(float v)
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-/* N elements of a query column (a lane's quarter of them, or zeros) as hi + lo fp16
- * parts of 2^e times themselves (or, without BOTH, the one that `low` says in hi);
- * gives back 2^-e.  2^e times the column's largest
- * element lies in [2^13, 2^14), e within what a float's exponent holds. */
+__device__ __forceinline__ f16x2 to_half(float x, float y) { return __builtin_convertvector((f32x2){ x, y }, f16x2); }
+/* What `to_half` left of x and y, times f (0 or 1). */
+__device__ __forceinline__ f16x2 rest_half(f16x2 h, float f, float x, float y)
+{
+    return to_half(fmaf(-(float)h.x, f, x), fmaf(-(float)h.y, f, y));
+}
+__device__ __forceinline__ f16x8 join8(const f16x2 *h)
+{
+    return (f16x8){ h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y };
+}
+
+/* N elements of a query column (a lane's quarter of them) as hi + lo fp16 parts of
+ * 2^e times themselves (without BOTH only the one that `low`, 0 or 1, says, in
+ * hi); gives back 2^-e.  2^e times the column's largest element lies in [2^13,
+ * 2^14), e within what a float's exponent holds. */
 template <int N, bool BOTH>
-__device__ __forceinline__ float split_q(const float4 *x, bool on, f16x8 *hi, f16x8 *lo, bool low = false)
+__device__ __forceinline__ float split_q(const float4 *x, f16x8 *hi, f16x8 *lo, float low)
 {
     float top = 0;
 #pragma unroll
     for (int i = 0; i < N / 4; i++)
         top = fmaxf(fmaxf(fmaxf(top, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
-    top = max_g(on ? top : 0.0f);
+    top = max_g(top);
     const int b = (__builtin_bit_cast(int, top) >> 23) & 255, e = b == 255 ? 0 : min(13 + 127 - b, 120);
     const float up = __builtin_bit_cast(float, (127 + e) << 23);
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float4 f = x[i / 4];
-        const float y = on ? (i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w) * up : 0.0f;
-        const _Float16 h = (_Float16)y, r = (_Float16)(y - (float)h);
-        hi[i / 8][i % 8] = !BOTH && low ? r : h;
-        if constexpr (BOTH) lo[i / 8][i % 8] = r;
+    for (int i = 0; i < N / 8; i++) {
+        f16x2 h[4], r[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float4 f = x[2 * i + j / 2];
+            const float a = (j & 1 ? f.z : f.x) * up, c = (j & 1 ? f.w : f.y) * up;
+            h[j] = to_half(a, c);
+            r[j] = rest_half(h[j], BOTH ? 1.0f : low, a, c);
+        }
+        hi[i] = join8(BOTH ? h : r);
+        if constexpr (BOTH) lo[i] = join8(r);
     }
     return __builtin_bit_cast(float, (127 - e) << 23);
 }
@@ -110,7 +128,8 @@ struct AttWave {
     gu32x4 k[C::SUB][C::KS];
     gu32x4 v[C::VT][C::NB];
 
-    /* The unit's queries as they lie: column c's head, zeros where there is none. */
+    /* The unit's queries as they lie: column c's head (a column without one computes
+     * the first head's and is never stored). */
     static constexpr int QE = F16 ? 8 : 4;          /* elements of a product operand */
     struct Raw {
         float4 x[QE * C::KS / 4];
@@ -130,15 +149,13 @@ struct AttWave {
 #pragma unroll
         for (int i = 0; i < C::NB * C::VE; i++) o[i] = (f32x4){};
     }
-    __device__ void begin(const Raw &r, int c, int nh, float scale)
+    __device__ void begin(const Raw &r, int c, float scale)
     {
-        const bool on = (c & 7) < nh && (F16 || c < HPB);
         fac = scale * 1.44269504088896341f;
-        if constexpr (F16) {
-            fac *= split_q<8 * C::KS, false>(r.x, on, qh, qh, c >= 8);
-        } else {
+        if constexpr (F16) fac *= split_q<8 * C::KS, false>(r.x, qh, qh, c < 8 ? 0.0f : 1.0f);
+        else {
 #pragma unroll
-            for (int s = 0; s < C::KS; s++) qf[s] = on ? (f32x4){ r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w } : (f32x4){};
+            for (int s = 0; s < C::KS; s++) qf[s] = (f32x4){ r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w };
         }
     }
     /* Keys of the tile whose 16-token parts begin at at[] (bytes, uniform). */
@@ -147,7 +164,7 @@ struct AttWave {
         for (int u = 0; u < C::SUB; u++) {
             const char *b = kc + at[u];
             const unsigned off = c * D * C::SZ + g * 16;
-            for (int s = 0; s < C::KS; s++) k[u][s] = *(const GAS gu32x4 *)(b + off + 64 * s);
+            for (int s = 0; s < C::KS; s++) k[u][s] = __builtin_nontemporal_load((const GAS gu32x4 *)(b + off + 64 * s));
         }
     }
     __device__ void load_v(const char *vc, const size_t *at, int c, int g)
@@ -157,9 +174,9 @@ struct AttWave {
             const unsigned off = ((4 * g + (j & 3)) * D + C::VE * c) * C::SZ;
             for (int n = 0; n < C::NB; n++) {
                 const GAS char *p = (const GAS char *)(b + off + 16 * C::VE * C::SZ * n);
-                if (C::VE * C::SZ == 16) v[j][n] = *(const GAS gu32x4 *)p;
+                if (C::VE * C::SZ == 16) v[j][n] = __builtin_nontemporal_load((const GAS gu32x4 *)p);
                 else {
-                    const gu32x2 h = *(const GAS gu32x2 *)p;
+                    const gu32x2 h = __builtin_nontemporal_load((const GAS gu32x2 *)p);
                     v[j][n] = (gu32x4){ h.x, h.y, 0, 0 };
                 }
             }
@@ -209,16 +226,9 @@ struct AttWave {
                 if (4 * g + j >= left)
                     for (int n = 0; n < C::NB; n++) v[j][n] = (gu32x4){};
         if (F16) {
-            f16x4 b;
             const float low = c < 8 ? 0.0f : 1.0f;
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                typedef __fp16 h2 __attribute__((ext_vector_type(2)));
-                const h2 hi = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
-                const h2 r = __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)hi.x, low, p[j]), fmaf(-(float)hi.y, low, p[j + 1]));
-                b[j] = (_Float16)r.x;
-                b[j + 1] = (_Float16)r.y;
-            }
+            const f16x2 b0 = rest_half(to_half(p[0], p[1]), low, p[0], p[1]), b1 = rest_half(to_half(p[2], p[3]), low, p[2], p[3]);
+            const f16x4 b = { b0.x, b0.y, b1.x, b1.y };
 #pragma unroll
             for (int n = 0; n < C::NB; n++)
 #pragma unroll
@@ -236,6 +246,28 @@ struct AttWave {
                     for (int j = 0; j < 4; j++)
                         o[n * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, v[j][n])[e], p[j],
                                                                             o[n * 4 + e], 0, 0, 0);
+        }
+    }
+    /* The high parts' columns get the low parts' sums.  Where an infinite value made a
+     * high sum infinite it stands for itself: the low one is NaN, or infinite the
+     * other way. */
+    __device__ void add_parts()
+    {
+        float top = 0;
+#pragma unroll
+        for (int i = 0; i < C::NB * C::VE; i++)
+            top = fmaxf(fmaxf(fmaxf(top, fabsf(o[i][0])), fmaxf(fabsf(o[i][1]), fabsf(o[i][2]))), fabsf(o[i][3]));
+        if (__any(top == INFINITY)) {
+#pragma unroll
+            for (int i = 0; i < C::NB * C::VE; i++)
+                for (int j = 0; j < 4; j++) {
+                    const float lo = dpp_f<0x128>(o[i][j]);
+                    o[i][j] = fabsf(o[i][j]) == INFINITY ? o[i][j] : o[i][j] + lo;
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < C::NB * C::VE; i++)
+                for (int j = 0; j < 4; j++) o[i][j] += dpp_f<0x128>(o[i][j]);
         }
     }
 };
@@ -274,13 +306,16 @@ struct AttLds {
     float o[ATT_W][HPB][D + 4], m[ATT_W][HPB], l[ATT_W][HPB];
 };
 
-/* out of one row's head from the sums y and l, four elements at d. */
+/* out of one row's head from the sums y and l, four elements at d.  The reciprocals
+ * are off by one step, the exponential by |gate| 2^-24 more: as little as the
+ * sums themselves. */
 __device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int t, int h, int d, f32x4 y, float l)
 {
-    y *= 1.0f / l;
+    y *= __builtin_amdgcn_rcpf(l);
     if (a.gate) {
-        const float4 gt = *(const float4 *)(a.gate + t * a.gate_row + h * a.gate_head + d);
-        y[0] /= 1.0f + expf(-gt.x); y[1] /= 1.0f + expf(-gt.y); y[2] /= 1.0f + expf(-gt.z); y[3] /= 1.0f + expf(-gt.w);
+        const f32x4 gt = *(const f32x4 *)(a.gate + t * a.gate_row + h * a.gate_head + d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gt[i] * -1.44269504088896341f));
     }
     *(f32x4 *)(a.out + ((size_t)t * a.q_heads + h) * D + d) = y;
 }
@@ -329,7 +364,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *er
         wv.load_k(A.kc, b, c, g);
         if (i2 < last) pages(i2, p);
         wv.load_v(A.vc, b, c, g);
-        wv.begin(raw, c, nh, a.scale);
+        wv.begin(raw, c, a.scale);
         while (1) {
             const int left = n - i * C::TT;
             const bool more = i2 < last;
@@ -348,28 +383,19 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *er
             i2 += ATT_W;
         }
     }
-    /* the waves' parts into LDS; an infinite or NaN high part (an infinite value) stands for itself */
     const float l = sum_g(wv.l);
     if (g == 0 && c < HPB) { S.m[w][c] = wv.m; S.l[w][c] = l; }
+    if constexpr (F16) wv.add_parts();
 #pragma unroll
     for (int b = 0; b < C::NB; b++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float y[C::VE];
-#pragma unroll
-            for (int e = 0; e < C::VE; e++) {
-                const float hi = wv.o[b * C::VE + e][i];
-                y[e] = hi;
-                if (F16) {
-                    const float lo = dpp_f<0x128>(hi);
-                    y[e] = fabsf(hi) < INFINITY ? hi + lo : hi;
-                }
-            }
+        for (int i = 0; i < 4; i++)
             if (c < HPB)
 #pragma unroll
                 for (int e = 0; e < C::VE; e += 4)
-                    *(float4 *)&S.o[w][c][16 * C::VE * b + C::VE * (4 * g + i) + e] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-        }
+                    *(float4 *)&S.o[w][c][16 * C::VE * b + C::VE * (4 * g + i) + e] =
+                        make_float4(wv.o[b * C::VE + e][i], wv.o[b * C::VE + e + 1][i], wv.o[b * C::VE + e + 2][i],
+                                    wv.o[b * C::VE + e + 3][i]);
     const bool any = __syncthreads_or(bad);
     if (any && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
     for (int idx = tid * 4; idx < nh * D; idx += ATT_T * 4) {
@@ -660,7 +686,7 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
 #pragma unroll
             for (int s = 0; s < 2 * C::KS; s++) x[s] = *(const float4 *)(q + 32 * (s / 2) + 4 * (s % 2));
             nc[j] = on ? T.tokens(req, a.row_pos[t0 + i], shift) : 0;
-            fac[j] = split_q<8 * C::KS, true>(x, on, qh[j], ql[j]) * (a.scale * 1.44269504088896341f);
+            fac[j] = split_q<8 * C::KS, true>(x, qh[j], ql[j], 1.0f) * (a.scale * 1.44269504088896341f);
             m[j] = -INFINITY;
             l[j] = 0;
 #pragma unroll
@@ -723,15 +749,18 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
                         /* a column that has met no position yet keeps its terms 0 */
                         const float base = m[j] == -INFINITY ? 0.0f : m[j] - P_UP;
 #pragma unroll
-                        for (int k = 0; k < 8; k += 2) {
-                            typedef __fp16 h2 __attribute__((ext_vector_type(2)));
-                            const float x = __builtin_amdgcn_exp2f(p[k] - base), y = __builtin_amdgcn_exp2f(p[k + 1] - base);
-                            l[j] += x;
-                            l[j] += y;
-                            const h2 hi = __builtin_amdgcn_cvt_pkrtz(x, y), lo = __builtin_amdgcn_cvt_pkrtz(x - (float)hi.x, y - (float)hi.y);
-                            ph[j][k] = (_Float16)hi.x; ph[j][k + 1] = (_Float16)hi.y;
-                            pl[j][k] = (_Float16)lo.x; pl[j][k + 1] = (_Float16)lo.y;
+                        for (int k = 0; k < 8; k++) {
+                            p[k] = __builtin_amdgcn_exp2f(p[k] - base);
+                            l[j] += p[k];
                         }
+                        f16x2 hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            hi[k] = to_half(p[2 * k], p[2 * k + 1]);
+                            lo[k] = rest_half(hi[k], 1.0f, p[2 * k], p[2 * k + 1]);
+                        }
+                        ph[j] = join8(hi);
+                        pl[j] = join8(lo);
                     }
                     const int left = n - i * 32;
 #pragma unroll
@@ -861,14 +890,13 @@ __global__ __launch_bounds__(ATT_T) void attn_rows_join_kernel(RowsArgs A)
     att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, d, y, A.a.row_pos[t] == -1 ? 1.0f : l);
 }
 
-#define JOIN_T 512
-
-/* The parts of one cut unit's head, D/4 lanes to a part: each group of lanes
- * joins its parts as a running softmax does, the groups join in LDS. */
-template <int D>
-__global__ __launch_bounds__(JOIN_T) void attn_join_kernel(AttArgs A)
+/* The parts of one cut unit's head, L lanes with four elements each to a part:
+ * each group of lanes joins its parts as a running softmax does, the groups
+ * join in LDS. */
+template <int D, int L, int JT>
+__global__ __launch_bounds__(JT) void attn_join_kernel(AttArgs A)
 {
-    constexpr int L = D / 4, N = JOIN_T / L;
+    constexpr int N = JT / L;
     __shared__ float s_m[N], s_l[N];
     __shared__ f32x4 s_o[N][L];
     const RoasterAttnPaged &a = A.a;
@@ -881,7 +909,7 @@ __global__ __launch_bounds__(JOIN_T) void attn_join_kernel(AttArgs A)
     if (!A.by_unit) unit = e.x;
     const int t = unit / per_row, hb = unit % per_row, kh = hb / A.blocks, bk = hb % A.blocks;
     if (h >= A.group - bk * HPB) return;
-    const int sub = tid / L, d = tid % L * 4;
+    const int sub = tid / L, d = blockIdx.z * 4 * L + tid % L * 4;
     float m = -INFINITY, l = 0;
     f32x4 y = {};
     for (int k0 = sub; k0 < n; k0 += 4 * N) {
@@ -910,19 +938,20 @@ __global__ __launch_bounds__(JOIN_T) void attn_join_kernel(AttArgs A)
         }
         m = mn;
     }
-    if (d == 0) { s_m[sub] = m; s_l[sub] = l; }
+    if (tid % L == 0) { s_m[sub] = m; s_l[sub] = l; }
     s_o[sub][tid % L] = y;
     __syncthreads();
     if (tid >= L) return;
     float mx = -INFINITY, sum = 0;
     y = (f32x4){};
     for (int i = 0; i < N; i++) mx = fmaxf(mx, s_m[i]);
+#pragma unroll 8
     for (int i = 0; i < N; i++) {
         const float w = s_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - mx);
         sum += s_l[i] * w;
         y += s_o[i][tid] * w;
     }
-    att_store(a, D, t, kh * A.group + bk * HPB + h, 4 * tid, y, sum);
+    att_store(a, D, t, kh * A.group + bk * HPB + h, d, y, sum);
 }
 
 /* Workspace: the cut table, then m and l of the parts, then the parts. */
@@ -955,8 +984,11 @@ static void att_launch(const AttArgs &A, int *err)
     const long long units = (long long)A.a.rows * A.s.kv * A.blocks;
     if (A.few) hipLaunchKernelGGL((attn_few_kernel<D, F16>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
     else hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
-    hipLaunchKernelGGL((attn_join_kernel<D>), dim3(A.by_unit ? (int)units : A.grid, A.group < HPB ? A.group : HPB),
-                       dim3(JOIN_T), 0, rt().stream, A);
+    const int heads = A.group < HPB ? A.group : HPB;
+    /* few units have many parts each: 64 elements of a head to a workgroup, 32 parts at a time */
+    if (A.few) hipLaunchKernelGGL((attn_join_kernel<D, 16, 512>), dim3((int)units, heads, D / 64), dim3(512), 0, rt().stream, A);
+    else hipLaunchKernelGGL((attn_join_kernel<D, D / 4, 128>), dim3(A.by_unit ? (int)units : A.grid, heads), dim3(128), 0,
+                            rt().stream, A);
 }
 
 extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCache *c)
