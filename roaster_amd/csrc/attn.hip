@@ -273,6 +273,7 @@ struct AttWave {
 };
 
 /* Inclusive sums over the workgroup of 64-bit values; `tot` gets the whole. */
+template <int W>
 __device__ __forceinline__ long long att_scan(long long v, long long *s_wave, long long &tot)
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -284,7 +285,7 @@ __device__ __forceinline__ long long att_scan(long long v, long long *s_wave, lo
     if (lane == 63) s_wave[w] = v;
     __syncthreads();
     long long before = 0, all = 0;
-    for (int i = 0; i < ATT_W; i++) {
+    for (int i = 0; i < W; i++) {
         if (i == w) before = all;
         all += s_wave[i];
     }
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
         const int t = tid * each + i;
         if (t < rows) mine += att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift);
     }
-    const long long upto = att_scan(mine, s_wave, tot);
+    const long long upto = att_scan<ATT_W>(mine, s_wave, tot);
     const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
     long long at = blockIdx.x * share;
     const long long end = min(all, at + share);
@@ -543,7 +544,9 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
  * heads.  Four waves of up to 512 registers: queries (two parts) and sums of
  * two groups take 256 of them at dim 256. */
 #define ROWS_G 256            /* workgroups: one per CU */
-#define ROWS_COLS 128         /* columns of a unit: 4 waves of 2 groups of 16 */
+#define ROWS_T 512
+#define ROWS_W (ROWS_T / 64)
+#define ROWS_COLS 128         /* columns of a unit: 16 a wave */
 
 struct RowsCut {
     int row, n, hb, k;        /* first row, rows and head block of a unit, and its number of shares (0: not to be joined) */
@@ -588,25 +591,25 @@ __device__ __forceinline__ int rows_tiles(const RowsArgs &A, const KvTable &T, i
 }
 
 template <int D>
-__global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *err)
+__global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *err)
 {
     using C = AttCfg<D, true>;
-    constexpr int CH = D / 8, PT = CH / 8, NO = C::NB * C::VE;         /* 16-byte pieces of a token, of a thread; sums of a lane */
+    constexpr int CH = D / 8, PT = (32 * CH + ROWS_T - 1) / ROWS_T, NO = C::NB * C::VE;         /* 16-byte pieces of a token, of a thread; sums of a lane */
     __shared__ gu32x4 s_k[2][32 * CH], s_v[2][32 * CH];
-    __shared__ long long s_wave[ATT_W], s_at;
+    __shared__ long long s_wave[ROWS_W], s_at;
     __shared__ int s_row;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
     const int per_row = A.s.kv * A.blocks, rows = a.rows;
 
-    const int each = (rows + ATT_T - 1) / ATT_T;
+    const int each = (rows + ROWS_T - 1) / ROWS_T;
     long long mine = 0, tot;
     for (int i = 0; i < each; i++) {
         const int t = tid * each + i;
         if (t < rows) mine += rows_tiles(A, T, t);
     }
-    const long long upto = att_scan(mine, s_wave, tot);
+    const long long upto = att_scan<ROWS_W>(mine, s_wave, tot);
     const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
     long long at = blockIdx.x * share;
     const long long end = min(all, at + share);
@@ -631,29 +634,40 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
     while (1) {
         const int last = uni((int)min((long long)tiles, first + (end - at)));
         const bool whole = first == 0 && last == tiles, cuts = first == 0 && !whole;
+        /* the run's first row: as many rows back as go on with the one before them, 64 at a time */
         int t0 = t1;
-        while (t0 % A.R && uni(rows_at(A, T, t0).joined)) t0--;
+        for (bool on = true; on;) {
+            const int t = t0 - lane;
+            const unsigned long long j = __ballot(t > 0 && rows_at(A, T, t).joined);
+            on = j == ~0ull;
+            t0 -= on ? 64 : __builtin_ctzll(~j);
+        }
         const int nr = t1 - t0 + 1, req = uni(a.row_req[t1]), n = uni(T.tokens(req, a.row_pos[t1], shift));
         const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(A.hpb, A.group - bk * A.hpb);
         const int h0 = kh * A.group + bk * A.hpb;
         bool bad = n < 0;
 
-        /* the tile's bytes, 16-token part by part, as in att_part */
-        auto where = [&](int i, size_t *b) {
+        /* page numbers of tile i's two 16-token parts (a part past the run's end repeats
+         * the first), then the bytes at which the parts begin */
+        auto pages = [&](int i, int *p) {
+            p[0] = a.table[T.entry(req, i * 32, shift)];
+            p[1] = i * 32 + 16 < n ? a.table[T.entry(req, i * 32 + 16, shift)] : p[0];
+        };
+        auto where = [&](int i, const int *p, size_t *b) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int tok = i * 32 + 16 * u;
-                if (u && tok >= n) { b[1] = b[0]; continue; }
-                int pg = uni(a.table[T.entry(req, tok, shift)]);
+                int pg = uni(p[u]);
                 if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
-                b[u] = A.s.at(pg, kh, tok & ((1 << shift) - 1)) * 2;
+                b[u] = A.s.at(pg, kh, (u && tok >= n ? tok - 16 : tok) & ((1 << shift) - 1)) * 2;
             }
         };
         gu32x4 sk[PT], sv[PT];
         auto fetch = [&](const size_t *b) {
 #pragma unroll
             for (int i = 0; i < PT; i++) {
-                const int x = tid + ATT_T * i, row = x / CH;
+                const int x = tid + ROWS_T * i, row = x / CH;
+                if (32 * CH < ROWS_T && x >= 32 * CH) break;
                 const size_t off = (row < 16 ? b[0] : b[1]) + (size_t)((row & 15) * CH + x % CH) * 16;
                 sk[i] = *(const GAS gu32x4 *)(A.kc + off);
                 sv[i] = *(const GAS gu32x4 *)(A.vc + off);
@@ -663,39 +677,38 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
         auto put = [&](int buf) {
 #pragma unroll
             for (int i = 0; i < PT; i++) {
-                const int x = tid + ATT_T * i, row = x / CH, at = row * CH + ((x % CH) ^ (row & 7));
+                const int x = tid + ROWS_T * i, row = x / CH, at = row * CH + ((x % CH) ^ (row & 7));
+                if (32 * CH < ROWS_T && x >= 32 * CH) break;
                 s_k[buf][at] = sk[i];
                 s_v[buf][at] = sv[i];
             }
         };
         size_t b[2];
+        int p2[2];
         if (n > 0) {
-            where(first, b);
+            pages(first, p2);
+            where(first, p2, b);
             fetch(b);
+            if (first + 1 < last) pages(first + 1, p2);
         }
-        f16x8 qh[2][C::KS], ql[2][C::KS];
-        f32x4 o[2][NO];
-        float m[2], l[2], fac[2];
-        int nc[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int i = (2 * w + j) * A.rpg + cr;
-            const bool on = cr < A.rpg && i < nr && ch < nh;
-            const float *q = a.q + ((size_t)(t0 + (on ? i : 0)) * a.q_heads + h0 + (on ? ch : 0)) * D + 8 * g;
+        /* this lane's column */
+        const int ri = w * A.rpg + cr;
+        const bool on = cr < A.rpg && ri < nr && ch < nh;
+        f16x8 qh[C::KS], ql[C::KS];
+        f32x4 o[NO];
+        float m = -INFINITY, l = 0, fac;
+        const int nc = on ? T.tokens(req, a.row_pos[t0 + ri], shift) : 0;
+        {
+            const float *q = a.q + ((size_t)(t0 + (on ? ri : 0)) * a.q_heads + h0 + (on ? ch : 0)) * D + 8 * g;
             float4 x[2 * C::KS];
 #pragma unroll
             for (int s = 0; s < 2 * C::KS; s++) x[s] = *(const float4 *)(q + 32 * (s / 2) + 4 * (s % 2));
-            nc[j] = on ? T.tokens(req, a.row_pos[t0 + i], shift) : 0;
-            fac[j] = split_q<8 * C::KS, true>(x, qh[j], ql[j], 1.0f) * (a.scale * 1.44269504088896341f);
-            m[j] = -INFINITY;
-            l[j] = 0;
-#pragma unroll
-            for (int k = 0; k < NO; k++) o[j][k] = (f32x4){};
+            fac = split_q<8 * C::KS, true>(x, qh, ql, 1.0f) * (a.scale * 1.44269504088896341f);
         }
-        if (n > 0) {
-            int most = max(nc[0], nc[1]), least = INT32_MAX;            /* over the wave's columns in use */
 #pragma unroll
-            for (int j = 0; j < 2; j++) least = min(least, nc[j] > 0 ? nc[j] : INT32_MAX);
+        for (int k = 0; k < NO; k++) o[k] = (f32x4){};
+        if (n > 0) {
+            int most = nc, least = nc > 0 ? nc : INT32_MAX;            /* over the wave's columns in use */
             for (int x = 32; x; x >>= 1) {
                 most = max(most, __shfl_xor(most, x));
                 least = min(least, __shfl_xor(least, x));
@@ -710,58 +723,52 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
             for (; i < mine; i++) {
                 const int buf = (i - first) & 1;
                 if (i + 1 < last) {
-                    where(i + 1, b);
+                    where(i + 1, p2, b);
                     fetch(b);
+                    if (i + 2 < last) pages(i + 2, p2);
                 }
                 {
-                    f32x4 acc[2][2] = {};
+                    f32x4 acc[2] = {};
 #pragma unroll
                     for (int s = 0; s < C::KS; s++)
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const int row = 16 * u + c;
                             const f16x8 kf = __builtin_bit_cast(f16x8, s_k[buf][row * CH + ((4 * s + g) ^ (row & 7))]);
-#pragma unroll
-                            for (int j = 0; j < 2; j++) acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[j][s], acc[j][u], 0, 0, 0);
-#pragma unroll
-                            for (int j = 0; j < 2; j++) acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[j][s], acc[j][u], 0, 0, 0);
+                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[s], acc[u], 0, 0, 0);
+                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[s], acc[u], 0, 0, 0);
                         }
-                    f16x8 ph[2], pl[2];
+                    float p[8], mx = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        float p[8], mx = -INFINITY;
+                    for (int k = 0; k < 8; k++) p[k] = acc[k / 4][k & 3] * fac;
+                    if ((i + 1) * 32 > least) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++) p[k] = acc[j][k / 4][k & 3] * fac[j];
-                        if ((i + 1) * 32 > least) {
-#pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                if (i * 32 + 16 * (k / 4) + 4 * g + (k & 3) >= nc[j]) p[k] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; k++) mx = fmaxf(mx, p[k]);
-                        if (__any(mx > m[j] + M_LATE)) {
-                            const float mn = fmaxf(m[j], max_g(mx)), f = m[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[j] - mn);
-                            l[j] *= f;
-#pragma unroll
-                            for (int k = 0; k < NO; k++) o[j][k] *= f;
-                            m[j] = mn;
-                        }
-                        /* a column that has met no position yet keeps its terms 0 */
-                        const float base = m[j] == -INFINITY ? 0.0f : m[j] - P_UP;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            p[k] = __builtin_amdgcn_exp2f(p[k] - base);
-                            l[j] += p[k];
-                        }
-                        f16x2 hi[4], lo[4];
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            hi[k] = to_half(p[2 * k], p[2 * k + 1]);
-                            lo[k] = rest_half(hi[k], 1.0f, p[2 * k], p[2 * k + 1]);
-                        }
-                        ph[j] = join8(hi);
-                        pl[j] = join8(lo);
+                        for (int k = 0; k < 8; k++)
+                            if (i * 32 + 16 * (k / 4) + 4 * g + (k & 3) >= nc) p[k] = -INFINITY;
                     }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) mx = fmaxf(mx, p[k]);
+                    if (__any(mx > m + M_LATE)) {
+                        const float mn = fmaxf(m, max_g(mx)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                        l *= f;
+#pragma unroll
+                        for (int k = 0; k < NO; k++) o[k] *= f;
+                        m = mn;
+                    }
+                    /* a column that has met no position yet keeps its terms 0 */
+                    const float base = m == -INFINITY ? 0.0f : m - P_UP;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        p[k] = __builtin_amdgcn_exp2f(p[k] - base);
+                        l += p[k];
+                    }
+                    f16x2 hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        hi[k] = to_half(p[2 * k], p[2 * k + 1]);
+                        lo[k] = rest_half(hi[k], 1.0f, p[2 * k], p[2 * k + 1]);
+                    }
+                    const f16x8 ph = join8(hi), pl = join8(lo);
                     const int left = n - i * 32;
 #pragma unroll
                     for (int nb = 0; nb < C::NB; nb++) {
@@ -774,7 +781,11 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
                                 const gu32x2 h = ((const gu32x2 *)&s_v[buf][row * CH + ((c >> 1) ^ (row & 7))])[c & 1];
                                 v[k] = (gu32x4){ h.x, h.y, 0, 0 };
                             }
-                            if (left < 32 && row >= left) v[k] = (gu32x4){};     /* behind the run: may be anything */
+                        }
+                        if (left < 32) {                 /* behind the run: may be anything */
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if (4 * g + (k & 3) + 16 * (k / 4) >= left) v[k] = (gu32x4){};
                         }
 #pragma unroll
                         for (int e = 0; e < C::VE; e++) {
@@ -783,12 +794,8 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
                             for (int k = 0; k < 4; k++)
                                 x[k] = __builtin_amdgcn_perm(v[2 * k + 1][e / 2], v[2 * k][e / 2], e & 1 ? 0x07060302 : 0x05040100);
                             const f16x8 vf = __builtin_bit_cast(f16x8, x);
-#pragma unroll
-                            for (int j = 0; j < 2; j++)
-                                o[j][nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[j], o[j][nb * C::VE + e], 0, 0, 0);
-#pragma unroll
-                            for (int j = 0; j < 2; j++)
-                                o[j][nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[j], o[j][nb * C::VE + e], 0, 0, 0);
+                            o[nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[nb * C::VE + e], 0, 0, 0);
+                            o[nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[nb * C::VE + e], 0, 0, 0);
                         }
                     }
                 }
@@ -797,8 +804,9 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
             }
             for (; i < last; i++) {
                 if (i + 1 < last) {
-                    where(i + 1, b);
+                    where(i + 1, p2, b);
                     fetch(b);
+                    if (i + 2 < last) pages(i + 2, p2);
                     put((i - first + 1) & 1);
                 }
                 __syncthreads();
@@ -806,17 +814,14 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
         }
         if (bad && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
         const int slot = 2 * blockIdx.x + (first == 0);
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int i = (2 * w + j) * A.rpg + cr;
-            if (!(cr < A.rpg && i < nr && ch < nh)) continue;
-            float sum = sum_g(l[j]);
-            if (bad) sum = NAN;
-            const int col = i * A.hpb + ch;
-            if (!whole && g == 0) {
-                A.pm[slot * ROWS_COLS + col] = m[j];
-                A.pl[slot * ROWS_COLS + col] = sum;
-            }
+        float sum = sum_g(l);
+        if (bad) sum = NAN;
+        const int col = ri * A.hpb + ch;
+        if (on && !whole && g == 0) {
+            A.pm[slot * ROWS_COLS + col] = m;
+            A.pl[slot * ROWS_COLS + col] = sum;
+        }
+        if (on)
 #pragma unroll
             for (int nb = 0; nb < C::NB; nb++)
 #pragma unroll
@@ -825,12 +830,11 @@ __global__ __launch_bounds__(ATT_T, 1) void attn_rows_kernel(RowsArgs A, int *er
                     for (int e = 0; e < C::VE; e += 4) {
                         f32x4 y;
 #pragma unroll
-                        for (int z = 0; z < 4; z++) y[z] = o[j][nb * C::VE + e + z][k];
+                        for (int z = 0; z < 4; z++) y[z] = o[nb * C::VE + e + z][k];
                         const int d = 16 * C::VE * nb + C::VE * (4 * g + k) + e;
-                        if (whole) att_store(a, D, t0 + i, h0 + ch, d, y, nc[j] == 0 ? 1.0f : sum);
+                        if (whole) att_store(a, D, t0 + ri, h0 + ch, d, y, nc == 0 ? 1.0f : sum);
                         else *(f32x4 *)(A.po + ((size_t)slot * ROWS_COLS + col) * D + d) = y;
                     }
-        }
         at += last - first;
         if (tid == 0 && at == end) {
             const RowsCut x = { t0, nr, hb, cuts ? (int)((at - last + tiles - 1) / share) - (int)blockIdx.x + 1 : 0 };
@@ -974,7 +978,7 @@ extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCa
 template <int D>
 static void rows_launch(const RowsArgs &A, int *err)
 {
-    hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ATT_T), 0, rt().stream, A, err);
+    hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ROWS_T), 0, rt().stream, A, err);
     hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_G, ROWS_COLS * D / 4 / ATT_T), dim3(ATT_T), 0, rt().stream, A);
 }
 
@@ -1033,7 +1037,7 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
         A.hpb = A.group < 16 ? A.group : 16;
         A.blocks = (A.group + A.hpb - 1) / A.hpb;
         A.rpg = 16 / A.hpb;
-        A.R = 2 * ATT_W * A.rpg;
+        A.R = ROWS_W * A.rpg;
         A.cut = (RowsCut *)p->ws;
         A.pm = (float *)((char *)p->ws + ROWS_CUT);
         A.pl = (float *)((char *)p->ws + ROWS_CUT + ROWS_ML);
