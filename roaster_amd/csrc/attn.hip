@@ -546,7 +546,44 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
+#define ROWS_BUF 4            /* tiles in LDS: the one in use and three under way */
 #define ROWS_COLS 128         /* columns of a unit: 16 a wave */
+
+/* s_waitcnt's operand for at most n loads under way, LDS and exports not waited for. */
+#define ROWS_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
+#define CAS __attribute__((address_space(4)))
+
+/* Pieces of 16 bytes (8 with an h) from LDS bytes a0..a3, further O0 and further O1
+ * for the second four.  In one block with their wait: a read that the compiler sees
+ * would wait for every tile under way into LDS. */
+template <int O0, int O1>
+__device__ __forceinline__ void lds_read8(gu32x4 *r, int a0, int a1, int a2, int a3)
+{
+    asm volatile("ds_read_b128 %0, %8 offset:%12\n\tds_read_b128 %1, %9 offset:%12\n\t"
+                 "ds_read_b128 %2, %10 offset:%12\n\tds_read_b128 %3, %11 offset:%12\n\t"
+                 "ds_read_b128 %4, %8 offset:%13\n\tds_read_b128 %5, %9 offset:%13\n\t"
+                 "ds_read_b128 %6, %10 offset:%13\n\tds_read_b128 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(O0), "n"(O1) : "memory");
+}
+__device__ __forceinline__ void lds_read4(gu32x4 *r, int a0, int a1, int a2, int a3)
+{
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]) : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
+}
+template <int O1>
+__device__ __forceinline__ void lds_read8h(gu32x4 *r, int a0, int a1, int a2, int a3)
+{
+    gu32x2 h[8];
+    asm volatile("ds_read_b64 %0, %8\n\tds_read_b64 %1, %9\n\tds_read_b64 %2, %10\n\tds_read_b64 %3, %11\n\t"
+                 "ds_read_b64 %4, %8 offset:%12\n\tds_read_b64 %5, %9 offset:%12\n\t"
+                 "ds_read_b64 %6, %10 offset:%12\n\tds_read_b64 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7])
+                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(O1) : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = (gu32x4){ h[i].x, h[i].y, 0, 0 };
+}
 
 struct RowsCut {
     int row, n, hb, k;        /* first row, rows and head block of a unit, and its number of shares (0: not to be joined) */
@@ -594,8 +631,9 @@ template <int D>
 __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *err)
 {
     using C = AttCfg<D, true>;
-    constexpr int CH = D / 8, PT = (32 * CH + ROWS_T - 1) / ROWS_T, NO = C::NB * C::VE;         /* 16-byte pieces of a token, of a thread; sums of a lane */
-    __shared__ gu32x4 s_k[2][32 * CH], s_v[2][32 * CH];
+    constexpr int CH = D / 8, NO = C::NB * C::VE;         /* 16-byte pieces of a token; sums of a lane */
+    constexpr int SW = CH < 16 ? CH : 16, KJ = SW / 4;
+    __shared__ gu32x4 s_t[ROWS_BUF][2][32 * CH];          /* tiles of keys and values */
     __shared__ long long s_wave[ROWS_W], s_at;
     __shared__ int s_row;
     const RoasterAttnPaged &a = A.a;
@@ -630,6 +668,17 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     __syncthreads();
     int t1 = uni(s_row), tiles = uni(rows_tiles(A, T, t1));
     int hb = uni((int)((at - s_at) / tiles)), first = uni((int)((at - s_at) % tiles));
+    /* Where this lane's operands lie in a tile, in bytes: its key's piece 4 s + g at kb[s % KJ]
+     * + 64 (s - s % KJ), its value piece of token 4 g + k at vb[k], further 256 for the next
+     * 16 pieces.  (4 s + g) ^ r = 4 (s ^ r / 4) + (g ^ r % 4). */
+    int kb[KJ], vb[4];
+    const int t0_at = (int)(uintptr_t)(__attribute__((address_space(3))) void *)&s_t[0][0][0];
+#pragma unroll
+    for (int k = 0; k < KJ; k++) kb[k] = t0_at + (c * CH + 4 * (k ^ (c % SW) / 4) + (g ^ c % 4)) * 16;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        vb[k] = t0_at + (C::VE == 8 ? ((4 * g + k) * CH + (c ^ (4 * g + k) % SW)) * 16
+                                    : ((4 * g + k) * CH + ((c >> 1) ^ (4 * g + k) % SW)) * 16 + 8 * (c & 1));
     const int cr = c / A.hpb, ch = c - cr * A.hpb;                      /* this lane's column: its row and head within the group */
     while (1) {
         const int last = uni((int)min((long long)tiles, first + (end - at)));
@@ -650,46 +699,40 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         /* page numbers of tile i's two 16-token parts (a part past the run's end repeats
          * the first), then the bytes at which the parts begin */
         auto pages = [&](int i, int *p) {
-            p[0] = a.table[T.entry(req, i * 32, shift)];
-            p[1] = i * 32 + 16 < n ? a.table[T.entry(req, i * 32 + 16, shift)] : p[0];
+            const CAS int *t = (const CAS int *)a.table;              /* scalar loads: they stay out of the tiles' count */
+            p[0] = t[T.entry(req, i * 32, shift)];
+            p[1] = i * 32 + 16 < n ? t[T.entry(req, i * 32 + 16, shift)] : p[0];
         };
         auto where = [&](int i, const int *p, size_t *b) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int tok = i * 32 + 16 * u;
-                int pg = uni(p[u]);
+                int pg = p[u];
                 if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
                 b[u] = A.s.at(pg, kh, (u && tok >= n ? tok - 16 : tok) & ((1 << shift) - 1)) * 2;
             }
         };
-        gu32x4 sk[PT], sv[PT];
-        auto fetch = [&](const size_t *b) {
+        /* The tile's 64 CH pieces straight into LDS, 64 to a wave and load, in the order
+         * they lie there: piece x of a token's row lies at x ^ (row % SW), so that the rows
+         * which an operand read takes fall on different banks. */
+        auto fetch = [&](int buf, const size_t *b) {
 #pragma unroll
-            for (int i = 0; i < PT; i++) {
-                const int x = tid + ROWS_T * i, row = x / CH;
-                if (32 * CH < ROWS_T && x >= 32 * CH) break;
-                const size_t off = (row < 16 ? b[0] : b[1]) + (size_t)((row & 15) * CH + x % CH) * 16;
-                sk[i] = *(const GAS gu32x4 *)(A.kc + off);
-                sv[i] = *(const GAS gu32x4 *)(A.vc + off);
-            }
-        };
-        /* piece x of a token's row lies at x ^ (row & 7): the 16 rows that an operand read takes fall on different banks */
-        auto put = [&](int buf) {
-#pragma unroll
-            for (int i = 0; i < PT; i++) {
-                const int x = tid + ROWS_T * i, row = x / CH, at = row * CH + ((x % CH) ^ (row & 7));
-                if (32 * CH < ROWS_T && x >= 32 * CH) break;
-                s_k[buf][at] = sk[i];
-                s_v[buf][at] = sv[i];
+            for (int i = 0; i < CH / ROWS_W; i++) {
+                const int q = i * ROWS_W + w, v = q >= CH / 2, at = (q - v * (CH / 2)) * 64, row = (at + lane) / CH;
+                const size_t off = (row < 16 ? b[0] : b[1]) + (size_t)((row & 15) * CH + ((at + lane) % CH ^ (row % SW))) * 16;
+                __builtin_amdgcn_global_load_lds((const GAS void *)((v ? A.vc : A.kc) + off),
+                                                 (__attribute__((address_space(3))) void *)&s_t[buf][v][at], 16, 0, 0);
             }
         };
         size_t b[2];
         int p2[2];
         if (n > 0) {
-            pages(first, p2);
-            where(first, p2, b);
-            fetch(b);
-            if (first + 1 < last) pages(first + 1, p2);
+            for (int k = 0; k < ROWS_BUF - 1 && first + k < last; k++) {
+                pages(first + k, p2);
+                where(first + k, p2, b);
+                fetch(k, b);
+            }
+            if (first + ROWS_BUF - 1 < last) pages(first + ROWS_BUF - 1, p2);
         }
         /* this lane's column */
         const int ri = w * A.rpg + cr;
@@ -715,29 +758,49 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             }
             most = uni(most);
             least = uni(least);
-            put(0);
-            __syncthreads();
             /* this wave's own rows may end before the run does: then it only brings tiles */
             const int mine = min(last, (int)(((long long)most + 31) / 32));
+            /* tile i has come, to this wave and the others, and tile i - 1 is done with */
+            auto next = [&](int i) {
+                const int under_way = min(ROWS_BUF - 2, last - 1 - i);
+                if (under_way >= 2) __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(2 * CH / ROWS_W));
+                else if (under_way == 1) __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(CH / ROWS_W));
+                else __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(0));
+                __syncthreads();
+                const int far = i + ROWS_BUF - 1;
+                if (far < last) {
+                    where(far, p2, b);
+                    fetch((far - first) % ROWS_BUF, b);
+                    if (far + 1 < last) pages(far + 1, p2);
+                }
+            };
             int i = first;
             for (; i < mine; i++) {
-                const int buf = (i - first) & 1;
-                if (i + 1 < last) {
-                    where(i + 1, p2, b);
-                    fetch(b);
-                    if (i + 2 < last) pages(i + 2, p2);
+                next(i);
+                const int at = ((i - first) % ROWS_BUF) * (int)sizeof(s_t[0]);
+                int kt[4], vt[4];                      /* this tile's operands */
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    kt[k] = at + (KJ == 4 ? kb[k % KJ] : kb[k % 2] + k / 2 * CH * 256);
+                    vt[k] = at + (int)sizeof(s_t[0][0]) + vb[k];
                 }
                 {
                     f32x4 acc[2] = {};
+                    gu32x4 kf[8];
 #pragma unroll
-                    for (int s = 0; s < C::KS; s++)
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const int row = 16 * u + c;
-                            const f16x8 kf = __builtin_bit_cast(f16x8, s_k[buf][row * CH + ((4 * s + g) ^ (row & 7))]);
-                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[s], acc[u], 0, 0, 0);
-                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[s], acc[u], 0, 0, 0);
+                    for (int u = 0; u < 2; u++) {
+                        if constexpr (D == 256) lds_read8<0, 256>(kf, kt[0] + u * CH * 256, kt[1] + u * CH * 256, kt[2] + u * CH * 256, kt[3] + u * CH * 256);
+                        else if (u == 0) {
+                            if constexpr (D == 128) lds_read8<0, CH * 256>(kf, kt[0], kt[1], kt[2], kt[3]);
+                            else lds_read4(kf, kt[0], kt[1], kt[2], kt[3]);
                         }
+#pragma unroll
+                        for (int s = 0; s < C::KS; s++) {
+                            const f16x8 x = __builtin_bit_cast(f16x8, kf[D == 256 ? s : u * C::KS + s]);
+                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[s], acc[u], 0, 0, 0);
+                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[s], acc[u], 0, 0, 0);
+                        }
+                    }
                     float p[8], mx = -INFINITY;
 #pragma unroll
                     for (int k = 0; k < 8; k++) p[k] = acc[k / 4][k & 3] * fac;
@@ -773,15 +836,10 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
                     for (int nb = 0; nb < C::NB; nb++) {
                         gu32x4 v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const int row = 4 * g + (k & 3) + 16 * (k / 4);
-                            if constexpr (C::VE == 8) v[k] = s_v[buf][row * CH + ((16 * nb + c) ^ (row & 7))];
-                            else {
-                                const gu32x2 h = ((const gu32x2 *)&s_v[buf][row * CH + ((c >> 1) ^ (row & 7))])[c & 1];
-                                v[k] = (gu32x4){ h.x, h.y, 0, 0 };
-                            }
-                        }
+                        if constexpr (C::VE == 8) {
+                            if (nb == 0) lds_read8<0, CH * 256>(v, vt[0], vt[1], vt[2], vt[3]);
+                            else lds_read8<256, CH * 256 + 256>(v, vt[0], vt[1], vt[2], vt[3]);
+                        } else lds_read8h<CH * 256>(v, vt[0], vt[1], vt[2], vt[3]);
                         if (left < 32) {                 /* behind the run: may be anything */
 #pragma unroll
                             for (int k = 0; k < 8; k++)
@@ -799,18 +857,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                         }
                     }
                 }
-                if (i + 1 < last) put(buf ^ 1);
-                __syncthreads();
             }
-            for (; i < last; i++) {
-                if (i + 1 < last) {
-                    where(i + 1, p2, b);
-                    fetch(b);
-                    if (i + 2 < last) pages(i + 2, p2);
-                    put((i - first + 1) & 1);
-                }
-                __syncthreads();
-            }
+            for (; i < last; i++) next(i);
         }
         if (bad && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
         const int slot = 2 * blockIdx.x + (first == 0);
@@ -841,6 +889,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             A.cut[blockIdx.x] = x;
         }
         if (at >= end) break;
+        __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(0));     /* no store is counted among the next unit's tiles */
+        __syncthreads();                               /* the tiles in LDS are done with */
         first = 0;
         if (++hb == per_row) {
             hb = 0;
