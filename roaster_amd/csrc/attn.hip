@@ -546,14 +546,13 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
-#define ROWS_BUF 4            /* tiles in LDS: the one in use and three under way */
 #define ROWS_COLS 128         /* columns of a unit: 16 a wave */
 
-/* s_waitcnt's operand for at most n loads under way, LDS and exports not waited for. */
-#define ROWS_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
+/* s_waitcnt's operand for no load and no store under way, LDS and exports not waited for. */
+#define ROWS_ALL_CAME ((7 << 4) | (15 << 8))
 #define CAS __attribute__((address_space(4)))
 
-/* Pieces of 16 bytes (8 with an h) from LDS bytes a0..a3, further O0 and further O1
+/* Pieces of 16 bytes from LDS bytes a0..a3, further O0 and further O1
  * for the second four.  In one block with their wait: a read that the compiler sees
  * would wait for every tile under way into LDS. */
 template <int O0, int O1>
@@ -572,17 +571,39 @@ __device__ __forceinline__ void lds_read4(gu32x4 *r, int a0, int a1, int a2, int
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]) : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
 }
-template <int O1>
-__device__ __forceinline__ void lds_read8h(gu32x4 *r, int a0, int a1, int a2, int a3)
+/* Eight operands of 16 elements' values each from the addresses a[], tokens of the first
+ * half at O0 and of the second at O1: the transposing read takes 4 rows of 16 elements
+ * from 16 lanes (lane 4 r + q: elements 4 q .. of row r) and gives lane c the four
+ * elements of column c. */
+template <int O0, int O1>
+__device__ __forceinline__ void lds_cols8(gu32x2 (*r)[2], const int *a)
 {
-    gu32x2 h[8];
-    asm volatile("ds_read_b64 %0, %8\n\tds_read_b64 %1, %9\n\tds_read_b64 %2, %10\n\tds_read_b64 %3, %11\n\t"
-                 "ds_read_b64 %4, %8 offset:%12\n\tds_read_b64 %5, %9 offset:%12\n\t"
-                 "ds_read_b64 %6, %10 offset:%12\n\tds_read_b64 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7])
-                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(O1) : "memory");
-#pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = (gu32x4){ h[i].x, h[i].y, 0, 0 };
+    asm volatile("ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %1, %16 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %2, %17 offset:%24\n\tds_read_b64_tr_b16 %3, %17 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %4, %18 offset:%24\n\tds_read_b64_tr_b16 %5, %18 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %6, %19 offset:%24\n\tds_read_b64_tr_b16 %7, %19 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %8, %20 offset:%24\n\tds_read_b64_tr_b16 %9, %20 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %10, %21 offset:%24\n\tds_read_b64_tr_b16 %11, %21 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %12, %22 offset:%24\n\tds_read_b64_tr_b16 %13, %22 offset:%25\n\t"
+                 "ds_read_b64_tr_b16 %14, %23 offset:%24\n\tds_read_b64_tr_b16 %15, %23 offset:%25\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]),
+                   "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[4][0]), "=&v"(r[4][1]), "=&v"(r[5][0]), "=&v"(r[5][1]),
+                   "=&v"(r[6][0]), "=&v"(r[6][1]), "=&v"(r[7][0]), "=&v"(r[7][1])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "n"(O0), "n"(O1)
+                 : "memory");
+}
+template <int O0, int O1>
+__device__ __forceinline__ void lds_cols4(gu32x2 (*r)[2], const int *a)
+{
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]),
+                   "=&v"(r[3][0]), "=&v"(r[3][1])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(O0), "n"(O1) : "memory");
 }
 
 struct RowsCut {
@@ -596,46 +617,40 @@ struct RowsArgs {
     int group, blocks, hpb;   /* query heads of a key/value head, their blocks, heads of a block */
     int rpg, R;               /* rows of a column group, of a run */
     RowsCut *cut;             /* [ROWS_G] by the share that began a unit and did not finish it */
-    float *pm, *pl, *po;      /* parts [2 ROWS_G][ROWS_COLS] and [..][D], slots as in AttArgs */
+    float *pm, *pl, *po;      /* parts [2 ROWS_G][waves][16 columns], and [..][waves][D / 16][64 lanes][4]; slots as in AttArgs */
 };
 
-/* Tokens of row t; where they are, the row goes on with the run of row t - 1. */
+/* Row t's request and tokens, and whether it goes on with the run of row t - 1. */
 struct RowsAt {
     int req, n;
     bool joined;
 };
 __device__ __forceinline__ RowsAt rows_at(const RowsArgs &A, const KvTable &T, int t)
 {
+    const int b = max(t - 1, 0), r = A.a.row_req[b], p = A.a.row_pos[b];
     RowsAt x;
     x.req = A.a.row_req[t];
-    x.n = x.req == -1 ? -1 : T.tokens(x.req, A.a.row_pos[t], A.s.shift);
-    x.joined = false;
-    if (t % A.R && x.n >= 0) {
-        const int r = A.a.row_req[t - 1];
-        if (r == x.req) {
-            const int n = T.tokens(r, A.a.row_pos[t - 1], A.s.shift);
-            x.joined = n >= 0 && n <= x.n;
-        }
-    }
+    x.n = T.tokens(x.req, A.a.row_pos[t], A.s.shift);      /* -1 for a row that is skipped, too */
+    const int n = T.tokens(r, p, A.s.shift);
+    x.joined = t % A.R && r == x.req && n >= 0 && n <= x.n;
     return x;
 }
 /* Tiles of the run that ends with row t, 0 if none does. */
 __device__ __forceinline__ int rows_tiles(const RowsArgs &A, const KvTable &T, int t)
 {
-    const RowsAt x = rows_at(A, T, t);
-    if (x.req == -1 || (t + 1 < A.a.rows && rows_at(A, T, t + 1).joined)) return 0;
+    const RowsAt x = rows_at(A, T, t), y = rows_at(A, T, min(t + 1, A.a.rows - 1));
+    if (x.req == -1 || (t + 1 < A.a.rows && y.joined)) return 0;
     return x.n <= 32 ? 1 : (int)(((long long)x.n + 31) / 32);
 }
 
 template <int D>
 __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *err)
 {
-    using C = AttCfg<D, true>;
-    constexpr int CH = D / 8, NO = C::NB * C::VE;         /* 16-byte pieces of a token; sums of a lane */
-    constexpr int SW = CH < 16 ? CH : 16, KJ = SW / 4;
-    __shared__ gu32x4 s_t[ROWS_BUF][2][32 * CH];          /* tiles of keys and values */
+    constexpr int CH = D / 8, KS = D / 32, NO = D / 16;   /* 16-byte pieces of a token; steps of a score; sums of a lane */
+    constexpr int SW = CH < 16 ? CH : 16, KJ = SW / 4, VJ = SW / 2;
+    __shared__ gu32x4 s_t[4][2][32 * CH];          /* tiles of keys and values: two in use, two under way */
     __shared__ long long s_wave[ROWS_W], s_at;
-    __shared__ int s_row;
+    __shared__ int s_row, s_tiles;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
@@ -643,9 +658,10 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 
     const int each = (rows + ROWS_T - 1) / ROWS_T;
     long long mine = 0, tot;
+    int tl = 0;
     for (int i = 0; i < each; i++) {
         const int t = tid * each + i;
-        if (t < rows) mine += rows_tiles(A, T, t);
+        if (t < rows) mine += tl = rows_tiles(A, T, t);
     }
     const long long upto = att_scan<ROWS_W>(mine, s_wave, tot);
     const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
@@ -657,28 +673,30 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     }
     if (at < upto * per_row && at >= (upto - mine) * per_row) {
         long long b = (upto - mine) * per_row;
-        int t = tid * each, n;
-        while (at >= b + (n = rows_tiles(A, T, t)) * (long long)per_row) {
-            b += n * (long long)per_row;
-            t++;
-        }
+        int t = tid * each;
+        if (each > 1)
+            while (at >= b + (tl = rows_tiles(A, T, t)) * (long long)per_row) {
+                b += tl * (long long)per_row;
+                t++;
+            }
         s_row = t;
+        s_tiles = tl;
         s_at = b;
     }
     __syncthreads();
-    int t1 = uni(s_row), tiles = uni(rows_tiles(A, T, t1));
+    int t1 = uni(s_row), tiles = uni(s_tiles);
     int hb = uni((int)((at - s_at) / tiles)), first = uni((int)((at - s_at) % tiles));
     /* Where this lane's operands lie in a tile, in bytes: its key's piece 4 s + g at kb[s % KJ]
-     * + 64 (s - s % KJ), its value piece of token 4 g + k at vb[k], further 256 for the next
-     * 16 pieces.  (4 s + g) ^ r = 4 (s ^ r / 4) + (g ^ r % 4). */
-    int kb[KJ], vb[4];
-    const int t0_at = (int)(uintptr_t)(__attribute__((address_space(3))) void *)&s_t[0][0][0];
+     * + 64 (s - s % KJ), its share of the values' 16 elements j at vb[j % VJ] + 32 (j - j % VJ):
+     * four elements of token 4 g + c / 4.  (4 s + g) ^ r = 4 (s ^ r / 4) + (g ^ r % 4), and
+     * alike for the pieces 2 j + (c & 2) / 2. */
+    int kb[KJ], vb[VJ];
+    const int t0_at = (int)(uintptr_t)(__attribute__((address_space(3))) void *)&s_t[0][0][0], vr = 4 * g + c / 4;
 #pragma unroll
     for (int k = 0; k < KJ; k++) kb[k] = t0_at + (c * CH + 4 * (k ^ (c % SW) / 4) + (g ^ c % 4)) * 16;
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        vb[k] = t0_at + (C::VE == 8 ? ((4 * g + k) * CH + (c ^ (4 * g + k) % SW)) * 16
-                                    : ((4 * g + k) * CH + ((c >> 1) ^ (4 * g + k) % SW)) * 16 + 8 * (c & 1));
+    for (int k = 0; k < VJ; k++)
+        vb[k] = t0_at + (vr * CH + 2 * (k ^ (vr % SW) / 2) + ((c >> 1 & 1) ^ (vr & 1))) * 16 + 8 * (c & 1);
     const int cr = c / A.hpb, ch = c - cr * A.hpb;                      /* this lane's column: its row and head within the group */
     while (1) {
         const int last = uni((int)min((long long)tiles, first + (end - at)));
@@ -714,40 +732,57 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         };
         /* The tile's 64 CH pieces straight into LDS, 64 to a wave and load, in the order
          * they lie there: piece x of a token's row lies at x ^ (row % SW), so that the rows
-         * which an operand read takes fall on different banks. */
+         * which an operand read takes fall on different banks.  A load's rows lie in one
+         * 16-token part. */
         auto fetch = [&](int buf, const size_t *b) {
 #pragma unroll
             for (int i = 0; i < CH / ROWS_W; i++) {
                 const int q = i * ROWS_W + w, v = q >= CH / 2, at = (q - v * (CH / 2)) * 64, row = (at + lane) / CH;
-                const size_t off = (row < 16 ? b[0] : b[1]) + (size_t)((row & 15) * CH + ((at + lane) % CH ^ (row % SW))) * 16;
-                __builtin_amdgcn_global_load_lds((const GAS void *)((v ? A.vc : A.kc) + off),
+                const char *from = (v ? A.vc : A.kc) + (at / CH < 16 ? b[0] : b[1]);
+                const unsigned off = ((row & 15) * CH + ((at + lane) % CH ^ row % SW)) * 16;
+                __builtin_amdgcn_global_load_lds((const GAS void *)(from + off),
                                                  (__attribute__((address_space(3))) void *)&s_t[buf][v][at], 16, 0, 0);
             }
         };
         size_t b[2];
-        int p2[2];
+        int pg[2][2];
         if (n > 0) {
-            for (int k = 0; k < ROWS_BUF - 1 && first + k < last; k++) {
-                pages(first + k, p2);
-                where(first + k, p2, b);
-                fetch(k, b);
-            }
-            if (first + ROWS_BUF - 1 < last) pages(first + ROWS_BUF - 1, p2);
+            pages(first, pg[0]);
+            pages(min(first + 1, last - 1), pg[1]);
         }
         /* this lane's column */
         const int ri = w * A.rpg + cr;
         const bool on = cr < A.rpg && ri < nr && ch < nh;
-        f16x8 qh[C::KS], ql[C::KS];
+        f16x8 qh[KS], ql[KS];
         f32x4 o[NO];
         float m = -INFINITY, l = 0, fac;
         const int nc = on ? T.tokens(req, a.row_pos[t0 + ri], shift) : 0;
+        float4 qx[2 * KS];
         {
             const float *q = a.q + ((size_t)(t0 + (on ? ri : 0)) * a.q_heads + h0 + (on ? ch : 0)) * D + 8 * g;
-            float4 x[2 * C::KS];
 #pragma unroll
-            for (int s = 0; s < 2 * C::KS; s++) x[s] = *(const float4 *)(q + 32 * (s / 2) + 4 * (s % 2));
-            fac = split_q<8 * C::KS, true>(x, qh, ql, 1.0f) * (a.scale * 1.44269504088896341f);
+            for (int s = 0; s < 2 * KS; s++) qx[s] = *(const float4 *)(q + 32 * (s / 2) + 4 * (s % 2));
         }
+        /* tiles i and i + 1, and the page numbers of the two behind them */
+        auto bring = [&](int i, int buf) {
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (i + k < last) {
+                    where(i + k, pg[k], b);
+                    fetch(buf + k, b);
+                }
+        };
+        if (n > 0) {
+            bring(first, 0);
+            pages(min(first + 2, last - 1), pg[0]);
+            pages(min(first + 3, last - 1), pg[1]);
+        }
+        #pragma unroll
+        for (int s = 0; s < 2 * KS; s++) {
+            const float f = a.scale * 1.44269504088896341f;
+            qx[s].x *= f; qx[s].y *= f; qx[s].z *= f; qx[s].w *= f;
+        }
+        fac = split_q<8 * KS, true>(qx, qh, ql, 1.0f);
 #pragma unroll
         for (int k = 0; k < NO; k++) o[k] = (f32x4){};
         if (n > 0) {
@@ -760,50 +795,44 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             least = uni(least);
             /* this wave's own rows may end before the run does: then it only brings tiles */
             const int mine = min(last, (int)(((long long)most + 31) / 32));
-            /* tile i has come, to this wave and the others, and tile i - 1 is done with */
-            auto next = [&](int i) {
-                const int under_way = min(ROWS_BUF - 2, last - 1 - i);
-                if (under_way >= 2) __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(2 * CH / ROWS_W));
-                else if (under_way == 1) __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(CH / ROWS_W));
-                else __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(0));
+            for (int i0 = first; i0 < last; i0 += 2) {
+                /* both tiles have come, to this wave and the others, and the two before are done
+                 * with; a barrier for two tiles lets a SIMD's two waves drift apart, so that
+                 * one's MFMAs run beside the other's softmax */
+                const int buf = (i0 - first) & 2;
+                __builtin_amdgcn_s_waitcnt(ROWS_ALL_CAME);
                 __syncthreads();
-                const int far = i + ROWS_BUF - 1;
-                if (far < last) {
-                    where(far, p2, b);
-                    fetch((far - first) % ROWS_BUF, b);
-                    if (far + 1 < last) pages(far + 1, p2);
-                }
-            };
-            int i = first;
-            for (; i < mine; i++) {
-                next(i);
-                const int at = ((i - first) % ROWS_BUF) * (int)sizeof(s_t[0]);
-                int kt[4], vt[4];                      /* this tile's operands */
+                bring(i0 + 2, buf ^ 2);
+                const int to = min(i0 + 2, mine);
+#pragma unroll 1
+                for (int i = i0; i < to; i++) {
+                const int at = (buf + i - i0) * (int)sizeof(s_t[0]);
+                int kt[4], vt[VJ];                     /* this tile's operands */
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    kt[k] = at + (KJ == 4 ? kb[k % KJ] : kb[k % 2] + k / 2 * CH * 256);
-                    vt[k] = at + (int)sizeof(s_t[0][0]) + vb[k];
-                }
+                for (int k = 0; k < 4; k++) kt[k] = at + (KJ == 4 ? kb[k % KJ] : kb[k % 2] + k / 2 * CH * 256);
+#pragma unroll
+                for (int k = 0; k < VJ; k++) vt[k] = at + (int)sizeof(s_t[0][0]) + vb[k];
                 {
                     f32x4 acc[2] = {};
-                    gu32x4 kf[8];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        if constexpr (D == 256) lds_read8<0, 256>(kf, kt[0] + u * CH * 256, kt[1] + u * CH * 256, kt[2] + u * CH * 256, kt[3] + u * CH * 256);
-                        else if (u == 0) {
-                            if constexpr (D == 128) lds_read8<0, CH * 256>(kf, kt[0], kt[1], kt[2], kt[3]);
-                            else lds_read4(kf, kt[0], kt[1], kt[2], kt[3]);
-                        }
+                    for (int q = 0; q < (D == 256 ? 2 : 1); q++) {
+                        constexpr int S = D == 64 ? 2 : 4;             /* products of a chain that one block's reads feed */
+                        gu32x4 kf[8];
+                        if constexpr (D == 64) lds_read4(kf, kt[0], kt[1], kt[2], kt[3]);
+                        else if (q == 0) lds_read8<0, CH * 256>(kf, kt[0], kt[1], kt[2], kt[3]);
+                        else lds_read8<256, CH * 256 + 256>(kf, kt[0], kt[1], kt[2], kt[3]);
 #pragma unroll
-                        for (int s = 0; s < C::KS; s++) {
-                            const f16x8 x = __builtin_bit_cast(f16x8, kf[D == 256 ? s : u * C::KS + s]);
-                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[s], acc[u], 0, 0, 0);
-                            acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[s], acc[u], 0, 0, 0);
-                        }
+                        for (int s = 0; s < S; s++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const f16x8 x = __builtin_bit_cast(f16x8, kf[u * S + s]);
+                                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[q * S + s], acc[u], 0, 0, 0);
+                                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[q * S + s], acc[u], 0, 0, 0);
+                            }
                     }
                     float p[8], mx = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) p[k] = acc[k / 4][k & 3] * fac;
+                    for (int k = 0; k < 8; k++) p[k] = acc[k / 4][k & 3];
                     if ((i + 1) * 32 > least) {
 #pragma unroll
                         for (int k = 0; k < 8; k++)
@@ -811,6 +840,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                     }
 #pragma unroll
                     for (int k = 0; k < 8; k++) mx = fmaxf(mx, p[k]);
+                    mx *= fac;
                     if (__any(mx > m + M_LATE)) {
                         const float mn = fmaxf(m, max_g(mx)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
                         l *= f;
@@ -819,10 +849,10 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                         m = mn;
                     }
                     /* a column that has met no position yet keeps its terms 0 */
-                    const float base = m == -INFINITY ? 0.0f : m - P_UP;
+                    const float base = m == -INFINITY ? 0.0f : P_UP - m;
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
-                        p[k] = __builtin_amdgcn_exp2f(p[k] - base);
+                        p[k] = __builtin_amdgcn_exp2f(fmaf(p[k], fac, base));
                         l += p[k];
                     }
                     f16x2 hi[4], lo[4];
@@ -834,62 +864,63 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                     const f16x8 ph = join8(hi), pl = join8(lo);
                     const int left = n - i * 32;
 #pragma unroll
-                    for (int nb = 0; nb < C::NB; nb++) {
-                        gu32x4 v[8];
-                        if constexpr (C::VE == 8) {
-                            if (nb == 0) lds_read8<0, CH * 256>(v, vt[0], vt[1], vt[2], vt[3]);
-                            else lds_read8<256, CH * 256 + 256>(v, vt[0], vt[1], vt[2], vt[3]);
-                        } else lds_read8h<CH * 256>(v, vt[0], vt[1], vt[2], vt[3]);
+                    for (int q = 0; q < (NO + 7) / 8; q++) {
+                        constexpr int NV = NO < 8 ? NO : 8;
+                        gu32x2 v[NV][2];
+                        if constexpr (NO < 8) lds_cols4<0, CH * 256>(v, vt);
+                        else if (q == 0) lds_cols8<0, CH * 256>(v, vt);
+                        else lds_cols8<256, CH * 256 + 256>(v, vt);
                         if (left < 32) {                 /* behind the run: may be anything */
 #pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                if (4 * g + (k & 3) + 16 * (k / 4) >= left) v[k] = (gu32x4){};
+                            for (int u = 0; u < 2; u++) {
+                                const int in = left - 16 * u - 4 * g;
+                                const unsigned m0 = in >= 2 ? ~0u : in == 1 ? 0xffffu : 0u, m1 = in >= 4 ? ~0u : in == 3 ? 0xffffu : 0u;
+#pragma unroll
+                                for (int z = 0; z < NV; z++) { v[z][u].x &= m0; v[z][u].y &= m1; }
+                            }
                         }
 #pragma unroll
-                        for (int e = 0; e < C::VE; e++) {
-                            gu32x4 x;
+                        for (int z = 0; z < NV; z += 4) {
+                            f32x4 *to = o + 8 * q + z;
+                            f16x8 vf[4];
 #pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                x[k] = __builtin_amdgcn_perm(v[2 * k + 1][e / 2], v[2 * k][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-                            const f16x8 vf = __builtin_bit_cast(f16x8, x);
-                            o[nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[nb * C::VE + e], 0, 0, 0);
-                            o[nb * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[nb * C::VE + e], 0, 0, 0);
+                            for (int y = 0; y < 4; y++)
+                                vf[y] = __builtin_bit_cast(f16x8, (gu32x4){ v[z + y][0].x, v[z + y][0].y, v[z + y][1].x, v[z + y][1].y });
+#pragma unroll
+                            for (int y = 0; y < 4; y++) to[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[y], ph, to[y], 0, 0, 0);
+#pragma unroll
+                            for (int y = 0; y < 4; y++) to[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[y], pl, to[y], 0, 0, 0);
                         }
                     }
                 }
+                }
+                pages(min(i0 + 4, last - 1), pg[0]);
+                pages(min(i0 + 5, last - 1), pg[1]);
             }
-            for (; i < last; i++) next(i);
         }
         if (bad && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
         const int slot = 2 * blockIdx.x + (first == 0);
         float sum = sum_g(l);
         if (bad) sum = NAN;
-        const int col = ri * A.hpb + ch;
-        if (on && !whole && g == 0) {
-            A.pm[slot * ROWS_COLS + col] = m;
-            A.pl[slot * ROWS_COLS + col] = sum;
+        if (whole) {
+            if (on)
+#pragma unroll
+                for (int k = 0; k < NO; k++) att_store(a, D, t0 + ri, h0 + ch, 16 * k + 4 * g, o[k], nc == 0 ? 1.0f : sum);
+        } else {                                       /* as the registers lie: the join needs no other order */
+            const size_t at = slot * ROWS_W + w;
+            if (g == 0) {
+                A.pm[at * 16 + c] = m;
+                A.pl[at * 16 + c] = sum;
+            }
+#pragma unroll
+            for (int k = 0; k < NO; k++) ((f32x4 *)A.po)[(at * NO + k) * 64 + lane] = o[k];
         }
-        if (on)
-#pragma unroll
-            for (int nb = 0; nb < C::NB; nb++)
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-#pragma unroll
-                    for (int e = 0; e < C::VE; e += 4) {
-                        f32x4 y;
-#pragma unroll
-                        for (int z = 0; z < 4; z++) y[z] = o[nb * C::VE + e + z][k];
-                        const int d = 16 * C::VE * nb + C::VE * (4 * g + k) + e;
-                        if (whole) att_store(a, D, t0 + ri, h0 + ch, d, y, nc == 0 ? 1.0f : sum);
-                        else *(f32x4 *)(A.po + ((size_t)slot * ROWS_COLS + col) * D + d) = y;
-                    }
         at += last - first;
         if (tid == 0 && at == end) {
             const RowsCut x = { t0, nr, hb, cuts ? (int)((at - last + tiles - 1) / share) - (int)blockIdx.x + 1 : 0 };
             A.cut[blockIdx.x] = x;
         }
         if (at >= end) break;
-        __builtin_amdgcn_s_waitcnt(ROWS_VMCNT(0));     /* no store is counted among the next unit's tiles */
         __syncthreads();                               /* the tiles in LDS are done with */
         first = 0;
         if (++hb == per_row) {
@@ -902,46 +933,52 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     }
 }
 
-/* The parts of a cut run's columns, D/4 lanes to a column. */
+/* The parts of a cut run, one wave's columns to a workgroup: a thread joins what one
+ * lane held of four sums, its column's elements 16 j + 4 g .. for four j. */
 template <int D>
-__global__ __launch_bounds__(ATT_T) void attn_rows_join_kernel(RowsArgs A)
+__global__ __launch_bounds__(D) void attn_rows_join_kernel(RowsArgs A)
 {
-    constexpr int L = D / 4;
+    constexpr int NO = D / 16;                         /* 64 threads for four sums */
     const RowsCut x = A.cut[blockIdx.x];
-    const int col = blockIdx.y * (ATT_T / L) + threadIdx.x / L, d = threadIdx.x % L * 4, g0 = blockIdx.x;
-    const int i = col / A.hpb, ch = col - i * A.hpb;
+    const int w = blockIdx.y, lane = threadIdx.x & 63, q = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, g0 = blockIdx.x;
+    const int cr = c / A.hpb, ch = c - cr * A.hpb, ri = w * A.rpg + cr;
     const int kh = x.hb / A.blocks, bk = x.hb - kh * A.blocks;
-    if (x.k == 0 || i >= x.n || ch >= A.group - bk * A.hpb) return;
+    if (x.k == 0 || cr >= A.rpg || ri >= x.n || ch >= A.group - bk * A.hpb) return;
     float m = -INFINITY, l = 0;
-    f32x4 y = {};
+    f32x4 y[4] = {};
     for (int k0 = 0; k0 < x.k; k0 += 4) {
         float pm[4], pl[4];
-        f32x4 po[4];
+        f32x4 po[4][4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int k = min(k0 + j, x.k - 1);
-            const size_t at = (size_t)(k ? 2 * (g0 + k) : 2 * g0 + 1) * ROWS_COLS + col;
-            pm[j] = k0 + j < x.k ? A.pm[at] : -INFINITY;
-            pl[j] = A.pl[at];
-            po[j] = *(const f32x4 *)(A.po + at * D + d);
+            const size_t at = (size_t)(k ? 2 * (g0 + k) : 2 * g0 + 1) * ROWS_W + w;
+            pm[j] = k0 + j < x.k ? A.pm[at * 16 + c] : -INFINITY;
+            pl[j] = A.pl[at * 16 + c];
+#pragma unroll
+            for (int z = 0; z < 4; z++) po[j][z] = ((const f32x4 *)A.po)[(at * NO + 4 * q + z) * 64 + lane];
         }
         float mn = m;
 #pragma unroll
         for (int j = 0; j < 4; j++) mn = fmaxf(mn, pm[j]);
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
-        y *= f;
+#pragma unroll
+        for (int z = 0; z < 4; z++) y[z] *= f;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (k0 + j >= x.k) continue;
-            const float w = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
-            l += pl[j] * w;
-            y += po[j] * w;
+            const float p = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
+            l += pl[j] * p;
+#pragma unroll
+            for (int z = 0; z < 4; z++) y[z] += po[j][z] * p;
         }
         m = mn;
     }
-    const int t = x.row + i;
-    att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, d, y, A.a.row_pos[t] == -1 ? 1.0f : l);
+    const int t = x.row + ri;
+    const float sum = A.a.row_pos[t] == -1 ? 1.0f : l;
+#pragma unroll
+    for (int z = 0; z < 4; z++) att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, 16 * (4 * q + z) + 4 * g, y[z], sum);
 }
 
 /* The parts of one cut unit's head, L lanes with four elements each to a part:
@@ -1029,7 +1066,7 @@ template <int D>
 static void rows_launch(const RowsArgs &A, int *err)
 {
     hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ROWS_T), 0, rt().stream, A, err);
-    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_G, ROWS_COLS * D / 4 / ATT_T), dim3(ATT_T), 0, rt().stream, A);
+    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_G, ROWS_W), dim3(D), 0, rt().stream, A);
 }
 
 template <int D, bool F16>

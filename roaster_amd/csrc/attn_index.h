@@ -21,10 +21,12 @@ struct KvShape {
 
     ATTN_FN bool page_ok(int p) const { return p >= 0 && p < n_pages; }
     ATTN_FN bool slot_ok(int s) const { return s >= 0 && (s >> shift) < n_pages; }
-    /* Element 0 of token `in` (0 .. page size - 1) of head h in page p. */
-    ATTN_FN size_t at(int p, int h, int in) const { return ((((size_t)p * kv + h) << shift) + in) * dim; }
+    /* Element 0 of token `in` (0 .. page size - 1) of head h in page p.  A page has at most
+     * 1024 heads of 4096 tokens of 256 elements: 2^30. */
+    ATTN_FN unsigned page_elements() const { return (unsigned)(kv << shift) * dim; }
+    ATTN_FN size_t at(int p, int h, int in) const { return (uint64_t)(unsigned)p * page_elements() + (unsigned)(((h << shift) + in) * dim); }
     ATTN_FN size_t at_slot(int s, int h) const { return at(s >> shift, h, s & ((1 << shift) - 1)); }
-    ATTN_FN size_t elements() const { return (((size_t)n_pages * kv) << shift) * dim; }
+    ATTN_FN size_t elements() const { return (size_t)n_pages * page_elements(); }
 };
 
 /* Block tables of n_req requests, max_pages entries each. */
