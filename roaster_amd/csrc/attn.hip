@@ -547,6 +547,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
 #define ROWS_COLS 128         /* columns of a unit: 16 a wave */
+#define ROWS_PART(D) (ROWS_COLS * (D) / 4 + 80)       /* a part in units of four sums, off a power of two: its unit's parts are read together */
 
 /* s_waitcnt's operand for no load and no store under way, LDS and exports not waited for. */
 #define ROWS_ALL_CAME ((7 << 4) | (15 << 8))
@@ -650,42 +651,84 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     constexpr int SW = CH < 16 ? CH : 16, KJ = SW / 4, VJ = SW / 2;
     __shared__ gu32x4 s_t[4][2][32 * CH];          /* tiles of keys and values: two in use, two under way */
     __shared__ long long s_wave[ROWS_W], s_at;
-    __shared__ int s_row, s_tiles;
+    __shared__ int s_row, s_tiles, s_parts;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
     const int per_row = A.s.kv * A.blocks, rows = a.rows;
 
+    /* this share: the tiles [at, end) of all units' laid end to end, or with few units one of
+     * np equal parts of one unit (a share that two units meet in begins twice) */
     const int each = (rows + ROWS_T - 1) / ROWS_T;
-    long long mine = 0, tot;
-    int tl = 0;
+    long long mine = 0, at = 0, end = 0, share = 1;
+    int tl = 0, np = 0, hb, first;
     for (int i = 0; i < each; i++) {
         const int t = tid * each + i;
         if (t < rows) mine += tl = rows_tiles(A, T, t);
     }
-    const long long upto = att_scan<ROWS_W>(mine, s_wave, tot);
-    const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
-    long long at = blockIdx.x * share;
-    const long long end = min(all, at + share);
-    if (at >= end) {
-        if (tid == 0) A.cut[blockIdx.x].k = 0;
-        return;
-    }
-    if (at < upto * per_row && at >= (upto - mine) * per_row) {
-        long long b = (upto - mine) * per_row;
-        int t = tid * each;
-        if (each > 1)
-            while (at >= b + (tl = rows_tiles(A, T, t)) * (long long)per_row) {
-                b += tl * (long long)per_row;
-                t++;
+    if (each == 1) {                                   /* at most 512 runs of at most 2^26 tiles: counts above bit 44 */
+        long long sum, parts;
+        (void)att_scan<ROWS_W>(mine | (long long)(tl > 0) << 44, s_wave, sum);
+        const int G = gridDim.x, units = (int)(sum >> 44) * per_row;
+        if (units > 0 && units <= G / 4) {
+            /* parts of S tiles: as small as they may be if their number then fits, else so that it
+             * must, a unit of n tiles having ceil(n / S) */
+            const long long W = (sum & ((1ll << 44) - 1)) * per_row;
+            const int lo = max(ATT_MIN, (int)((W + G - 1) / G)), hi = max(ATT_MIN, (int)((W + G - units - 1) / (G - units)));
+            const int p0 = (int)(((long long)tl + lo - 1) / lo), p1 = (int)(((long long)tl + hi - 1) / hi);
+            __syncthreads();                           /* s_wave is read */
+            const long long in = att_scan<ROWS_W>(p0 | (long long)p1 << 32, s_wave, parts);
+            const bool small = (parts & 0xffffffff) * per_row <= G;
+            const int mp = small ? p0 : p1, upto = (int)(small ? in & 0xffffffff : in >> 32), all = (int)(small ? parts & 0xffffffff : parts >> 32);
+            const int me = blockIdx.x;
+            if (me >= all * per_row) {
+                if (tid == 0) A.cut[me].k = 0;
+                return;
             }
-        s_row = t;
-        s_tiles = tl;
-        s_at = b;
+            if (me < upto * per_row && me >= (upto - mp) * per_row) {
+                s_row = tid;
+                s_tiles = tl;
+                s_parts = mp;
+                s_at = (upto - mp) * per_row;
+            }
+            __syncthreads();
+            np = uni(s_parts);
+            const int tiles = uni(s_tiles), k0 = me - (int)s_at;
+            hb = uni(k0 / np);
+            const int k = k0 - hb * np, base = uni(tiles / np), rem = tiles - base * np;
+            first = k * base + min(k, rem);
+            end = base + (k < rem);
+        }
+        __syncthreads();
     }
-    __syncthreads();
+    if (np == 0) {
+        long long tot;
+        const long long upto = att_scan<ROWS_W>(mine, s_wave, tot);
+        const long long all = tot * per_row;
+        share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
+        at = blockIdx.x * share;
+        end = min(all, at + share);
+        if (at >= end) {
+            if (tid == 0) A.cut[blockIdx.x].k = 0;
+            return;
+        }
+        if (at < upto * per_row && at >= (upto - mine) * per_row) {
+            long long b = (upto - mine) * per_row;
+            int t = tid * each;
+            if (each > 1)
+                while (at >= b + (tl = rows_tiles(A, T, t)) * (long long)per_row) {
+                    b += tl * (long long)per_row;
+                    t++;
+                }
+            s_row = t;
+            s_tiles = tl;
+            s_at = b;
+        }
+        __syncthreads();
+        hb = uni((int)((at - s_at) / s_tiles));
+        first = uni((int)((at - s_at) % s_tiles));
+    }
     int t1 = uni(s_row), tiles = uni(s_tiles);
-    int hb = uni((int)((at - s_at) / tiles)), first = uni((int)((at - s_at) % tiles));
     /* Where this lane's operands lie in a tile, in bytes: its key's piece 4 s + g at kb[s % KJ]
      * + 64 (s - s % KJ), its share of the values' 16 elements j at vb[j % VJ] + 32 (j - j % VJ):
      * four elements of token 4 g + c / 4.  (4 s + g) ^ r = 4 (s ^ r / 4) + (g ^ r % 4), and
@@ -899,7 +942,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             }
         }
         if (bad && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
-        const int slot = 2 * blockIdx.x + (first == 0);
+        const size_t slot = 2 * blockIdx.x + (first == 0);
         float sum = sum_g(l);
         if (bad) sum = NAN;
         if (whole) {
@@ -913,11 +956,11 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                 A.pl[at * 16 + c] = sum;
             }
 #pragma unroll
-            for (int k = 0; k < NO; k++) ((f32x4 *)A.po)[(at * NO + k) * 64 + lane] = o[k];
+            for (int k = 0; k < NO; k++) ((f32x4 *)A.po)[slot * ROWS_PART(D) + (w * NO + k) * 64 + lane] = o[k];
         }
         at += last - first;
         if (tid == 0 && at == end) {
-            const RowsCut x = { t0, nr, hb, cuts ? (int)((at - last + tiles - 1) / share) - (int)blockIdx.x + 1 : 0 };
+            const RowsCut x = { t0, nr, hb, !cuts ? 0 : np ? np : (int)((at - last + tiles - 1) / share) - (int)blockIdx.x + 1 };
             A.cut[blockIdx.x] = x;
         }
         if (at >= end) break;
@@ -934,39 +977,41 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 }
 
 /* The parts of a cut run, one wave's columns to a workgroup: a thread joins what one
- * lane held of four sums, its column's elements 16 j + 4 g .. for four j. */
+ * lane held of four sums, its column's elements 16 j + 4 g .. for four j.  The waves
+ * come first in the grid: with equal parts every eighth share, say, begins a unit, and
+ * the workgroups of those would all be on one XCD (38 us instead of 9). */
 template <int D>
 __global__ __launch_bounds__(D) void attn_rows_join_kernel(RowsArgs A)
 {
     constexpr int NO = D / 16;                         /* 64 threads for four sums */
-    const RowsCut x = A.cut[blockIdx.x];
-    const int w = blockIdx.y, lane = threadIdx.x & 63, q = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, g0 = blockIdx.x;
+    const RowsCut x = A.cut[blockIdx.y];
+    const int w = blockIdx.x, lane = threadIdx.x & 63, q = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, g0 = blockIdx.y;
     const int cr = c / A.hpb, ch = c - cr * A.hpb, ri = w * A.rpg + cr;
     const int kh = x.hb / A.blocks, bk = x.hb - kh * A.blocks;
     if (x.k == 0 || cr >= A.rpg || ri >= x.n || ch >= A.group - bk * A.hpb) return;
     float m = -INFINITY, l = 0;
     f32x4 y[4] = {};
-    for (int k0 = 0; k0 < x.k; k0 += 4) {
-        float pm[4], pl[4];
-        f32x4 po[4][4];
+    for (int k0 = 0; k0 < x.k; k0 += 8) {
+        float pm[8], pl[8];
+        f32x4 po[8][4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 8; j++) {
             const int k = min(k0 + j, x.k - 1);
-            const size_t at = (size_t)(k ? 2 * (g0 + k) : 2 * g0 + 1) * ROWS_W + w;
+            const size_t sl = k ? 2 * (g0 + k) : 2 * g0 + 1, at = sl * ROWS_W + w;
             pm[j] = k0 + j < x.k ? A.pm[at * 16 + c] : -INFINITY;
             pl[j] = A.pl[at * 16 + c];
 #pragma unroll
-            for (int z = 0; z < 4; z++) po[j][z] = ((const f32x4 *)A.po)[(at * NO + 4 * q + z) * 64 + lane];
+            for (int z = 0; z < 4; z++) po[j][z] = ((const f32x4 *)A.po)[sl * ROWS_PART(D) + (w * NO + 4 * q + z) * 64 + lane];
         }
         float mn = m;
 #pragma unroll
-        for (int j = 0; j < 4; j++) mn = fmaxf(mn, pm[j]);
+        for (int j = 0; j < 8; j++) mn = fmaxf(mn, pm[j]);
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
 #pragma unroll
         for (int z = 0; z < 4; z++) y[z] *= f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 8; j++) {
             if (k0 + j >= x.k) continue;
             const float p = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
             l += pl[j] * p;
@@ -1058,7 +1103,7 @@ extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCa
 {
     if (!attn_cache_ok(c) || rows < 0 || rows > (1 << 20) || q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads) return 0;
     const size_t one = ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * HPB * c->head_dim * 4,
-                 run = ROWS_CUT + 2 * ROWS_ML + (size_t)2 * ROWS_G * ROWS_COLS * c->head_dim * 4;
+                 run = ROWS_CUT + 2 * ROWS_ML + (size_t)2 * ROWS_G * ROWS_PART(c->head_dim) * 16;
     return rows_may(rows, c->type) && run > one ? run : one;
 }
 
@@ -1066,7 +1111,7 @@ template <int D>
 static void rows_launch(const RowsArgs &A, int *err)
 {
     hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ROWS_T), 0, rt().stream, A, err);
-    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_G, ROWS_W), dim3(D), 0, rt().stream, A);
+    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_W, ROWS_G), dim3(D), 0, rt().stream, A);
 }
 
 template <int D, bool F16>
