@@ -69,7 +69,7 @@ typedef struct {
     int n_req;                /* 1 .. 2048 */
     int page_size;            /* a power of two, 16 .. 4096 */
     int n_pages;              /* of the caches, and entries of the ring */
-    int max_pages;            /* entries of a table row; max_pages * page_size <= 2^31 - 1 */
+    int max_pages;            /* entries of a table row; max_pages * page_size <= 2^30 */
     int max_rows;             /* 1 .. 262144 */
     const int *len, *add;     /* [n_req] */
     int *len_out;             /* [n_req] */
@@ -110,7 +110,7 @@ typedef struct {
     float eps;
     int rot_dim;              /* a multiple of 8, 0 .. head_dim */
     int pair_adjacent;
-    double theta;             /* > 0 */
+    double theta;             /* 1 .. 1e30 */
     const int *row_pos, *row_slot;       /* [rows] */
     float *q_out;
 } RoasterQkRope;
@@ -126,9 +126,17 @@ int roaster_qk_rope_store(const RoasterQkRope *rope, const RoasterKvCache *cache
  * are a draft or a prompt's chunk.  row_pos[t] = -1: no position, out is 0.
  * row_req[t] = -1: the row is skipped, out untouched.  A request, position or
  * page number out of range gives that row NaN outputs and is reported.
- * Keys and values behind a row's position are never used, whatever they hold.
- * Sums and softmax are in 32 bits; with an fp16 cache the queries and
- * probabilities enter the products with 22 bits (two fp16 parts).
+ * Keys and values behind the positions that a request's rows of the call attend to
+ * are never used, whatever they hold; between a row's own position and the last of
+ * its request's rows in the call, values must be finite (they are multiplied by 0).
+ * Infinite or NaN keys and values in use make the elements that they reach
+ * infinite or NaN.  Sums and softmax are in 32 bits; with an fp16 cache the queries
+ * and probabilities enter the products with 22 bits (two fp16 parts).  How a call's
+ * work is split goes by all its rows: the last bits of a row's output depend on
+ * them, and are the same for the same call.
+ * An fp16 call of 16 rows or more, and of four times n_req or more, takes the rows
+ * of a request that stand together together (16 query heads on 2: 16 rows at a
+ * time); it is right, but slow, where most of its rows are one to a request.
  * gate: element d of head h of row t at [t * gate_row + h * gate_head + d].
  * out and ws must not overlap the inputs.  rows = 0 does nothing. */
 typedef struct {
@@ -137,7 +145,7 @@ typedef struct {
     const float *q;           /* [rows][q_heads][head_dim], 16-byte aligned */
     const int *row_req, *row_pos;        /* [rows] */
     const int *table;         /* [n_req][max_pages] */
-    int n_req, max_pages;
+    int n_req, max_pages;     /* max_pages * page_size <= 2^30 */
     float scale;
     const float *gate;        /* or NULL; 16-byte aligned, strides multiples of 4 */
     size_t gate_row, gate_head;

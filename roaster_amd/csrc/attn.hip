@@ -829,7 +829,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
         for (int k = 0; k < NO; k++) o[k] = (f32x4){};
         if (n > 0) {
-            int most = nc, least = nc > 0 ? nc : INT32_MAX;            /* over the wave's columns in use */
+            int most = nc, least = on ? nc : INT32_MAX;                /* over the wave's columns in use */
             for (int x = 32; x; x >>= 1) {
                 most = max(most, __shfl_xor(most, x));
                 least = min(least, __shfl_xor(least, x));
@@ -979,7 +979,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 /* The parts of a cut run, one wave's columns to a workgroup: a thread joins what one
  * lane held of four sums, its column's elements 16 j + 4 g .. for four j.  The waves
  * come first in the grid: with equal parts every eighth share, say, begins a unit, and
- * the workgroups of those would all be on one XCD (38 us instead of 9). */
+ * the workgroups of those would all be on one XCD (the join of 256 rows' parts 38 us
+ * instead of 14). */
 template <int D>
 __global__ __launch_bounds__(D) void attn_rows_join_kernel(RowsArgs A)
 {
@@ -1132,9 +1133,9 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     std::lock_guard<std::recursive_mutex> g(rt_lock());
     if (!attn_cache_ok(c)) return rt_fail(ROASTER_EINVAL, "roaster_attn_paged: bad cache description");
     if (!p || p->rows < 0 || p->rows > (1 << 20) || p->q_heads < 1 || p->q_heads > 1024 || p->q_heads % c->kv_heads ||
-        p->n_req < 1 || p->max_pages < 1 || (int64_t)p->max_pages * c->page_size > INT32_MAX || !(fabsf(p->scale) < INFINITY))
+        p->n_req < 1 || p->max_pages < 1 || (int64_t)p->max_pages * c->page_size > (1 << 30) || !(fabsf(p->scale) < INFINITY))
         return rt_fail(ROASTER_EINVAL, "roaster_attn_paged: need 0 <= rows <= 2^20, q_heads a multiple of kv_heads up to 1024, "
-                       "n_req >= 1, max_pages * page_size below 2^31, a finite scale");
+                       "n_req >= 1, max_pages * page_size at most 2^30, a finite scale");
     if (!p->rows) return 0;
     if (!p->q || !p->out || !p->row_req || !p->row_pos || !p->table || !attn_aligned(p->q, 16) || !attn_aligned(p->out, 16) ||
         !attn_aligned(p->row_req, 4) || !attn_aligned(p->row_pos, 4) || !attn_aligned(p->table, 4) ||

@@ -157,9 +157,9 @@ extern "C" int roaster_kv_plan(const RoasterKvPlan *p)
     std::lock_guard<std::recursive_mutex> g(rt_lock());
     if (!p || p->n_req < 1 || p->n_req > KVP_MAX_REQ || !attn_page_ok(p->page_size) || p->n_pages < 1 ||
         (int64_t)p->n_pages * p->page_size > INT32_MAX || p->max_pages < 1 ||
-        (int64_t)p->max_pages * p->page_size > INT32_MAX || p->max_rows < 1 || p->max_rows > KVP_MAX_ROWS)
+        (int64_t)p->max_pages * p->page_size > (1 << 30) || p->max_rows < 1 || p->max_rows > KVP_MAX_ROWS)
         return rt_fail(ROASTER_EINVAL, "roaster_kv_plan: need 1 <= n_req <= %d, 1 <= max_rows <= %d, page_size a power of two "
-                       "in 16..4096, and page_size times n_pages and max_pages below 2^31", KVP_MAX_REQ, KVP_MAX_ROWS);
+                       "in 16..4096, page_size * n_pages below 2^31, page_size * max_pages at most 2^30", KVP_MAX_REQ, KVP_MAX_ROWS);
     const void *at[] = { p->len, p->add, p->len_out, p->table, p->ring, p->ctl, p->ctl_out,
                          p->row_req, p->row_pos, p->row_slot, p->first };
     const size_t n4 = 4 * (size_t)p->n_req, r4 = 4 * (size_t)p->max_rows;
@@ -177,10 +177,12 @@ extern "C" int roaster_kv_plan(const RoasterKvPlan *p)
     const AttnDevice dev;
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
-    /* four rows a thread; where the outputs replace inputs that every workgroup
-     * reads, one workgroup, or for many rows a second launch for those outputs */
-    int blocks = (p->max_rows + 4 * KVP_T - 1) / (4 * KVP_T);
-    if (blocks > 256) blocks = 256;
+    /* a row a thread: a row's search and its page's load are one chain of waits (22700 rows of
+     * 512 requests 9.7 us with four rows a thread, 6.9 with one); where the outputs replace
+     * inputs that every workgroup reads, one workgroup, or for many rows a second launch for
+     * those outputs */
+    int blocks = (p->max_rows + KVP_T - 1) / KVP_T;
+    if (blocks > 1024) blocks = 1024;
     const bool in_place = p->len_out == p->len || p->ctl_out == p->ctl, two = in_place && blocks > 8;
     if (in_place && !two) blocks = 1;
     int shift = 0;

@@ -117,9 +117,9 @@ extern "C" int roaster_qk_rope_store(const RoasterQkRope *p, const RoasterKvCach
     if (!attn_cache_ok(c)) return rt_fail(ROASTER_EINVAL, "roaster_qk_rope_store: bad cache description");
     const int D = c->head_dim;
     if (!p || p->rows < 0 || p->rows > (1 << 20) || p->q_heads < 1 || p->q_heads > 1024 || p->rot_dim < 0 ||
-        p->rot_dim > D || p->rot_dim % 8 || !(p->theta > 0) || !(p->theta < 1e30))
+        p->rot_dim > D || p->rot_dim % 8 || !(p->theta >= 1) || !(p->theta <= 1e30))
         return rt_fail(ROASTER_EINVAL, "roaster_qk_rope_store: need 0 <= rows <= 2^20, 1 <= q_heads <= 1024, rot_dim a multiple "
-                       "of 8 up to head_dim, theta > 0");
+                       "of 8 up to head_dim, 1 <= theta <= 1e30");
     if (!p->rows) return 0;
     const void *at[] = { p->q, p->k, p->v, p->q_out };
     const size_t str[] = { p->q_row, p->q_head, p->k_row, p->k_head, p->v_row, p->v_head };

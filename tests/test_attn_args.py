@@ -68,7 +68,7 @@ def test_good_arguments_come_as_far_as_the_device():
 
 @pytest.mark.parametrize("kw", [
     dict(n_req=0), dict(n_req=2049), dict(max_rows=0), dict(max_rows=(1 << 18) + 1), dict(page_size=8), dict(page_size=48),
-    dict(page_size=8192), dict(n_pages=0), dict(n_pages=1 << 25), dict(max_pages=0), dict(max_pages=1 << 25),
+    dict(page_size=8192), dict(n_pages=0), dict(n_pages=1 << 25), dict(max_pages=0), dict(max_pages=(1 << 24) + 1),
     dict(len=None), dict(add=None), dict(len_out=None), dict(table=None), dict(ring=None), dict(ctl=None),
     dict(ctl_out=None), dict(row_req=None), dict(row_pos=None), dict(row_slot=None), dict(len=mem(3) + 2),
     dict(ctl=mem(8) + 4), dict(len_out=mem(3) + 4), dict(ctl_out=mem(8) + 8), dict(table=mem(7)), dict(first=mem(4) + 28),
@@ -91,7 +91,7 @@ def test_cache_refused(kw):
 
 @pytest.mark.parametrize("kw", [
     dict(rows=-1), dict(rows=(1 << 20) + 1), dict(q_heads=0), dict(q_heads=1025), dict(rot_dim=-8), dict(rot_dim=12),
-    dict(rot_dim=264), dict(theta=0.0), dict(theta=-1.0), dict(theta=float("nan")), dict(theta=float("inf")), dict(q=None),
+    dict(rot_dim=264), dict(theta=0.0), dict(theta=-1.0), dict(theta=0.5), dict(theta=float("nan")), dict(theta=float("inf")), dict(q=None),
     dict(k=None), dict(v=None), dict(q_out=None), dict(q=mem(3) + 4), dict(v=mem(5) + 8), dict(q_out=mem(10) + 4),
     dict(q_row=4098), dict(k_head=255), dict(v_row=1 << 40), dict(row_pos=None), dict(row_slot=None),
     dict(row_pos=mem(8) + 1), dict(q_norm=mem(6) + 4), dict(q_out=mem(3)), dict(q_out=mem(3) + 4096), dict(q_out=mem(4)),
@@ -106,7 +106,7 @@ def test_rope_refuses_keys_over_values():
 
 @pytest.mark.parametrize("kw", [
     dict(rows=-1), dict(rows=(1 << 20) + 1), dict(q_heads=0), dict(q_heads=17), dict(q_heads=1026), dict(n_req=0),
-    dict(max_pages=0), dict(max_pages=1 << 25), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
+    dict(max_pages=0), dict(max_pages=(1 << 24) + 1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
     dict(row_req=None), dict(row_pos=None), dict(table=None), dict(out=None), dict(q=mem(3) + 8), dict(out=mem(8) + 4),
     dict(table=mem(6) + 2), dict(gate=mem(7) + 4), dict(gate_row=8190), dict(gate_head=510), dict(gate_row=1 << 40),
     dict(ws=None), dict(ws=mem(9) + 8), dict(ws_bytes=0), dict(out=mem(3)), dict(out=mem(1)), dict(ws=mem(2)),

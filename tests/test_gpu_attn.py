@@ -105,6 +105,7 @@ CHUNKS = [
     ([900], [(0, p) for p in range(644, 900)]),                                       # a chunk behind a context
     ([70, 200, 33], [(0, p) for p in range(60, 70)] + [(1, p) for p in range(100, 200)] + [(2, p) for p in range(33)]),
     ([40, 50], [(0, 39), (1, 49), (0, 38), (1, 3), (-1, -1), (0, 5), (0, 5), (1, -1), (0, 39)]),      # no order at all
+    ([200], [(0, -1), (0, -1), (0, 100), (0, 150)] + [(0, -1)] + [(0, p) for p in range(120, 140)] + [(0, 7)]),
     ([120, 64], [(0, p) for p in range(100, 120)] + [(-1, -1)] * 5 + [(1, p) for p in range(60, 64)] + [(-1, -1)] * 40),
 ]
 
