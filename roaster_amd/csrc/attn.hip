@@ -55,10 +55,12 @@ struct AttArgs {
 
 template <int D, bool F16>
 struct AttCfg {
-    static constexpr int TT = 16, SUB = 1, SZ = F16 ? 2 : 4;
+    static constexpr int TT = 16, SZ = F16 ? 2 : 4;                  /* tokens of a tile */
     static constexpr int VE = F16 ? (D >= 128 ? 8 : 4) : 4;       /* elements of a value load */
     static constexpr int NB = D / (16 * VE);                        /* value loads of a token */
-    static constexpr int KS = F16 ? D / 32 : D / 16;                 /* 16-byte key loads of a token */
+    static constexpr int NCH = D * SZ / 16;                          /* 16-byte pieces of a token's key */
+    static constexpr int KS = NCH / 4;                               /* key loads of a tile, and operands of a score */
+    static constexpr int SW = NCH < 16 ? NCH : 16;
     static constexpr int VT = 4;                                     /* tokens of a lane's value operand */
     static constexpr int LD = D + 4;                                 /* LDS row */
 };
@@ -125,7 +127,7 @@ struct AttWave {
     float fac;                      /* log2 score of a product */
     float m, l;
     f32x4 o[C::NB * C::VE];
-    gu32x4 k[C::SUB][C::KS];
+    gu32x4 k[C::KS];
     gu32x4 v[C::VT][C::NB];
 
     /* The unit's queries as they lie: column c's head (a column without one computes
@@ -158,20 +160,30 @@ struct AttWave {
             for (int s = 0; s < C::KS; s++) qf[s] = (f32x4){ r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w };
         }
     }
-    /* Keys of the tile whose 16-token parts begin at at[] (bytes, uniform). */
-    __device__ void load_k(const char *kc, const size_t *at, int c, int g)
+    /* Keys of the tile that begins at byte `at`, a kilobyte to a load: with 64 bytes of each
+     * of 16 tokens to a load, as the products take them, they come at 5.9 TB/s, so at 6.8. */
+    __device__ void load_k(const char *kc, size_t at, int lane)
     {
-        for (int u = 0; u < C::SUB; u++) {
-            const char *b = kc + at[u];
-            const unsigned off = c * D * C::SZ + g * 16;
-            for (int s = 0; s < C::KS; s++) k[u][s] = __builtin_nontemporal_load((const GAS gu32x4 *)(b + off + 64 * s));
+#pragma unroll
+        for (int i = 0; i < C::KS; i++) k[i] = __builtin_nontemporal_load((const GAS gu32x4 *)(kc + at + (i * 64 + lane) * 16));
+    }
+    /* The keys through this wave's own LDS into the products' order: piece x of token r lies
+     * at x ^ (r % SW). */
+    __device__ void store_k(gu32x4 *t, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < C::KS; i++) {
+            const int r = (i * 64 + lane) / C::NCH, x = lane % C::NCH;
+            t[r * C::NCH + (x ^ r % C::SW)] = k[i];
         }
     }
-    __device__ void load_v(const char *vc, const size_t *at, int c, int g)
+    __device__ void load_v(const char *vc, size_t at, int c, int g)
     {
+#pragma unroll
         for (int j = 0; j < C::VT; j++) {
-            const char *b = vc + at[j / 4];
-            const unsigned off = ((4 * g + (j & 3)) * D + C::VE * c) * C::SZ;
+            const char *b = vc + at;
+            const unsigned off = ((4 * g + j) * D + C::VE * c) * C::SZ;
+#pragma unroll
             for (int n = 0; n < C::NB; n++) {
                 const GAS char *p = (const GAS char *)(b + off + 16 * C::VE * C::SZ * n);
                 if (C::VE * C::SZ == 16) v[j][n] = __builtin_nontemporal_load((const GAS gu32x4 *)p);
@@ -182,21 +194,21 @@ struct AttWave {
             }
         }
     }
-    /* Scores of the tile in k: a lane gets VT tokens of its column, those at 4g + j % 4 of part j / 4. */
-    __device__ void scores(float *s)
+    /* Scores of the tile in t: a lane gets its column's for tokens 4 g .. */
+    __device__ void scores(float *s, const gu32x4 *t, int c, int g)
     {
-        for (int u = 0; u < C::SUB; u++) {
-            f32x4 a = {};
-            if (F16)
-                for (int i = 0; i < C::KS; i++)
-                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[u][i]), qh[i], a, 0, 0, 0);
+        f32x4 a = {};
+#pragma unroll
+        for (int i = 0; i < C::KS; i++) {
+            const gu32x4 x = t[c * C::NCH + ((4 * i + g) ^ c % C::SW)];
+            if (F16) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), qh[i], a, 0, 0, 0);
             else
-                for (int i = 0; i < C::KS; i++) {
-                    const f32x4 x = __builtin_bit_cast(f32x4, k[u][i]);
-                    for (int j = 0; j < 4; j++) a = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], qf[i][j], a, 0, 0, 0);
-                }
-            for (int j = 0; j < 4; j++) s[4 * u + j] = F16 ? a[j] + dpp_f<0x128>(a[j]) : a[j];     /* row_ror:8: the other part's column */
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    a = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, x)[j], qf[i][j], a, 0, 0, 0);
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] = F16 ? a[j] + dpp_f<0x128>(a[j]) : a[j];     /* row_ror:8: the other part's column */
     }
     /* The tile's softmax terms, p in place of the scores; `left` tokens of the tile count. */
     __device__ void soften(float *s, int left, int g)
@@ -302,9 +314,13 @@ __device__ __forceinline__ int att_tiles(const KvTable &T, int req, int pos, int
     return n <= TT ? 1 : (int)(((long long)n + TT - 1) / TT);
 }
 
-template <int D>
+/* A wave's share holds its tile's keys, after its last tile its sums [HPB][D + 4]. */
+template <int D, bool F16>
 struct AttLds {
-    float o[ATT_W][HPB][D + 4], m[ATT_W][HPB], l[ATT_W][HPB];
+    static constexpr int KEYS = 16 * D * (F16 ? 2 : 4), SUMS = HPB * (D + 4) * 4;
+    gu32x4 own[ATT_W][(KEYS > SUMS ? KEYS : SUMS) / 16];
+    float m[ATT_W][HPB], l[ATT_W][HPB];
+    __device__ float *sums(int w, int h) { return (float *)own[w] + h * (D + 4); }
 };
 
 /* out of one row's head from the sums y and l, four elements at d.  The reciprocals
@@ -324,7 +340,7 @@ __device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int 
 /* Tiles [first, last) of unit (t, hb) by one workgroup: to out if that is all of
  * them, else to part `slot`. */
 template <int D, bool F16>
-__device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *err, int t, int req, int pos, int hb, int first,
+__device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16> &S, int *err, int t, int req, int pos, int hb, int first,
                                          int last, bool whole, int slot)
 {
     using C = AttCfg<D, F16>;
@@ -336,46 +352,34 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *er
     bool bad = n < 0;
     AttWave<D, F16> wv;
     typename AttWave<D, F16>::Raw raw;
-    /* page numbers of tile i's 16-token parts (a part past the row's end repeats the
-     * first), then the bytes at which the parts begin */
-    auto pages = [&](int i, int *p) {
-#pragma unroll
-        for (int u = 0; u < C::SUB; u++) {
-            const int tok = i * C::TT + 16 * u;
-            p[u] = u && tok >= n ? p[0] : a.table[T.entry(req, tok, shift)];
-        }
-    };
-    auto where = [&](int i, const int *p, size_t *b) {
-#pragma unroll
-        for (int u = 0; u < C::SUB; u++) {
-            const int tok = i * C::TT + 16 * u;
-            int pg = uni(p[u]);
-            if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
-            b[u] = A.s.at(pg, kh, (u && tok >= n ? i * C::TT : tok) & ((1 << shift) - 1)) * C::SZ;
-        }
+    /* the page of tile i, then the byte at which the tile begins */
+    auto page = [&](int i) { return a.table[T.entry(req, i * 16, shift)]; };
+    auto where = [&](int i, int p) {
+        int pg = uni(p);
+        if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
+        return A.s.at(pg, kh, i * 16 & ((1 << shift) - 1)) * C::SZ;
     };
     wv.clear();
     int i = first + w;
     if (n > 0 && i < last) {
-        int p[C::SUB], i2 = i + ATT_W;
-        size_t b[C::SUB];
-        pages(i, p);
+        int p = page(i), i2 = i + ATT_W;
         wv.load_q(raw, a.q + ((size_t)t * a.q_heads + h0) * D, c, g, nh);
-        where(i, p, b);
-        wv.load_k(A.kc, b, c, g);
-        if (i2 < last) pages(i2, p);
+        size_t b = where(i, p);
+        wv.load_k(A.kc, b, lane);
+        if (i2 < last) p = page(i2);
         wv.load_v(A.vc, b, c, g);
         wv.begin(raw, c, a.scale);
         while (1) {
-            const int left = n - i * C::TT;
+            const int left = n - i * 16;
             const bool more = i2 < last;
             float s[C::VT];
-            wv.scores(s);
+            wv.store_k(S.own[w], lane);
             if (more) {
-                where(i2, p, b);
-                wv.load_k(A.kc, b, c, g);
-                if (i2 + ATT_W < last) pages(i2 + ATT_W, p);
+                b = where(i2, p);
+                wv.load_k(A.kc, b, lane);
+                if (i2 + ATT_W < last) p = page(i2 + ATT_W);
             }
+            wv.scores(s, S.own[w], c, g);
             wv.soften(s, left, g);
             wv.values(s, left, c, g);
             if (!more) break;
@@ -394,7 +398,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *er
             if (c < HPB)
 #pragma unroll
                 for (int e = 0; e < C::VE; e += 4)
-                    *(float4 *)&S.o[w][c][16 * C::VE * b + C::VE * (4 * g + i) + e] =
+                    *(float4 *)(S.sums(w, c) + 16 * C::VE * b + C::VE * (4 * g + i) + e) =
                         make_float4(wv.o[b * C::VE + e][i], wv.o[b * C::VE + e + 1][i], wv.o[b * C::VE + e + 2][i],
                                     wv.o[b * C::VE + e + 3][i]);
     const bool any = __syncthreads_or(bad);
@@ -409,7 +413,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D> &S, int *er
         for (int i = 0; i < ATT_W; i++) {
             const float f = S.m[i][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(S.m[i][h] - mx);
             sum += S.l[i][h] * f;
-            y += *(const f32x4 *)&S.o[i][h][d] * f;
+            y += *(const f32x4 *)(S.sums(i, h) + d) * f;
         }
         if (any) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
         if (whole) att_store(a, D, t, h0 + h, d, y, n == 0 ? 1.0f : sum);      /* without positions: y is 0 */
@@ -431,7 +435,7 @@ template <int D, bool F16>
 __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kernel(AttArgs A, int *err)
 {
     using C = AttCfg<D, F16>;
-    __shared__ AttLds<D> S;
+    __shared__ AttLds<D, F16> S;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int lane = threadIdx.x & 63, shift = A.s.shift, rows = a.rows, per_row = A.s.kv * A.blocks;
@@ -473,7 +477,7 @@ template <int D, bool F16>
 __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(AttArgs A, int *err)
 {
     using C = AttCfg<D, F16>;
-    __shared__ AttLds<D> S;
+    __shared__ AttLds<D, F16> S;
     __shared__ long long s_wave[ATT_W], s_at;
     __shared__ int s_row;
     const RoasterAttnPaged &a = A.a;
