@@ -640,12 +640,15 @@ __device__ __forceinline__ RowsAt rows_at(const RowsArgs &A, const KvTable &T, i
     x.joined = t % A.R && r == x.req && n >= 0 && n <= x.n;
     return x;
 }
-/* Tiles of the run that ends with row t, 0 if none does. */
+/* Tiles of the run that ends with row x, 0 if none does: its request is none or it goes on. */
+__device__ __forceinline__ int rows_tiles(const RowsAt &x, bool goes_on)
+{
+    if (x.req == -1 || goes_on) return 0;
+    return x.n <= 32 ? 1 : (int)(((long long)x.n + 31) / 32);
+}
 __device__ __forceinline__ int rows_tiles(const RowsArgs &A, const KvTable &T, int t)
 {
-    const RowsAt x = rows_at(A, T, t), y = rows_at(A, T, min(t + 1, A.a.rows - 1));
-    if (x.req == -1 || (t + 1 < A.a.rows && y.joined)) return 0;
-    return x.n <= 32 ? 1 : (int)(((long long)x.n + 31) / 32);
+    return rows_tiles(rows_at(A, T, t), t + 1 < A.a.rows && rows_at(A, T, min(t + 1, A.a.rows - 1)).joined);
 }
 
 template <int D>
@@ -655,7 +658,10 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     constexpr int SW = CH < 16 ? CH : 16, KJ = SW / 4, VJ = SW / 2;
     __shared__ gu32x4 s_t[4][2][32 * CH];          /* tiles of keys and values: two in use, two under way */
     __shared__ long long s_wave[ROWS_W], s_at;
-    __shared__ int s_row, s_tiles, s_parts;
+    __shared__ int s_row, s_tiles, s_np, s_runs[ROWS_W];
+    __shared__ unsigned s_parts[ROWS_W];
+    __shared__ unsigned long long s_join[ROWS_W];          /* the rows that go on with a run, a bit each */
+    __shared__ float s_sum[ROWS_W];
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
@@ -666,45 +672,70 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     const int each = (rows + ROWS_T - 1) / ROWS_T;
     long long mine = 0, at = 0, end = 0, share = 1;
     int tl = 0, np = 0, hb, first;
-    for (int i = 0; i < each; i++) {
-        const int t = tid * each + i;
-        if (t < rows) mine += tl = rows_tiles(A, T, t);
-    }
-    if (each == 1) {                                   /* at most 512 runs of at most 2^26 tiles: counts above bit 44 */
-        long long sum, parts;
-        (void)att_scan<ROWS_W>(mine | (long long)(tl > 0) << 44, s_wave, sum);
-        const int G = gridDim.x, units = (int)(sum >> 44) * per_row;
+    if (each == 1) {                                   /* at most 512 runs, one a thread */
+        const int G = gridDim.x, t = min(tid, rows - 1);
+        const RowsAt x = rows_at(A, T, t), y = rows_at(A, T, min(t + 1, rows - 1));
+        if (tid < rows) mine = tl = rows_tiles(x, t + 1 < rows && y.joined);
+        const float some = group_sum<64>((float)tl);
+        const unsigned long long on = __ballot(x.joined), runs = __ballot(tl > 0);
+        if (lane == 0) {
+            s_sum[w] = some;
+            s_runs[w] = __popcll(runs);
+            s_join[w] = on;
+        }
+        __syncthreads();
+        float W = 0;
+        int units = 0;
+#pragma unroll
+        for (int i = 0; i < ROWS_W; i++) { W += s_sum[i]; units += s_runs[i]; }
+        W *= per_row;
+        units *= per_row;
         if (units > 0 && units <= G / 4) {
-            /* parts of S tiles: as small as they may be if their number then fits, else so that it
-             * must, a unit of n tiles having ceil(n / S) */
-            const long long W = (sum & ((1ll << 44) - 1)) * per_row;
-            const int lo = max(ATT_MIN, (int)((W + G - 1) / G)), hi = max(ATT_MIN, (int)((W + G - units - 1) / (G - units)));
-            const int p0 = (int)(((long long)tl + lo - 1) / lo), p1 = (int)(((long long)tl + hi - 1) / hi);
-            __syncthreads();                           /* s_wave is read */
-            const long long in = att_scan<ROWS_W>(p0 | (long long)p1 << 32, s_wave, parts);
-            const bool small = (parts & 0xffffffff) * per_row <= G;
-            const int mp = small ? p0 : p1, upto = (int)(small ? in & 0xffffffff : in >> 32), all = (int)(small ? parts & 0xffffffff : parts >> 32);
-            const int me = blockIdx.x;
-            if (me >= all * per_row) {
+            /* parts of S tiles: as small as all tiles over all workgroups if there are then not
+             * too many, else so that there cannot be, a unit of n tiles having ceil(n / S) (the
+             * quotients in f32: `hi` is taken a little too large) */
+            const unsigned lo = max(ATT_MIN, (int)ceilf(W / G)), hi = max(ATT_MIN, (int)(W * 1.0001f / (G - units)) + 1);
+            const unsigned p0 = (tl + lo - 1) / lo, p1 = (tl + hi - 1) / hi;
+            /* at most G + 512 and G parts, so both fit one word */
+            unsigned in = p0 | p1 << 16;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const unsigned u = __shfl_up(in, o);
+                if (lane >= o) in += u;
+            }
+            if (lane == 63) s_parts[w] = in;
+            __syncthreads();
+            unsigned all = 0;
+#pragma unroll
+            for (int i = 0; i < ROWS_W; i++) {
+                if (i == w) in += all;
+                all += s_parts[i];
+            }
+            const bool small = (int)(all & 0xffff) * per_row <= G;
+            const int mp = small ? p0 : p1, upto = small ? in & 0xffff : in >> 16, me = blockIdx.x;
+            if (me >= (int)(small ? all & 0xffff : all >> 16) * per_row) {
                 if (tid == 0) A.cut[me].k = 0;
                 return;
             }
             if (me < upto * per_row && me >= (upto - mp) * per_row) {
                 s_row = tid;
                 s_tiles = tl;
-                s_parts = mp;
+                s_np = mp;
                 s_at = (upto - mp) * per_row;
             }
             __syncthreads();
-            np = uni(s_parts);
+            np = uni(s_np);
             const int tiles = uni(s_tiles), k0 = me - (int)s_at;
             hb = uni(k0 / np);
             const int k = k0 - hb * np, base = uni(tiles / np), rem = tiles - base * np;
             first = k * base + min(k, rem);
             end = base + (k < rem);
         }
-        __syncthreads();
-    }
+    } else
+        for (int i = 0; i < each; i++) {
+            const int t = tid * each + i;
+            if (t < rows) mine += tl = rows_tiles(A, T, t);
+        }
     if (np == 0) {
         long long tot;
         const long long upto = att_scan<ROWS_W>(mine, s_wave, tot);
@@ -748,14 +779,20 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     while (1) {
         const int last = uni((int)min((long long)tiles, first + (end - at)));
         const bool whole = first == 0 && last == tiles, cuts = first == 0 && !whole;
-        /* the run's first row: as many rows back as go on with the one before them, 64 at a time */
+        /* the run's first row: the last one up to t1 that does not go on with the one before it */
         int t0 = t1;
-        for (bool on = true; on;) {
-            const int t = t0 - lane;
-            const unsigned long long j = __ballot(t > 0 && rows_at(A, T, t).joined);
-            on = j == ~0ull;
-            t0 -= on ? 64 : __builtin_ctzll(~j);
-        }
+        if (each == 1) {
+            int k = t1 >> 6;
+            unsigned long long j = ~s_join[k] & (~0ull >> (63 - (t1 & 63)));
+            while (!j) j = ~s_join[--k];               /* row 0 goes on with none */
+            t0 = uni(64 * k + 63 - __builtin_clzll(j));
+        } else
+            for (bool on = true; on;) {                /* 64 rows at a time */
+                const int t = t0 - lane;
+                const unsigned long long j = __ballot(t > 0 && rows_at(A, T, t).joined);
+                on = j == ~0ull;
+                t0 -= on ? 64 : __builtin_ctzll(~j);
+            }
         const int nr = t1 - t0 + 1, req = uni(a.row_req[t1]), n = uni(T.tokens(req, a.row_pos[t1], shift));
         const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(A.hpb, A.group - bk * A.hpb);
         const int h0 = kh * A.group + bk * A.hpb;
@@ -980,17 +1017,17 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     }
 }
 
-/* The parts of a cut run, one wave's columns to a workgroup: a thread joins what one
- * lane held of four sums, its column's elements 16 j + 4 g .. for four j.  The waves
+/* The parts of a cut run, four sums of one wave's lanes to a workgroup of one wave: a
+ * thread joins what one lane held, its column's elements 16 j + 4 g .. for four j.  The waves
  * come first in the grid: with equal parts every eighth share, say, begins a unit, and
  * the workgroups of those would all be on one XCD (the join of 256 rows' parts 38 us
  * instead of 14). */
 template <int D>
-__global__ __launch_bounds__(D) void attn_rows_join_kernel(RowsArgs A)
+__global__ __launch_bounds__(64) void attn_rows_join_kernel(RowsArgs A)
 {
-    constexpr int NO = D / 16;                         /* 64 threads for four sums */
+    constexpr int NO = D / 16;
     const RowsCut x = A.cut[blockIdx.y];
-    const int w = blockIdx.x, lane = threadIdx.x & 63, q = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, g0 = blockIdx.y;
+    const int w = blockIdx.x / (NO / 4), q = blockIdx.x % (NO / 4), lane = threadIdx.x, c = lane & 15, g = lane >> 4, g0 = blockIdx.y;
     const int cr = c / A.hpb, ch = c - cr * A.hpb, ri = w * A.rpg + cr;
     const int kh = x.hb / A.blocks, bk = x.hb - kh * A.blocks;
     if (x.k == 0 || cr >= A.rpg || ri >= x.n || ch >= A.group - bk * A.hpb) return;
@@ -1116,7 +1153,7 @@ template <int D>
 static void rows_launch(const RowsArgs &A, int *err)
 {
     hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ROWS_T), 0, rt().stream, A, err);
-    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_W, ROWS_G), dim3(D), 0, rt().stream, A);
+    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_W * D / 64, ROWS_G), dim3(64), 0, rt().stream, A);
 }
 
 template <int D, bool F16>
