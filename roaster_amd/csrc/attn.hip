@@ -305,6 +305,13 @@ __device__ __forceinline__ long long att_scan(long long v, long long *s_wave, lo
     return v + before;
 }
 
+/* What beginning a unit costs, in tiles, where shares are made equal: its row, page and
+ * queries have to come before its first keys, and its sums go through LDS (700 requests of 1
+ * to 500 tokens 82 us without it, 47 with it).  A unit of n tiles lies on LEAD + n
+ * places, its tiles on the last n. */
+#define ATT_LEAD 8
+#define ROWS_LEAD 4           /* of 32 tokens */
+
 /* Tiles of a row: at least one for a row that has an output to write. */
 template <int TT>
 __device__ __forceinline__ int att_tiles(const KvTable &T, int req, int pos, int shift)
@@ -484,12 +491,16 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, shift = A.s.shift, per_row = A.s.kv * A.blocks, rows = a.rows;
 
-    /* this share: where it begins in all units' tiles laid end to end */
+    /* this share: the places [at, end) of all units' laid end to end */
     const int each = (rows + ATT_T - 1) / ATT_T;
+    auto places = [&](int t) {
+        const int k = att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift);
+        return k ? ATT_LEAD + k : 0;
+    };
     long long mine = 0, tot;
     for (int i = 0; i < each; i++) {
         const int t = tid * each + i;
-        if (t < rows) mine += att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift);
+        if (t < rows) mine += places(t);
     }
     const long long upto = att_scan<ATT_W>(mine, s_wave, tot);
     const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
@@ -502,7 +513,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
     if (at < upto * per_row && at >= (upto - mine) * per_row) {        /* one thread's rows hold it */
         long long b = (upto - mine) * per_row;
         int t = tid * each, n;
-        while (at >= b + (n = att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift)) * (long long)per_row) {
+        while (at >= b + (n = places(t)) * (long long)per_row) {
             b += n * (long long)per_row;
             t++;
         }
@@ -512,26 +523,38 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
     __syncthreads();
     int t = uni(s_row), req = uni(a.row_req[t]), pos = uni(a.row_pos[t]);
     int tiles = att_tiles<C::TT>(T, req, pos, shift);
-    int hb = uni((int)((at - s_at) / tiles)), first = uni((int)((at - s_at) % tiles));
+    int hb = uni((int)((at - s_at) / (ATT_LEAD + tiles))), x0 = uni((int)((at - s_at) % (ATT_LEAD + tiles)));
     while (1) {
-        const int last = uni((int)min((long long)tiles, first + (end - at)));       /* tiles [first, last) of unit (t, hb) */
-        const bool whole = first == 0 && last == tiles, cuts = first == 0 && !whole;
-        att_part<D, F16>(A, S, err, t, req, pos, hb, first, last, whole, 2 * blockIdx.x + (first == 0));
-        if (tid == 0) {                                /* for the join: the shares of a unit begun and cut here */
-            const int k = cuts ? (int)((at + tiles - 1) / share) - (int)blockIdx.x + 1 : 0;
-            if (A.by_unit && first == 0) A.cut[t * per_row + hb] = make_int2(blockIdx.x, k);
-            if (!A.by_unit && at + (last - first) == end) A.cut[blockIdx.x] = make_int2(t * per_row + hb, k);
+        /* places [x0, x1) and tiles [first, last) of unit (t, hb) */
+        const int x1 = uni((int)min((long long)ATT_LEAD + tiles, x0 + (end - at)));
+        const int first = max(0, x0 - ATT_LEAD), last = max(0, x1 - ATT_LEAD);
+        const bool cuts = first == 0 && last > 0 && last < tiles, over = at + (x1 - x0) == end;
+        const bool step = !over && hb + 1 == per_row;
+        int req1 = -1, pos1 = 0;
+        if (step) {                                    /* the next row, while this one is worked on */
+            req1 = a.row_req[t + 1];
+            pos1 = a.row_pos[t + 1];
         }
-        at += last - first;
-        if (at >= end) break;
-        first = 0;
-        if (++hb == per_row) {
+        if (last > first) att_part<D, F16>(A, S, err, t, req, pos, hb, first, last, first == 0 && last == tiles, 2 * blockIdx.x + (first == 0));
+        if (tid == 0) {                                /* for the join: the shares of a unit begun and cut here */
+            const int k = cuts ? (int)((at - x0 + ATT_LEAD + tiles - 1) / share) - (int)blockIdx.x + 1 : 0;
+            if (A.by_unit && first == 0 && last > 0) A.cut[t * per_row + hb] = make_int2(blockIdx.x, k);
+            if (!A.by_unit && over) A.cut[blockIdx.x] = make_int2(t * per_row + hb, k);
+        }
+        if (over) break;
+        at += x1 - x0;
+        x0 = 0;
+        hb++;
+        if (step) {
             hb = 0;
-            do {
+            t++;
+            req = uni(req1);
+            pos = uni(pos1);
+            while (req == -1) {
                 t++;
                 req = uni(a.row_req[t]);
-            } while (req == -1);
-            pos = uni(a.row_pos[t]);
+                pos = uni(a.row_pos[t]);
+            }
             tiles = att_tiles<C::TT>(T, req, pos, shift);
         }
         __syncthreads();                               /* S is free again */
@@ -671,11 +694,13 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
      * np equal parts of one unit (a share that two units meet in begins twice) */
     const int each = (rows + ROWS_T - 1) / ROWS_T;
     long long mine = 0, at = 0, end = 0, share = 1;
-    int tl = 0, np = 0, hb, first;
+    int tl = 0, np = 0, hb, x0;
+    auto places = [](int k) { return k ? ROWS_LEAD + k : 0; };
     if (each == 1) {                                   /* at most 512 runs, one a thread */
         const int G = gridDim.x, t = min(tid, rows - 1);
         const RowsAt x = rows_at(A, T, t), y = rows_at(A, T, min(t + 1, rows - 1));
-        if (tid < rows) mine = tl = rows_tiles(x, t + 1 < rows && y.joined);
+        if (tid < rows) tl = rows_tiles(x, t + 1 < rows && y.joined);
+        mine = places(tl);
         const float some = group_sum<64>((float)tl);
         const unsigned long long on = __ballot(x.joined), runs = __ballot(tl > 0);
         if (lane == 0) {
@@ -728,13 +753,13 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             const int tiles = uni(s_tiles), k0 = me - (int)s_at;
             hb = uni(k0 / np);
             const int k = k0 - hb * np, base = uni(tiles / np), rem = tiles - base * np;
-            first = k * base + min(k, rem);
+            x0 = ROWS_LEAD + k * base + min(k, rem);
             end = base + (k < rem);
         }
     } else
         for (int i = 0; i < each; i++) {
             const int t = tid * each + i;
-            if (t < rows) mine += tl = rows_tiles(A, T, t);
+            if (t < rows) mine += places(tl = rows_tiles(A, T, t));
         }
     if (np == 0) {
         long long tot;
@@ -751,8 +776,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             long long b = (upto - mine) * per_row;
             int t = tid * each;
             if (each > 1)
-                while (at >= b + (tl = rows_tiles(A, T, t)) * (long long)per_row) {
-                    b += tl * (long long)per_row;
+                while (at >= b + places(tl = rows_tiles(A, T, t)) * (long long)per_row) {
+                    b += places(tl) * (long long)per_row;
                     t++;
                 }
             s_row = t;
@@ -760,8 +785,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             s_at = b;
         }
         __syncthreads();
-        hb = uni((int)((at - s_at) / s_tiles));
-        first = uni((int)((at - s_at) % s_tiles));
+        hb = uni((int)((at - s_at) / (ROWS_LEAD + s_tiles)));
+        x0 = uni((int)((at - s_at) % (ROWS_LEAD + s_tiles)));
     }
     int t1 = uni(s_row), tiles = uni(s_tiles);
     /* Where this lane's operands lie in a tile, in bytes: its key's piece 4 s + g at kb[s % KJ]
@@ -777,7 +802,13 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         vb[k] = t0_at + (vr * CH + 2 * (k ^ (vr % SW) / 2) + ((c >> 1 & 1) ^ (vr & 1))) * 16 + 8 * (c & 1);
     const int cr = c / A.hpb, ch = c - cr * A.hpb;                      /* this lane's column: its row and head within the group */
     while (1) {
-        const int last = uni((int)min((long long)tiles, first + (end - at)));
+        /* places [x0, x1) and tiles [first, last) of this unit */
+        const int x1 = uni((int)min((long long)ROWS_LEAD + tiles, x0 + (end - at)));
+        const int first = max(0, x0 - ROWS_LEAD), last = max(0, x1 - ROWS_LEAD);
+        if (last == 0) {                               /* the next share begins it */
+            if (tid == 0) A.cut[blockIdx.x].k = 0;
+            break;
+        }
         const bool whole = first == 0 && last == tiles, cuts = first == 0 && !whole;
         /* the run's first row: the last one up to t1 that does not go on with the one before it */
         int t0 = t1;
@@ -999,20 +1030,24 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
             for (int k = 0; k < NO; k++) ((f32x4 *)A.po)[slot * ROWS_PART(D) + (w * NO + k) * 64 + lane] = o[k];
         }
-        at += last - first;
+        at += x1 - x0;
         if (tid == 0 && at == end) {
-            const RowsCut x = { t0, nr, hb, !cuts ? 0 : np ? np : (int)((at - last + tiles - 1) / share) - (int)blockIdx.x + 1 };
+            const RowsCut x = { t0, nr, hb, !cuts ? 0 : np ? np : (int)((at - x1 + ROWS_LEAD + tiles - 1) / share) - (int)blockIdx.x + 1 };
             A.cut[blockIdx.x] = x;
         }
         if (at >= end) break;
         __syncthreads();                               /* the tiles in LDS are done with */
-        first = 0;
+        x0 = 0;
         if (++hb == per_row) {
             hb = 0;
-            do {
-                t1++;
-                tiles = uni(rows_tiles(A, T, t1));
-            } while (tiles == 0);
+            for (bool on = true; on;) {                /* the next row that ends a run, 64 rows at a time */
+                const int t = t1 + 1 + lane, k = t < rows ? rows_tiles(A, T, t) : 0;
+                const unsigned long long j = __ballot(k > 0);
+                on = j == 0;
+                const int i = on ? 0 : __builtin_ctzll(j);
+                t1 += on ? 64 : 1 + i;
+                tiles = __builtin_amdgcn_readlane(k, i);
+            }
         }
     }
 }
