@@ -2,25 +2,32 @@
  * attn.hip -- softmax attention of new rows over a paged key/value cache
  * (roaster_attn_paged; model.c:755-863, 1536-1602).
  *
- * A unit of work is one row and up to HPB query heads of one key/value head; it
- * goes over the row's positions in tiles of TT tokens.  Every workgroup sums
- * the rows' tiles by itself and takes an even share of all units' tiles laid
- * end to end, whatever the rows' lengths; its waves take a unit's tiles in turn,
- * each with its own running maximum and sums, and join them in LDS.  A unit that
- * lies within one share is finished there.  Of one that a share's end cuts, the
- * parts go to the workspace and attn_join_kernel joins them.
+ * A unit of work is one row, or a few of one request, and up to 8 or 16 query heads
+ * of one key/value head; it goes over the row's positions in tiles of 16 tokens.
+ * Every workgroup sums the rows' tiles by itself and takes an even share of all
+ * units' tiles laid end to end, whatever the rows' lengths; its waves take a unit's
+ * tiles in turn, each with its own running maximum and sums, and join them in LDS.
+ * A unit that lies within one share is finished there.  Of one that a share's end
+ * cuts, the parts go to the workspace and attn_join_kernel joins them.
  *
- * Both products are MFMAs whose sixteen columns are the heads, and whose operands
- * come from global memory straight into registers:
- *   S^T = K Q^T   rows: 16 tokens, a lane holds 16 bytes of its token's key;
- *   O^T = V^T P^T rows: 16 elements, a lane holds 16 bytes of each of its tokens'
- *                 values, transposed among its own registers; a lane's scores
- *                 are the very probabilities that its operand needs, so P
- *                 never moves between lanes.
+ * Both products are MFMAs whose sixteen columns are heads (of one row or several):
+ *   S^T = K Q^T   rows: 16 tokens; keys come a kilobyte to a load and go through a
+ *                 wave's own LDS into the operands' order;
+ *   O^T = V^T P^T rows: 16 elements; a lane holds 16 bytes of each of its tokens'
+ *                 values, transposed among its own registers, and its scores are
+ *                 the very probabilities that its operand needs, so P never moves
+ *                 between lanes.
  * fp16 cache: a query row is scaled by a power of two and split into two fp16
- * parts, the probabilities likewise, and the parts are the columns h and h + 8:
- * the eight heads fill the sixteen columns, and products are exact up to 2^-22
- * of an operand.  f32 cache: f32 MFMAs, columns 8..15 unused.
+ * parts, the probabilities likewise, so that products are exact up to 2^-22 of an
+ * operand.  For one row of up to eight heads the parts are the columns h and h + 8:
+ * one product does both.  For more heads or rows (WIDE) the columns are sixteen of
+ * them, and each operand read is multiplied by high and low parts in turn.
+ * f32 cache: f32 MFMAs, always WIDE.
+ *
+ * What bounds it: the cache's bytes.  A large read reaches 6.8 TB/s here; 64
+ * requests of 300..16000 tokens come to 5.65 (94 us), one of 200001 to 5.7 (72 us, 5 of
+ * them for the join), f32 to 5.0.  437 tokens take 12 us: two launches and a chain of
+ * waits for a row, its page, keys and values.
  */
 #include "attn.h"
 #include "qdot.h"
@@ -29,7 +36,6 @@
 #define ATT_W (ATT_T / 64)
 #define ATT_G 512             /* workgroups at most: two per CU */
 #define ATT_MIN 4             /* tiles of a share at least: one a wave */
-#define HPB 8                 /* query heads of a unit */
 #define P_UP 7.0f             /* probabilities are kept times 2^7 (relative to the running maximum, which they
                                  may pass by 2^8): the low fp16 part of one of 2^-10 is still normal */
 #define M_LATE 8.0f           /* the running maximum moves only when a score passes it by this much */
@@ -40,21 +46,29 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+/* A unit whose parts are to be joined: first row and rows, head block, the share that began
+ * it, and its shares (0: none to join). */
+struct AttCut {
+    int row, n, hb, g0, k;
+};
+
 struct AttArgs {
     RoasterAttnPaged a;
     const char *kc, *vc;
     KvShape s;
-    int group, blocks;        /* query heads of a key/value head, and their blocks of HPB */
+    int group, blocks, hpb;   /* query heads of a key/value head, their blocks, heads of a block */
+    int R;                    /* rows of a unit at most */
     int by_unit;              /* the join's table goes by unit (else by the share that began the unit) */
     int grid;                 /* workgroups */
     int few;                  /* attn_few_kernel's parts: one a workgroup */
-    int2 *cut;                /* [.] first share and number of shares of a unit to join; 0 shares: none */
-    float *pm, *pl, *po;      /* parts [2 ATT_G][HPB], [..][HPB], [..][HPB][D]: slot g with `few`, else 2g + 1 the unit
+    AttCut *cut;              /* [units] or [grid] */
+    float *pm, *pl, *po;      /* parts [2 ATT_G][COLS], [..][COLS], [..][COLS][D]: slot g with `few`, else 2g + 1 the unit
                                  that share g began and did not finish, 2g the one that it found begun */
 };
 
-template <int D, bool F16>
+template <int D, bool F16, bool WIDE>
 struct AttCfg {
+    static constexpr int COLS = WIDE ? 16 : 8;                       /* columns with sums of their own */
     static constexpr int TT = 16, SZ = F16 ? 2 : 4;                  /* tokens of a tile */
     static constexpr int VE = F16 ? (D >= 128 ? 8 : 4) : 4;       /* elements of a value load */
     static constexpr int NB = D / (16 * VE);                        /* value loads of a token */
@@ -62,7 +76,6 @@ struct AttCfg {
     static constexpr int KS = NCH / 4;                               /* key loads of a tile, and operands of a score */
     static constexpr int SW = NCH < 16 ? NCH : 16;
     static constexpr int VT = 4;                                     /* tokens of a lane's value operand */
-    static constexpr int LD = D + 4;                                 /* LDS row */
 };
 
 __device__ __forceinline__ float max_g(float v)       /* over the four lanes of a column */
@@ -119,10 +132,10 @@ __device__ __forceinline__ float split_q(const float4 *x, f16x8 *hi, f16x8 *lo, 
 }
 
 /* One wave's state of a unit: lane (c = lane % 16, g = lane / 16) holds column c. */
-template <int D, bool F16>
+template <int D, bool F16, bool WIDE>
 struct AttWave {
-    using C = AttCfg<D, F16>;
-    f16x8 qh[F16 ? C::KS : 1];
+    using C = AttCfg<D, F16, WIDE>;
+    f16x8 qh[F16 ? C::KS : 1], ql[F16 && WIDE ? C::KS : 1];
     f32x4 qf[F16 ? 1 : C::KS];
     float fac;                      /* log2 score of a product */
     float m, l;
@@ -130,19 +143,18 @@ struct AttWave {
     gu32x4 k[C::KS];
     gu32x4 v[C::VT][C::NB];
 
-    /* The unit's queries as they lie: column c's head (a column without one computes
-     * the first head's and is never stored). */
+    /* Column c's query as it lies, from q (a column without one computes another's and is
+     * never stored). */
     static constexpr int QE = F16 ? 8 : 4;          /* elements of a product operand */
     struct Raw {
         float4 x[QE * C::KS / 4];
     };
-    __device__ static void load_q(Raw &r, const float *q, int c, int g, int nh)
+    __device__ static void load_q(Raw &r, const float *q, int g)
     {
-        const float *p = q + ((c & 7) < nh ? (c & 7) : 0) * D + QE * g;
 #pragma unroll
         for (int s = 0; s < C::KS; s++)
 #pragma unroll
-            for (int j = 0; j < QE / 4; j++) r.x[QE / 4 * s + j] = *(const float4 *)(p + 4 * QE * s + 4 * j);
+            for (int j = 0; j < QE / 4; j++) r.x[QE / 4 * s + j] = *(const float4 *)(q + QE * g + 4 * QE * s + 4 * j);
     }
     __device__ void clear()
     {
@@ -154,7 +166,7 @@ struct AttWave {
     __device__ void begin(const Raw &r, int c, float scale)
     {
         fac = scale * 1.44269504088896341f;
-        if constexpr (F16) fac *= split_q<8 * C::KS, false>(r.x, qh, qh, c < 8 ? 0.0f : 1.0f);
+        if constexpr (F16) fac *= split_q<8 * C::KS, WIDE>(r.x, qh, ql, c < 8 ? 0.0f : 1.0f);
         else {
 #pragma unroll
             for (int s = 0; s < C::KS; s++) qf[s] = (f32x4){ r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w };
@@ -201,21 +213,24 @@ struct AttWave {
 #pragma unroll
         for (int i = 0; i < C::KS; i++) {
             const gu32x4 x = t[c * C::NCH + ((4 * i + g) ^ c % C::SW)];
-            if (F16) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), qh[i], a, 0, 0, 0);
-            else
+            if constexpr (F16) {
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), qh[i], a, 0, 0, 0);
+                if constexpr (WIDE) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), ql[i], a, 0, 0, 0);
+            } else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     a = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, x)[j], qf[i][j], a, 0, 0, 0);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[j] = F16 ? a[j] + dpp_f<0x128>(a[j]) : a[j];     /* row_ror:8: the other part's column */
+        for (int j = 0; j < 4; j++) s[j] = F16 && !WIDE ? a[j] + dpp_f<0x128>(a[j]) : a[j];     /* row_ror:8: the other part's column */
     }
-    /* The tile's softmax terms, p in place of the scores; `left` tokens of the tile count. */
-    __device__ void soften(float *s, int left, int g)
+    /* The tile's softmax terms, p in place of the scores; `left` tokens of the tile count for
+     * this column, all of them for every column unless `some`. */
+    __device__ void soften(float *s, int left, bool some, int g)
     {
         float mx = -INFINITY;
         for (int j = 0; j < C::VT; j++) s[j] *= fac;
-        if (left < C::TT)
+        if (some)
             for (int j = 0; j < C::VT; j++)
                 if (4 * g + j >= left) s[j] = -INFINITY;
         for (int j = 0; j < C::VT; j++) mx = fmaxf(mx, s[j]);
@@ -225,7 +240,8 @@ struct AttWave {
             for (int i = 0; i < C::NB * C::VE; i++) o[i] *= w;
             m = mn;
         }
-        const float base = m - P_UP;
+        /* a column that has met no position yet keeps its terms 0 */
+        const float base = m == -INFINITY ? 0.0f : m - P_UP;
         for (int j = 0; j < C::VT; j++) {
             s[j] = __builtin_amdgcn_exp2f(s[j] - base);
             l += s[j];
@@ -233,14 +249,15 @@ struct AttWave {
     }
     __device__ void values(const float *p, int left, int c, int g)
     {
-        if (left < C::TT)                              /* what lies behind the row may be anything: 0 * NaN is NaN */
+        if (left < C::TT)                              /* what lies behind the rows or a bad page may be anything: 0 * NaN is NaN */
             for (int j = 0; j < C::VT; j++)
                 if (4 * g + j >= left)
                     for (int n = 0; n < C::NB; n++) v[j][n] = (gu32x4){};
         if (F16) {
-            const float low = c < 8 ? 0.0f : 1.0f;
-            const f16x2 b0 = rest_half(to_half(p[0], p[1]), low, p[0], p[1]), b1 = rest_half(to_half(p[2], p[3]), low, p[2], p[3]);
-            const f16x4 b = { b0.x, b0.y, b1.x, b1.y };
+            const float low = WIDE || c >= 8 ? 1.0f : 0.0f;
+            const f16x2 h0 = to_half(p[0], p[1]), h1 = to_half(p[2], p[3]);
+            const f16x2 r0 = rest_half(h0, low, p[0], p[1]), r1 = rest_half(h1, low, p[2], p[3]);
+            const f16x4 hi = { h0.x, h0.y, h1.x, h1.y }, lo = { r0.x, r0.y, r1.x, r1.y };      /* not WIDE: lo is this column's part */
 #pragma unroll
             for (int n = 0; n < C::NB; n++)
 #pragma unroll
@@ -249,8 +266,9 @@ struct AttWave {
 #pragma unroll
                     for (int j = 0; j < 2; j++)
                         a[j] = __builtin_amdgcn_perm(v[2 * j + 1][n][e / 2], v[2 * j][n][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-                    o[n * C::VE + e] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), b,
-                                                                             o[n * C::VE + e], 0, 0, 0);
+                    f32x4 &to = o[n * C::VE + e];
+                    if constexpr (WIDE) to = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), hi, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), lo, to, 0, 0, 0);
                 }
         } else {
             for (int n = 0; n < C::NB; n++)
@@ -312,21 +330,50 @@ __device__ __forceinline__ long long att_scan(long long v, long long *s_wave, lo
 #define ATT_LEAD 8
 #define ROWS_LEAD 4           /* of 32 tokens */
 
-/* Tiles of a row: at least one for a row that has an output to write. */
-template <int TT>
-__device__ __forceinline__ int att_tiles(const KvTable &T, int req, int pos, int shift)
+/* Row t's request and tokens, and whether it goes on with the unit of row t - 1: runs of up to
+ * R rows of one request, one behind the other with positions that do not fall, between
+ * multiples of R. */
+struct RowsAt {
+    int req, n;
+    bool joined;
+};
+__device__ __forceinline__ RowsAt rows_at(const RoasterAttnPaged &a, const KvTable &T, int shift, int R, int t)
 {
-    if (req == -1) return 0;
-    const int n = T.tokens(req, pos, shift);
-    return n <= TT ? 1 : (int)(((long long)n + TT - 1) / TT);
+    RowsAt x = { a.row_req[t], 0, false };
+    x.n = T.tokens(x.req, a.row_pos[t], shift);            /* -1 for a row that is skipped, too */
+    const int b = max(t - 1, 0), r = a.row_req[b], n = T.tokens(r, a.row_pos[b], shift);
+    x.joined = t % R && r == x.req && n >= 0 && n <= x.n;
+    return x;
+}
+/* Tiles of TT tokens of the unit that ends with row x, at least one for rows that have an
+ * output to write; 0 if none ends there: its request is none or it goes on. */
+template <int TT>
+__device__ __forceinline__ int rows_tiles(const RowsAt &x, bool goes_on)
+{
+    if (x.req == -1 || goes_on) return 0;
+    return x.n <= TT ? 1 : (int)(((long long)x.n + TT - 1) / TT);
+}
+template <int TT>
+__device__ __forceinline__ int rows_tiles(const RoasterAttnPaged &a, const KvTable &T, int shift, int R, int t)
+{
+    const RowsAt x = rows_at(a, T, shift, R, t);
+    return rows_tiles<TT>(x, R > 1 && t + 1 < a.rows && rows_at(a, T, shift, R, min(t + 1, a.rows - 1)).joined);
+}
+/* The first row of the unit that ends with row t1 (R at most 64), by a whole wave. */
+__device__ __forceinline__ int rows_first(const RoasterAttnPaged &a, const KvTable &T, int shift, int R, int t1)
+{
+    if (R == 1) return t1;
+    const int t = max(t1 - ((int)threadIdx.x & 63), 0);    /* row 0 goes on with none */
+    return t1 - __builtin_ctzll(~__ballot(rows_at(a, T, shift, R, t).joined));
 }
 
-/* A wave's share holds its tile's keys, after its last tile its sums [HPB][D + 4]. */
-template <int D, bool F16>
+/* A wave's share holds its tile's keys, after its last tile its sums [COLS][D + 4]. */
+template <int D, bool F16, bool WIDE>
 struct AttLds {
-    static constexpr int KEYS = 16 * D * (F16 ? 2 : 4), SUMS = HPB * (D + 4) * 4;
+    static constexpr int COLS = WIDE ? 16 : 8, KEYS = 16 * D * (F16 ? 2 : 4), SUMS = COLS * (D + 4) * 4;
     gu32x4 own[ATT_W][(KEYS > SUMS ? KEYS : SUMS) / 16];
-    float m[ATT_W][HPB], l[ATT_W][HPB];
+    float m[ATT_W][COLS], l[ATT_W][COLS];
+    int n[COLS], good[ATT_W];
     __device__ float *sums(int w, int h) { return (float *)own[w] + h * (D + 4); }
 };
 
@@ -344,40 +391,50 @@ __device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int 
     *(f32x4 *)(a.out + ((size_t)t * a.q_heads + h) * D + d) = y;
 }
 
-/* Tiles [first, last) of unit (t, hb) by one workgroup: to out if that is all of
- * them, else to part `slot`. */
-template <int D, bool F16>
-__device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16> &S, int *err, int t, int req, int pos, int hb, int first,
-                                         int last, bool whole, int slot)
+/* Tiles [first, last) of the unit of rows t0 .. t0 + nr - 1 and head block hb by one
+ * workgroup: to out if that is all of them, else to part `slot`.  n: tokens of its last row. */
+template <int D, bool F16, bool WIDE>
+__device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> &S, int *err, int t0, int nr, int req, int n, int hb,
+                                         int first, int last, bool whole, int slot)
 {
-    using C = AttCfg<D, F16>;
+    using C = AttCfg<D, F16, WIDE>;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
-    const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(HPB, A.group - bk * HPB);
-    const int h0 = kh * A.group + bk * HPB, n = T.tokens(req, pos, shift);
-    bool bad = n < 0;
-    AttWave<D, F16> wv;
-    typename AttWave<D, F16>::Raw raw;
+    const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(A.hpb, A.group - bk * A.hpb);
+    const int h0 = kh * A.group + bk * A.hpb;
+    /* this lane's column: its row and head, and the tokens that count for it */
+    const int cr = WIDE ? c / A.hpb : 0, ch = WIDE ? c - cr * A.hpb : c & 7;
+    const bool on = cr < nr && ch < nh;
+    int nc = n;
+    if (WIDE && nr > 1) nc = on ? T.tokens(req, a.row_pos[t0 + cr], shift) : 0;
+    int good = n < 0 ? -2 : n;     /* tokens before the first bad page: rows of more are NaN, all if the row itself is bad */
+    AttWave<D, F16, WIDE> wv;
+    typename AttWave<D, F16, WIDE>::Raw raw;
     /* the page of tile i, then the byte at which the tile begins */
     auto page = [&](int i) { return a.table[T.entry(req, i * 16, shift)]; };
     auto where = [&](int i, int p) {
         int pg = uni(p);
-        if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
+        if (!A.s.page_ok(pg)) { good = min(good, i * 16); pg = 0; }
         return A.s.at(pg, kh, i * 16 & ((1 << shift) - 1)) * C::SZ;
     };
     wv.clear();
     int i = first + w;
     if (n > 0 && i < last) {
         int p = page(i), i2 = i + ATT_W;
-        wv.load_q(raw, a.q + ((size_t)t * a.q_heads + h0) * D, c, g, nh);
+        wv.load_q(raw, a.q + ((size_t)(t0 + (on ? cr : 0)) * a.q_heads + h0 + (on ? ch : 0)) * D, g);
         size_t b = where(i, p);
         wv.load_k(A.kc, b, lane);
         if (i2 < last) p = page(i2);
         wv.load_v(A.vc, b, c, g);
         wv.begin(raw, c, a.scale);
+        int least = n;                                 /* over the columns in use */
+        if (WIDE && nr > 1) {
+            least = on ? nc : n;
+            for (int x = 1; x < 16; x <<= 1) least = min(least, __shfl_xor(least, x));
+            least = uni(least);
+        }
         while (1) {
-            const int left = n - i * 16;
             const bool more = i2 < last;
             float s[C::VT];
             wv.store_k(S.own[w], lane);
@@ -387,8 +444,8 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16> &S, in
                 if (i2 + ATT_W < last) p = page(i2 + ATT_W);
             }
             wv.scores(s, S.own[w], c, g);
-            wv.soften(s, left, g);
-            wv.values(s, left, c, g);
+            wv.soften(s, nc - i * 16, least < (i + 1) * 16, g);
+            wv.values(s, good - i * 16, c, g);
             if (!more) break;
             wv.load_v(A.vc, b, c, g);
             i = i2;
@@ -396,22 +453,29 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16> &S, in
         }
     }
     const float l = sum_g(wv.l);
-    if (g == 0 && c < HPB) { S.m[w][c] = wv.m; S.l[w][c] = l; }
-    if constexpr (F16) wv.add_parts();
+    if (g == 0 && c < C::COLS) {
+        S.m[w][c] = wv.m;
+        S.l[w][c] = l;
+        if (w == 0) S.n[c] = nc;
+    }
+    if (lane == 0) S.good[w] = good;
+    if constexpr (F16 && !WIDE) wv.add_parts();
 #pragma unroll
     for (int b = 0; b < C::NB; b++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (c < HPB)
+            if (c < C::COLS)
 #pragma unroll
                 for (int e = 0; e < C::VE; e += 4)
                     *(float4 *)(S.sums(w, c) + 16 * C::VE * b + C::VE * (4 * g + i) + e) =
                         make_float4(wv.o[b * C::VE + e][i], wv.o[b * C::VE + e + 1][i], wv.o[b * C::VE + e + 2][i],
                                     wv.o[b * C::VE + e + 3][i]);
-    const bool any = __syncthreads_or(bad);
-    if (any && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
-    for (int idx = tid * 4; idx < nh * D; idx += ATT_T * 4) {
-        const int h = idx / D, d = idx % D;
+    __syncthreads();
+    for (int i = 0; i < ATT_W; i++) good = min(good, S.good[i]);
+    if (good < n && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
+    for (int idx = tid * 4; idx < C::COLS * D; idx += ATT_T * 4) {
+        const int h = idx / D, d = idx % D, row = WIDE ? h / A.hpb : 0, head = h - row * A.hpb;
+        if (row >= nr || head >= nh) continue;
         float mx = -INFINITY, sum = 0;
         f32x4 y = {};
 #pragma unroll
@@ -422,40 +486,45 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16> &S, in
             sum += S.l[i][h] * f;
             y += *(const f32x4 *)(S.sums(i, h) + d) * f;
         }
-        if (any) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
-        if (whole) att_store(a, D, t, h0 + h, d, y, n == 0 ? 1.0f : sum);      /* without positions: y is 0 */
+        if (S.n[h] > good) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
+        if (whole) att_store(a, D, t0 + row, h0 + head, d, y, S.n[h] == 0 ? 1.0f : sum);      /* without positions: y is 0 */
         else {
-            *(f32x4 *)(A.po + ((size_t)slot * HPB + h) * D + d) = y;
+            *(f32x4 *)(A.po + ((size_t)slot * C::COLS + h) * D + d) = y;
             if (d == 0) {
-                A.pm[slot * HPB + h] = mx;
-                A.pl[slot * HPB + h] = sum;
+                A.pm[slot * C::COLS + h] = mx;
+                A.pl[slot * C::COLS + h] = sum;
             }
         }
     }
 }
 
-/* Few units (at most ATT_G / 4, of at most 128 rows): every workgroup takes one
- * unit's part.  All tiles over (ATT_G - units) is a part's size S that gives at
- * most ATT_G parts, since a unit of n tiles has ceil(n / S); a unit's parts are
- * equal.  Each wave finds its part from the rows by itself, without a barrier. */
-template <int D, bool F16>
+/* Few units (at most an eighth of the workgroups, of at most 128 rows): every workgroup
+ * takes one unit's part.  All tiles over (workgroups - units) is a part's size that gives
+ * no more parts than workgroups, since a unit of n tiles has ceil(n / size); a unit's
+ * parts are equal.  Each wave finds its part from the rows by itself, without a barrier.
+ * 8 requests of 100..8000 tokens, 2 key/value heads: 18 us, with even shares 26; 32 of them
+ * (above the bound): 32 either way. */
+template <int D, bool F16, bool WIDE>
 __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kernel(AttArgs A, int *err)
 {
-    using C = AttCfg<D, F16>;
-    __shared__ AttLds<D, F16> S;
+    using C = AttCfg<D, F16, WIDE>;
+    __shared__ AttLds<D, F16, WIDE> S;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int lane = threadIdx.x & 63, shift = A.s.shift, rows = a.rows, per_row = A.s.kv * A.blocks;
-    int req[2], pos[2], tl[2] = { 0, 0 };
+    int req[2], tok[2], tl[2] = { 0, 0 };
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const int t = min(lane + 64 * k, rows - 1);
-        req[k] = a.row_req[t];
-        pos[k] = a.row_pos[t];
+        const RowsAt x = rows_at(a, T, shift, 1, t);
+        req[k] = x.req;
+        tok[k] = x.n;
+        if (lane + 64 * k < rows) {
+            tl[k] = rows_tiles<C::TT>(x, false);
+            if (tl[k] == 0 && blockIdx.x == 0 && threadIdx.x < 64)       /* no unit: nothing to join */
+                for (int u = 0; u < per_row; u++) A.cut[t * per_row + u].k = 0;
+        }
     }
-#pragma unroll
-    for (int k = 0; k < 2; k++)
-        if (lane + 64 * k < rows) tl[k] = att_tiles<C::TT>(T, req[k], pos[k], shift);
     /* the sum in f32, a little too large if anything */
     const float all = group_sum<64>((float)tl[0] + (float)tl[1]) * per_row;
     const int size = max(ATT_MIN, (int)(all * (1.0001f / ((int)gridDim.x - rows * per_row))) + 1);
@@ -476,38 +545,42 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kern
     const int chunks = pick(ch), tiles = pick(tl), at = me - (pick(in) - chunks) * per_row;
     const int hb = uni(at / chunks), k = at - hb * chunks, base = uni(tiles / chunks), rem = tiles - base * chunks;
     const int first = k * base + min(k, rem), last = first + base + (k < rem);
-    att_part<D, F16>(A, S, err, t, pick(req), pick(pos), hb, first, last, chunks == 1, me);
-    if (k == 0 && threadIdx.x == 0) A.cut[t * per_row + hb] = make_int2(me, chunks == 1 ? 0 : chunks);
+    att_part<D, F16, WIDE>(A, S, err, t, 1, pick(req), pick(tok), hb, first, last, chunks == 1, me);
+    if (k == 0 && threadIdx.x == 0) A.cut[t * per_row + hb] = (AttCut){ t, 1, hb, me, chunks == 1 ? 0 : chunks };
 }
 
-template <int D, bool F16>
+template <int D, bool F16, bool WIDE>
 __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(AttArgs A, int *err)
 {
-    using C = AttCfg<D, F16>;
-    __shared__ AttLds<D, F16> S;
+    using C = AttCfg<D, F16, WIDE>;
+    __shared__ AttLds<D, F16, WIDE> S;
     __shared__ long long s_wave[ATT_W], s_at;
     __shared__ int s_row;
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
-    const int tid = threadIdx.x, shift = A.s.shift, per_row = A.s.kv * A.blocks, rows = a.rows;
+    const int tid = threadIdx.x, shift = A.s.shift, per_row = A.s.kv * A.blocks, rows = a.rows, R = WIDE ? A.R : 1;
 
     /* this share: the places [at, end) of all units' laid end to end */
     const int each = (rows + ATT_T - 1) / ATT_T;
     auto places = [&](int t) {
-        const int k = att_tiles<C::TT>(T, a.row_req[t], a.row_pos[t], shift);
+        const int k = rows_tiles<C::TT>(a, T, shift, R, t);
         return k ? ATT_LEAD + k : 0;
     };
     long long mine = 0, tot;
     for (int i = 0; i < each; i++) {
         const int t = tid * each + i;
-        if (t < rows) mine += places(t);
+        if (t >= rows) break;
+        const int k = places(t);
+        mine += k;
+        if (k == 0 && A.by_unit && blockIdx.x == 0)    /* no unit: nothing to join */
+            for (int u = 0; u < per_row; u++) A.cut[t * per_row + u].k = 0;
     }
     const long long upto = att_scan<ATT_W>(mine, s_wave, tot);
     const long long all = tot * per_row, share = max((long long)ATT_MIN, (all + gridDim.x - 1) / gridDim.x);
     long long at = blockIdx.x * share;
     const long long end = min(all, at + share);
     if (at >= end) {
-        if (!A.by_unit && tid == 0) A.cut[blockIdx.x] = make_int2(0, 0);
+        if (!A.by_unit && tid == 0) A.cut[blockIdx.x].k = 0;
         return;
     }
     if (at < upto * per_row && at >= (upto - mine) * per_row) {        /* one thread's rows hold it */
@@ -521,8 +594,8 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
         s_at = b;
     }
     __syncthreads();
-    int t = uni(s_row), req = uni(a.row_req[t]), pos = uni(a.row_pos[t]);
-    int tiles = att_tiles<C::TT>(T, req, pos, shift);
+    int t = uni(s_row), req = uni(a.row_req[t]), n = uni(T.tokens(req, a.row_pos[t], shift));
+    int tiles = rows_tiles<C::TT>((RowsAt){ req, n, false }, false);
     int hb = uni((int)((at - s_at) / (ATT_LEAD + tiles))), x0 = uni((int)((at - s_at) % (ATT_LEAD + tiles)));
     while (1) {
         /* places [x0, x1) and tiles [first, last) of unit (t, hb) */
@@ -531,15 +604,18 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
         const bool cuts = first == 0 && last > 0 && last < tiles, over = at + (x1 - x0) == end;
         const bool step = !over && hb + 1 == per_row;
         int req1 = -1, pos1 = 0;
-        if (step) {                                    /* the next row, while this one is worked on */
+        if (step && R == 1) {                          /* the next row, while this one is worked on */
             req1 = a.row_req[t + 1];
             pos1 = a.row_pos[t + 1];
         }
-        if (last > first) att_part<D, F16>(A, S, err, t, req, pos, hb, first, last, first == 0 && last == tiles, 2 * blockIdx.x + (first == 0));
+        const int t0 = uni(rows_first(a, T, shift, R, t)), nr = t - t0 + 1;
+        if (last > first)
+            att_part<D, F16, WIDE>(A, S, err, t0, nr, req, n, hb, first, last, first == 0 && last == tiles, 2 * blockIdx.x + (first == 0));
         if (tid == 0) {                                /* for the join: the shares of a unit begun and cut here */
             const int k = cuts ? (int)((at - x0 + ATT_LEAD + tiles - 1) / share) - (int)blockIdx.x + 1 : 0;
-            if (A.by_unit && first == 0 && last > 0) A.cut[t * per_row + hb] = make_int2(blockIdx.x, k);
-            if (!A.by_unit && over) A.cut[blockIdx.x] = make_int2(t * per_row + hb, k);
+            const AttCut x = { t0, nr, hb, (int)blockIdx.x, k };
+            if (A.by_unit && first == 0 && last > 0) A.cut[t * per_row + hb] = x;
+            if (!A.by_unit && over) A.cut[blockIdx.x] = x;
         }
         if (over) break;
         at += x1 - x0;
@@ -548,14 +624,21 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
         if (step) {
             hb = 0;
             t++;
-            req = uni(req1);
-            pos = uni(pos1);
-            while (req == -1) {
-                t++;
-                req = uni(a.row_req[t]);
-                pos = uni(a.row_pos[t]);
-            }
-            tiles = att_tiles<C::TT>(T, req, pos, shift);
+            if (R == 1 && uni(req1) != -1) {
+                req = uni(req1);
+                n = uni(T.tokens(req, pos1, shift));
+            } else
+                for (bool on = true; on;) {            /* the next row that ends a unit, 64 rows at a time */
+                    const int u = t + (tid & 63), k = u < rows ? rows_tiles<C::TT>(a, T, shift, R, u) : 0;
+                    const unsigned long long j = __ballot(k > 0);
+                    on = j == 0;
+                    t += on ? 64 : __builtin_ctzll(j);
+                    if (!on) {
+                        req = uni(a.row_req[t]);
+                        n = uni(T.tokens(req, a.row_pos[t], shift));
+                    }
+                }
+            tiles = rows_tiles<C::TT>((RowsAt){ req, n, false }, false);
         }
         __syncthreads();                               /* S is free again */
     }
@@ -563,13 +646,15 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
 
 /* ---- several rows of a request together (fp16 cache) ------------------------
  * A run is up to R rows of one request, one behind the other with positions that
- * do not fall: a prompt's chunk.  The workgroup brings each tile of the run's
- * keys and values into LDS once; a wave has two groups of 16 columns (row, head)
- * and multiplies every operand it reads by both groups' high and low parts, so
- * that the scores come out whole and no two lanes compute the same.  Shares,
- * cuts and the join go as in attn_kernel, a unit being a run and a block of
- * heads.  Four waves of up to 512 registers: queries (two parts) and sums of
- * two groups take 256 of them at dim 256. */
+ * do not fall: a prompt's chunk.  The workgroup brings each tile of 32 tokens into LDS
+ * once, straight from memory, for its eight waves of 16 columns (row, head), which
+ * multiply every operand they read by their columns' high and low parts.  Shares, cuts
+ * and the join go as in attn_kernel, a unit being a run and a block of heads.
+ * What bounds it: a tile is 64 MFMAs and 32 KB of LDS reads a wave, 2048 cycles of the
+ * matrix cores and as many of LDS, which overlap in part (4700 measured); of 256 rows
+ * behind 2048 tokens (43 us) the tiles take 20 us, beginning 9, and the parts' way
+ * through memory 10, 33 MB each way: 32 units on 256 CUs are cut in eight.  1024 rows of
+ * one prompt take 71 us. */
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
@@ -648,32 +733,6 @@ struct RowsArgs {
     float *pm, *pl, *po;      /* parts [2 ROWS_G][waves][16 columns], and [..][waves][D / 16][64 lanes][4]; slots as in AttArgs */
 };
 
-/* Row t's request and tokens, and whether it goes on with the run of row t - 1. */
-struct RowsAt {
-    int req, n;
-    bool joined;
-};
-__device__ __forceinline__ RowsAt rows_at(const RowsArgs &A, const KvTable &T, int t)
-{
-    const int b = max(t - 1, 0), r = A.a.row_req[b], p = A.a.row_pos[b];
-    RowsAt x;
-    x.req = A.a.row_req[t];
-    x.n = T.tokens(x.req, A.a.row_pos[t], A.s.shift);      /* -1 for a row that is skipped, too */
-    const int n = T.tokens(r, p, A.s.shift);
-    x.joined = t % A.R && r == x.req && n >= 0 && n <= x.n;
-    return x;
-}
-/* Tiles of the run that ends with row x, 0 if none does: its request is none or it goes on. */
-__device__ __forceinline__ int rows_tiles(const RowsAt &x, bool goes_on)
-{
-    if (x.req == -1 || goes_on) return 0;
-    return x.n <= 32 ? 1 : (int)(((long long)x.n + 31) / 32);
-}
-__device__ __forceinline__ int rows_tiles(const RowsArgs &A, const KvTable &T, int t)
-{
-    return rows_tiles(rows_at(A, T, t), t + 1 < A.a.rows && rows_at(A, T, min(t + 1, A.a.rows - 1)).joined);
-}
-
 template <int D>
 __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *err)
 {
@@ -688,9 +747,10 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     const RoasterAttnPaged &a = A.a;
     const KvTable T = { a.n_req, a.max_pages };
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, g = lane >> 4, shift = A.s.shift;
-    const int per_row = A.s.kv * A.blocks, rows = a.rows;
+    const int per_row = A.s.kv * A.blocks, rows = a.rows, R = A.R;
+    __builtin_assume(R > 1);
 
-    /* this share: the tiles [at, end) of all units' laid end to end, or with few units one of
+    /* this share: the places [at, end) of all units' laid end to end, or with few units one of
      * np equal parts of one unit (a share that two units meet in begins twice) */
     const int each = (rows + ROWS_T - 1) / ROWS_T;
     long long mine = 0, at = 0, end = 0, share = 1;
@@ -698,8 +758,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     auto places = [](int k) { return k ? ROWS_LEAD + k : 0; };
     if (each == 1) {                                   /* at most 512 runs, one a thread */
         const int G = gridDim.x, t = min(tid, rows - 1);
-        const RowsAt x = rows_at(A, T, t), y = rows_at(A, T, min(t + 1, rows - 1));
-        if (tid < rows) tl = rows_tiles(x, t + 1 < rows && y.joined);
+        const RowsAt x = rows_at(a, T, shift, R, t), y = rows_at(a, T, shift, R, min(t + 1, rows - 1));
+        if (tid < rows) tl = rows_tiles<32>(x, t + 1 < rows && y.joined);
         mine = places(tl);
         const float some = group_sum<64>((float)tl);
         const unsigned long long on = __ballot(x.joined), runs = __ballot(tl > 0);
@@ -759,7 +819,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
     } else
         for (int i = 0; i < each; i++) {
             const int t = tid * each + i;
-            if (t < rows) mine += places(tl = rows_tiles(A, T, t));
+            if (t < rows) mine += places(tl = rows_tiles<32>(a, T, shift, R, t));
         }
     if (np == 0) {
         long long tot;
@@ -776,7 +836,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             long long b = (upto - mine) * per_row;
             int t = tid * each;
             if (each > 1)
-                while (at >= b + places(tl = rows_tiles(A, T, t)) * (long long)per_row) {
+                while (at >= b + places(tl = rows_tiles<32>(a, T, shift, R, t)) * (long long)per_row) {
                     b += places(tl) * (long long)per_row;
                     t++;
                 }
@@ -820,7 +880,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         } else
             for (bool on = true; on;) {                /* 64 rows at a time */
                 const int t = t0 - lane;
-                const unsigned long long j = __ballot(t > 0 && rows_at(A, T, t).joined);
+                const unsigned long long j = __ballot(t > 0 && rows_at(a, T, shift, R, t).joined);
                 on = j == ~0ull;
                 t0 -= on ? 64 : __builtin_ctzll(~j);
             }
@@ -840,9 +900,14 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int tok = i * 32 + 16 * u;
-                int pg = p[u];
-                if (!A.s.page_ok(pg)) { bad = true; pg = 0; }
-                b[u] = A.s.at(pg, kh, (u && tok >= n ? tok - 16 : tok) & ((1 << shift) - 1)) * 2;
+                int pg = p[u], in = (u && tok >= n ? tok - 16 : tok) & ((1 << shift) - 1);
+                if (__builtin_expect(!A.s.page_ok(pg), 0)) {                /* the first part's page in its place, whose values rows may meet times 0 */
+                    bad = true;
+                    pg = ((const CAS int *)a.table)[T.entry(req, 0, shift)];
+                    if (!A.s.page_ok(pg)) pg = 0;
+                    in = 0;
+                }
+                b[u] = A.s.at(pg, kh, in) * 2;
             }
         };
         /* The tile's 64 CH pieces straight into LDS, 64 to a wave and load, in the order
@@ -1013,10 +1078,17 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                 pages(min(i0 + 5, last - 1), pg[1]);
             }
         }
-        if (bad && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
         const size_t slot = 2 * blockIdx.x + (first == 0);
         float sum = sum_g(l);
-        if (bad) sum = NAN;
+        if (__builtin_expect(bad, 0)) {
+            /* NaN for rows of more tokens than there are before the first bad page, or if the row itself is bad */
+            if (tid == 0) atomicOr(err, ATTN_ERR_INDEX);
+            int good = n < 0 ? -2 : first * 32;
+            while (good >= 0 && good < n && A.s.page_ok(a.table[T.entry(req, good, shift)])) good += 16;
+            if (nc > good) sum = NAN;
+            else if (nc <= 32 * first)                 /* met nothing but, maybe, a bad page's substitute */
+                for (int k = 0; k < NO; k++) o[k] = (f32x4){};
+        }
         if (whole) {
             if (on)
 #pragma unroll
@@ -1041,7 +1113,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         if (++hb == per_row) {
             hb = 0;
             for (bool on = true; on;) {                /* the next row that ends a run, 64 rows at a time */
-                const int t = t1 + 1 + lane, k = t < rows ? rows_tiles(A, T, t) : 0;
+                const int t = t1 + 1 + lane, k = t < rows ? rows_tiles<32>(a, T, shift, R, t) : 0;
                 const unsigned long long j = __ballot(k > 0);
                 on = j == 0;
                 const int i = on ? 0 : __builtin_ctzll(j);
@@ -1103,25 +1175,22 @@ __global__ __launch_bounds__(64) void attn_rows_join_kernel(RowsArgs A)
     for (int z = 0; z < 4; z++) att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, 16 * (4 * q + z) + 4 * g, y[z], sum);
 }
 
-/* The parts of one cut unit's head, L lanes with four elements each to a part:
+/* The parts of one cut unit's column, L lanes with four elements each to a part:
  * each group of lanes joins its parts as a running softmax does, the groups
  * join in LDS. */
-template <int D, int L, int JT>
+template <int D, int COLS, int L, int JT>
 __global__ __launch_bounds__(JT) void attn_join_kernel(AttArgs A)
 {
     constexpr int N = JT / L;
     __shared__ float s_m[N], s_l[N];
     __shared__ f32x4 s_o[N][L];
     const RoasterAttnPaged &a = A.a;
-    const int tid = threadIdx.x, h = blockIdx.y, per_row = A.s.kv * A.blocks;
-    int unit = blockIdx.x;
-    const int2 e = A.cut[unit];
-    if (A.by_unit && a.row_req[unit / per_row] == -1) return;
-    const int n = e.y, g0 = A.by_unit ? e.x : unit;
+    const int tid = threadIdx.x, col = blockIdx.y, row = col / A.hpb, head = col - row * A.hpb;
+    const AttCut e = A.cut[blockIdx.x];
+    const int n = e.k, g0 = e.g0;
     if (n == 0) return;
-    if (!A.by_unit) unit = e.x;
-    const int t = unit / per_row, hb = unit % per_row, kh = hb / A.blocks, bk = hb % A.blocks;
-    if (h >= A.group - bk * HPB) return;
+    const int kh = e.hb / A.blocks, bk = e.hb - kh * A.blocks;
+    if (row >= e.n || head >= A.group - bk * A.hpb) return;
     const int sub = tid / L, d = blockIdx.z * 4 * L + tid % L * 4;
     float m = -INFINITY, l = 0;
     f32x4 y = {};
@@ -1131,7 +1200,7 @@ __global__ __launch_bounds__(JT) void attn_join_kernel(AttArgs A)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int k = k0 + j * N, q = k < n ? k : k0;
-            const size_t at = (size_t)(A.few ? g0 + q : q ? 2 * (g0 + q) : 2 * g0 + 1) * HPB + h;
+            const size_t at = (size_t)(A.few ? g0 + q : q ? 2 * (g0 + q) : 2 * g0 + 1) * COLS + col;
             pm[j] = k < n ? A.pm[at] : -INFINITY;
             pl[j] = A.pl[at];
             po[j] = *(const f32x4 *)(A.po + at * D + d);
@@ -1164,22 +1233,25 @@ __global__ __launch_bounds__(JT) void attn_join_kernel(AttArgs A)
         sum += s_l[i] * w;
         y += s_o[i][tid] * w;
     }
-    att_store(a, D, t, kh * A.group + bk * HPB + h, d, y, sum);
+    const int t = e.row + row;
+    att_store(a, D, t, kh * A.group + bk * A.hpb + head, d, y, a.row_pos[t] == -1 ? 1.0f : sum);
 }
 
-/* Workspace: the cut table, then m and l of the parts, then the parts. */
-static const size_t ATT_CUT = (size_t)ATT_G * sizeof(int2), ATT_ML = (size_t)2 * ATT_G * HPB * 4;
+/* Workspace: the cut table, then m and l of the parts, then the parts (16 columns). */
+static const size_t ATT_CUT = (size_t)ATT_G * sizeof(AttCut), ATT_ML = (size_t)2 * ATT_G * 16 * 4;
 
 /* The same of attn_rows_kernel. */
 static const size_t ROWS_CUT = (size_t)ROWS_G * sizeof(RowsCut), ROWS_ML = (size_t)2 * ROWS_G * ROWS_COLS * 4;
 
-/* Calls that may go by runs of rows: with fewer rows there is little to share. */
+/* Calls that may go by runs of rows.  With fewer rows there is little to share: of one request
+ * behind 2048 tokens 8 take 23 us so and 19 apart, 16 take 26 and 21, 32 take 27 and 29;
+ * behind 16000 tokens 16 take 47 and 71. */
 static bool rows_may(int rows, int type) { return type == ROASTER_KV_F16 && rows >= 16; }
 
 extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCache *c)
 {
     if (!attn_cache_ok(c) || rows < 0 || rows > (1 << 20) || q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads) return 0;
-    const size_t one = ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * HPB * c->head_dim * 4,
+    const size_t one = ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * 16 * c->head_dim * 4,
                  run = ROWS_CUT + 2 * ROWS_ML + (size_t)2 * ROWS_G * ROWS_PART(c->head_dim) * 16;
     return rows_may(rows, c->type) && run > one ? run : one;
 }
@@ -1191,17 +1263,16 @@ static void rows_launch(const RowsArgs &A, int *err)
     hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_W * D / 64, ROWS_G), dim3(64), 0, rt().stream, A);
 }
 
-template <int D, bool F16>
+template <int D, bool F16, bool WIDE>
 static void att_launch(const AttArgs &A, int *err)
 {
-    const long long units = (long long)A.a.rows * A.s.kv * A.blocks;
-    if (A.few) hipLaunchKernelGGL((attn_few_kernel<D, F16>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
-    else hipLaunchKernelGGL((attn_kernel<D, F16>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
-    const int heads = A.group < HPB ? A.group : HPB;
-    /* few units have many parts each: 64 elements of a head to a workgroup, 32 parts at a time */
-    if (A.few) hipLaunchKernelGGL((attn_join_kernel<D, 16, 512>), dim3((int)units, heads, D / 64), dim3(512), 0, rt().stream, A);
-    else hipLaunchKernelGGL((attn_join_kernel<D, D / 4, 128>), dim3(A.by_unit ? (int)units : A.grid, heads), dim3(128), 0,
-                            rt().stream, A);
+    constexpr int COLS = AttCfg<D, F16, WIDE>::COLS;
+    const int units = A.by_unit ? A.a.rows * A.s.kv * A.blocks : A.grid, cols = A.hpb * A.R;
+    if (A.few) hipLaunchKernelGGL((attn_few_kernel<D, F16, WIDE>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
+    else hipLaunchKernelGGL((attn_kernel<D, F16, WIDE>), dim3(A.grid), dim3(ATT_T), 0, rt().stream, A, err);
+    /* few units have many parts each: 64 elements of a column to a workgroup, 32 parts at a time */
+    if (A.few) hipLaunchKernelGGL((attn_join_kernel<D, COLS, 16, 512>), dim3(units, cols, D / 64), dim3(512), 0, rt().stream, A);
+    else hipLaunchKernelGGL((attn_join_kernel<D, COLS, D / 4, 128>), dim3(units, cols), dim3(128), 0, rt().stream, A);
 }
 
 extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCache *c)
@@ -1235,7 +1306,8 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
     /* Runs of rows pay where requests have several rows each, which the two counts
-     * tell on average (a call of other rows is right as well, only slower). */
+     * tell on average (a call of other rows is right as well, only slower): 256 rows behind
+     * 2048 tokens take 43 us so, 114 row by row. */
     if (rows_may(p->rows, c->type) && p->rows >= 4 * (long long)p->n_req) {
         RowsArgs A;
         A.a = *p;
@@ -1262,18 +1334,31 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     A.vc = (const char *)c->v;
     A.s = attn_shape(c);
     A.group = p->q_heads / c->kv_heads;
-    A.blocks = (A.group + HPB - 1) / HPB;
+    /* Sixteen columns of their own for more than eight heads (32 requests, 16 heads on one:
+     * 53 us, with two blocks of eight 90) and for several rows of a request (32 requests of two
+     * rows: 72 us, row by row 95; f32, 256 rows: 165 instead of 302).  With one row of few
+     * heads the high and low parts fill them: half the MFMAs. */
+    const bool f16 = c->type == ROASTER_KV_F16;
+    bool wide = !f16 || A.group > 8;
+    A.hpb = std::min(A.group, wide ? 16 : 8);
+    A.blocks = (A.group + A.hpb - 1) / A.hpb;
+    /* two workgroups a CU, but for the f32 cache's registers at dim 256 */
+    A.grid = D == 256 && !f16 ? ATT_G / 2 : ATT_G;
     const long long units = (long long)p->rows * c->kv_heads * A.blocks;
-    A.grid = D == 256 && c->type == ROASTER_KV_F32 ? ATT_G / 2 : ATT_G;
     A.by_unit = units <= A.grid;
+    /* With few units the rows of a request stay apart: what they share comes from the caches,
+     * and there are more parts (three rows behind 437 tokens: 11.8 us, 14.6 together). */
     A.few = units <= A.grid / 8 && p->rows <= 128;
-    A.cut = (int2 *)p->ws;
+    A.R = A.few || p->rows < 2 * (long long)p->n_req ? 1 : 16 / A.hpb;
+    wide |= A.R > 1;
+    A.cut = (AttCut *)p->ws;
     A.pm = (float *)((char *)p->ws + ATT_CUT);
     A.pl = (float *)((char *)p->ws + ATT_CUT + ATT_ML);
     A.po = (float *)((char *)p->ws + ATT_CUT + 2 * ATT_ML);
-    const bool f16 = c->type == ROASTER_KV_F16;
-    if (D == 256) f16 ? att_launch<256, true>(A, err) : att_launch<256, false>(A, err);
-    else if (D == 128) f16 ? att_launch<128, true>(A, err) : att_launch<128, false>(A, err);
-    else f16 ? att_launch<64, true>(A, err) : att_launch<64, false>(A, err);
+#define ATT(DD) (f16 ? wide ? att_launch<DD, true, true>(A, err) : att_launch<DD, true, false>(A, err) : att_launch<DD, false, true>(A, err))
+    if (D == 256) ATT(256);
+    else if (D == 128) ATT(128);
+    else ATT(64);
+#undef ATT
     return rt_check(hipGetLastError(), "attention launch") ? ROASTER_EDEVICE : 0;
 }

@@ -119,6 +119,24 @@ def test_several_rows_a_request(i, H, KV, D, f16):
     run_case(lens, rows, H, KV, D, 32, f16, gate=True)
 
 
+@pytest.mark.parametrize("H,KV,D", HEADS)
+@pytest.mark.parametrize("f16", [True, False])
+def test_drafts_of_many_requests(H, KV, D, f16):
+    """Two or three rows to a request, some skipped or without a position, of lengths that end
+    within a tile and at its edge: 80 units at least."""
+    rng = np.random.default_rng(H + D)
+    lens = rng.integers(3, 200, 40).tolist() + [3, 16, 17, 18, 33, 3000]
+    rows = []
+    for r, l in enumerate(lens):
+        n = 2 + r % 2
+        rows += [(r, l - n + i) for i in range(n)]
+        if r % 7 == 3:
+            rows[-1] = (-1, 5)
+        if r % 7 == 5:
+            rows[-2] = (r, -1)
+    run_case(lens, rows, H, KV, D, 16, f16, gate=True)
+
+
 def test_many_rows_of_many_requests():
     """More rows than a launch has workgroups."""
     rng = np.random.default_rng(4)
@@ -207,6 +225,30 @@ def test_bad_rows_are_nan_and_reported(f16):
     assert all(np.isnan(got[i]).all() for i in range(len(rows)) if i not in good)
     want = attn_oracle(q[good], kc, vc, table, rows[good, 0], rows[good, 1], np.float64(np.float32(0.1)))
     check_attn(got[good], *want, 3000, 128)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("T,at", [(3, 60), (24, 60), (24, 3000), (4, 3000)])
+def test_a_bad_page_is_of_the_rows_that_reach_it(f16, T, at):
+    """Rows of one request before and behind a bad page, together in one call: the
+    former are right, the latter NaN."""
+    rng = np.random.default_rng(T + at)
+    kc, vc, table = make(rng, [at + T], 2, 128, 16, f16)
+    bad = table.copy()
+    split = (at + T // 2) // 16 * 16                   # the bad page's first token
+    bad[0, split // 16] = kc.shape[0]
+    pos = np.array([split - 1 - T // 2 + i for i in range(T)], np.int32)
+    req = np.zeros(T, np.int32)
+    q = rng.standard_normal((T, 8, 128)).astype(np.float32)
+    a = Attn(Cache(kc, vc), q, req, pos, bad, 0.1)
+    R.check(a.call(), "attn")
+    assert R.lib().roaster_sync() == R.EINVAL
+    sync()
+    got = a.out.get()
+    good = np.flatnonzero(pos < split)
+    assert 0 < len(good) < T and np.isnan(got[len(good):]).all()
+    want = attn_oracle(q[good], kc, vc, table, req[good], pos[good], np.float64(np.float32(0.1)))
+    check_attn(got[good], *want, int(pos[-1]) + 1, 128)
 
 
 def test_cache_past_32_bit_offsets():
