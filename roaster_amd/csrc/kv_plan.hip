@@ -53,7 +53,9 @@ __device__ __forceinline__ int kvp_find(const int *c, int n, int i)
  * gives the same memory for len_out and ctl_out: then one workgroup, which has
  * read both before its first barrier, does all, or a second launch of one
  * workgroup writes them (`what`: bit 0 rows, table and ring, bit 1 len_out,
- * ctl_out, first and the error word). */
+ * ctl_out, first and the error word).  What bounds it: latency, a chain of the
+ * lengths' load, three scans, a search and a page's load; 8 requests of one row 4.5
+ * us, 512 requests with 22700 rows 6.9. */
 __global__ __launch_bounds__(KVP_T) void kv_plan_kernel(RoasterKvPlan A, int shift, int what, int *err)
 {
     __shared__ int c_row[KVP_MAX_REQ + 1], c_new[KVP_MAX_REQ + 1], c_old[KVP_MAX_REQ + 1], s_len[KVP_MAX_REQ];

@@ -73,7 +73,7 @@ def test_heads(H, KV, D, rot, adjacent, f16):
         run_case(T, H, KV, D, rot, f16, page=page, adjacent=adjacent, seed=T)
 
 
-@pytest.mark.parametrize("T", [511, 512, 1100])
+@pytest.mark.parametrize("T", [511, 767, 768, 1100])
 def test_many_rows(T):
     run_case(T, 16, 2, 256, 64, True, page=64, skip=(0, 3, T - 1))
     run_case(T, 20, 4, 64, 64, False, page=32, skip=(7,))
