@@ -137,7 +137,7 @@ struct AttWave {
     using C = AttCfg<D, F16, WIDE>;
     f16x8 qh[F16 ? C::KS : 1], ql[F16 && WIDE ? C::KS : 1];
     f32x4 qf[F16 ? 1 : C::KS];
-    float fac;                      /* log2 score of a product */
+    float fac;                      /* log2 score of a product, a power of two */
     float m, l;
     f32x4 o[C::NB * C::VE];
     gu32x4 k[C::KS];
@@ -163,10 +163,13 @@ struct AttWave {
 #pragma unroll
         for (int i = 0; i < C::NB * C::VE; i++) o[i] = (f32x4){};
     }
-    __device__ void begin(const Raw &r, int c, float scale)
+    __device__ void begin(Raw &r, int c, float scale)
     {
-        fac = scale * 1.44269504088896341f;
-        if constexpr (F16) fac *= split_q<8 * C::KS, WIDE>(r.x, qh, ql, c < 8 ? 0.0f : 1.0f);
+        const float f = scale * 1.44269504088896341f;
+#pragma unroll
+        for (int i = 0; i < QE * C::KS / 4; i++) { r.x[i].x *= f; r.x[i].y *= f; r.x[i].z *= f; r.x[i].w *= f; }
+        fac = 1.0f;
+        if constexpr (F16) fac = split_q<8 * C::KS, WIDE>(r.x, qh, ql, c < 8 ? 0.0f : 1.0f);
         else {
 #pragma unroll
             for (int s = 0; s < C::KS; s++) qf[s] = (f32x4){ r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w };
@@ -206,34 +209,42 @@ struct AttWave {
             }
         }
     }
-    /* Scores of the tile in t: a lane gets its column's for tokens 4 g .. */
+    /* Scores of the tile in t, over fac: a lane gets its column's for tokens 4 g ..  In N sums
+     * of their own (WIDE: high and low parts'), which wait less for each other and round less: of one
+     * sum of 256 f32 products the outputs were off by 1.65e-6 (6 requests of 2700 tokens)
+     * where those of four are by 0.54e-6. */
+    template <int N>
     __device__ void scores(float *s, const gu32x4 *t, int c, int g)
     {
-        f32x4 a = {};
+        f32x4 a[N] = {};
 #pragma unroll
         for (int i = 0; i < C::KS; i++) {
             const gu32x4 x = t[c * C::NCH + ((4 * i + g) ^ c % C::SW)];
             if constexpr (F16) {
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), qh[i], a, 0, 0, 0);
-                if constexpr (WIDE) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), ql[i], a, 0, 0, 0);
+                f32x4 &to = a[WIDE ? 0 : i % N];
+                to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), qh[i], to, 0, 0, 0);
+                if constexpr (WIDE) a[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), ql[i], a[1], 0, 0, 0);
             } else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    a = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, x)[j], qf[i][j], a, 0, 0, 0);
+                    a[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, x)[j], qf[i][j], a[j], 0, 0, 0);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[j] = F16 && !WIDE ? a[j] + dpp_f<0x128>(a[j]) : a[j];     /* row_ror:8: the other part's column */
+        for (int j = 0; j < 4; j++) {
+            s[j] = N == 2 ? a[0][j] + a[1][j] : (a[0][j] + a[1][j]) + (a[N - 2][j] + a[N - 1][j]);
+            if (F16 && !WIDE) s[j] += dpp_f<0x128>(s[j]);              /* row_ror:8: the other part's column */
+        }
     }
     /* The tile's softmax terms, p in place of the scores; `left` tokens of the tile count for
      * this column, all of them for every column unless `some`. */
     __device__ void soften(float *s, int left, bool some, int g)
     {
         float mx = -INFINITY;
-        for (int j = 0; j < C::VT; j++) s[j] *= fac;
         if (some)
             for (int j = 0; j < C::VT; j++)
                 if (4 * g + j >= left) s[j] = -INFINITY;
         for (int j = 0; j < C::VT; j++) mx = fmaxf(mx, s[j]);
+        mx *= fac;
         if (__any(mx > m + M_LATE)) {
             const float mn = fmaxf(m, max_g(mx)), w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             l *= w;
@@ -241,9 +252,9 @@ struct AttWave {
             m = mn;
         }
         /* a column that has met no position yet keeps its terms 0 */
-        const float base = m == -INFINITY ? 0.0f : m - P_UP;
+        const float base = m == -INFINITY ? 0.0f : P_UP - m;
         for (int j = 0; j < C::VT; j++) {
-            s[j] = __builtin_amdgcn_exp2f(s[j] - base);
+            s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], fac, base));
             l += s[j];
         }
     }
@@ -393,7 +404,7 @@ __device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int 
 
 /* Tiles [first, last) of the unit of rows t0 .. t0 + nr - 1 and head block hb by one
  * workgroup: to out if that is all of them, else to part `slot`.  n: tokens of its last row. */
-template <int D, bool F16, bool WIDE>
+template <int D, bool F16, bool WIDE, int N>
 __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> &S, int *err, int t0, int nr, int req, int n, int hb,
                                          int first, int last, bool whole, int slot)
 {
@@ -443,7 +454,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
                 wv.load_k(A.kc, b, lane);
                 if (i2 + ATT_W < last) p = page(i2 + ATT_W);
             }
-            wv.scores(s, S.own[w], c, g);
+            wv.template scores<N>(s, S.own[w], c, g);
             wv.soften(s, nc - i * 16, least < (i + 1) * 16, g);
             wv.values(s, good - i * 16, c, g);
             if (!more) break;
@@ -545,7 +556,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kern
     const int chunks = pick(ch), tiles = pick(tl), at = me - (pick(in) - chunks) * per_row;
     const int hb = uni(at / chunks), k = at - hb * chunks, base = uni(tiles / chunks), rem = tiles - base * chunks;
     const int first = k * base + min(k, rem), last = first + base + (k < rem);
-    att_part<D, F16, WIDE>(A, S, err, t, 1, pick(req), pick(tok), hb, first, last, chunks == 1, me);
+    att_part<D, F16, WIDE, F16 && WIDE ? 2 : 4>(A, S, err, t, 1, pick(req), pick(tok), hb, first, last, chunks == 1, me);
     if (k == 0 && threadIdx.x == 0) A.cut[t * per_row + hb] = (AttCut){ t, 1, hb, me, chunks == 1 ? 0 : chunks };
 }
 
@@ -609,8 +620,9 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
             pos1 = a.row_pos[t + 1];
         }
         const int t0 = uni(rows_first(a, T, shift, R, t)), nr = t - t0 + 1;
-        if (last > first)
-            att_part<D, F16, WIDE>(A, S, err, t0, nr, req, n, hb, first, last, first == 0 && last == tiles, 2 * blockIdx.x + (first == 0));
+        if (last > first)                              /* at dim 256 four sums would spill: 102 us instead of 94 (64 requests) */
+            att_part<D, F16, WIDE, F16 && (WIDE || D == 256) ? 2 : 4>(A, S, err, t0, nr, req, n, hb, first, last, first == 0 && last == tiles,
+                                                                 2 * blockIdx.x + (first == 0));
         if (tid == 0) {                                /* for the join: the shares of a unit begun and cut here */
             const int k = cuts ? (int)((at - x0 + ATT_LEAD + tiles - 1) / share) - (int)blockIdx.x + 1 : 0;
             const AttCut x = { t0, nr, hb, (int)blockIdx.x, k };
@@ -993,7 +1005,9 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
                 for (int k = 0; k < VJ; k++) vt[k] = at + (int)sizeof(s_t[0][0]) + vb[k];
                 {
-                    f32x4 acc[2] = {};
+                    /* a block's low parts first, whose small sums round little, and blocks apart: outputs
+                     * off by 0.5e-6, in one sum by 1.1e-6 */
+                    f32x4 acc[D == 256 ? 2 : 1][2] = {};
 #pragma unroll
                     for (int q = 0; q < (D == 256 ? 2 : 1); q++) {
                         constexpr int S = D == 64 ? 2 : 4;             /* products of a chain that one block's reads feed */
@@ -1006,13 +1020,19 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
                                 const f16x8 x = __builtin_bit_cast(f16x8, kf[u * S + s]);
-                                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[q * S + s], acc[u], 0, 0, 0);
-                                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[q * S + s], acc[u], 0, 0, 0);
+                                acc[q][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[q * S + s], acc[q][u], 0, 0, 0);
+                            }
+#pragma unroll
+                        for (int s = 0; s < S; s++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const f16x8 x = __builtin_bit_cast(f16x8, kf[u * S + s]);
+                                acc[q][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[q * S + s], acc[q][u], 0, 0, 0);
                             }
                     }
                     float p[8], mx = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) p[k] = acc[k / 4][k & 3];
+                    for (int k = 0; k < 8; k++) p[k] = D == 256 ? acc[0][k / 4][k & 3] + acc[D == 256][k / 4][k & 3] : acc[0][k / 4][k & 3];
                     if ((i + 1) * 32 > least) {
 #pragma unroll
                         for (int k = 0; k < 8; k++)
