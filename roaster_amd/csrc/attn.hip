@@ -31,6 +31,7 @@
  */
 #include "attn.h"
 #include "qdot.h"
+#include <type_traits>
 
 #define ATT_T 256
 #define ATT_W (ATT_T / 64)
@@ -339,7 +340,7 @@ __device__ __forceinline__ long long att_scan(long long v, long long *s_wave, lo
  * to 500 tokens 82 us without it, 47 with it).  A unit of n tiles lies on LEAD + n
  * places, its tiles on the last n. */
 #define ATT_LEAD 8
-#define ROWS_LEAD 4           /* of 32 tokens */
+#define ROWS_LEAD 12          /* of 32 tokens; 4 requests of 1000 rows: 444 us with 4, 295 with 12, 304 with 24 */
 
 /* Row t's request and tokens, and whether it goes on with the unit of row t - 1: runs of up to
  * R rows of one request, one behind the other with positions that do not fall, between
@@ -662,16 +663,18 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
  * once, straight from memory, for its eight waves of 16 columns (row, head), which
  * multiply every operand they read by their columns' high and low parts.  Shares, cuts
  * and the join go as in attn_kernel, a unit being a run and a block of heads.
- * What bounds it: a tile is 64 MFMAs and 32 KB of LDS reads a wave, 2048 cycles of the
- * matrix cores and as many of LDS, which overlap in part (4700 measured); of 256 rows
- * behind 2048 tokens (43 us) the tiles take 20 us, beginning 9, and the parts' way
- * through memory 10, 33 MB each way: 32 units on 256 CUs are cut in eight.  1024 rows of
- * one prompt take 71 us. */
+ * With HALVES 2 a run has half as many columns, and two waves share theirs, taking
+ * the tiles in turn and joining in LDS: half the bytes of parts, twice the tiles to bring.
+ * What bounds it: a tile is 64 MFMAs, 200 other vector instructions and 32 KB of LDS reads a
+ * wave, about 2 us of the two waves on a SIMD, a third of the matrix cores' rate; before a
+ * unit's first tile lie 9 to 12 us (rows, page, queries and tile, each a wait), behind its last 1 to
+ * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 43 us, 512 rows 63, a prompt of 1024
+ * 63, of 2000 126, four prompts' 1000 rows behind 0..3000 tokens 295. */
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
-#define ROWS_COLS 128         /* columns of a unit: 16 a wave */
-#define ROWS_PART(D) (ROWS_COLS * (D) / 4 + 80)       /* a part in units of four sums, off a power of two: its unit's parts are read together */
+#define ROWS_COLS 128         /* columns of a unit: 16 a wave; half as many where two waves share theirs */
+#define ROWS_PART(D, COLS) ((COLS) * (D) / 4 + 80)       /* a part in units of four sums, off a power of two: its unit's parts are read together */
 
 /* s_waitcnt's operand for no load and no store under way, LDS and exports not waited for. */
 #define ROWS_ALL_CAME ((7 << 4) | (15 << 8))
@@ -745,15 +748,17 @@ struct RowsArgs {
     float *pm, *pl, *po;      /* parts [2 ROWS_G][waves][16 columns], and [..][waves][D / 16][64 lanes][4]; slots as in AttArgs */
 };
 
-template <int D>
+template <int D, int HALVES>
 __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *err)
 {
     constexpr int CH = D / 8, KS = D / 32, NO = D / 16;   /* 16-byte pieces of a token; steps of a score; sums of a lane */
     constexpr int SW = CH < 16 ? CH : 16, KJ = SW / 4, VJ = SW / 2;
+    constexpr int GROUPS = ROWS_W / HALVES;        /* of 16 columns: HALVES waves each, taking its tiles in turn */
     __shared__ gu32x4 s_t[4][2][32 * CH];          /* tiles of keys and values: two in use, two under way */
     __shared__ long long s_wave[ROWS_W], s_at;
-    __shared__ int s_row, s_tiles, s_np, s_runs[ROWS_W];
-    __shared__ unsigned s_parts[ROWS_W];
+    __shared__ int s_row, s_tiles, s_np, s_req, s_n, s_runs[ROWS_W];
+    __shared__ int s_parts[ROWS_W];
+    __shared__ float4 s_try[ROWS_W];
     __shared__ unsigned long long s_join[ROWS_W];          /* the rows that go on with a run, a bit each */
     __shared__ float s_sum[ROWS_W];
     const RoasterAttnPaged &a = A.a;
@@ -766,12 +771,14 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
      * np equal parts of one unit (a share that two units meet in begins twice) */
     const int each = (rows + ROWS_T - 1) / ROWS_T;
     long long mine = 0, at = 0, end = 0, share = 1;
-    int tl = 0, np = 0, hb, x0;
+    int tl = 0, np = 0, hb, x0, req = 0, n = 0;
     auto places = [](int k) { return k ? ROWS_LEAD + k : 0; };
     if (each == 1) {                                   /* at most 512 runs, one a thread */
         const int G = gridDim.x, t = min(tid, rows - 1);
         const RowsAt x = rows_at(a, T, shift, R, t), y = rows_at(a, T, shift, R, min(t + 1, rows - 1));
         if (tid < rows) tl = rows_tiles<32>(x, t + 1 < rows && y.joined);
+        req = x.req;
+        n = x.n;
         mine = places(tl);
         const float some = group_sum<64>((float)tl);
         const unsigned long long on = __ballot(x.joined), runs = __ballot(tl > 0);
@@ -787,30 +794,45 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         for (int i = 0; i < ROWS_W; i++) { W += s_sum[i]; units += s_runs[i]; }
         W *= per_row;
         units *= per_row;
-        if (units > 0 && units <= G / 4) {
-            /* parts of S tiles: as small as all tiles over all workgroups if there are then not
-             * too many, else so that there cannot be, a unit of n tiles having ceil(n / S) (the
-             * quotients in f32: `hi` is taken a little too large) */
-            const unsigned lo = max(ATT_MIN, (int)ceilf(W / G)), hi = max(ATT_MIN, (int)(W * 1.0001f / (G - units)) + 1);
-            const unsigned p0 = (tl + lo - 1) / lo, p1 = (tl + hi - 1) / hi;
-            /* at most G + 512 and G parts, so both fit one word */
-            unsigned in = p0 | p1 << 16;
+        /* Equal parts of S tiles, S the least of five with no more parts than workgroups, a unit
+         * of n tiles having ceil(n / S): from all tiles over all workgroups to where there cannot
+         * be too many (the quotients in f32: `hi` is a little too large).  Worth it while its
+         * excess is less than a second beginning. */
+        const bool parts = units > 0 && units <= G - G / 4;
+        const unsigned lo = max(ATT_MIN, (int)ceilf(W / G)), hi = max(lo, (unsigned)(W * 1.0001f / max(G - units, G / 4)) + 1);
+        unsigned S = hi;
+        if (parts && hi > lo) {
+            const unsigned d = (hi - lo) / 8;
+            const unsigned at[4] = { lo, min(lo + max(1u, d), hi), min(lo + max(2u, 2 * d), hi), min(lo + max(3u, 4 * d), hi) };
+            float4 f;
+            f.x = group_sum<64>((float)((tl + at[0] - 1) / at[0]));
+            f.y = group_sum<64>((float)((tl + at[1] - 1) / at[1]));
+            f.z = group_sum<64>((float)((tl + at[2] - 1) / at[2]));
+            f.w = group_sum<64>((float)((tl + at[3] - 1) / at[3]));
+            if (lane == 0) s_try[w] = f;
+            __syncthreads();
+            f = s_try[0];
+#pragma unroll
+            for (int i = 1; i < ROWS_W; i++) { f.x += s_try[i].x; f.y += s_try[i].y; f.z += s_try[i].z; f.w += s_try[i].w; }
+            const float most = G / per_row;
+            S = f.x <= most ? at[0] : f.y <= most ? at[1] : f.z <= most ? at[2] : f.w <= most ? at[3] : hi;
+        }
+        if (parts && S <= lo + ROWS_LEAD) {
+            const int me = blockIdx.x, mp = (tl + S - 1) / S;
+            int upto = mp, all = 0;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const unsigned u = __shfl_up(in, o);
-                if (lane >= o) in += u;
+                const int u = __shfl_up(upto, o);
+                if (lane >= o) upto += u;
             }
-            if (lane == 63) s_parts[w] = in;
+            if (lane == 63) s_parts[w] = upto;
             __syncthreads();
-            unsigned all = 0;
 #pragma unroll
             for (int i = 0; i < ROWS_W; i++) {
-                if (i == w) in += all;
+                if (i == w) upto += all;
                 all += s_parts[i];
             }
-            const bool small = (int)(all & 0xffff) * per_row <= G;
-            const int mp = small ? p0 : p1, upto = small ? in & 0xffff : in >> 16, me = blockIdx.x;
-            if (me >= (int)(small ? all & 0xffff : all >> 16) * per_row) {
+            if (me >= all * per_row) {
                 if (tid == 0) A.cut[me].k = 0;
                 return;
             }
@@ -818,6 +840,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                 s_row = tid;
                 s_tiles = tl;
                 s_np = mp;
+                s_req = req;
+                s_n = n;
                 s_at = (upto - mp) * per_row;
             }
             __syncthreads();
@@ -852,15 +876,23 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                     b += places(tl) * (long long)per_row;
                     t++;
                 }
+            if (each > 1) {
+                req = a.row_req[t];
+                n = T.tokens(req, a.row_pos[t], shift);
+            }
             s_row = t;
             s_tiles = tl;
             s_at = b;
+            s_req = req;
+            s_n = n;
         }
         __syncthreads();
         hb = uni((int)((at - s_at) / (ROWS_LEAD + s_tiles)));
         x0 = uni((int)((at - s_at) % (ROWS_LEAD + s_tiles)));
     }
     int t1 = uni(s_row), tiles = uni(s_tiles);
+    req = uni(s_req);
+    n = uni(s_n);
     /* Where this lane's operands lie in a tile, in bytes: its key's piece 4 s + g at kb[s % KJ]
      * + 64 (s - s % KJ), its share of the values' 16 elements j at vb[j % VJ] + 32 (j - j % VJ):
      * four elements of token 4 g + c / 4.  (4 s + g) ^ r = 4 (s ^ r / 4) + (g ^ r % 4), and
@@ -896,7 +928,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                 on = j == ~0ull;
                 t0 -= on ? 64 : __builtin_ctzll(~j);
             }
-        const int nr = t1 - t0 + 1, req = uni(a.row_req[t1]), n = uni(T.tokens(req, a.row_pos[t1], shift));
+        const int nr = t1 - t0 + 1;
         const int kh = A.blocks == 1 ? hb : hb / A.blocks, bk = hb - kh * A.blocks, nh = min(A.hpb, A.group - bk * A.hpb);
         const int h0 = kh * A.group + bk * A.hpb;
         bool bad = n < 0;
@@ -943,7 +975,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             pages(min(first + 1, last - 1), pg[1]);
         }
         /* this lane's column */
-        const int ri = w * A.rpg + cr;
+        const int grp = HALVES == 1 ? w : w % GROUPS, half = HALVES == 1 ? 0 : w / GROUPS, ri = grp * A.rpg + cr;
         const bool on = cr < A.rpg && ri < nr && ch < nh;
         f16x8 qh[KS], ql[KS];
         f32x4 o[NO];
@@ -997,7 +1029,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                 bring(i0 + 2, buf ^ 2);
                 const int to = min(i0 + 2, mine);
 #pragma unroll 1
-                for (int i = i0; i < to; i++) {
+                for (int i = i0 + half; i < to; i += HALVES) {
                 const int at = (buf + i - i0) * (int)sizeof(s_t[0]);
                 int kt[4], vt[VJ];                     /* this tile's operands */
 #pragma unroll
@@ -1100,6 +1132,25 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         }
         const size_t slot = 2 * blockIdx.x + (first == 0);
         float sum = sum_g(l);
+        if constexpr (HALVES == 2) {                   /* the second half's sums to the first's waves */
+            f32x4 *t = (f32x4 *)s_t + grp * (NO + 1) * 64 + lane;
+            __syncthreads();                           /* the tiles in LDS are done with */
+            if (half) {
+#pragma unroll
+                for (int k = 0; k < NO; k++) t[k * 64] = o[k];
+                t[NO * 64] = (f32x4){ m, sum, 0, 0 };
+            }
+            __syncthreads();
+            if (!half) {
+                const f32x4 ml = t[NO * 64];
+                const float mn = fmaxf(m, ml[0]), f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn),
+                            f1 = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - mn);
+                sum = sum * f0 + ml[1] * f1;
+                m = mn;
+#pragma unroll
+                for (int k = 0; k < NO; k++) o[k] = o[k] * f0 + t[k * 64] * f1;
+            }
+        }
         if (__builtin_expect(bad, 0)) {
             /* NaN for rows of more tokens than there are before the first bad page, or if the row itself is bad */
             if (tid == 0) atomicOr(err, ATTN_ERR_INDEX);
@@ -1109,18 +1160,19 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             else if (nc <= 32 * first)                 /* met nothing but, maybe, a bad page's substitute */
                 for (int k = 0; k < NO; k++) o[k] = (f32x4){};
         }
-        if (whole) {
+        if (half) {
+        } else if (whole) {
             if (on)
 #pragma unroll
                 for (int k = 0; k < NO; k++) att_store(a, D, t0 + ri, h0 + ch, 16 * k + 4 * g, o[k], nc == 0 ? 1.0f : sum);
         } else {                                       /* as the registers lie: the join needs no other order */
-            const size_t at = slot * ROWS_W + w;
+            const size_t at = slot * GROUPS + grp;
             if (g == 0) {
                 A.pm[at * 16 + c] = m;
                 A.pl[at * 16 + c] = sum;
             }
 #pragma unroll
-            for (int k = 0; k < NO; k++) ((f32x4 *)A.po)[slot * ROWS_PART(D) + (w * NO + k) * 64 + lane] = o[k];
+            for (int k = 0; k < NO; k++) ((f32x4 *)A.po)[slot * ROWS_PART(D, 16 * GROUPS) + (grp * NO + k) * 64 + lane] = o[k];
         }
         at += x1 - x0;
         if (tid == 0 && at == end) {
@@ -1140,6 +1192,8 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                 t1 += on ? 64 : 1 + i;
                 tiles = __builtin_amdgcn_readlane(k, i);
             }
+            req = uni(a.row_req[t1]);
+            n = uni(T.tokens(req, a.row_pos[t1], shift));
         }
     }
 }
@@ -1149,10 +1203,10 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
  * come first in the grid: with equal parts every eighth share, say, begins a unit, and
  * the workgroups of those would all be on one XCD (the join of 256 rows' parts 38 us
  * instead of 14). */
-template <int D>
+template <int D, int HALVES>
 __global__ __launch_bounds__(64) void attn_rows_join_kernel(RowsArgs A)
 {
-    constexpr int NO = D / 16;
+    constexpr int NO = D / 16, GROUPS = ROWS_W / HALVES;
     const RowsCut x = A.cut[blockIdx.y];
     const int w = blockIdx.x / (NO / 4), q = blockIdx.x % (NO / 4), lane = threadIdx.x, c = lane & 15, g = lane >> 4, g0 = blockIdx.y;
     const int cr = c / A.hpb, ch = c - cr * A.hpb, ri = w * A.rpg + cr;
@@ -1160,35 +1214,40 @@ __global__ __launch_bounds__(64) void attn_rows_join_kernel(RowsArgs A)
     if (x.k == 0 || cr >= A.rpg || ri >= x.n || ch >= A.group - bk * A.hpb) return;
     float m = -INFINITY, l = 0;
     f32x4 y[4] = {};
-    for (int k0 = 0; k0 < x.k; k0 += 8) {
-        float pm[8], pl[8];
-        f32x4 po[8][4];
+    auto join = [&](auto N) {                          /* N parts at a time */
+        for (int k0 = 0; k0 < x.k; k0 += N()) {
+            float pm[N()], pl[N()];
+            f32x4 po[N()][4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int k = min(k0 + j, x.k - 1);
-            const size_t sl = k ? 2 * (g0 + k) : 2 * g0 + 1, at = sl * ROWS_W + w;
-            pm[j] = k0 + j < x.k ? A.pm[at * 16 + c] : -INFINITY;
-            pl[j] = A.pl[at * 16 + c];
+            for (int j = 0; j < N(); j++) {
+                const int k = min(k0 + j, x.k - 1);
+                const size_t sl = k ? 2 * (g0 + k) : 2 * g0 + 1, at = sl * GROUPS + w;
+                pm[j] = k0 + j < x.k ? A.pm[at * 16 + c] : -INFINITY;
+                pl[j] = A.pl[at * 16 + c];
 #pragma unroll
-            for (int z = 0; z < 4; z++) po[j][z] = ((const f32x4 *)A.po)[sl * ROWS_PART(D) + (w * NO + 4 * q + z) * 64 + lane];
+                for (int z = 0; z < 4; z++) po[j][z] = ((const f32x4 *)A.po)[sl * ROWS_PART(D, 16 * GROUPS) + (w * NO + 4 * q + z) * 64 + lane];
+            }
+            float mn = m;
+#pragma unroll
+            for (int j = 0; j < N(); j++) mn = fmaxf(mn, pm[j]);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+#pragma unroll
+            for (int z = 0; z < 4; z++) y[z] *= f;
+#pragma unroll
+            for (int j = 0; j < N(); j++) {
+                if (k0 + j >= x.k) continue;
+                const float p = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
+                l += pl[j] * p;
+#pragma unroll
+                for (int z = 0; z < 4; z++) y[z] += po[j][z] * p;
+            }
+            m = mn;
         }
-        float mn = m;
-#pragma unroll
-        for (int j = 0; j < 8; j++) mn = fmaxf(mn, pm[j]);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        l *= f;
-#pragma unroll
-        for (int z = 0; z < 4; z++) y[z] *= f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (k0 + j >= x.k) continue;
-            const float p = pm[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[j] - mn);
-            l += pl[j] * p;
-#pragma unroll
-            for (int z = 0; z < 4; z++) y[z] += po[j][z] * p;
-        }
-        m = mn;
-    }
+    };
+    if (x.k == 2) join(std::integral_constant<int, 2>());
+    else if (x.k <= 4) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, 8>());
     const int t = x.row + ri;
     const float sum = A.a.row_pos[t] == -1 ? 1.0f : l;
 #pragma unroll
@@ -1272,15 +1331,16 @@ extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCa
 {
     if (!attn_cache_ok(c) || rows < 0 || rows > (1 << 20) || q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads) return 0;
     const size_t one = ATT_CUT + 2 * ATT_ML + (size_t)2 * ATT_G * 16 * c->head_dim * 4,
-                 run = ROWS_CUT + 2 * ROWS_ML + (size_t)2 * ROWS_G * ROWS_PART(c->head_dim) * 16;
+                 run = ROWS_CUT + 2 * ROWS_ML + (size_t)2 * ROWS_G * ROWS_PART(c->head_dim, ROWS_COLS) * 16;
     return rows_may(rows, c->type) && run > one ? run : one;
 }
 
-template <int D>
-static void rows_launch(const RowsArgs &A, int *err)
+template <int D, int HALVES>
+static void rows_launch(RowsArgs &A, int *err)
 {
-    hipLaunchKernelGGL((attn_rows_kernel<D>), dim3(ROWS_G), dim3(ROWS_T), 0, rt().stream, A, err);
-    hipLaunchKernelGGL((attn_rows_join_kernel<D>), dim3(ROWS_W * D / 64, ROWS_G), dim3(64), 0, rt().stream, A);
+    A.R = ROWS_W / HALVES * A.rpg;
+    hipLaunchKernelGGL((attn_rows_kernel<D, HALVES>), dim3(ROWS_G), dim3(ROWS_T), 0, rt().stream, A, err);
+    hipLaunchKernelGGL((attn_rows_join_kernel<D, HALVES>), dim3(ROWS_W / HALVES * D / 64, ROWS_G), dim3(64), 0, rt().stream, A);
 }
 
 template <int D, bool F16, bool WIDE>
@@ -1338,14 +1398,18 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
         A.hpb = A.group < 16 ? A.group : 16;
         A.blocks = (A.group + A.hpb - 1) / A.hpb;
         A.rpg = 16 / A.hpb;
-        A.R = ROWS_W * A.rpg;
         A.cut = (RowsCut *)p->ws;
         A.pm = (float *)((char *)p->ws + ROWS_CUT);
         A.pl = (float *)((char *)p->ws + ROWS_CUT + ROWS_ML);
         A.po = (float *)((char *)p->ws + ROWS_CUT + 2 * ROWS_ML);
-        if (D == 256) rows_launch<256>(A, err);
-        else if (D == 128) rows_launch<128>(A, err);
-        else rows_launch<64>(A, err);
+        /* Few units are cut into many parts: 16 rows behind 2048 tokens take 24 us in halves and 26
+         * without, 8 requests of six rows 45 and 50, 256 rows 43 and 44, but 512 rows 68 and 63. */
+        const bool halves = (long long)p->rows * A.hpb * A.blocks * c->kv_heads <= ROWS_G / 8 * ROWS_COLS;
+#define ROWS(DD) (halves ? rows_launch<DD, 2>(A, err) : rows_launch<DD, 1>(A, err))
+        if (D == 256) ROWS(256);
+        else if (D == 128) ROWS(128);
+        else ROWS(64);
+#undef ROWS
         return rt_check(hipGetLastError(), "attention launch") ? ROASTER_EDEVICE : 0;
     }
     AttArgs A;
