@@ -748,6 +748,15 @@ struct RowsArgs {
     float *pm, *pl, *po;      /* parts [2 ROWS_G][waves][16 columns], and [..][waves][D / 16][64 lanes][4]; slots as in AttArgs */
 };
 
+/* What the pieces' numbers in row r of 16 are turned by: keys' reads take one piece of
+ * each row, values' two neighbours of eight rows (0..7 or 8..15), each all over the banks, 16
+ * pieces wide.  A row of 64 elements is half as wide. */
+template <int SW>
+__device__ __forceinline__ int rows_turn(int r)
+{
+    return SW == 16 ? (r & 7) << 1 | r >> 3 : (r & 6) | r >> 3;
+}
+
 template <int D, int HALVES>
 __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *err)
 {
@@ -898,12 +907,13 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
      * four elements of token 4 g + c / 4.  (4 s + g) ^ r = 4 (s ^ r / 4) + (g ^ r % 4), and
      * alike for the pieces 2 j + (c & 2) / 2. */
     int kb[KJ], vb[VJ];
-    const int t0_at = (int)(uintptr_t)(__attribute__((address_space(3))) void *)&s_t[0][0][0], vr = 4 * g + c / 4;
+    const int t0_at = (int)(uintptr_t)(__attribute__((address_space(3))) void *)&s_t[0][0][0], vr = 4 * g + c / 4,
+              fk = rows_turn<SW>(c), fv = rows_turn<SW>(vr);
 #pragma unroll
-    for (int k = 0; k < KJ; k++) kb[k] = t0_at + (c * CH + 4 * (k ^ (c % SW) / 4) + (g ^ c % 4)) * 16;
+    for (int k = 0; k < KJ; k++) kb[k] = t0_at + (c * CH + 4 * (k ^ fk / 4) + (g ^ fk % 4)) * 16;
 #pragma unroll
     for (int k = 0; k < VJ; k++)
-        vb[k] = t0_at + (vr * CH + 2 * (k ^ (vr % SW) / 2) + ((c >> 1 & 1) ^ (vr & 1))) * 16 + 8 * (c & 1);
+        vb[k] = t0_at + (vr * CH + 2 * (k ^ fv / 2) + ((c >> 1 & 1) ^ (fv & 1))) * 16 + 8 * (c & 1);
     const int cr = c / A.hpb, ch = c - cr * A.hpb;                      /* this lane's column: its row and head within the group */
     while (1) {
         /* places [x0, x1) and tiles [first, last) of this unit */
@@ -955,15 +965,15 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
             }
         };
         /* The tile's 64 CH pieces straight into LDS, 64 to a wave and load, in the order
-         * they lie there: piece x of a token's row lies at x ^ (row % SW), so that the rows
-         * which an operand read takes fall on different banks.  A load's rows lie in one
+         * they lie there: piece x of a token's row lies at x ^ rows_turn(row), so that what
+         * an operand read takes falls on different banks.  A load's rows lie in one
          * 16-token part. */
         auto fetch = [&](int buf, const size_t *b) {
 #pragma unroll
             for (int i = 0; i < CH / ROWS_W; i++) {
                 const int q = i * ROWS_W + w, v = q >= CH / 2, at = (q - v * (CH / 2)) * 64, row = (at + lane) / CH;
                 const char *from = (v ? A.vc : A.kc) + (at / CH < 16 ? b[0] : b[1]);
-                const unsigned off = ((row & 15) * CH + ((at + lane) % CH ^ row % SW)) * 16;
+                const unsigned off = ((row & 15) * CH + ((at + lane) % CH ^ rows_turn<SW>(row & 15))) * 16;
                 __builtin_amdgcn_global_load_lds((const GAS void *)(from + off),
                                                  (__attribute__((address_space(3))) void *)&s_t[buf][v][at], 16, 0, 0);
             }
