@@ -251,6 +251,17 @@ def test_a_bad_page_is_of_the_rows_that_reach_it(f16, T, at):
     check_attn(got[good], *want, int(pos[-1]) + 1, 128)
 
 
+@pytest.mark.parametrize("H,KV,D,lens,each", [
+    (2, 1, 64, [730], 700),                            # more rows than a workgroup has threads, few columns
+    (32, 8, 128, [600], 512),                          # 128 units in equal parts
+    (4, 4, 64, [900, 40, 17, 300, 2000], 40),          # unequal requests
+    (16, 2, 64, [5000] + [24] * 30, 24),               # one long request among short ones: equal parts would be too long
+])
+def test_chunks_of_every_split(H, KV, D, lens, each):
+    rows = [(r, max(l - each, 0) + i) for r, l in enumerate(lens) for i in range(min(each, l))]
+    run_case(lens, rows, H, KV, D, 32, True, gate=True)
+
+
 def test_cache_past_32_bit_offsets():
     """Pages beyond 2^32 elements of a cache of 9 GB for the keys and as much for the values."""
     L = R.lib()
