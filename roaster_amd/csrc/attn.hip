@@ -666,10 +666,11 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
  * With HALVES 2 a run has half as many columns, and two waves share theirs, taking
  * the tiles in turn and joining in LDS: half the bytes of parts, twice the tiles to bring.
  * What bounds it: a tile is 64 MFMAs, 200 other vector instructions and 32 KB of LDS reads a
- * wave, about 2 us of the two waves on a SIMD, a third of the matrix cores' rate; before a
+ * wave, about 2 us of the two waves on a SIMD, a third of the matrix cores' rate (each wave a
+ * chain of reads, products and softmax, which 256 registers let no third wave fill); before a
  * unit's first tile lie 9 to 12 us (rows, page, queries and tile, each a wait), behind its last 1 to
- * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 43 us, 512 rows 63, a prompt of 1024
- * 63, of 2000 126, four prompts' 1000 rows behind 0..3000 tokens 295. */
+ * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 42 us, 512 rows 62, a prompt of 1024
+ * 61, of 2000 123, four prompts' 1000 rows behind 0..3000 tokens 290. */
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
