@@ -134,9 +134,10 @@ int roaster_qk_rope_store(const RoasterQkRope *rope, const RoasterKvCache *cache
  * and probabilities enter the products with 22 bits (two fp16 parts).  How a call's
  * work is split goes by all its rows: the last bits of a row's output depend on
  * them, and are the same for the same call.
- * An fp16 call of 16 rows or more, and of four times n_req or more, takes the rows
- * of a request that stand together together (16 query heads on 2: 16 rows at a
- * time); it is right, but slow, where most of its rows are one to a request.
+ * An fp16 call of 16 rows or more, and of more rows for each of the n_req requests than
+ * 16 / (q_heads / kv_heads), two at least, takes the rows of a request that stand
+ * together together (8 query heads on one: 8 or 16 rows at a time); it is right, but slow,
+ * where most of its rows are one to a request.
  * gate: element d of head h of row t at [t * gate_row + h * gate_head + d].
  * out and ws must not overlap the inputs.  rows = 0 does nothing. */
 typedef struct {

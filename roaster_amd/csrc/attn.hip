@@ -1396,10 +1396,14 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     const AttnDevice dev;
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
-    /* Runs of rows pay where requests have several rows each, which the two counts
-     * tell on average (a call of other rows is right as well, only slower): 256 rows behind
-     * 2048 tokens take 43 us so, 114 row by row. */
-    if (rows_may(p->rows, c->type) && p->rows >= 4 * (long long)p->n_req) {
+    /* Runs of rows pay where requests have more rows each than sixteen columns hold, which
+     * the two counts tell on average (a call of other rows is right as well, only slower): 256
+     * rows behind 2048 tokens take 42 us so, 99 otherwise; requests of 300..16000 tokens and 8
+     * heads (two rows fill the columns) with three rows 56 and 71, with two 75 and 73; with 4
+     * heads (four rows do) and 75..4000 tokens four rows 53 and 42, six 63 and 67; with 16, 77 and
+     * 113 for two rows. */
+    const int per16 = 16 / std::min(p->q_heads / c->kv_heads, 16);
+    if (rows_may(p->rows, c->type) && p->rows >= std::max(2, per16 + 1) * (long long)p->n_req) {
         RowsArgs A;
         A.a = *p;
         A.kc = (const char *)c->k;
@@ -1408,7 +1412,7 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
         A.group = p->q_heads / c->kv_heads;
         A.hpb = A.group < 16 ? A.group : 16;
         A.blocks = (A.group + A.hpb - 1) / A.hpb;
-        A.rpg = 16 / A.hpb;
+        A.rpg = per16;
         A.cut = (RowsCut *)p->ws;
         A.pm = (float *)((char *)p->ws + ROWS_CUT);
         A.pl = (float *)((char *)p->ws + ROWS_CUT + ROWS_ML);
