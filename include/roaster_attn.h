@@ -126,9 +126,7 @@ int roaster_qk_rope_store(const RoasterQkRope *rope, const RoasterKvCache *cache
  * are a draft or a prompt's chunk.  row_pos[t] = -1: no position, out is 0.
  * row_req[t] = -1: the row is skipped, out untouched.  A request, position or
  * page number out of range gives that row NaN outputs and is reported.
- * Keys and values behind the positions that a request's rows of the call attend to
- * are never used, whatever they hold; between a row's own position and the last of
- * its request's rows in the call, values must be finite (they are multiplied by 0).
+ * Keys and values behind a row's position are never used, whatever they hold.
  * Infinite or NaN keys and values in use make the elements that they reach
  * infinite or NaN.  Sums and softmax are in 32 bits; with an fp16 cache the queries
  * and probabilities enter the products with 22 bits (two fp16 parts).  How a call's

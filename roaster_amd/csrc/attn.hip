@@ -132,6 +132,9 @@ __device__ __forceinline__ float split_q(const float4 *x, f16x8 *hi, f16x8 *lo, 
     return __builtin_bit_cast(float, (127 - e) << 23);
 }
 
+/* Not 0 if one of two fp16 values is infinite or NaN. */
+__device__ __forceinline__ unsigned odd_half(unsigned x) { return (x & 0x7c007c00u) + 0x04000400u & 0x80008000u; }
+
 /* One wave's state of a unit: lane (c = lane % 16, g = lane / 16) holds column c. */
 template <int D, bool F16, bool WIDE>
 struct AttWave {
@@ -259,6 +262,22 @@ struct AttWave {
             l += s[j];
         }
     }
+    /* Whether the tile's first `left` tokens have infinite or NaN values. */
+    __device__ bool odd(int left, int g)
+    {
+        unsigned x = 0;
+#pragma unroll
+        for (int j = 0; j < C::VT; j++) {
+            unsigned y = 0;
+#pragma unroll
+            for (int n = 0; n < C::NB; n++)
+#pragma unroll
+                for (int i = 0; i < C::VE * C::SZ / 4; i++)
+                    y |= F16 ? odd_half(v[j][n][i]) : (v[j][n][i] & 0x7f800000u) + 0x00800000u & 0x80000000u;
+            x |= 4 * g + j < left ? y : 0;
+        }
+        return __any(x != 0);
+    }
     __device__ void values(const float *p, int left, int c, int g)
     {
         if (left < C::TT)                              /* what lies behind the rows or a bad page may be anything: 0 * NaN is NaN */
@@ -385,7 +404,7 @@ struct AttLds {
     static constexpr int COLS = WIDE ? 16 : 8, KEYS = 16 * D * (F16 ? 2 : 4), SUMS = COLS * (D + 4) * 4;
     gu32x4 own[ATT_W][(KEYS > SUMS ? KEYS : SUMS) / 16];
     float m[ATT_W][COLS], l[ATT_W][COLS];
-    int n[COLS], good[ATT_W];
+    int n[COLS], good[ATT_W], odd[ATT_W];
     __device__ float *sums(int w, int h) { return (float *)own[w] + h * (D + 4); }
 };
 
@@ -404,10 +423,12 @@ __device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int 
 }
 
 /* Tiles [first, last) of the unit of rows t0 .. t0 + nr - 1 and head block hb by one
- * workgroup: to out if that is all of them, else to part `slot`.  n: tokens of its last row. */
+ * workgroup: to out if that is all of them, else to part `slot` from column `off` on.  n: tokens
+ * of its last row.  Gives back whether it found infinite or NaN values that some of the rows use and
+ * others must not (0 * NaN is NaN): then it has written nothing, and the rows go one by one. */
 template <int D, bool F16, bool WIDE, int N>
-__device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> &S, int *err, int t0, int nr, int req, int n, int hb,
-                                         int first, int last, bool whole, int slot)
+__device__ __forceinline__ bool att_part(const AttArgs &A, AttLds<D, F16, WIDE> &S, int *err, int t0, int nr, int req, int n, int hb,
+                                         int first, int last, bool whole, int slot, int off)
 {
     using C = AttCfg<D, F16, WIDE>;
     const RoasterAttnPaged &a = A.a;
@@ -421,6 +442,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
     int nc = n;
     if (WIDE && nr > 1) nc = on ? T.tokens(req, a.row_pos[t0 + cr], shift) : 0;
     int good = n < 0 ? -2 : n;     /* tokens before the first bad page: rows of more are NaN, all if the row itself is bad */
+    int odd = 0;
     AttWave<D, F16, WIDE> wv;
     typename AttWave<D, F16, WIDE>::Raw raw;
     /* the page of tile i, then the byte at which the tile begins */
@@ -457,6 +479,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
             }
             wv.template scores<N>(s, S.own[w], c, g);
             wv.soften(s, nc - i * 16, least < (i + 1) * 16, g);
+            if (WIDE && nr > 1 && least < (i + 1) * 16 && wv.odd(good - i * 16, g)) odd = 1;
             wv.values(s, good - i * 16, c, g);
             if (!more) break;
             wv.load_v(A.vc, b, c, g);
@@ -470,7 +493,7 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
         S.l[w][c] = l;
         if (w == 0) S.n[c] = nc;
     }
-    if (lane == 0) S.good[w] = good;
+    if (lane == 0) { S.good[w] = good; S.odd[w] = odd; }
     if constexpr (F16 && !WIDE) wv.add_parts();
 #pragma unroll
     for (int b = 0; b < C::NB; b++)
@@ -484,6 +507,10 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
                                     wv.o[b * C::VE + e + 3][i]);
     __syncthreads();
     for (int i = 0; i < ATT_W; i++) good = min(good, S.good[i]);
+    if (WIDE && nr > 1) {
+        for (int i = 0; i < ATT_W; i++) odd |= S.odd[i];
+        if (odd) return true;
+    }
     if (good < n && tid == 0) atomicOr(err, ATTN_ERR_INDEX);
     for (int idx = tid * 4; idx < C::COLS * D; idx += ATT_T * 4) {
         const int h = idx / D, d = idx % D, row = WIDE ? h / A.hpb : 0, head = h - row * A.hpb;
@@ -501,13 +528,14 @@ __device__ __forceinline__ void att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
         if (S.n[h] > good) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
         if (whole) att_store(a, D, t0 + row, h0 + head, d, y, S.n[h] == 0 ? 1.0f : sum);      /* without positions: y is 0 */
         else {
-            *(f32x4 *)(A.po + ((size_t)slot * C::COLS + h) * D + d) = y;
+            *(f32x4 *)(A.po + ((size_t)slot * C::COLS + off + h) * D + d) = y;
             if (d == 0) {
-                A.pm[slot * C::COLS + h] = mx;
-                A.pl[slot * C::COLS + h] = sum;
+                A.pm[slot * C::COLS + off + h] = mx;
+                A.pl[slot * C::COLS + off + h] = sum;
             }
         }
     }
+    return false;
 }
 
 /* Few units (at most an eighth of the workgroups, of at most 128 rows): every workgroup
@@ -557,7 +585,7 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kern
     const int chunks = pick(ch), tiles = pick(tl), at = me - (pick(in) - chunks) * per_row;
     const int hb = uni(at / chunks), k = at - hb * chunks, base = uni(tiles / chunks), rem = tiles - base * chunks;
     const int first = k * base + min(k, rem), last = first + base + (k < rem);
-    att_part<D, F16, WIDE, F16 && WIDE ? 2 : 4>(A, S, err, t, 1, pick(req), pick(tok), hb, first, last, chunks == 1, me);
+    att_part<D, F16, WIDE, F16 && WIDE ? 2 : 4>(A, S, err, t, 1, pick(req), pick(tok), hb, first, last, chunks == 1, me, 0);
     if (k == 0 && threadIdx.x == 0) A.cut[t * per_row + hb] = (AttCut){ t, 1, hb, me, chunks == 1 ? 0 : chunks };
 }
 
@@ -621,9 +649,20 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
             pos1 = a.row_pos[t + 1];
         }
         const int t0 = uni(rows_first(a, T, shift, R, t)), nr = t - t0 + 1;
-        if (last > first)                              /* at dim 256 four sums would spill: 102 us instead of 94 (64 requests) */
-            att_part<D, F16, WIDE, F16 && (WIDE || D == 256) ? 2 : 4>(A, S, err, t0, nr, req, n, hb, first, last, first == 0 && last == tiles,
-                                                                 2 * blockIdx.x + (first == 0));
+        if (last > first) {
+            int t = t0, rows_n = nr, row_n = n;        /* the unit's rows together, or one by one */
+            while (1) {
+                /* at dim 256 four sums of scores would spill: 102 us instead of 94 (64 requests) */
+                const bool odd = att_part<D, F16, WIDE, F16 && (WIDE || D == 256) ? 2 : 4>(
+                    A, S, err, t, rows_n, req, row_n, hb, first, last, first == 0 && last == tiles, 2 * blockIdx.x + (first == 0),
+                    (t - t0) * A.hpb);
+                if (!WIDE || (rows_n == nr && !odd) || (rows_n != nr && t == t0 + nr - 1)) break;
+                t = rows_n == nr ? t0 : t + 1;
+                rows_n = 1;
+                row_n = uni(T.tokens(req, a.row_pos[t], shift));
+                __syncthreads();                       /* S is free again */
+            }
+        }
         if (tid == 0) {                                /* for the join: the shares of a unit begun and cut here */
             const int k = cuts ? (int)((at - x0 + ATT_LEAD + tiles - 1) / share) - (int)blockIdx.x + 1 : 0;
             const AttCut x = { t0, nr, hb, (int)blockIdx.x, k };
@@ -1120,6 +1159,32 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
                                 const unsigned m0 = in >= 2 ? ~0u : in == 1 ? 0xffffu : 0u, m1 = in >= 4 ? ~0u : in == 3 ? 0xffffu : 0u;
 #pragma unroll
                                 for (int z = 0; z < NV; z++) { v[z][u].x &= m0; v[z][u].y &= m1; }
+                            }
+                        }
+                        if ((i + 1) * 32 > least) {    /* tokens that some of the wave's rows use and others must not */
+                            unsigned odd = 0;
+#pragma unroll
+                            for (int z = 0; z < NV; z++)
+                                odd |= odd_half(v[z][0].x) | odd_half(v[z][0].y) | odd_half(v[z][1].x) | odd_half(v[z][1].y);
+                            if (__any(odd != 0)) {     /* 0 * NaN is NaN: row by row, each with its own tokens' values alone */
+#pragma unroll 1
+                                for (int r = 0; r < A.rpg; r++) {
+                                    const int in = __builtin_amdgcn_readlane(nc, r * A.hpb) - i * 32 - 4 * g;
+#pragma unroll
+                                    for (int z = 0; z < NV; z++) {
+                                        gu32x4 x;
+#pragma unroll
+                                        for (int u = 0; u < 2; u++) {
+                                            const int k = in - 16 * u;
+                                            x[2 * u] = v[z][u].x & (k >= 2 ? ~0u : k == 1 ? 0xffffu : 0u);
+                                            x[2 * u + 1] = v[z][u].y & (k >= 4 ? ~0u : k == 3 ? 0xffffu : 0u);
+                                        }
+                                        f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), ph, (f32x4){}, 0, 0, 0);
+                                        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pl, y, 0, 0, 0);
+                                        if (cr == r) o[8 * q + z] += y;
+                                    }
+                                }
+                                continue;
                             }
                         }
 #pragma unroll

@@ -262,6 +262,34 @@ def test_chunks_of_every_split(H, KV, D, lens, each):
     run_case(lens, rows, H, KV, D, 32, True, gate=True)
 
 
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("H,KV,D", [(16, 2, 256), (32, 8, 128), (4, 4, 64)])
+@pytest.mark.parametrize("n,each", [(1, 3), (1, 40), (40, 2), (40, 3), (20, 5)])
+def test_odd_values_reach_only_the_rows_that_use_them(n, each, H, KV, D, f16):
+    """Infinite and NaN values at positions of a call's own rows: the rows before them are
+    right, in those from there on the elements of these values are infinite or NaN, the others right."""
+    rng = np.random.default_rng(n + each + D)
+    lens = [int(l) for l in rng.integers(each, 260, n)]
+    kc, vc, table = make(rng, lens, KV, D, 16, f16)
+    rows = np.array([(r, l - each + i) for r, l in enumerate(lens) for i in range(each)], np.int32)
+    for r, l in enumerate(lens):
+        if r % 4 != 3:
+            at = l - each + 1 + int(rng.integers(0, each - 1))
+            for e in rng.integers(0, D, 4):
+                vc[table[r, at // 16], :, at % 16, e] = [np.nan, np.inf, -np.inf][int(e) % 3]
+    q = rng.standard_normal((len(rows), H, D)).astype(np.float32)
+    a = Attn(Cache(kc, vc), q, rows[:, 0].copy(), rows[:, 1].copy(), table, D ** -0.5)
+    R.check(a.call(), "attn")
+    sync()
+    got = a.out.get()
+    with np.errstate(invalid="ignore"):
+        want, mass, reach = attn_oracle(q, kc, vc, table, rows[:, 0], rows[:, 1], np.float64(np.float32(D ** -0.5)))
+    fin = np.isfinite(want)
+    assert not fin.all() and fin[::each].all()
+    assert np.array_equal(np.isfinite(got), fin)
+    check_attn(np.where(fin, got, 0), np.where(fin, want, 0), np.where(fin, mass, 0), reach, 260, D)
+
+
 def test_cache_past_32_bit_offsets():
     """Pages beyond 2^32 elements of a cache of 9 GB for the keys and as much for the values."""
     L = R.lib()
