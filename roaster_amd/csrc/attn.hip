@@ -708,8 +708,8 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
  * wave, about 2 us of the two waves on a SIMD, a third of the matrix cores' rate (each wave a
  * chain of reads, products and softmax, which 256 registers let no third wave fill); before a
  * unit's first tile lie 9 to 12 us (rows, page, queries and tile, each a wait), behind its last 1 to
- * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 42 us, 512 rows 62, a prompt of 1024
- * 61, of 2000 123, four prompts' 1000 rows behind 0..3000 tokens 290. */
+ * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 43 us, 512 rows 62, a prompt of 1024
+ * 62, of 2000 124, four prompts' 1000 rows behind 0..3000 tokens 291. */
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
