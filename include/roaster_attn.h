@@ -129,7 +129,11 @@ int roaster_qk_rope_store(const RoasterQkRope *rope, const RoasterKvCache *cache
  * Keys and values behind a row's position are never used, whatever they hold.
  * Infinite or NaN keys and values in use make the elements that they reach
  * infinite or NaN.  Sums and softmax are in 32 bits; with an fp16 cache the queries
- * and probabilities enter the products with 22 bits (two fp16 parts).  How a call's
+ * enter the products with 22 bits (two fp16 parts, relative to the row's largest element),
+ * and probabilities off by at most 2^-22 of themselves or 2^-24 of the largest in
+ * their tile (up to 32 positions one behind the other).  Where a position outweighs all
+ * before it, those in its tile are off by up to 2^-38 of its probability, and tiles
+ * below 2^-70 of it may be left out.  How a call's
  * work is split goes by all its rows: the last bits of a row's output depend on
  * them, and are the same for the same call.
  * An fp16 call of 16 rows or more, and of more rows for each of the n_req requests than

@@ -37,9 +37,20 @@
 #define ATT_W (ATT_T / 64)
 #define ATT_G 512             /* workgroups at most: two per CU */
 #define ATT_MIN 4             /* tiles of a share at least: one a wave */
-#define P_UP 7.0f             /* probabilities are kept times 2^7 (relative to the running maximum, which they
-                                 may pass by 2^8): the low fp16 part of one of 2^-10 is still normal */
-#define M_LATE 8.0f           /* the running maximum moves only when a score passes it by this much */
+/* A column's terms are 2^(score - m) with a base m that follows its scores, its sums keeping the base's
+ * scale.  fp16: a term is kept times 2^13 and may reach 2^15; its two parts hold 22 bits of it down to 2^-3
+ * and are off by 2^-25 below.  So the base goes up when a score passes it by LATE octaves, and down when
+ * all of a tile stays M_DOWN below it: a term is then off by at most 2^-22 of itself or 2^-24 of its
+ * tile's largest, also behind a position that outweighs the rest by 2^20 and whose value is nothing;
+ * only in that position's own tile it is 2^-38 of the position's term.  (With a base that only rises
+ * and terms up to 2^15 at LATE 8, a first position 2^22 above 700 others, its value 0, left outputs off by
+ * 1.5e-4; so 1.4e-6.  It costs a prompt's rows 3%, single tokens nothing.) */
+template <bool F16>
+struct Soft {
+    static constexpr float UP = F16 ? 13.0f : 7.0f, LATE = F16 ? 2.0f : 8.0f;
+};
+#define M_DOWN 14.0f
+#define M_MID 6.0f            /* a base that goes down stays this much above the tile's largest, for the next ones */
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -130,6 +141,31 @@ __device__ __forceinline__ float split_q(const float4 *x, f16x8 *hi, f16x8 *lo, 
         if constexpr (BOTH) lo[i] = join8(r);
     }
     return __builtin_bit_cast(float, (127 - e) << 23);
+}
+
+/* Moves the bases of a wave's columns for a tile where one has to, mx being a lane's largest score, and
+ * the sums l along; w is what a column's other sums are to be multiplied by, if it says so.  Bases are
+ * whole, so that this rounds nothing.  Down only while the sums stay below 2^80 (values: 2^96). */
+template <bool F16>
+__device__ __forceinline__ bool base_moves(float mx, float &m, float &l, float &w)
+{
+    bool down = false;
+    if (F16) {
+        const unsigned long long near = __ballot(!(mx < m - M_DOWN));
+        const unsigned c = (unsigned)near | (unsigned)(near >> 32);
+        down = ((c | c >> 16) & 0xffff) != 0xffff;
+    }
+    if (!down && !__any(mx > m + Soft<F16>::LATE)) return false;
+    const float top = floorf(max_g(mx));
+    float to = fmaxf(m, top);
+    if (down) {
+        const float sum = max_g(l) * __builtin_amdgcn_exp2f(m - (top + M_MID));
+        if (top < m - M_DOWN && top > -INFINITY && sum <= 0x1p80f) to = top + M_MID;       /* -inf: no position in the tile */
+    }
+    w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+    l *= w;
+    m = to;
+    return true;
 }
 
 /* Not 0 if one of two fp16 values is infinite or NaN. */
@@ -249,14 +285,11 @@ struct AttWave {
                 if (4 * g + j >= left) s[j] = -INFINITY;
         for (int j = 0; j < C::VT; j++) mx = fmaxf(mx, s[j]);
         mx *= fac;
-        if (__any(mx > m + M_LATE)) {
-            const float mn = fmaxf(m, max_g(mx)), w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            l *= w;
+        float w;
+        if (base_moves<F16>(mx, m, l, w))
             for (int i = 0; i < C::NB * C::VE; i++) o[i] *= w;
-            m = mn;
-        }
         /* a column that has met no position yet keeps its terms 0 */
-        const float base = m == -INFINITY ? 0.0f : P_UP - m;
+        const float base = m == -INFINITY ? 0.0f : Soft<F16>::UP - m;
         for (int j = 0; j < C::VT; j++) {
             s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], fac, base));
             l += s[j];
@@ -1123,15 +1156,12 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
 #pragma unroll
                     for (int k = 0; k < 8; k++) mx = fmaxf(mx, p[k]);
                     mx *= fac;
-                    if (__any(mx > m + M_LATE)) {
-                        const float mn = fmaxf(m, max_g(mx)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                        l *= f;
+                    float f;
+                    if (base_moves<true>(mx, m, l, f))
 #pragma unroll
                         for (int k = 0; k < NO; k++) o[k] *= f;
-                        m = mn;
-                    }
                     /* a column that has met no position yet keeps its terms 0 */
-                    const float base = m == -INFINITY ? 0.0f : P_UP - m;
+                    const float base = m == -INFINITY ? 0.0f : Soft<true>::UP - m;
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         p[k] = __builtin_amdgcn_exp2f(fmaf(p[k], fac, base));
