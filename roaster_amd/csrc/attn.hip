@@ -43,11 +43,13 @@
  * all of a tile stays M_DOWN below it: a term is then off by at most 2^-22 of itself or 2^-24 of its
  * tile's largest, also behind a position that outweighs the rest by 2^20 and whose value is nothing;
  * only in that position's own tile it is 2^-38 of the position's term.  (With a base that only rises
- * and terms up to 2^15 at LATE 8, a first position 2^22 above 700 others, its value 0, left outputs off by
- * 1.5e-4; so 1.4e-6.  It costs a prompt's rows 3%, single tokens nothing.) */
+ * and LATE 8, a first position 2^22 above 700 others, its value 0, left outputs off by
+ * 1.5e-4; so 1.4e-6.  It costs a prompt's rows 3%, single tokens nothing.)
+ * f32: terms stay below 2^-14, so that 2^14 values of any size can be added up. */
+#define LATE 2.0f
 template <bool F16>
 struct Soft {
-    static constexpr float UP = F16 ? 13.0f : 7.0f, LATE = F16 ? 2.0f : 8.0f;
+    static constexpr float UP = F16 ? 13.0f : -16.0f;
 };
 #define M_DOWN 14.0f
 #define M_MID 6.0f            /* a base that goes down stays this much above the tile's largest, for the next ones */
@@ -155,7 +157,7 @@ __device__ __forceinline__ bool base_moves(float mx, float &m, float &l, float &
         const unsigned c = (unsigned)near | (unsigned)(near >> 32);
         down = ((c | c >> 16) & 0xffff) != 0xffff;
     }
-    if (!down && !__any(mx > m + Soft<F16>::LATE)) return false;
+    if (!down && !__any(mx > m + LATE)) return false;
     const float top = floorf(max_g(mx));
     float to = fmaxf(m, top);
     if (down) {

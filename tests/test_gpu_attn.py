@@ -320,3 +320,20 @@ def test_cache_past_32_bit_offsets():
     finally:
         L.roaster_dev_free(k)
         L.roaster_dev_free(v)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e34, 3e38])
+@pytest.mark.parametrize("H,KV,D", [(16, 2, 256), (32, 8, 128), (7, 1, 64)])
+def test_f32_values_of_any_size(H, KV, D, size):
+    """Outputs are means of values, within f32 where the values are."""
+    rng = np.random.default_rng(D)
+    for lens, each in (([300], 1), ([70, 3, 41], 1), ([60 + i for i in range(40)], 2), ([80], 30)):
+        kc, vc, table = make(rng, lens, KV, D, 16, False)
+        vc = np.where(np.isfinite(vc), np.float32(size) * rng.uniform(-1, 1, vc.shape), vc).astype(np.float32)
+        rows = np.array([(r, l - each + i) for r, l in enumerate(lens) for i in range(each)], np.int32)
+        q = rng.standard_normal((len(rows), H, D)).astype(np.float32)
+        a = Attn(Cache(kc, vc), q, rows[:, 0].copy(), rows[:, 1].copy(), table, D ** -0.5)
+        R.check(a.call(), "attn")
+        sync()
+        want, mass, reach = attn_oracle(q, kc, vc, table, rows[:, 0], rows[:, 1], np.float64(np.float32(D ** -0.5)))
+        check_attn(a.out.get() / size, want / size, mass / size, reach, int(rows[:, 1].max()) + 1, D)
