@@ -443,13 +443,14 @@ struct AttLds {
     __device__ float *sums(int w, int h) { return (float *)own[w] + h * (D + 4); }
 };
 
-/* out of one row's head from the sums y and l, four elements at d.  The reciprocals
+/* out of one row's head from the sums y and l, four elements at d; 0, whatever the gate holds, for a row
+ * without positions (`none`).  The reciprocals
  * are off by one step, the exponential by |gate| 2^-24 more: as little as the
  * sums themselves. */
-__device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int t, int h, int d, f32x4 y, float l)
+__device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int t, int h, int d, f32x4 y, float l, bool none)
 {
-    y *= __builtin_amdgcn_rcpf(l);
-    if (a.gate) {
+    y = none ? (f32x4){} : y * __builtin_amdgcn_rcpf(l);
+    if (a.gate && !none) {
         const f32x4 gt = *(const f32x4 *)(a.gate + t * a.gate_row + h * a.gate_head + d);
 #pragma unroll
         for (int i = 0; i < 4; i++) y[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gt[i] * -1.44269504088896341f));
@@ -561,7 +562,7 @@ __device__ __forceinline__ bool att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
             y += *(const f32x4 *)(S.sums(i, h) + d) * f;
         }
         if (S.n[h] > good) { y = (f32x4){ NAN, NAN, NAN, NAN }; sum = NAN; }
-        if (whole) att_store(a, D, t0 + row, h0 + head, d, y, S.n[h] == 0 ? 1.0f : sum);      /* without positions: y is 0 */
+        if (whole) att_store(a, D, t0 + row, h0 + head, d, y, sum, S.n[h] == 0);
         else {
             *(f32x4 *)(A.po + ((size_t)slot * C::COLS + off + h) * D + d) = y;
             if (d == 0) {
@@ -1272,7 +1273,7 @@ __global__ __launch_bounds__(ROWS_T, 2) void attn_rows_kernel(RowsArgs A, int *e
         } else if (whole) {
             if (on)
 #pragma unroll
-                for (int k = 0; k < NO; k++) att_store(a, D, t0 + ri, h0 + ch, 16 * k + 4 * g, o[k], nc == 0 ? 1.0f : sum);
+                for (int k = 0; k < NO; k++) att_store(a, D, t0 + ri, h0 + ch, 16 * k + 4 * g, o[k], sum, nc == 0);
         } else {                                       /* as the registers lie: the join needs no other order */
             const size_t at = slot * GROUPS + grp;
             if (g == 0) {
@@ -1357,9 +1358,9 @@ __global__ __launch_bounds__(64) void attn_rows_join_kernel(RowsArgs A)
     else if (x.k <= 4) join(std::integral_constant<int, 4>());
     else join(std::integral_constant<int, 8>());
     const int t = x.row + ri;
-    const float sum = A.a.row_pos[t] == -1 ? 1.0f : l;
+    const bool none = A.a.row_pos[t] == -1;
 #pragma unroll
-    for (int z = 0; z < 4; z++) att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, 16 * (4 * q + z) + 4 * g, y[z], sum);
+    for (int z = 0; z < 4; z++) att_store(A.a, D, t, kh * A.group + bk * A.hpb + ch, 16 * (4 * q + z) + 4 * g, y[z], l, none);
 }
 
 /* The parts of one cut unit's column, L lanes with four elements each to a part:
@@ -1421,7 +1422,7 @@ __global__ __launch_bounds__(JT) void attn_join_kernel(AttArgs A)
         y += s_o[i][tid] * w;
     }
     const int t = e.row + row;
-    att_store(a, D, t, kh * A.group + bk * A.hpb + head, d, y, a.row_pos[t] == -1 ? 1.0f : sum);
+    att_store(a, D, t, kh * A.group + bk * A.hpb + head, d, y, sum, a.row_pos[t] == -1);
 }
 
 /* Workspace: the cut table, then m and l of the parts, then the parts (16 columns). */

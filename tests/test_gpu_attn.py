@@ -337,3 +337,29 @@ def test_f32_values_of_any_size(H, KV, D, size):
         sync()
         want, mass, reach = attn_oracle(q, kc, vc, table, rows[:, 0], rows[:, 1], np.float64(np.float32(D ** -0.5)))
         check_attn(a.out.get() / size, want / size, mass / size, reach, int(rows[:, 1].max()) + 1, D)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("H,KV,D", [(16, 2, 256), (16, 1, 64), (8, 2, 128)])
+def test_rows_without_a_position_are_zero_whatever_their_gate(H, KV, D, f16):
+    """Alone, among requests' rows, at the beginning of a run, and where a run's parts are joined."""
+    rng = np.random.default_rng(D + H)
+    for lens, rows in (([50], [(0, -1)]), ([50, 9], [(0, 49), (1, -1), (0, -1)]),
+                       ([40 + i for i in range(60)], [(r, -1 if r % 3 else 39 + r) for r in range(60)]),
+                       ([40 + i for i in range(40)], [(r, p) for r in range(40) for p in (-1, 39 + r)]),
+                       ([3000], [(0, -1)] * 5 + [(0, 2970 + i) for i in range(25)])):
+        kc, vc, table = make(rng, lens, KV, D, 16, f16)
+        rows = np.array(rows, np.int32)
+        q = rng.standard_normal((len(rows), H, D)).astype(np.float32)
+        none = rows[:, 1] == -1
+        g = rng.standard_normal((len(rows), H, 2, D)).astype(np.float32)
+        g[none, :, 1] = rng.choice(np.array([np.nan, np.inf, -np.inf, 1], np.float32), (int(none.sum()), H, D))
+        a = Attn(Cache(kc, vc), q, rows[:, 0].copy(), rows[:, 1].copy(), table, D ** -0.5, g)
+        R.check(a.call(), "attn")
+        sync()
+        got = a.out.get()
+        assert not got[none].any(), np.isnan(got[none]).sum()
+        if not none.all():
+            want = attn_oracle(q, kc, vc, table, rows[:, 0], rows[:, 1], np.float64(np.float32(D ** -0.5)),
+                               np.where(np.isfinite(g[:, :, 1]), g[:, :, 1], 0))
+            check_attn(got[~none], *(w[~none] for w in want), int(rows[:, 1].max()) + 1, D)
