@@ -64,7 +64,9 @@ typedef struct {
  * range, a ring that is not one) is refused as a whole: len_out = len, ctl_out =
  * ctl, table and ring untouched, first all 0, every row -1, and roaster_sync
  * reports it.  A page number out of range in the ring or in a table row gives
- * its rows slot -1 (a new one is entered as -1) and is reported. */
+ * its rows slot -1 (a new one is entered as -1) and is reported; one that an ended
+ * request gives back is reported, stands in the ring as -1, and counts as a free page
+ * until it is taken. */
 typedef struct {
     int n_req;                /* 1 .. 2048 */
     int page_size;            /* a power of two, 16 .. 4096 */

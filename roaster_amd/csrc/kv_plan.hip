@@ -148,8 +148,10 @@ __global__ __launch_bounds__(KVP_T) void kv_plan_kernel(RoasterKvPlan A, int shi
     }
     for (int i = gt; i < t_old; i += gn) {
         const int r = kvp_find(c_old, n, i);
-        const int at = e0 + i;
-        A.ring[at - (at >= N ? N : 0)] = A.table[(size_t)r * A.max_pages + i - c_old[r]];
+        const int at = e0 + i, p = A.table[(size_t)r * A.max_pages + i - c_old[r]];
+        const bool in = (unsigned)p < (unsigned)N;
+        if (!in) lost = 1;
+        A.ring[at - (at >= N ? N : 0)] = in ? p : -1;
     }
     if (lost) atomicOr(err, ATTN_ERR_INDEX);
 }

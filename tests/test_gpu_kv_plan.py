@@ -142,3 +142,27 @@ def test_bad_page_numbers_are_marked():
     got = p.got()
     assert got["row_slot"].tolist() == [-1, -1, 16 + 8, -1] and got["row_req"].tolist() == [0, 1, 2, -1]
     assert got["table"].tolist() == [[4, 99, -1], [2, -1, -1], [5, 3, 1]] and got["ctl_out"].tolist() == [1, 3]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_bad_pages_of_an_ended_request(in_place):
+    """Page numbers out of range among those that come back: reported in this step and entered as
+    -1, the others as they are; reported again in the step that takes one."""
+    ln, add = np.array([50, 16], np.int32), np.array([-1, 0], np.int32)
+    table = np.array([[4, 99, -7, 2, 55], [6, -1, -1, -1, -1]], np.int32)
+    ring = np.array([0, 0, 0, 0, 0, 0, 0, 1, 8, 0], np.int32)
+    ctl = np.array([7, 9], np.int64)
+    p = Plan(16, 10, 4, ln, add, table, ring, ctl, in_place)
+    R.check(p.call(), "plan")
+    assert R.lib().roaster_sync() == R.EINVAL
+    sync()
+    got = p.got()
+    assert got["ring"].tolist() == [-1, -1, 2, 0, 0, 0, 0, 1, 8, 4] and got["ctl_out"].tolist() == [7, 13]
+    assert got["table"].tolist() == table.tolist() and got["len_out"].tolist() == [0, 16]
+    p = Plan(16, 10, 64, got["len_out"], np.array([49, 0], np.int32), got["table"], got["ring"], got["ctl_out"], in_place)
+    R.check(p.call(), "plan")
+    assert R.lib().roaster_sync() == R.EINVAL
+    sync()
+    got = p.got()
+    assert got["table"].tolist()[0] == [1, 8, 4, -1, 55] and got["ctl_out"].tolist() == [11, 13]
+    assert got["row_slot"].tolist()[:49] == [pg * 16 + i for pg in (1, 8, 4) for i in range(16)] + [-1]
