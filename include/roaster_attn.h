@@ -13,7 +13,7 @@
  * (lengths, page numbers, slots) is checked by the kernels, which neither read
  * nor write out of bounds for any value, and reported by roaster_sync:
  * ROASTER_ENOMEM for a plan without enough free pages, ROASTER_EINVAL for the
- * others.  No call allocates, copies to the host or waits: after roaster_init
+ * others, each in a call of its own where there are several.  No call allocates, copies to the host or waits: after roaster_init
  * all of them can be captured into a HIP graph on roaster_stream, the rows
  * that a replay does not use being marked by -1.  Two calls, or two captured
  * graphs, that may run at the same time need output buffers, a page ring and

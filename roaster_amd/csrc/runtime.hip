@@ -174,6 +174,8 @@ int rt_take_err()
     return rt_fail(ROASTER_EROUTE, "router produced fewer than 8 finite logits for some token");
 }
 
+__global__ void clear_bits_kernel(int *word, int bits) { atomicAnd(word, ~bits); }
+
 extern "C" int roaster_sync(void)
 {
     std::lock_guard<std::recursive_mutex> g(g_lock);
@@ -189,7 +191,12 @@ extern "C" int roaster_sync(void)
         return ROASTER_EDEVICE;
     const int rc = rt_take_err(), e = g_err_pin[2];
     if (rc || !e) return rc;
-    if (rt_check(hipMemset(word, 0, sizeof(int)), "error word reset")) return ROASTER_EDEVICE;
+    /* only what is reported is cleared, on the stream and in one piece: other bits, and those that a
+     * graph on another stream sets meanwhile, are the next calls' */
+    const int said = e & ATTN_ERR_PAGES ? ATTN_ERR_PAGES : e & ATTN_ERR_PLAN ? ATTN_ERR_PLAN : e;
+    const AttnDevice dev;
+    hipLaunchKernelGGL(clear_bits_kernel, dim3(1), dim3(1), 0, g_rt.stream, word, said);
+    if (rt_check(hipGetLastError(), "error word reset")) return ROASTER_EDEVICE;
     if (e & ATTN_ERR_PAGES) return rt_fail(ROASTER_ENOMEM, "roaster_kv_plan: too few free pages; the step was not planned");
     if (e & ATTN_ERR_PLAN)
         return rt_fail(ROASTER_EINVAL, "roaster_kv_plan: a length, the row count or the page ring out of range; the step was not planned");

@@ -245,3 +245,26 @@ def test_errors_wait_for_their_sync():
         assert math.isnan(a.out.get().ravel()[0])
     finally:
         t.destroy()
+
+
+def test_errors_of_several_calls_are_reported_one_by_one():
+    """A plan without pages, a plan whose lengths are out of range and a bad row before one sync:
+    each is reported once, then none is left."""
+    from test_gpu_attn import make
+    rng = np.random.default_rng(4)
+    L = R.lib()
+    n_pages, table, ring, ctl = pool(rng, 16, np.array([16]), 0, 4, slack=0)
+    few = Plan(16, n_pages, 8, [16], [3], table, ring, ctl)
+    bad = Plan(16, n_pages, 8, [-4], [3], table, ring, ctl)
+    kc, vc, table = make(rng, [20], 2, 64, 16, True)
+    a = Attn(Cache(kc, vc), np.zeros((1, 4, 64), np.float32), np.array([5], np.int32), np.array([3], np.int32), table, 1.0)
+    for calls, codes in (([few.call, a.call], [R.ENOMEM, R.EINVAL]), ([a.call, bad.call, few.call], [R.ENOMEM, R.EINVAL, R.EINVAL]),
+                         ([a.call, a.call], [R.EINVAL]), ([bad.call, a.call], [R.EINVAL, R.EINVAL])):
+        for c in calls:
+            R.check(c(), "call")
+        said = []
+        for code in codes:
+            assert L.roaster_sync() == code, (codes, said)
+            said.append(R.last_error())
+        assert len(set(said)) == len(codes)
+        assert L.roaster_sync() == R.OK
