@@ -151,7 +151,7 @@ typedef struct {
     const int *row_req, *row_pos;        /* [rows] */
     const int *table;         /* [n_req][max_pages] */
     int n_req, max_pages;     /* max_pages * page_size <= 2^30 */
-    float scale;
+    float scale;              /* at most 2e38 in size */
     const float *gate;        /* or NULL; 16-byte aligned, strides multiples of 4 */
     size_t gate_row, gate_head;
     float *out;               /* [rows][q_heads][head_dim], 16-byte aligned */

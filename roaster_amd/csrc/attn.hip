@@ -1469,9 +1469,9 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     std::lock_guard<std::recursive_mutex> g(rt_lock());
     if (!attn_cache_ok(c)) return rt_fail(ROASTER_EINVAL, "roaster_attn_paged: bad cache description");
     if (!p || p->rows < 0 || p->rows > (1 << 20) || p->q_heads < 1 || p->q_heads > 1024 || p->q_heads % c->kv_heads ||
-        p->n_req < 1 || p->max_pages < 1 || (int64_t)p->max_pages * c->page_size > (1 << 30) || !(fabsf(p->scale) < INFINITY))
+        p->n_req < 1 || p->max_pages < 1 || (int64_t)p->max_pages * c->page_size > (1 << 30) || !(fabsf(p->scale) <= 2e38f))
         return rt_fail(ROASTER_EINVAL, "roaster_attn_paged: need 0 <= rows <= 2^20, q_heads a multiple of kv_heads up to 1024, "
-                       "n_req >= 1, max_pages * page_size at most 2^30, a finite scale");
+                       "n_req >= 1, max_pages * page_size at most 2^30, a scale within 2e38");
     if (!p->rows) return 0;
     if (!p->q || !p->out || !p->row_req || !p->row_pos || !p->table || !attn_aligned(p->q, 16) || !attn_aligned(p->out, 16) ||
         !attn_aligned(p->row_req, 4) || !attn_aligned(p->row_pos, 4) || !attn_aligned(p->table, 4) ||

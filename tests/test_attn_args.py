@@ -171,3 +171,14 @@ def test_index_functions_stay_inside(tmp_path):
     subprocess.check_call(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-I", CSRC, "-o", str(exe), str(src)])
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and not r.stderr, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, 2.4e38, float("-inf")])
+def test_scales_whose_product_with_log2_e_overflows_are_refused(scale):
+    assert attn(scale=scale) == R.EINVAL
+
+
+@no_gpu
+def test_scales_up_to_that_are_taken():
+    for scale in (2e38, -2e38, 0.0, 1e-38):
+        assert attn(scale=scale) == R.EDEVICE
