@@ -130,7 +130,7 @@ int roaster_qk_rope_store(const RoasterQkRope *rope, const RoasterKvCache *cache
  * page number out of range gives that row NaN outputs and is reported.
  * Keys and values behind a row's position are never used, whatever they hold.
  * Infinite or NaN keys and values in use make the elements that they reach
- * infinite or NaN.  Sums and softmax are in 32 bits; with an fp16 cache the queries
+ * infinite or NaN; so does a scale * log2(e) * q past f32's range.  Sums and softmax are in 32 bits; with an fp16 cache the queries
  * enter the products with 22 bits (two fp16 parts, relative to the row's largest element),
  * and probabilities off by at most 2^-22 of themselves or 2^-24 of the largest in
  * their tile (up to 32 positions one behind the other).  Where a position outweighs all

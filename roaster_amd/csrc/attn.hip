@@ -24,10 +24,12 @@
  * them, and each operand read is multiplied by high and low parts in turn.
  * f32 cache: f32 MFMAs, always WIDE.
  *
- * What bounds it: the cache's bytes.  A large read reaches 6.8 TB/s here; 64
- * requests of 300..16000 tokens come to 5.65 (94 us), one of 200001 to 5.7 (72 us, 5 of
- * them for the join), f32 to 5.0.  437 tokens take 12 us: two launches and a chain of
- * waits for a row, its page, keys and values.
+ * What bounds it: the cache's bytes.  A large read reaches 7.2 TB/s here; 64
+ * requests of 300..16000 tokens come to 5.65 (94 us; of four times the lengths to 6.4), one
+ * of 200001 to 5.7 (72 us, 5 of them for the join), an f32 cache's 12 of 500..5000 to 4.9 (41 us;
+ * of ten times the lengths to 6.5): what is missing are the units' beginnings and the
+ * join.  437 tokens take 12 us: two launches and a chain of waits for a row, its page,
+ * keys and values.
  */
 #include "attn.h"
 #include "qdot.h"
@@ -44,7 +46,7 @@
  * tile's largest, also behind a position that outweighs the rest by 2^20 and whose value is nothing;
  * only in that position's own tile it is 2^-38 of the position's term.  (With a base that only rises
  * and LATE 8, a first position 2^22 above 700 others, its value 0, left outputs off by
- * 1.5e-4; so 1.4e-6.  It costs a prompt's rows 3%, single tokens nothing.)
+ * 1.5e-4; so 1.4e-6.  It costs a prompt's rows 3 to 5%, single tokens nothing.)
  * f32: terms stay below 2^-14, so that 2^14 values of any size can be added up. */
 #define LATE 2.0f
 template <bool F16>
@@ -218,7 +220,8 @@ struct AttWave {
         }
     }
     /* Keys of the tile that begins at byte `at`, a kilobyte to a load: with 64 bytes of each
-     * of 16 tokens to a load, as the products take them, they come at 5.9 TB/s, so at 6.8. */
+     * of 16 tokens to a load, as the products take them, a read of nothing else comes at 5.9 TB/s, so
+     * at 6.8. */
     __device__ void load_k(const char *kc, size_t at, int lane)
     {
 #pragma unroll
@@ -391,10 +394,10 @@ __device__ __forceinline__ long long att_scan(long long v, long long *s_wave, lo
 
 /* What beginning a unit costs, in tiles, where shares are made equal: its row, page and
  * queries have to come before its first keys, and its sums go through LDS (700 requests of 1
- * to 500 tokens 82 us without it, 47 with it).  A unit of n tiles lies on LEAD + n
+ * to 500 tokens 84 us without it, 48 with it).  A unit of n tiles lies on LEAD + n
  * places, its tiles on the last n. */
 #define ATT_LEAD 8
-#define ROWS_LEAD 12          /* of 32 tokens; 4 requests of 1000 rows: 444 us with 4, 295 with 12, 304 with 24 */
+#define ROWS_LEAD 12          /* of 32 tokens; 4 requests of 1000 rows: 415 us with 4, 301 with 12, 313 with 24 */
 
 /* Row t's request and tokens, and whether it goes on with the unit of row t - 1: runs of up to
  * R rows of one request, one behind the other with positions that do not fall, between
@@ -578,8 +581,8 @@ __device__ __forceinline__ bool att_part(const AttArgs &A, AttLds<D, F16, WIDE> 
  * takes one unit's part.  All tiles over (workgroups - units) is a part's size that gives
  * no more parts than workgroups, since a unit of n tiles has ceil(n / size); a unit's
  * parts are equal.  Each wave finds its part from the rows by itself, without a barrier.
- * 8 requests of 100..8000 tokens, 2 key/value heads: 18 us, with even shares 26; 32 of them
- * (above the bound): 32 either way. */
+ * 8 requests of 100..8000 tokens, 2 key/value heads: 19 us, with even shares 27; 32 of them,
+ * the most there may be: 33, with even shares 32; 64 of them 54 and 50. */
 template <int D, bool F16, bool WIDE>
 __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_few_kernel(AttArgs A, int *err)
 {
@@ -744,8 +747,8 @@ __global__ __launch_bounds__(ATT_T, D == 256 && !F16 ? 1 : 2) void attn_kernel(A
  * wave, about 2 us of the two waves on a SIMD, a third of the matrix cores' rate (each wave a
  * chain of reads, products and softmax, which 256 registers let no third wave fill); before a
  * unit's first tile lie 9 to 12 us (rows, page, queries and tile, each a wait), behind its last 1 to
- * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 43 us, 512 rows 62, a prompt of 1024
- * 62, of 2000 124, four prompts' 1000 rows behind 0..3000 tokens 291. */
+ * 2, and the join takes 8 to 20.  256 rows behind 2048 tokens 45 us, 512 rows 65, a prompt of 1024
+ * 62, of 2000 120, four prompts' 1000 rows behind 0..3000 tokens 301. */
 #define ROWS_G 256            /* workgroups: one per CU */
 #define ROWS_T 512
 #define ROWS_W (ROWS_T / 64)
@@ -1431,9 +1434,10 @@ static const size_t ATT_CUT = (size_t)ATT_G * sizeof(AttCut), ATT_ML = (size_t)2
 /* The same of attn_rows_kernel. */
 static const size_t ROWS_CUT = (size_t)ROWS_G * sizeof(RowsCut), ROWS_ML = (size_t)2 * ROWS_G * ROWS_COLS * 4;
 
-/* Calls that may go by runs of rows.  With fewer rows there is little to share: of one request
- * behind 2048 tokens 8 take 23 us so and 19 apart, 16 take 26 and 21, 32 take 27 and 29;
- * behind 16000 tokens 16 take 47 and 71. */
+/* Calls that may go by runs of rows.  With fewer rows there is little to share, with short contexts too: of
+ * one request behind 2048 tokens 8 rows take 24 us so and 18 apart, 16 take 25 and 20, 32 take 27
+ * and 25, but behind 16000 tokens 16 take 39 and 69.  The host sees no lengths, so this is a
+ * compromise: it loses a quarter on 16 rows behind a short context, and would lose more behind a long one. */
 static bool rows_may(int rows, int type) { return type == ROASTER_KV_F16 && rows >= 16; }
 
 extern "C" size_t roaster_attn_ws_bytes(int rows, int q_heads, const RoasterKvCache *c)
@@ -1495,11 +1499,13 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
     /* Runs of rows pay where requests have more rows each than sixteen columns hold, which
-     * the two counts tell on average (a call of other rows is right as well, only slower): 256
-     * rows behind 2048 tokens take 42 us so, 99 otherwise; requests of 300..16000 tokens and 8
-     * heads (two rows fill the columns) with three rows 56 and 71, with two 75 and 73; with 4
-     * heads (four rows do) and 75..4000 tokens four rows 53 and 42, six 63 and 67; with 16, 77 and
-     * 113 for two rows. */
+     * the two counts tell on average (the host sees neither lengths nor which request a row is of; a
+     * call of other rows is right as well, only slower): 256 rows behind 2048 tokens take 45 us so, 107
+     * otherwise, a prompt of 2000 120 and 444; 16 requests of 300..16000 tokens and 8 heads (two
+     * rows fill the columns) with three rows 57 and 75, with 16 heads two rows 36.5 and 38; with 4
+     * heads (four rows do) and 75..4000 tokens six rows 39 and 39, four 32 and 28.  Two rows of 8
+     * heads are on the slower side, 45 and 53 (32 requests: 70 and 75).  One request's 256 rows with 63
+     * requests' single rows in one call take 159, in two calls 136. */
     const int per16 = 16 / std::min(p->q_heads / c->kv_heads, 16);
     if (rows_may(p->rows, c->type) && p->rows >= std::max(2, per16 + 1) * (long long)p->n_req) {
         RowsArgs A;
@@ -1515,8 +1521,8 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
         A.pm = (float *)((char *)p->ws + ROWS_CUT);
         A.pl = (float *)((char *)p->ws + ROWS_CUT + ROWS_ML);
         A.po = (float *)((char *)p->ws + ROWS_CUT + 2 * ROWS_ML);
-        /* Few units are cut into many parts: 16 rows behind 2048 tokens take 24 us in halves and 26
-         * without, 8 requests of six rows 45 and 50, 256 rows 43 and 44, but 512 rows 68 and 63. */
+        /* Few units are cut into many parts: 16 rows behind 2048 tokens take 25 us in halves and 26
+         * without, 8 requests of six rows 40 and 45, 256 rows 45 and 46, but 512 rows 70 and 66. */
         const bool halves = (long long)p->rows * A.hpb * A.blocks * c->kv_heads <= ROWS_G / 8 * ROWS_COLS;
 #define ROWS(DD) (halves ? rows_launch<DD, 2>(A, err) : rows_launch<DD, 1>(A, err))
         if (D == 256) ROWS(256);
@@ -1531,9 +1537,9 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     A.vc = (const char *)c->v;
     A.s = attn_shape(c);
     A.group = p->q_heads / c->kv_heads;
-    /* Sixteen columns of their own for more than eight heads (32 requests, 16 heads on one:
-     * 53 us, with two blocks of eight 90) and for several rows of a request (32 requests of two
-     * rows: 72 us, row by row 95; f32, 256 rows: 165 instead of 302).  With one row of few
+    /* Sixteen columns of their own for more than eight heads (32 requests of
+     * 300..16000 tokens, 16 heads on one: 38 us, with two blocks of eight 53) and for several rows of a
+     * request (32 requests of two rows: 76 us, row by row 93; f32, 256 rows: 153 instead of 270).  With one row of few
      * heads the high and low parts fill them: half the MFMAs. */
     const bool f16 = c->type == ROASTER_KV_F16;
     bool wide = !f16 || A.group > 8;
@@ -1544,7 +1550,7 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     const long long units = (long long)p->rows * c->kv_heads * A.blocks;
     A.by_unit = units <= A.grid;
     /* With few units the rows of a request stay apart: what they share comes from the caches,
-     * and there are more parts (three rows behind 437 tokens: 11.8 us, 14.6 together). */
+     * and there are more parts (three rows behind 437 tokens: 12.7 us, together in even shares 18.5). */
     A.few = units <= A.grid / 8 && p->rows <= 128;
     A.R = A.few || p->rows < 2 * (long long)p->n_req ? 1 : 16 / A.hpb;
     wide |= A.R > 1;
