@@ -13,9 +13,10 @@
  * (lengths, page numbers, slots) is checked by the kernels, which neither read
  * nor write out of bounds for any value, and reported by roaster_sync:
  * ROASTER_ENOMEM for a plan without enough free pages, ROASTER_EINVAL for the
- * others, each in a call of its own where there are several.  No call allocates, copies to the host or waits: after roaster_init
- * all of them can be captured into a HIP graph on roaster_stream, the rows
- * that a replay does not use being marked by -1.  Two calls, or two captured
+ * others, each in a call of its own where there are several.  No call
+ * allocates, copies to the host or waits: after roaster_init all of them can be
+ * captured into a HIP graph on roaster_stream, the rows that a replay does not
+ * use being marked by -1.  Two calls, or two captured
  * graphs, that may run at the same time need output buffers, a page ring and
  * workspaces of their own.
  */
@@ -130,13 +131,13 @@ int roaster_qk_rope_store(const RoasterQkRope *rope, const RoasterKvCache *cache
  * page number out of range gives that row NaN outputs and is reported.
  * Keys and values behind a row's position are never used, whatever they hold.
  * Infinite or NaN keys and values in use make the elements that they reach
- * infinite or NaN; so does a scale * log2(e) * q past f32's range.  Sums and softmax are in 32 bits; with an fp16 cache the queries
- * enter the products with 22 bits (two fp16 parts, relative to the row's largest element),
- * and probabilities off by at most 2^-22 of themselves or 2^-24 of the largest in
- * their tile (up to 32 positions one behind the other).  Where a position outweighs all
- * before it, those in its tile are off by up to 2^-38 of its probability, and tiles
- * below 2^-70 of it may be left out.  How a call's
- * work is split goes by all its rows: the last bits of a row's output depend on
+ * infinite or NaN; so does a scale * log2(e) * q past f32's range.  Sums and softmax
+ * are in 32 bits; with an fp16 cache the queries enter the products with 22 bits (two
+ * fp16 parts, relative to a head's largest element), and probabilities off by at
+ * most 2^-22 of themselves or 2^-24 of the largest in their tile (up to 32 positions one
+ * behind the other).  Where a position outweighs all before it, those in its tile are
+ * off by up to 2^-38 of its probability, and tiles below 2^-70 of it may be left out.
+ * How a call's work is split goes by all its rows: the last bits of a row's output depend on
  * them, and are the same for the same call.
  * An fp16 call of 16 rows or more, and of more rows for each of the n_req requests than
  * 16 / (q_heads / kv_heads), two at least, takes the rows of a request that stand

@@ -446,10 +446,9 @@ struct AttLds {
     __device__ float *sums(int w, int h) { return (float *)own[w] + h * (D + 4); }
 };
 
-/* out of one row's head from the sums y and l, four elements at d; 0, whatever the gate holds, for a row
- * without positions (`none`).  The reciprocals
- * are off by one step, the exponential by |gate| 2^-24 more: as little as the
- * sums themselves. */
+/* out of one row's head from the sums y and l, four elements at d; 0, whatever the gate holds,
+ * for a row without positions (`none`).  The reciprocals are off by one step, the
+ * exponential by |gate| 2^-24 more: as little as the sums themselves. */
 __device__ __forceinline__ void att_store(const RoasterAttnPaged &a, int D, int t, int h, int d, f32x4 y, float l, bool none)
 {
     y = none ? (f32x4){} : y * __builtin_amdgcn_rcpf(l);
@@ -1539,8 +1538,8 @@ extern "C" int roaster_attn_paged(const RoasterAttnPaged *p, const RoasterKvCach
     A.group = p->q_heads / c->kv_heads;
     /* Sixteen columns of their own for more than eight heads (32 requests of
      * 300..16000 tokens, 16 heads on one: 38 us, with two blocks of eight 53) and for several rows of a
-     * request (32 requests of two rows: 76 us, row by row 93; f32, 256 rows: 153 instead of 270).  With one row of few
-     * heads the high and low parts fill them: half the MFMAs. */
+     * request (32 requests of two rows: 76 us, row by row 93; f32, 256 rows: 153 instead of 270).  With one
+     * row of few heads the high and low parts fill them: half the MFMAs. */
     const bool f16 = c->type == ROASTER_KV_F16;
     bool wide = !f16 || A.group > 8;
     A.hpb = std::min(A.group, wide ? 16 : 8);

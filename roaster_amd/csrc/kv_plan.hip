@@ -55,7 +55,8 @@ __device__ __forceinline__ int kvp_find(const int *c, int n, int i)
  * workgroup writes them (`what`: bit 0 rows, table and ring, bit 1 len_out,
  * ctl_out, first and the error word).  What bounds it: latency, a chain of the
  * lengths' load, three scans, a search and a page's load; 8 requests of one row 4.5
- * us, 512 requests with 22700 rows 6.9; in place, a call by itself, 5.8 in one workgroup and 13.6 in two launches. */
+ * us, 512 requests with 22700 rows 6.9; in place, a call by itself, 5.8 in one workgroup
+ * and 13.6 in two launches. */
 __global__ __launch_bounds__(KVP_T) void kv_plan_kernel(RoasterKvPlan A, int shift, int what, int *err)
 {
     __shared__ int c_row[KVP_MAX_REQ + 1], c_new[KVP_MAX_REQ + 1], c_old[KVP_MAX_REQ + 1], s_len[KVP_MAX_REQ];
