@@ -1,8 +1,9 @@
 """roaster_amd -- Python access to libroaster_moe.so, the MI355X MoE-FFN hot path.
 
 The product is the C ABI declared in include/kernels.h (the reference's kernel API),
-include/roaster_moe.h (expert table, whole-layer decode / prefill) and
-include/roaster_attn.h (attention over a paged key/value cache).  This module
+include/roaster_moe.h (expert table, whole-layer decode / prefill),
+include/roaster_attn.h (attention over a paged key/value cache) and
+include/roaster_mixer.h (norm, 8-bit product, state space scan).  This module
 only loads that library with ctypes and declares its signatures, so that tests and
 the benchmark can call the same entry points a C caller would.  It fails loudly
 when the library has not been built: there is no Python or CPU fallback.
@@ -23,6 +24,8 @@ OK, EINVAL, EDEVICE, EROUTE, ENOMEM = 0, -1, -2, -3, -4
 GATE, UP, DOWN = 0, 1, 2
 PREC_F16, PREC_SPLIT, PREC_BF16 = 0, 1, 2
 KV_F32, KV_F16 = 0, 1
+I8_FROM_F32, I8_FROM_Q4K, I8_FROM_Q6K, I8_FROM_I8 = 0, 1, 2, 3
+SCAN_DELTA, SCAN_STATE = 0, 1
 
 
 class KernelMatvecJob(C.Structure):
@@ -102,6 +105,35 @@ class RoasterAttnPaged(C.Structure):
                 ("out", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
+class RoasterNorm(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("group", C.c_int), ("x", C.c_void_p), ("x_row", C.c_size_t),
+                ("res", C.c_void_p), ("res_row", C.c_size_t), ("weight", C.c_void_p), ("gate", C.c_void_p),
+                ("gate_row", C.c_size_t), ("eps", C.c_float), ("y", C.c_void_p), ("y_row", C.c_size_t), ("q", C.c_void_p),
+                ("q_row", C.c_size_t), ("q_scale", C.c_void_p)]
+
+
+class RoasterI8(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scale", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int)]
+
+
+class RoasterMatmulI8(C.Structure):
+    _fields_ = [("rows", C.c_int), ("x", C.c_void_p), ("x_row", C.c_size_t), ("x_scale", C.c_void_p), ("y", C.c_void_p),
+                ("y_row", C.c_size_t)]
+
+
+class RoasterSsmState(C.Structure):
+    _fields_ = [("n_req", C.c_int), ("k_heads", C.c_int), ("v_heads", C.c_int), ("k_dim", C.c_int), ("v_dim", C.c_int),
+                ("taps", C.c_int), ("conv", C.c_void_p), ("state", C.c_void_p)]
+
+
+class RoasterSsmScan(C.Structure):
+    _fields_ = [("rows", C.c_int), ("most", C.c_int), ("mode", C.c_int), ("x", C.c_void_p), ("x_row", C.c_size_t),
+                ("a", C.c_void_p), ("a_row", C.c_size_t), ("b", C.c_void_p), ("b_row", C.c_size_t), ("conv_w", C.c_void_p),
+                ("conv_b", C.c_void_p), ("a_coef", C.c_void_p), ("dt_bias", C.c_void_p), ("skip", C.c_void_p),
+                ("scale", C.c_float), ("eps", C.c_float), ("first", C.c_void_p), ("row_pos", C.c_void_p), ("out", C.c_void_p),
+                ("out_row", C.c_size_t), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
 _P = C.c_void_p
 _SIG = {
     # kernels.h
@@ -179,6 +211,13 @@ _SIG = {
     "roaster_qk_rope_store": (C.c_int, [C.POINTER(RoasterQkRope), C.POINTER(RoasterKvCache)]),
     "roaster_attn_ws_bytes": (C.c_size_t, [C.c_int, C.c_int, C.POINTER(RoasterKvCache)]),
     "roaster_attn_paged": (C.c_int, [C.POINTER(RoasterAttnPaged), C.POINTER(RoasterKvCache)]),
+    # roaster_mixer.h
+    "roaster_norm": (C.c_int, [C.POINTER(RoasterNorm)]),
+    "roaster_i8_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "roaster_i8_pack": (C.c_int, [_P, C.c_int, C.POINTER(RoasterI8)]),
+    "roaster_matmul_i8": (C.c_int, [C.POINTER(RoasterMatmulI8), C.POINTER(RoasterI8)]),
+    "roaster_ssm_ws_bytes": (C.c_size_t, [C.c_int, C.c_int, C.POINTER(RoasterSsmState)]),
+    "roaster_ssm_scan": (C.c_int, [C.POINTER(RoasterSsmScan), C.POINTER(RoasterSsmState)]),
 }
 
 _lib = None

@@ -9,10 +9,11 @@
 #include "../../include/roaster_attn.h"
 #include "attn_index.h"
 
-/* Error bits of the attention operators' device word (rt_attn_err). */
+/* Error bits of the attention operators' device word (rt_attn_err), which the state space scan shares. */
 #define ATTN_ERR_PAGES 1      /* a plan found too few free pages */
 #define ATTN_ERR_PLAN 2       /* a plan's lengths, sizes or ring out of range */
 #define ATTN_ERR_INDEX 4      /* a request, position, page or slot out of range */
+#define ATTN_ERR_SCAN 8       /* ssm.hip: a request's rows, their number or its position out of range */
 
 /* Makes the library's device current for the calls of one entry point and
  * gives the caller's back: the library's stream belongs to that device. */

@@ -1,0 +1,300 @@
+/*
+ * i8.hip -- matrix product in 8-bit integers with scales for each token and each
+ * channel (roaster_matmul_i8), and the layout of its weights (roaster_i8_pack):
+ * the projections on either side of the mixers (model.c:1284-1290, 1344-1347 one
+ * token, 1604-1660 a prompt's chunk) for any number of rows.
+ *
+ * v_mfma_i32_32x32x32_i8, channels as its rows and tokens as its columns.  Lane layout:
+ *   A[m][k]: lane l holds m = l%32, k = 16*(l/32) + i, i = 0..15      (B[k][n] likewise)
+ *   D[m][n]: lane l holds m = 8*(i/4) + 4*(l/32) + i%4, n = l%32, i = 0..15
+ * Weights lie as [rows/32][cols/16][32 rows][16 columns], so that an operand of 32
+ * channels by 32 columns is a kilobyte in lane order.
+ */
+#include "mixer.h"
+#include "qdot.h"
+
+#define I8_T 256
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+static inline size_t i8_rows(int rows) { return ((size_t)rows + 31) & ~(size_t)31; }
+static inline size_t i8_cols(int cols) { return ((size_t)cols + 127) & ~(size_t)127; }
+
+/* ---- weights -------------------------------------------------------------------- */
+/* Weight i of a super-block (kernels.c:1839-1874). */
+__device__ __forceinline__ float q4k_weight(const uint8_t *blk, int i)
+{
+    const float d = f16_bits_to_f32(gld_u16(blk)), dmin = f16_bits_to_f32(gld_u16(blk + 2));
+    const uint8_t *s = blk + 4;
+    const int j = i / 32, q = blk[16 + 32 * (i / 64) + i % 32] >> (j & 1) * 4 & 15;
+    const int sc = j < 4 ? s[j] & 63 : (s[j + 4] & 15) | (s[j - 4] >> 6) << 4;
+    const int mn = j < 4 ? s[j + 4] & 63 : s[j + 4] >> 4 | (s[j] >> 6) << 4;
+    return fmaf(d * sc, (float)q, -(dmin * mn));
+}
+
+__device__ __forceinline__ float q6k_weight(const uint8_t *blk, int i)
+{
+    const int n = i / 128, s = i % 128 / 32, l = i % 32;
+    const int lo = blk[64 * n + 32 * (s & 1) + l] >> (s >> 1) * 4 & 15, hi = blk[128 + 32 * n + l] >> 2 * s & 3;
+    const int8_t sc = (int8_t)blk[192 + 8 * n + 2 * s + l / 16];
+    return f16_bits_to_f32(gld_u16(blk + 208)) * sc * (float)((lo | hi << 4) - 32);
+}
+
+/* One workgroup a row of the padded matrix; 16 columns a thread at a time. */
+template <int FROM>
+__global__ __launch_bounds__(I8_T) void i8_pack_kernel(const uint8_t *W, RoasterI8 to, int padded)
+{
+    __shared__ unsigned s_top[I8_T / 64];
+    const int r = blockIdx.x, tid = threadIdx.x, n16 = to.cols / 16;
+    auto weight = [&](int c) {
+        if (FROM == ROASTER_I8_FROM_F32) return ((const float *)W)[(size_t)r * to.cols + c];
+        const int bytes = FROM == ROASTER_I8_FROM_Q6K ? RQ6K_BYTES : RQ4K_BYTES;
+        const uint8_t *blk = W + ((size_t)r * (to.cols / RQK) + c / RQK) * bytes;
+        return FROM == ROASTER_I8_FROM_Q6K ? q6k_weight(blk, c % RQK) : q4k_weight(blk, c % RQK);
+    };
+    float mul = 0;
+    if (FROM != ROASTER_I8_FROM_I8 && r < to.rows) {
+        unsigned top = 0;
+        for (int c = tid; c < to.cols; c += I8_T) top = max(top, __float_as_uint(weight(c)) & 0x7FFFFFFFu);
+        for (int o = 1; o < 64; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+        if (tid % 64 == 0) s_top[tid / 64] = top;
+        __syncthreads();
+        for (int w = 0; w < I8_T / 64; w++) top = max(top, s_top[w]);
+        const I8Scale s = i8_scale(top);
+        mul = s.mul;
+        if (tid == 0) to.scale[r] = s.scale;
+    }
+    for (int c = tid; c < padded / 16; c += I8_T) {
+        int v[4] = { 0, 0, 0, 0 };
+        if (r < to.rows && c < n16) {
+            if (FROM == ROASTER_I8_FROM_I8) {
+                const uint4 u = gld_u4(W + (size_t)r * to.cols + 16 * c);
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+            } else
+                for (int j = 0; j < 16; j++) v[j / 4] |= (i8_round(weight(16 * c + j), mul) & 255) << 8 * (j % 4);
+        }
+        int8_t *at = (int8_t *)to.data + (((size_t)(r / 32) * (padded / 16) + c) * 32 + r % 32) * 16;
+        *(i32x4 *)at = (i32x4){ v[0], v[1], v[2], v[3] };
+    }
+}
+
+/* ---- product -------------------------------------------------------------------- */
+struct I8Args {
+    const int8_t *w, *x;
+    const float *ws, *xs;
+    float *y;
+    size_t x_row, y_row;
+    int T, N, n16, k32;          /* tokens, channels, 16-byte pieces of a token, blocks of 32 padded columns */
+};
+
+__device__ __forceinline__ i32x4 i8_ld(const void *p) { return *(const GAS i32x4 *)p; }
+
+/* Up to 32 tokens: a workgroup takes 32 channels, its waves a part of the columns each and join in LDS
+ * (integers, so in any order).  Weights go from memory straight into the products, tokens too (from the L2).
+ * Padded columns of the weights are zeros, so any byte of the token may stand there. */
+__global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a)
+{
+    __shared__ int s_sum[32 * 32];                     /* [token][channel] */
+    const int tid = threadIdx.x, l = tid % 64, w = tid / 64, W = blockDim.x / 64;
+    for (int i = tid; i < 1024; i += blockDim.x) s_sum[i] = 0;
+    const int k0 = a.k32 * w / W, k1 = a.k32 * (w + 1) / W;
+    const int8_t *wp = a.w + ((size_t)blockIdx.x * a.k32 + k0) * 1024 + 16 * l;
+    const int8_t *xp = a.x + min(l % 32, a.T - 1) * a.x_row;
+    i32x16 acc = {};
+    int k = k0;
+    for (; k + 8 <= k1; k += 8, wp += 8192) {
+        i32x4 A[8], B[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) A[i] = i8_ld(wp + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < 8; i++) B[i] = i8_ld(xp + 16 * min(2 * (k + i) + l / 32, a.n16 - 1));
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(A[i], B[i], acc, 0, 0, 0);
+    }
+    for (; k < k1; k++, wp += 1024)
+        acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(i8_ld(wp), i8_ld(xp + 16 * min(2 * k + l / 32, a.n16 - 1)), acc, 0, 0, 0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) atomicAdd(&s_sum[(l % 32) * 32 + 8 * (i / 4) + 4 * (l / 32) + i % 4], acc[i]);
+    __syncthreads();
+    for (int i = tid; i < 32 * a.T; i += blockDim.x) {
+        const int t = i / 32, c = blockIdx.x * 32 + i % 32;
+        if (c < a.N) a.y[t * a.y_row + c] = (float)s_sum[i] * (a.xs[t] * a.ws[c]);
+    }
+}
+
+__device__ __forceinline__ void i8_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }   /* loads stay in flight */
+
+/* More tokens: a workgroup's tile is 32 TB tokens by 128 CB channels, a wave's all its tokens by 32 CB
+ * channels.  So no two waves read the same weights, which go from the L2 straight into registers, and only
+ * the tokens pass through LDS, 64 columns at a time, doubly buffered; both are loaded two such steps ahead.  Pieces of
+ * 16 bytes of a token are exchanged by (token / 2) % 4, so that eight lanes' reads fall on different banks. */
+template <int TB, int CB>
+__global__ __launch_bounds__(I8_T, 2) void i8_tile_kernel(I8Args a, int tiles, int per, int tblocks)
+{
+    constexpr int TM = 32 * TB, XL = (TM * 4 + I8_T - 1) / I8_T;
+    __shared__ __attribute__((aligned(16))) int8_t s_x[2][TM * 64];
+    /* workgroup b runs on XCD b % 8: each has a run of tiles, tokens' blocks of one channel block in turn */
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= tiles) return;
+    const int tid = threadIdx.x, l = tid % 64, w = tid / 64;
+    const int t0 = id % tblocks * TM, c0 = id / tblocks * (128 * CB) + 32 * CB * w;
+    const int steps = a.k32 / 2;
+    const int8_t *wp[CB];
+    for (int c = 0; c < CB; c++) {
+        const int cb = min(c0 / 32 + c, (a.N + 31) / 32 - 1);
+        wp[c] = a.w + (size_t)cb * a.k32 * 1024 + 16 * l;
+    }
+    const int8_t *xp[XL];
+    int xc[XL], xd[XL];
+    for (int i = 0; i < XL; i++) {
+        const int q = min(tid + i * I8_T, TM * 4 - 1), t = q / 4;
+        xp[i] = a.x + min(t0 + t, a.T - 1) * a.x_row;
+        xc[i] = q % 4;
+        xd[i] = t * 64 + ((q % 4 ^ (t >> 1 & 3)) << 4);
+    }
+    i32x4 W[2][2 * CB], X[2][XL];
+    auto load_w = [&](int s, i32x4 (&r)[2 * CB]) {
+        s = min(s, steps - 1);
+#pragma unroll
+        for (int c = 0; c < CB; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) r[2 * c + h] = i8_ld(wp[c] + (size_t)s * 2048 + 1024 * h);
+    };
+    auto load_x = [&](int s, i32x4 (&r)[XL]) {
+#pragma unroll
+        for (int i = 0; i < XL; i++) r[i] = i8_ld(xp[i] + 16 * min(4 * s + xc[i], a.n16 - 1));
+    };
+    auto store_x = [&](int b, const i32x4 (&r)[XL]) {
+#pragma unroll
+        for (int i = 0; i < XL; i++)
+            if (TM * 4 % I8_T == 0 || tid + i * I8_T < TM * 4) *(i32x4 *)(s_x[b] + xd[i]) = r[i];
+    };
+    i32x16 acc[CB][TB];
+    for (int c = 0; c < CB; c++)
+        for (int t = 0; t < TB; t++) acc[c][t] = (i32x16){};
+    auto step = [&](int s, int b) {
+        store_x(b ^ 1, X[b ^ 1]);                       /* step s + 1, whose buffer no wave reads any more */
+        load_x(s + 2, X[b]);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int t = 0; t < TB; t++) {
+                const int tok = 32 * t + l % 32, c16 = 2 * h + l / 32;
+                const i32x4 B = *(const i32x4 *)(s_x[b] + tok * 64 + ((c16 ^ (tok >> 1 & 3)) << 4));
+#pragma unroll
+                for (int c = 0; c < CB; c++) acc[c][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(W[b][2 * c + h], B, acc[c][t], 0, 0, 0);
+            }
+        load_w(s + 2, W[b]);
+        i8_barrier();
+    };
+    load_x(0, X[0]);
+    load_w(0, W[0]);
+    load_x(1, X[1]);
+    load_w(1, W[1]);
+    store_x(0, X[0]);
+    i8_barrier();
+    for (int s = 0; s < steps; s += 2) {                /* an even number */
+        step(s, 0);
+        step(s + 1, 1);
+    }
+    for (int c = 0; c < CB; c++)
+        for (int t = 0; t < TB; t++) {
+            const int tok = t0 + 32 * t + l % 32;
+            if (tok >= a.T) continue;
+            const float xs = a.xs[tok];
+            float *y = a.y + tok * a.y_row;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int ch = c0 + 32 * c + 8 * j + 4 * (l / 32);
+                f32x4_a4 v;
+                for (int i = 0; i < 4; i++) v[i] = (float)acc[c][t][4 * j + i] * (xs * a.ws[min(ch + i, a.N - 1)]);
+                if (ch + 4 <= a.N) *(f32x4_a4 *)(y + ch) = v;
+                else
+                    for (int i = 0; i < 4; i++)
+                        if (ch + i < a.N) y[ch + i] = v[i];
+            }
+        }
+}
+
+/* ---- entry points --------------------------------------------------------------- */
+static bool i8_sizes_ok(int rows, int cols)
+{
+    return rows >= 1 && rows <= (1 << 20) && cols >= 16 && cols <= 65536 && cols % 16 == 0;
+}
+
+static bool i8_ok(const RoasterI8 *w)
+{
+    return w && i8_sizes_ok(w->rows, w->cols) && w->data && w->scale && attn_aligned(w->data, 16) && attn_aligned(w->scale, 4);
+}
+
+extern "C" size_t roaster_i8_bytes(int rows, int cols) { return i8_sizes_ok(rows, cols) ? i8_rows(rows) * i8_cols(cols) : 0; }
+
+extern "C" int roaster_i8_pack(const void *W, int from, const RoasterI8 *to)
+{
+    std::lock_guard<std::recursive_mutex> g(rt_lock());
+    if (!i8_ok(to))
+        return rt_fail(ROASTER_EINVAL, "roaster_i8_pack: need 1 <= rows <= 2^20, cols a multiple of 16 up to 65536, data (16-byte "
+                       "aligned) and scale");
+    const bool quant = from == ROASTER_I8_FROM_Q4K || from == ROASTER_I8_FROM_Q6K;
+    if (from < ROASTER_I8_FROM_F32 || from > ROASTER_I8_FROM_I8 || (quant && to->cols % RQK))
+        return rt_fail(ROASTER_EINVAL, "roaster_i8_pack: bad source type, or Q4_K / Q6_K with cols no multiple of 256");
+    if (!W || !attn_aligned(W, quant ? 2 : 16))
+        return rt_fail(ROASTER_EINVAL, "roaster_i8_pack: W must be given and aligned (f32 and int8 to 16 bytes)");
+    const size_t rows = to->rows, cols = to->cols, nd = i8_rows(to->rows) * i8_cols(to->cols);
+    const size_t nw = from == ROASTER_I8_FROM_F32 ? 4 * rows * cols : from == ROASTER_I8_FROM_I8 ? rows * cols
+                                                                  : rq_mat_bytes(from == ROASTER_I8_FROM_Q6K, rows, cols);
+    if (attn_overlap(W, nw, to->data, nd) || attn_overlap(W, nw, to->scale, 4 * rows) || attn_overlap(to->data, nd, to->scale, 4 * rows))
+        return rt_fail(ROASTER_EINVAL, "roaster_i8_pack: W, data and scale overlap");
+    if (rt_init_locked()) return ROASTER_EDEVICE;
+    const AttnDevice dev;
+#define PACK(F) hipLaunchKernelGGL((i8_pack_kernel<F>), dim3(i8_rows(to->rows)), dim3(I8_T), 0, rt().stream, (const uint8_t *)W, *to, (int)i8_cols(to->cols))
+    if (from == ROASTER_I8_FROM_F32) PACK(ROASTER_I8_FROM_F32);
+    else if (from == ROASTER_I8_FROM_Q4K) PACK(ROASTER_I8_FROM_Q4K);
+    else if (from == ROASTER_I8_FROM_Q6K) PACK(ROASTER_I8_FROM_Q6K);
+    else PACK(ROASTER_I8_FROM_I8);
+#undef PACK
+    return rt_check(hipGetLastError(), "i8_pack launch") ? ROASTER_EDEVICE : 0;
+}
+
+extern "C" int roaster_matmul_i8(const RoasterMatmulI8 *p, const RoasterI8 *w)
+{
+    std::lock_guard<std::recursive_mutex> g(rt_lock());
+    if (!i8_ok(w))
+        return rt_fail(ROASTER_EINVAL, "roaster_matmul_i8: bad weights (1 <= rows <= 2^20, cols a multiple of 16 up to 65536, "
+                       "data 16-byte aligned)");
+    if (!p || p->rows < 0 || p->rows > (1 << 20)) return rt_fail(ROASTER_EINVAL, "roaster_matmul_i8: need 0 <= rows <= 2^20");
+    if (!p->rows) return 0;
+    const size_t T = p->rows, N = w->rows, K = w->cols;
+    if (!p->x || !p->x_scale || !p->y || !attn_aligned(p->x, 16) || !attn_aligned(p->x_scale, 4) || !attn_aligned(p->y, 4) ||
+        !stride_ok(p->x_row, 16) || !stride_ok(p->y_row, 1) || p->y_row < N)
+        return rt_fail(ROASTER_EINVAL, "roaster_matmul_i8: x (16-byte aligned, stride a multiple of 16 up to 2^32), x_scale and y "
+                       "(stride from w->rows up to 2^32) must be given");
+    const size_t ny = rows_span(T, N, p->y_row, 4);
+    if (attn_overlap(p->y, ny, p->x, rows_span(T, K, p->x_row, 1)) || attn_overlap(p->y, ny, p->x_scale, 4 * T) ||
+        attn_overlap(p->y, ny, w->data, i8_rows(w->rows) * i8_cols(w->cols)) || attn_overlap(p->y, ny, w->scale, 4 * N))
+        return rt_fail(ROASTER_EINVAL, "roaster_matmul_i8: y overlaps inputs");
+    if (rt_init_locked()) return ROASTER_EDEVICE;
+    const AttnDevice dev;
+    I8Args a = { (const int8_t *)w->data, p->x, w->scale, p->x_scale, p->y, p->x_row, p->y_row, p->rows, w->rows, w->cols / 16,
+                 (int)(i8_cols(w->cols) / 32) };
+    if (T <= 32) {
+        const int waves = N <= 8192 ? 16 : 4;
+        hipLaunchKernelGGL(i8_few_kernel, dim3((N + 31) / 32), dim3(64 * waves), 0, rt().stream, a);
+    } else {
+        auto tiles = [&](int tb, int cb) { return ((T + 32 * tb - 1) / (32 * tb)) * ((N + 128 * cb - 1) / (128 * cb)); };
+#define TILE(TB, CB)                                                                                                       \
+    do {                                                                                                                   \
+        const int n = (int)tiles(TB, CB), per = (n + 7) / 8;                                                               \
+        hipLaunchKernelGGL((i8_tile_kernel<TB, CB>), dim3(8 * per), dim3(I8_T), 0, rt().stream, a, n, per,                 \
+                           (int)((T + 32 * TB - 1) / (32 * TB)));                                                          \
+    } while (0)
+        if (tiles(4, 2) >= 384) TILE(4, 2);
+        else if (tiles(4, 1) >= 192) TILE(4, 1);
+        else TILE(2, 1);
+#undef TILE
+    }
+    return rt_check(hipGetLastError(), "matmul_i8 launch") ? ROASTER_EDEVICE : 0;
+}

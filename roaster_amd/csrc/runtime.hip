@@ -193,14 +193,16 @@ extern "C" int roaster_sync(void)
     if (rc || !e) return rc;
     /* only what is reported is cleared, on the stream and in one piece: other bits, and those that a
      * graph on another stream sets meanwhile, are the next calls' */
-    const int said = e & ATTN_ERR_PAGES ? ATTN_ERR_PAGES : e & ATTN_ERR_PLAN ? ATTN_ERR_PLAN : e;
+    const int said = e & ATTN_ERR_PAGES ? ATTN_ERR_PAGES : e & ATTN_ERR_PLAN ? ATTN_ERR_PLAN
+                     : e & ATTN_ERR_INDEX ? ATTN_ERR_INDEX : e;
     const AttnDevice dev;
     hipLaunchKernelGGL(clear_bits_kernel, dim3(1), dim3(1), 0, g_rt.stream, word, said);
     if (rt_check(hipGetLastError(), "error word reset")) return ROASTER_EDEVICE;
     if (e & ATTN_ERR_PAGES) return rt_fail(ROASTER_ENOMEM, "roaster_kv_plan: too few free pages; the step was not planned");
     if (e & ATTN_ERR_PLAN)
         return rt_fail(ROASTER_EINVAL, "roaster_kv_plan: a length, the row count or the page ring out of range; the step was not planned");
-    return rt_fail(ROASTER_EINVAL, "attention: a request, position, page or slot out of range");
+    if (e & ATTN_ERR_INDEX) return rt_fail(ROASTER_EINVAL, "attention: a request, position, page or slot out of range");
+    return rt_fail(ROASTER_EINVAL, "roaster_ssm_scan: a request's rows, their number or its position out of range; it was left out");
 }
 
 extern "C" int roaster_device_info(int *n_cu, int *n_xcd, size_t *hbm)

@@ -1,0 +1,162 @@
+"""roaster_ssm_scan against the recurrence in 64 bits, token by token (bounds: mixer_util.scan_oracle)."""
+import numpy as np
+import pytest
+
+import roaster_amd as R
+from attn_util import sync
+from gpu_util import log
+from mixer_util import Scan, ScanCall, check_scan, scan_oracle
+
+pytestmark = pytest.mark.gpu
+DELTA, STATE = R.SCAN_DELTA, R.SCAN_STATE
+
+
+def run(s, **kw):
+    c = ScanCall(s, **kw)
+    R.check(c.call(), "scan")
+    sync()
+    return c.got()
+
+
+SHAPES = [(2, 4, 128, 128), (3, 3, 64, 64), (1, 5, 128, 64), (2, 2, 64, 128)]
+
+
+@pytest.mark.parametrize("kh,vh,kd,vd", SHAPES)
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+@pytest.mark.parametrize("new,pos", [
+    ([1], [0]), ([1, 0, 1, 1], [7, 3, 0, 2]), ([3], [0]), ([5, 1, 0, 2], [2, 1, 9, 0]), ([64], [0]), ([65], [5]), ([20, 70, 0, 130], [0, 11, 4, 3]),
+    ([1, 2, 3, 33, 31], [1, 2, 3, 0, 1000000])])
+def test_scan(kh, vh, kd, vd, mode, new, pos):
+    rng = np.random.default_rng(sum(new) + kd + 2 * vd + mode)
+    for taps in (2, 3, 4):
+        s = Scan(rng, new, pos, mode, kh, vh, kd, vd, taps, pad=taps - 2, bias=taps != 3, dt_bias=taps != 2, skip=taps == 4, wide=taps - 2)
+        o, st = check_scan(run(s), scan_oracle(s))
+        log(f"taps {taps}: out {o:.2g}, state {st:.2g} of their bounds")
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+def test_a_long_prompt(mode):
+    s = Scan(np.random.default_rng(5), [700], [0], mode, 2, 4, 128, 128)
+    log(check_scan(run(s), scan_oracle(s)))
+
+
+@pytest.mark.parametrize("most", [6, 40, 200])
+def test_a_larger_most_gives_the_same(most):
+    """Requests of few tokens under bounds that allow more."""
+    s = Scan(np.random.default_rng(9), [3, 1, 6, 0], [0, 5, 2, 8], DELTA, 2, 4, 128, 64, pad=190)
+    check_scan(run(s, most=most), scan_oracle(s))
+
+
+def test_the_same_call_gives_the_same_bits():
+    s = Scan(np.random.default_rng(6), [90, 1, 40], [0, 3, 17], DELTA, 2, 4, 128, 128)
+    a, b = run(s), run(s)
+    assert all(np.array_equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [9, 4, 2], [150, 40, 70]])
+def test_a_first_token_starts_from_zeros(new):
+    """NaN in the states of a request that begins, and of one without new tokens."""
+    s = Scan(np.random.default_rng(8), new[:1] + [0] + new[1:], [0, 4, 3, 0], DELTA, 2, 2, 64, 64)
+    want = scan_oracle(s)
+    s.conv[0], s.state[0], s.conv[1], s.state[1], s.conv[3], s.state[3] = (np.nan,) * 6
+    out, conv, state = run(s)
+    for k, arr in ((1, conv), (2, state)):
+        assert np.isnan(arr[1]).all()
+        arr[1] = want[k][1]
+    n = min(s.taps, new[0]), min(s.taps, new[2])
+    for r, m in ((0, n[0]), (3, n[1])):                     # entries that no token has filled stay as they were
+        conv[r, m:] = want[1][r, m:]
+    check_scan((out, conv, state), want)
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+@pytest.mark.parametrize("what", ["v", "k", "q", "a", "state"])
+@pytest.mark.parametrize("new,at", [([1, 1, 1], 0), ([7, 9, 3], 4), ([130, 90, 20], 70)])
+def test_infinities_and_nan_reach_only_what_uses_them(mode, what, new, at):
+    """Request 1's row `at` holds a NaN or an infinity: the other requests, its rows before and the heads that
+    do not use it come out as without it."""
+    rng = np.random.default_rng(at + mode)
+    s = Scan(rng, new, [3, 4, 0], mode, 2, 4, 64, 64, skip=False)
+    want = scan_oracle(s)
+    row = s.first[1] + at
+    heads = range(2) if what in "kq" else range(1)
+    for bad in (np.nan, np.inf):
+        saved = {k: getattr(s, k).copy() for k in ("x", "a", "state")}
+        if what == "v":
+            s.x[row, 2 * 128 + 5] = bad
+        elif what == "k":
+            s.x[row, 128 + 9] = bad
+        elif what == "q":
+            s.x[row, 9] = bad
+        elif what == "a":
+            s.a[row, 0] = np.nan
+        else:
+            s.state[1, 0, 5, 3] = bad
+        out, conv, state = run(s)
+        assert not np.isfinite(out[row, 0, 5]) or what == "state" and at
+        fine = np.ones(out.shape, bool)
+        since = s.first[1] + (0 if what == "state" else at)
+        for h in heads:
+            if what in ("v", "state"):
+                fine[since:s.first[2], h, 5] = False
+            else:
+                fine[since:s.first[2], h] = False
+        lim = want[3] + 1e-30
+        assert np.all(np.abs(out - want[0])[fine] <= lim[fine]), np.argwhere(fine & ~(np.abs(out - want[0]) <= lim))[:4].tolist()
+        sf = np.ones(want[4].shape, bool)
+        for h in heads:
+            sf[1, h] = False
+        if what in ("v", "state"):
+            sf[1, 0] = True
+            sf[1, 0, 5] = False
+        es = np.linalg.norm(np.where(np.isfinite(state), state, 1e30) - want[2], axis=3)
+        assert np.all(es[sf] <= want[4][sf] + 1e-30)
+        for k, v in saved.items():
+            setattr(s, k, v)
+
+
+def test_bad_requests_are_left_out_and_reported():
+    """Too many tokens, a negative position, rows out of range: the rows within are NaN, the states as they were,
+    the others' results right, one report."""
+    rng = np.random.default_rng(12)
+    for most, pos, first in ((2, [0, 3, 5], None), (4, [0, -2, 5], None), (4, [0, 3, 5], [0, 2, 5, 70]), (4, [0, 3, 5], [0, 2, 1, 5]),
+                             (40, [0, -7, 1], None)):
+        big = most == 40
+        new = [30, 36, 33] if big else [2, 3, 2]
+        s = Scan(rng, new, pos, DELTA, 2, 2, 64, 64, pad=3)
+        bad = 2 if first and first[3] == 70 else 1
+        n = s.new[bad]
+        s.new[bad] = 0
+        want = scan_oracle(s)
+        s.new[bad] = n
+        if first:
+            s.first = np.array(first, np.int32)
+        c = ScanCall(s, most=most)
+        R.check(c.call(), "scan")
+        assert R.lib().roaster_sync() == R.EINVAL and "left out" in R.last_error()
+        assert R.lib().roaster_sync() == R.OK
+        out, conv, state = c.got()
+        assert np.array_equal(conv[bad], s.conv[bad]) and np.array_equal(state[bad], s.state[bad])
+        f = s.first
+        if not first:
+            assert np.isnan(out[f[1]:f[2]]).all()
+        elif bad == 2:
+            assert np.isnan(out[5:]).all()
+        rows = slice(f[0], min(f[1], f[2]))                # a row that two requests claim is either's
+        assert np.all(np.abs(out[rows] - want[0][rows]) <= want[3][rows] + 1e-30)
+        if not first:
+            rows = slice(f[2], None)
+            assert np.all(np.abs(out[rows] - want[0][rows]) <= want[3][rows] + 1e-30)
+
+
+def test_many_requests_mostly_idle():
+    """2048 requests, a few with tokens."""
+    rng = np.random.default_rng(15)
+    new, pos = [0] * 2048, [1] * 2048
+    for r, m in ((0, 1), (700, 3), (2047, 2)):
+        new[r] = m
+    s = Scan(rng, new, pos, STATE, 1, 1, 64, 64)
+    check_scan(run(s), scan_oracle(s))
+    new[5], new[1999] = 70, 40
+    s = Scan(rng, new, pos, DELTA, 1, 1, 64, 64)
+    check_scan(run(s), scan_oracle(s))
