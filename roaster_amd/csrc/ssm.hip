@@ -43,8 +43,16 @@ __device__ __forceinline__ bool ssm_request(const SsmArgs &A, int r, int col, in
     return false;
 }
 
-__device__ __forceinline__ float ssm_silu(float x) { return x / (1.0f + expf(-x)); }
-__device__ __forceinline__ float ssm_softplus(float x) { return fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))); }
+/* e^x as 2^(x log2 e), the product's rounding made good: to about 2^-23 of it in 8 instructions. */
+__device__ __forceinline__ float ssm_exp(float x)
+{
+    const float t = x * 1.44269502f, p = __builtin_amdgcn_exp2f(t);              /* log2 e = 1.44269502 + 1.93e-8 */
+    const float d = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -t)) * 0.693147182f;
+    return fabsf(t) < 126.0f ? fmaf(p, d, p) : p;
+}
+__device__ __forceinline__ float ssm_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ssm_exp(-x)); }
+__device__ __forceinline__ float ssm_silu(float x) { return x * ssm_sigmoid(x); }
+__device__ __forceinline__ float ssm_softplus(float x) { return fmaxf(x, 0.0f) + log1pf(ssm_exp(-fabsf(x))); }
 
 /* One channel of the convolution, row by row: the last taps - 1 inputs and the weights. */
 struct SsmChannel {
@@ -115,7 +123,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_token_kernel(SsmArgs A, int blocks,
     }
     for (int t = 0; t < q.n; t++) {
         const int b = t & 1;
-        const float dt = ssm_softplus(av + dtb), decay = expf(coef * dt), gain = DELTA ? 1.0f / (1.0f + expf(-bv)) : dt;
+        const float dt = ssm_softplus(av + dtb), decay = ssm_exp(coef * dt), gain = DELTA ? ssm_sigmoid(bv) : dt;
         float cqv = 0.0f;
         if (qk) s_qk[b][tid] = cqv = chq.next(xq, taps);
         if (val) s_v[b][tid] = chv.next(xv, taps);
@@ -192,34 +200,47 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
  *
  * Within a chunk, G_i = sum of a_coef dt up to token i and D_ij = exp(G_i - G_j) for j <= i:
  *   A_ij = beta_i D_ij k_i.k_j (j < i),   T = (1 + A)^-1 diag(beta)
- *   W = T (V - exp(G) K S)                the w of all tokens
- *   out = exp(G) Q S + (D o Q K^T) W,     S = exp(G_63) S + K^T (exp(G_63 - G) W)
- * (STATE: W = dt V).  ssm_prep_kernel makes what does not need S for all chunks at once, ssm_chunk_kernel
- * goes through a request's chunks with a block of 16 value elements.  Both multiply on
- * v_mfma_f32_16x16x4_f32:
- *   A[m][k]: lane l holds m = l%16, k = l/16     B[k][n]: k = l/16, n = l%16
+ *   R = V - exp(G) K S,   W = T R         the w of all tokens (STATE: W = dt V)
+ *   out = scale (exp(G) Q S + (D o Q K^T) W),     S = exp(G_63) S + K^T (exp(G_63 - G) W)
+ * ssm_prep_kernel makes what does not need S for all chunks at once, ssm_chunk_kernel goes through a
+ * request's chunks with a block of 16 value elements.
+ *
+ * Products run on v_mfma_f32_16x16x32_f16 with both operands in two fp16 parts (x = hi + lo, 22 bits),
+ * hi hi + hi lo + lo hi, since f32 MFMAs have a sixteenth of the rate:
+ *   A[m][k]: lane l holds m = l%16, k = 8*(l/16) + i, i = 0..7     (B[k][n] likewise)
  *   D[m][n]: lane l holds m = 4*(l/16) + i, n = l%16, i = 0..3
- * four of them over 16 columns, the lane's four being 4*(l/16) .. + 3, so that an operand is
- * one 16-byte piece of a lane and a kilobyte of a wave; the workspace holds all operands so.
+ * Q and K are unit vectors (STATE: powers of two make them such to a factor of two, K's going into dt and Q's into
+ * the output), so they, D o Q K^T and T are at most 4 in size and enter times 2^8.  S, R and W enter
+ * times a power of two for each value element, from bounds that need no look at them: the norm of an element's
+ * row of S is at most b and grows by the sum of gain |v| |k| alone, |R| <= |v| + b, |w| <= |v| + |S|.  fp16's
+ * range below the bound (2^-38 of it) leaves 22 bits where the bound is 2^15 too large.  That takes decays
+ * of at most 1: a chunk with a positive a_coef dt, or with an infinite or NaN input, goes token by token.
  * Tokens behind a request's last are zeros with gain 0 and the decay of the last. */
 #define SSM_C 64                 /* tokens of a chunk */
 #define SSM_HG 2                 /* value heads of a workgroup of ssm_prep_kernel */
+#define SSM_UP 256.0f            /* Q, K, T and D o Q K^T as operands */
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
-/* Workspace, in floats: of a chunk and key head the operands of Q and K (tokens as rows) and K^T, of a chunk and value
- * head those of T and D o Q K^T, then exp(G), exp(G_63 - G), gain and a_coef dt of its tokens, and a
- * word that tells whether some of it is infinite or NaN. */
+/* Workspace, in bytes: of a chunk and key head the operands of Q and K (tokens as rows) and K^T, of a chunk and value
+ * head those of T and D o Q K^T and the vectors below.  An operand of 16 rows by 32 columns is a kilobyte
+ * of high and one of low parts in lane order. */
 struct SsmWs {
-    float *p;
+    char *p;
     int kd, kh, vh;
 
-    __host__ __device__ size_t key_floats() const { return 3 * (size_t)SSM_C * kd; }
-    __host__ __device__ size_t head_floats() const { return 2 * SSM_C * SSM_C + 5 * SSM_C; }
-    __host__ __device__ size_t chunk_floats() const { return kh * key_floats() + vh * head_floats(); }
-    __device__ float *key(int c, int h) const { return p + c * chunk_floats() + h * key_floats(); }
-    __device__ float *head(int c, int h) const { return p + c * chunk_floats() + kh * key_floats() + h * head_floats(); }
+    __host__ __device__ size_t key_bytes() const { return 3 * (size_t)SSM_C * kd * 4; }
+    __host__ __device__ size_t head_bytes() const { return 2 * SSM_C * SSM_C * 4 + 7 * SSM_C * 4; }
+    __host__ __device__ size_t chunk_bytes() const { return kh * key_bytes() + vh * head_bytes(); }
+    __device__ char *key(int c, int h) const { return p + c * chunk_bytes() + h * key_bytes(); }
+    __device__ char *head(int c, int h) const { return p + c * chunk_bytes() + kh * key_bytes() + h * head_bytes(); }
+    __device__ float *vec(int c, int h) const { return (float *)(head(c, h) + 2 * SSM_C * SSM_C * 4); }
 };
+/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; then the largest
+ * gain, and 1 where the chunk has to go token by token. */
+enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_MOST = 384, SSM_BAD = 385 };
 
 /* Chunks of request r, 0 for one that is idle or left out. */
 __device__ __forceinline__ int ssm_chunks(const SsmArgs &A, int r)
@@ -262,16 +283,55 @@ __device__ __forceinline__ int ssm_base(const SsmArgs &A, int r)
     return base;
 }
 
-__device__ __forceinline__ f32x4 ssm_mfma4(float4 a, float4 b, f32x4 c)
-{
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ float4 f4(f32x4 v) { return make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ bool ssm_finite(float x) { return fabsf(x) < INFINITY; }
+/* 2^e of a finite x, 2^e <= |x| < 2^(e + 1), within 2^-100 .. 2^123; 1 for others. */
+__device__ __forceinline__ float ssm_pow2(float x)
+{
+    const int e = (int)(__float_as_uint(x) >> 23 & 255);
+    return e == 255 ? 1.0f : __uint_as_float((unsigned)min(max(e, 27), 250) << 23);
+}
+__device__ __forceinline__ float ssm_inv2(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }   /* 1 / 2^e */
+
+struct SsmOp { h16x8 hi, lo; };                         /* one lane's of an operand */
+__device__ __forceinline__ SsmOp ssm_split(const float (&v)[8])
+{
+    SsmOp o;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        o.hi[i] = (_Float16)v[i];
+        o.lo[i] = (_Float16)(v[i] - (float)o.hi[i]);
+    }
+    return o;
+}
+__device__ __forceinline__ void ssm_split4(f32x4 v, float by, _Float16 *hi, _Float16 *lo)
+{
+    h16x4 h, r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x = v[i] * by;
+        h[i] = (_Float16)x;
+        r[i] = (_Float16)(x - (float)h[i]);
+    }
+    *(h16x4 *)hi = h;
+    *(h16x4 *)lo = r;
+}
+__device__ __forceinline__ SsmOp ssm_ld(const char *at, int l)
+{
+    const unsigned off = 16 * l;                        /* the base is scalar */
+    return { *(const h16x8 *)(at + off), *(const h16x8 *)(at + 1024 + off) };
+}
+__device__ __forceinline__ void ssm_st(char *at, int l, const SsmOp &o)
+{
+    *(h16x8 *)(at + 16 * l) = o.hi;
+    *(h16x8 *)(at + 1024 + 16 * l) = o.lo;
+}
+/* c += hi hi, d += hi lo + lo hi: two chains */
+__device__ __forceinline__ void ssm_mfma(const SsmOp &a, const SsmOp &b, f32x4 &c, f32x4 &d)
+{
+    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, d, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, d, 0, 0, 0);
+}
 
 /* A chunk's tokens of one key head: convolution, norms, the products among tokens, and of SSM_HG of its value
  * heads the decays and T.  Waves 0 and 1 make a head's T each, by forward substitution with a column a lane,
@@ -279,16 +339,18 @@ __device__ __forceinline__ bool ssm_finite(float x) { return fabsf(x) < INFINITY
 template <int KD, bool DELTA>
 __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int groups)
 {
-    constexpr int LD = KD + 4, LG = SSM_C + 4, G16 = KD / 16;
+    constexpr int LD = KD + 4, LG = SSM_C + 4, KS = KD / 32, OPS = 4 * KS;           /* operands of Q, and of K */
     constexpr int F0 = 2 * SSM_C * LD, F1 = (2 + SSM_HG) * SSM_C * LG;
     __shared__ __attribute__((aligned(16))) float s_buf[F0 > F1 ? F0 : F1];
     __shared__ double s_G[4][SSM_C];
+    __shared__ float s_rq[SSM_C], s_rk[SSM_C], s_qf[SSM_C], s_kf[SSM_C];
     __shared__ int s_bad;
     const RoasterSsmScan &a = A.a;
-    const int tid = threadIdx.x, l = tid % 64, w = tid / 64, taps = A.s.taps;
+    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), taps = A.s.taps;
     const int kh = blockIdx.y / groups, hg = blockIdx.y % groups, nk = A.s.k_heads * KD;
     int of;
-    const int r = ssm_find(A, blockIdx.x, of);
+    const int r = __builtin_amdgcn_readfirstlane(ssm_find(A, blockIdx.x, of));
+    of = __builtin_amdgcn_readfirstlane(of);
     if (r < 0) return;
     const int f0 = a.first[r], n = a.first[r + 1] - f0, pos = a.row_pos[f0], i0 = of * SSM_C, width = min(SSM_C, n - i0);
     float *s_q = s_buf, *s_k = s_buf + SSM_C * LD;
@@ -308,7 +370,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
         for (int j = 0; j < RG; j += 16) {
             float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = j0 + j + i < width ? x[(size_t)(j0 + j + i) * a.x_row] : 0.0f;
+            for (int i = 0; i < 16; i++) v[i] = x[(size_t)min(j0 + j + i, width - 1) * a.x_row];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const float y = cv.next(v[i], taps);
@@ -320,48 +382,58 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
     {   /* norms: four threads a row */
         const int row = tid / 4;
         float sq = 0, sk = 0;
-        float4 q[KD / 16], k[KD / 16];
 #pragma unroll
         for (int j = 0; j < KD / 16; j++) {
-            q[j] = *(const float4 *)(s_q + row * LD + 4 * (tid % 4 + 4 * j));
-            k[j] = *(const float4 *)(s_k + row * LD + 4 * (tid % 4 + 4 * j));
-            sq += q[j].x * q[j].x + q[j].y * q[j].y + q[j].z * q[j].z + q[j].w * q[j].w;
-            sk += k[j].x * k[j].x + k[j].y * k[j].y + k[j].z * k[j].z + k[j].w * k[j].w;
+            const float4 q = *(const float4 *)(s_q + row * LD + 4 * (tid % 4 + 4 * j)), k = *(const float4 *)(s_k + row * LD + 4 * (tid % 4 + 4 * j));
+            sq += q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
+            sk += k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w;
         }
         for (int o = 1; o < 4; o <<= 1) { sq += __shfl_xor(sq, o); sk += __shfl_xor(sk, o); }
-        if (!ssm_finite(sq) || !ssm_finite(sk)) s_bad = 1;
-        const float rq = DELTA ? a.scale / sqrtf(sq + a.eps) : a.scale, rk = DELTA ? 1.0f / sqrtf(sk + a.eps) : 1.0f;
-#pragma unroll
-        for (int j = 0; j < KD / 16; j++) {
-            *(float4 *)(s_q + row * LD + 4 * (tid % 4 + 4 * j)) = make_float4(q[j].x * rq, q[j].y * rq, q[j].z * rq, q[j].w * rq);
-            *(float4 *)(s_k + row * LD + 4 * (tid % 4 + 4 * j)) = make_float4(k[j].x * rk, k[j].y * rk, k[j].z * rk, k[j].w * rk);
+        if (tid % 4 == 0) {
+            const float pq = DELTA ? 1.0f : ssm_pow2(sqrtf(sq)), pk = DELTA ? 1.0f : ssm_pow2(sqrtf(sk));
+            const float rq = DELTA ? 1.0f / sqrtf(sq + a.eps) : ssm_inv2(pq), rk = DELTA ? 1.0f / sqrtf(sk + a.eps) : ssm_inv2(pk);
+            if (row < width && !(ssm_finite(sq) && ssm_finite(sk) && ssm_finite(rq) && ssm_finite(rk) && ssm_finite(a.scale * pq))) s_bad = 1;
+            s_rq[row] = row < width ? rq : 0.0f;
+            s_rk[row] = row < width ? rk : 0.0f;
+            s_qf[row] = a.scale * pq;
+            s_kf[row] = pk;
         }
     }
     __syncthreads();
-    if (hg == 0) {
-        float4 *q = (float4 *)W.key(blockIdx.x, kh), *k = q + SSM_C * KD / 4, *kt = k + SSM_C * KD / 4;
-        for (int f = tid; f < SSM_C * KD / 4; f += SSM_T) {
-            const int g = f / 64 % G16, m = f / 64 / G16 * 16 + f % 16, at = m * LD + 16 * g + 4 * (f % 64 / 16);
-            q[f] = *(const float4 *)(s_q + at);
-            k[f] = *(const float4 *)(s_k + at);
-        }
-        for (int f = tid; f < SSM_C * KD / 4; f += SSM_T) {
-            const float *at = s_k + (f / 64 % 4 * 16 + 4 * (f % 64 / 16)) * LD + f / 256 * 16 + f % 16;
-            kt[f] = make_float4(at[0], at[LD], at[2 * LD], at[3 * LD]);
-        }
+    SsmOp ops[OPS / 2];                                 /* of 2 OPS, wave w's: Q's first, then K's */
+    char *key = W.key(blockIdx.x, kh), *sop = (char *)s_buf;
+#pragma unroll
+    for (int f = 0; f < OPS / 2; f++) {
+        const int g = w * (OPS / 2) + f, row = g % OPS / KS * 16 + l % 16, col = g % KS * 32 + l / 16 * 8;
+        const float *at = (g < OPS ? s_q : s_k) + row * LD + col, by = SSM_UP * (g < OPS ? s_rq : s_rk)[row];
+        const float4 u = *(const float4 *)at, v = *(const float4 *)(at + 4);
+        ops[f] = ssm_split({ u.x * by, u.y * by, u.z * by, u.w * by, v.x * by, v.y * by, v.z * by, v.w * by });
+        if (hg == 0) ssm_st(key + g * 2048, l, ops[f]);
     }
+    if (hg == 0)
+        for (int g = w; g < OPS; g += 4) {              /* K^T: 16 key elements by 32 tokens */
+            const int col = g / 2 * 16 + l % 16, row = g % 2 * 32 + l / 16 * 8;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = s_k[(row + i) * LD + col] * (SSM_UP * s_rk[row + i]);
+            ssm_st(key + (2 * OPS + g) * 2048, l, ssm_split(v));
+        }
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < OPS / 2; f++) ssm_st(sop + (w * (OPS / 2) + f) * 2048, l, ops[f]);
+    __syncthreads();
     /* products of tokens, lower blocks alone: wave w has rows 16 w of K K^T and rows 16 (3 - w) of Q K^T */
-    f32x4 kk[4] = {}, qk[4] = {};
+    f32x4 kk[4] = {}, qk[4] = {}, kx[4] = {}, qx[4] = {};
     const int wq = 3 - w;
-    for (int g = 0; g < G16; g++) {
-        const int col = 16 * g + 4 * (l / 16);
-        const float4 ak = *(const float4 *)(s_k + (16 * w + l % 16) * LD + col), aq = *(const float4 *)(s_q + (16 * wq + l % 16) * LD + col);
+    auto op = [&](int g) { return SsmOp{ *(const h16x8 *)(sop + g * 2048 + 16 * l), *(const h16x8 *)(sop + g * 2048 + 1024 + 16 * l) }; };
+    for (int s = 0; s < KS; s++) {
+        const SsmOp ak = op(OPS + w * KS + s), aq = op(wq * KS + s);
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             if (b > w && b > wq) continue;
-            const float4 bk = *(const float4 *)(s_k + (16 * b + l % 16) * LD + col);
-            if (DELTA && b <= w) kk[b] = ssm_mfma4(ak, bk, kk[b]);
-            if (b <= wq) qk[b] = ssm_mfma4(aq, bk, qk[b]);
+            const SsmOp bk = op(OPS + b * KS + s);
+            if (DELTA && b <= w) ssm_mfma(ak, bk, kk[b], kx[b]);
+            if (b <= wq) ssm_mfma(aq, bk, qk[b], qx[b]);
         }
     }
     __syncthreads();
@@ -370,8 +442,8 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
     for (int b = 0; b < 4; b++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (DELTA && b <= w) s_kk[(16 * w + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = kk[b][i];
-            if (b <= wq) s_qk[(16 * wq + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = qk[b][i];
+            if (DELTA && b <= w) s_kk[(16 * w + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = (kk[b][i] + kx[b][i]) * (1 / (SSM_UP * SSM_UP));
+            if (b <= wq) s_qk[(16 * wq + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = (qk[b][i] + qx[b][i]) * (1 / SSM_UP);
         }
     __syncthreads();
     const int hh = hg * SSM_HG + w % SSM_HG, h = kh * A.rep + hh;
@@ -381,7 +453,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
     const size_t row = (size_t)(f0 + i0 + l);
     const float dt = in ? ssm_softplus(a.a[row * a.a_row + h] + (a.dt_bias ? a.dt_bias[h] : 0.0f)) : 0.0f;
     const float gl = in ? a.a_coef[h] * dt : 0.0f;
-    const float gain = !in ? 0.0f : DELTA ? 1.0f / (1.0f + expf(-a.b[row * a.b_row + h])) : dt;
+    const float gain = !in ? 0.0f : DELTA ? ssm_sigmoid(a.b[row * a.b_row + h]) : dt * s_kf[l];
     double G = gl;
     for (int o = 1; o < 64; o <<= 1) {
         const double v = __shfl_up(G, o);
@@ -389,26 +461,31 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
     }
     s_G[w][l] = G;
     const double last = __shfl(G, 63);
-    float *out = W.head(blockIdx.x, h);
+    char *out = W.head(blockIdx.x, h);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (w >= SSM_HG) {                                  /* D o Q K^T, in the operands' order */
+    if (w >= SSM_HG) {                                  /* D o Q K^T */
         for (int m = 0; m < 4; m++)
-            for (int g = 0; g <= m; g++) {
-                const int i = 16 * m + l % 16, j = 16 * g + 4 * (l / 16);
-                const float4 p = *(const float4 *)(s_qk + i * LG + j);
-                const float v[4] = { p.x, p.y, p.z, p.w };
-                f32x4 d;
+            for (int s = 0; s <= m / 2; s++) {
+                const int i = 16 * m + l % 16, j = 32 * s + 8 * (l / 16);
+                float v[8];
 #pragma unroll
-                for (int c = 0; c < 4; c++) d[c] = j + c <= i ? v[c] * expf((float)(s_G[w][i] - s_G[w][j + c])) : 0.0f;
-                *(f32x4 *)(out + SSM_C * SSM_C + ((m * 4 + g) * 64 + l) * 4) = d;
+                for (int c = 0; c < 8; c++) v[c] = j + c <= i ? s_qk[i * LG + j + c] * ssm_exp((float)(s_G[w][i] - s_G[w][j + c])) : 0.0f;
+                ssm_st(out + (8 + m * 2 + s) * 2048, l, ssm_split(v));
             }
-        float *vec = out + 2 * SSM_C * SSM_C;
-        vec[l] = expf((float)G);
-        vec[SSM_C + l] = expf((float)(last - G));
-        vec[2 * SSM_C + l] = gain;
-        vec[3 * SSM_C + l] = gl;
-        const bool bad = __any(!ssm_finite(gl) || !ssm_finite(gain)) || s_bad;
-        if (l == 0) vec[4 * SSM_C] = bad ? 1.0f : 0.0f;
+        float *vec = W.vec(blockIdx.x, h), top = gain;
+        const float eg = ssm_exp((float)G), qf = s_qf[l];
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        vec[SSM_EQ + l] = eg * qf;
+        vec[SSM_QF + l] = qf;
+        vec[SSM_EG + l] = eg;
+        vec[SSM_EC + l] = ssm_exp((float)(last - G));
+        vec[SSM_GAIN + l] = gain;
+        vec[SSM_GL + l] = gl;
+        const bool bad = __any(!ssm_finite(gl) || gl > 0.0f || !ssm_finite(gain)) || s_bad;
+        if (l == 0) {
+            vec[SSM_MOST] = top;
+            vec[SSM_BAD] = bad ? 1.0f : 0.0f;
+        }
     } else if (DELTA) {
         float *s_A = s_buf + (2 + w) * SSM_C * LG;
         for (int m = 0; m < 4; m++)
@@ -419,7 +496,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
                 const float beta = __shfl(gain, i);
                 f32x4 d;
 #pragma unroll
-                for (int c = 0; c < 4; c++) d[c] = j + c < i ? beta * v[c] * expf((float)(s_G[w][i] - s_G[w][j + c])) : 0.0f;
+                for (int c = 0; c < 4; c++) d[c] = j + c < i ? beta * v[c] * ssm_exp((float)(s_G[w][i] - s_G[w][j + c])) : 0.0f;
                 *(f32x4 *)(s_A + i * LG + j) = d;
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -441,26 +518,33 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int i = 0; i < SSM_C; i++) s_A[i * LG + l] = x[i] * gain;
+        for (int i = 0; i < SSM_C; i++) s_A[i * LG + l] = x[i] * (gain * SSM_UP);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         for (int m = 0; m < 4; m++)
-            for (int g = 0; g <= m; g++)
-                *(f32x4 *)(out + ((m * 4 + g) * 64 + l) * 4) = *(const f32x4 *)(s_A + (16 * m + l % 16) * LG + 16 * g + 4 * (l / 16));
+            for (int s = 0; s <= m / 2; s++) {
+                const float *at = s_A + (16 * m + l % 16) * LG + 32 * s + 8 * (l / 16);
+                const float4 u = *(const float4 *)at, v = *(const float4 *)(at + 4);
+                ssm_st(out + (m * 2 + s) * 2048, l, ssm_split({ u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w }));
+            }
     }
 }
 
-/* A request's chunks in order, for 16 value elements of one head; S stays in registers as the products leave it (lane:
- * value element l%16, key elements 16 (KB w + b) + 4 (l/16) + i) and in LDS as they take it.  Wave w has tokens
- * 16 w .. of every product with tokens as rows.  Operands of the next chunk are loaded while this one is worked on. */
+/* A request's chunks in order, for 16 value elements of one head (v = l%16), with two groups of four waves: the first goes
+ * from S to W, the second makes the outputs and the next chunk's values; token rows 16 (w % 4) .. each, and each
+ * wave has 16 key elements of S.  S stays in registers as the products leave it (key elements 16 w + 4 (l/16) + i) and
+ * in LDS as they take it.  Operands of the next chunk are loaded while this one is worked on, without conditions, so that
+ * waits count those under way exactly. */
 template <int KD, bool DELTA>
-__global__ __launch_bounds__(SSM_T, 1) void ssm_chunk_kernel(SsmArgs A, SsmWs W, int blocks, int max_chunks, int *err)
+__global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmWs W, int blocks, int max_chunks, int *err)
 {
-    constexpr int KB = KD / 64, G16 = KD / 16, LS = KD + 4, LT = SSM_C + 4;
-    __shared__ __attribute__((aligned(16))) float s_S[16 * LS], s_R[16 * LT], s_W[16 * LT], s_We[16 * LT];
-    __shared__ float s_part[2][4][16];
-    __shared__ int s_bad;
+    constexpr int KS = KD / 32, OPS = 4 * KS, LS = KD + 8, LT = SSM_C + 8, LV = SSM_C + 4;
+    __shared__ __attribute__((aligned(16))) _Float16 s_S[2][16 * LS], s_R[2][16 * LT], s_W[2][16 * LT], s_We[2][16 * LT];
+    __shared__ __attribute__((aligned(16))) float s_V[2][16 * LV];
+    __shared__ float s_top[2][16][4], s_part[2][8][16];
     const RoasterSsmScan &a = A.a;
-    const int tid = threadIdx.x, l = tid % 64, w = tid / 64, taps = A.s.taps, VD = A.s.v_dim, VH = A.s.v_heads;
+    const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;    /* so that operands' addresses are scalar */
+    const int taps = A.s.taps, VD = A.s.v_dim, VH = A.s.v_heads;
+    const bool first = w8 < 4, holds = w8 < KD / 16;
     /* with a multiple of 8 heads, those of one key head and their blocks on one XCD (workgroup b runs on b % 8) */
     int h = blockIdx.x / blocks, vb = blockIdx.x % blocks;
     if (VH % 8 == 0) {
@@ -471,194 +555,226 @@ __global__ __launch_bounds__(SSM_T, 1) void ssm_chunk_kernel(SsmArgs A, SsmWs W,
     const int r = blockIdx.y, kh = h / A.rep, nk = A.s.k_heads * KD, v0 = h * VD + vb * 16;
     SsmReq q;
     if (!ssm_request(A, r, v0, 16, q, err)) return;
-    const int base = ssm_base(A, r), chunks = (q.n + SSM_C - 1) / SSM_C;
+    const int base = __builtin_amdgcn_readfirstlane(ssm_base(A, r)), chunks = (q.n + SSM_C - 1) / SSM_C;
     if (base + chunks > max_chunks) {                   /* requests that share rows, so that `first` is none of a plan */
         if (tid == 0) atomicOr(err, ATTN_ERR_SCAN);
-        for (int t = tid; t < q.n * 16; t += SSM_T) a.out[(size_t)(q.f0 + t / 16) * a.out_row + v0 + t % 16] = __uint_as_float(0x7FC00000u);
+        for (int t = tid; t < q.n * 16; t += 2 * SSM_T) a.out[(size_t)(q.f0 + t / 16) * a.out_row + v0 + t % 16] = __uint_as_float(0x7FC00000u);
         return;
     }
     const int v = l % 16, t4 = 16 * w + 4 * (l / 16), cv = 2 * nk + v0 + v;
-    float *state = A.s.state + ((size_t)r * VH * VD + v0 + v) * KD + 4 * (l / 16);
-    f32x4 S[KB];
-#pragma unroll
-    for (int b = 0; b < KB; b++) {
-        S[b] = q.pos ? *(const f32x4 *)(state + 16 * (KB * w + b)) : (f32x4){ 0, 0, 0, 0 };
-        *(f32x4 *)(s_S + v * LS + 16 * (KB * w + b) + 4 * (l / 16)) = S[b];
-    }
-    if (tid == 0) s_bad = 0;
+    float *state = A.s.state + ((size_t)r * VH * VD + v0 + v) * KD + 16 * w8 + 4 * (l / 16);
+    f32x4 S = {};
+    if (holds && q.pos) S = *(const f32x4 *)state;
     SsmChannel conv;                                    /* its history is that of the request's first row */
     conv.start(A, r, q.pos, cv);
     const float skip = a.skip ? a.skip[h] : 0.0f;
     const float *x = a.x + (size_t)q.f0 * a.x_row + cv;
 
     struct Ops {
-        float4 k[G16], q[G16], t[4], a[4], kt[KB][4];
-        float x[7];
-        f32x4 eg, ec, gain;
-        float last, bad;
+        SsmOp one[KS], two[2], kt[2];                   /* DELTA's first group: K and T; else Q and D o Q K^T; K^T */
+        f32x4 f, g;                                     /* exp(G) and exp(G_63 - G) (STATE: and gain), or the outputs' factors */
+        f32x4 gain;
+        float last, most, bad;
+    };
+    auto load_x = [&](int c, float (&xs)[7]) {
+#pragma unroll
+        for (int j = 0; j < 7; j++)                      /* rows before the first and behind the last are not used */
+            xs[j] = x[(size_t)min(max(c * SSM_C + t4 - 3 + j, 0), q.n - 1) * a.x_row];
     };
     auto load = [&](int c, Ops &o) {
-        const float4 *key = (const float4 *)W.key(base + c, kh), *head = (const float4 *)W.head(base + c, h);
-        const float *vec = (const float *)(head + 2 * SSM_C * SSM_C / 4);
+        const char *key = W.key(base + c, kh), *head = W.head(base + c, h);
+        const float *vec = W.vec(base + c, h);
 #pragma unroll
-        for (int g = 0; g < G16; g++) {
-            if (DELTA) o.k[g] = gld_f4(key + SSM_C * KD / 4 + (w * G16 + g) * 64 + l);
-            o.q[g] = gld_f4(key + (w * G16 + g) * 64 + l);
+        for (int s = 0; s < KS; s++) o.one[s] = ssm_ld(key + ((DELTA && first ? OPS : 0) + w * KS + s) * 2048, l);
+        o.f = *(const f32x4 *)(vec + (first ? SSM_EG : SSM_EQ) + t4);
+        o.g = *(const f32x4 *)(vec + (first ? SSM_EC : SSM_QF) + t4);
+        if (!DELTA) o.gain = *(const f32x4 *)(vec + SSM_GAIN + t4);
+        o.last = vec[SSM_EG + SSM_C - 1];
+        o.most = vec[SSM_MOST];
+        o.bad = vec[SSM_BAD];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {                    /* tokens 32 .. have no part in rows below */
+            o.two[s] = ssm_ld(head + ((DELTA && first ? 0 : 8) + w * 2 + min(s, w / 2)) * 2048, l);
+            o.kt[s] = ssm_ld(key + (2 * OPS + (holds ? w8 : 0) * 2 + s) * 2048, l);
         }
-#pragma unroll
-        for (int j = 0; j < 7; j++) {
-            const int i = c * SSM_C + t4 - 3 + j;
-            o.x[j] = i >= 0 && i < q.n ? x[(size_t)i * a.x_row] : 0.0f;
-        }
-        o.eg = *(const f32x4 *)(vec + t4);
-        o.ec = *(const f32x4 *)(vec + SSM_C + t4);
-        o.gain = *(const f32x4 *)(vec + 2 * SSM_C + t4);
-        o.last = vec[SSM_C - 1];
-        o.bad = vec[4 * SSM_C];
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-            if (g <= w) {
-                if (DELTA) o.t[g] = gld_f4(head + (w * 4 + g) * 64 + l);
-                o.a[g] = gld_f4(head + SSM_C * SSM_C / 4 + (w * 4 + g) * 64 + l);
-            }
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) o.kt[b][g] = gld_f4(key + 2 * SSM_C * KD / 4 + ((KB * w + b) * 4 + g) * 64 + l);
     };
-    auto chunk = [&](int c, const Ops &o) {
-        const int width = min(SSM_C, q.n - c * SSM_C);
-        /* values of tokens t4 .. t4 + 3 */
+    /* values of chunk c to LDS, and the largest of each element */
+    auto values = [&](int c, const float (&xs)[7]) {
         float xx[7];
 #pragma unroll
-        for (int j = 0; j < 7; j++) xx[j] = o.x[j];
+        for (int j = 0; j < 7; j++) xx[j] = xs[j];
         if (c == 0 && t4 == 0) {
 #pragma unroll
             for (int j = 0; j < 3; j++) xx[j] = conv.h[j];
         }
         f32x4 V;
-        bool odd = false;
+        float top = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             SsmChannel cc = conv;
             cc.h[0] = xx[i]; cc.h[1] = xx[i + 1]; cc.h[2] = xx[i + 2];
-            V[i] = t4 + i < width ? cc.next(xx[i + 3], taps) : 0.0f;
-            odd |= !ssm_finite(V[i]);
+            const float y = cc.next(xx[i + 3], taps);
+            V[i] = c * SSM_C + t4 + i < q.n ? y : 0.0f;
+            /* NaN and infinities stay: the largest tells whether all are finite */
+            top = ssm_finite(V[i]) ? fmaxf(top, fabsf(V[i])) : INFINITY;
         }
-        if (odd || o.bad != 0.0f) s_bad = c + 1;
-        f32x4 P = {}, Q = {};
-#pragma unroll
-        for (int g = 0; g < G16; g++) {
-            const float4 b = *(const float4 *)(s_S + v * LS + 16 * g + 4 * (l / 16));
-            if (DELTA) P = ssm_mfma4(o.k[g], b, P);
-            Q = ssm_mfma4(o.q[g], b, Q);
-        }
-        if (DELTA) {
-            f32x4 R;
-#pragma unroll
-            for (int i = 0; i < 4; i++) R[i] = V[i] - o.eg[i] * P[i];
-            *(f32x4 *)(s_R + v * LT + t4) = R;
-            __syncthreads();
-        }
-        f32x4 Wv = {};
-        if (DELTA) {
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                if (g <= w) Wv = ssm_mfma4(o.t[g], *(const float4 *)(s_R + v * LT + 16 * g + 4 * (l / 16)), Wv);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) Wv[i] = o.gain[i] * V[i];
-        }
-        f32x4 We;
-#pragma unroll
-        for (int i = 0; i < 4; i++) We[i] = o.ec[i] * Wv[i];
-        *(f32x4 *)(s_W + v * LT + t4) = Wv;
-        *(f32x4 *)(s_We + v * LT + t4) = We;
-        __syncthreads();
+        for (int o = 16; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        *(f32x4 *)(s_V[c & 1] + v * LV + t4) = V;
+        if (l < 16) s_top[c & 1][v][w] = top;
+    };
+    auto op = [&](const _Float16 *p, int ld, int s) {
+        const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
+        return SsmOp{ *(const h16x8 *)at, *(const h16x8 *)(at + 16 * ld) };
+    };
+    auto put_S = [&](float by) {
+        if (holds) ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
+    };
+
+    Ops o0, o1;
+    float xs[7];
+    load_x(0, xs);
+    load(0, o0);
+    if (!first) values(0, xs);
+    load_x(min(1, chunks - 1), xs);
+    /* the norm of the element's row of S */
+    float b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
+    b += __shfl_xor(b, 16);
+    b += __shfl_xor(b, 32);
+    if (l < 16) s_part[0][w8][l] = b;
+    __syncthreads();
+    b = 0;
+    for (int i = 0; i < 8; i++) b += s_part[0][i][v];
+    b = sqrtf(b) * 1.0001f;
+    float pS = ssm_pow2(b);                              /* |S| < 2 pS; as an operand times 2^13 / pS, so below 2^14 */
+    put_S(8192.0f * ssm_inv2(pS));
+    __syncthreads();
+
+    auto chunk = [&](int c, const Ops &o) {
+        const f32x4 tops = *(const f32x4 *)s_top[c & 1][v];
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        /* the wave's lanes have all 16 elements, with the same bounds in every wave */
+        const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
+        const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
         float *out = a.out + (size_t)(q.f0 + c * SSM_C) * a.out_row + v0 + v;
-        if (s_bad != c + 1) {
-            f32x4 O;
+        const float last = o.last;
+        if (!bad) {
+            /* bounds: of R, of W, and of the next S */
+            const float bR = top + b, bW = DELTA ? b + 65.0f * top : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
+            f32x4 X = {}, Y = {};
 #pragma unroll
-            for (int i = 0; i < 4; i++) O[i] = o.eg[i] * Q[i];
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                if (g <= w) O = ssm_mfma4(o.a[g], *(const float4 *)(s_W + v * LT + 16 * g + 4 * (l / 16)), O);
-#pragma unroll
-            for (int b = 0; b < KB; b++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) S[b][i] *= o.last;
-#pragma unroll
-                for (int g = 0; g < 4; g++) S[b] = ssm_mfma4(o.kt[b][g], *(const float4 *)(s_We + v * LT + 16 * g + 4 * (l / 16)), S[b]);
+            for (int s = 0; s < KS; s++)
+                if (DELTA || !first) ssm_mfma(o.one[s], op(s_S[0], LS, s), X, Y);
+            X = (X + Y) * (pS * (1 / (8192.0f * SSM_UP)));
+            const f32x4 V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
+            if (DELTA) {
+                if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
+                __syncthreads();
             }
+            if (first) {
+                f32x4 w4 = {};
+                if (DELTA) {
+                    f32x4 d = {};
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (t4 + i < width) out[(size_t)(t4 + i) * a.out_row] = a.skip ? fmaf(skip, V[i], O[i]) : O[i];
-        } else {
-            /* an infinite or NaN input: token by token, so that it does not reach those before it */
-            const float *key = W.key(base + c, kh), *vec = W.head(base + c, h) + 2 * SSM_C * SSM_C;
-            *(f32x4 *)(s_R + v * LT + t4) = V;
+                    for (int s = 0; s < 2; s++)
+                        if (s <= w / 2) ssm_mfma(o.two[s], op(s_R[0], LT, s), w4, d);
+                    w4 = (w4 + d) * (pR * (1 / (8192.0f * SSM_UP)));
+                } else w4 = o.gain * V;
+                ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
+                ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
+            } else if (c + 1 < chunks) values(c + 1, xs);
             __syncthreads();
-            for (int t = 0; t < width; t++) {
-                const float decay = expf(vec[3 * SSM_C + t]), gain = vec[2 * SSM_C + t], val = s_R[v * LT + t];
-                f32x4 kf[KB], qf[KB];
-                float sk = 0, so = 0;
+            const float back = pW * (1 / (8192.0f * SSM_UP));
+            if (holds) {
+                f32x4 s4 = {}, d = {};
 #pragma unroll
-                for (int b = 0; b < KB; b++) {
-                    const int at = ((t / 16 * G16 + KB * w + b) * 64 + t % 16 + l / 16 * 16) * 4;
-                    qf[b] = *(const f32x4 *)(key + at);
-                    kf[b] = *(const f32x4 *)(key + SSM_C * KD + at);
+                for (int s = 0; s < 2; s++) ssm_mfma(o.kt[s], op(s_We[0], LT, s), s4, d);
+                S = S * last + (s4 + d) * back;
+            }
+            b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
+            pS = ssm_pow2(b);
+            put_S(8192.0f * ssm_inv2(pS));
+            if (!first) {
+                f32x4 O = {}, d = {};
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sk = fmaf(S[b][i], kf[b][i], sk);
+                for (int s = 0; s < 2; s++)
+                    if (s <= w / 2) ssm_mfma(o.two[s], op(s_W[0], LT, s), O, d);
+                O = o.f * X + o.g * ((O + d) * back);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (c * SSM_C + t4 + i < q.n) out[(size_t)(t4 + i) * a.out_row] = a.skip ? fmaf(skip, V[i], O[i]) : O[i];
+            }
+        } else {
+            /* token by token, so that an infinite or NaN input does not reach those before it */
+            const char *key = W.key(base + c, kh);
+            const float *vec = W.vec(base + c, h);
+            for (int t = 0; t < min(SSM_C, q.n - c * SSM_C); t++) {
+                const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[c & 1][v * LV + t];
+                f32x4 kf = {}, qf = {};
+                if (holds) {
+                    const int k = 16 * w8 + 4 * (l / 16);
+                    const char *at = key + (t / 16 * KS + k / 32) * 2048 + (t % 16 + 16 * (k % 32 / 8)) * 16 + k % 8 * 2;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        qf[i] = ((float)((const _Float16 *)at)[i] + (float)((const _Float16 *)(at + 1024))[i]) * (1 / SSM_UP);
+                        kf[i] = ((float)((const _Float16 *)(at + OPS * 2048))[i] + (float)((const _Float16 *)(at + OPS * 2048 + 1024))[i]) * (1 / SSM_UP);
+                    }
                 }
                 float wt = gain * val;
                 if (DELTA) {
+                    float sk = S[0] * kf[0] + S[1] * kf[1] + S[2] * kf[2] + S[3] * kf[3];
                     sk += __shfl_xor(sk, 16);
                     sk += __shfl_xor(sk, 32);
-                    if (l < 16) s_part[0][w][l] = sk;
+                    if (l < 16) s_part[0][w8][l] = sk;
                     __syncthreads();
-                    wt = gain * (val - decay * (s_part[0][0][v] + s_part[0][1][v] + s_part[0][2][v] + s_part[0][3][v]));
+                    sk = 0;
+                    for (int i = 0; i < KD / 16; i++) sk += s_part[0][i][v];
+                    wt = gain * (val - decay * sk);
                 }
-#pragma unroll
-                for (int b = 0; b < KB; b++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        S[b][i] = fmaf(wt, kf[b][i], decay * S[b][i]);
-                        so = fmaf(S[b][i], qf[b][i], so);
-                    }
+                S = decay * S + wt * kf;
+                float so = S[0] * qf[0] + S[1] * qf[1] + S[2] * qf[2] + S[3] * qf[3];
                 so += __shfl_xor(so, 16);
                 so += __shfl_xor(so, 32);
-                if (l < 16) s_part[1][w][l] = so;
+                if (l < 16) s_part[1][w8][l] = so;
                 __syncthreads();
                 if (tid < 16) {
-                    const float o4 = s_part[1][0][v] + s_part[1][1][v] + s_part[1][2][v] + s_part[1][3][v];
-                    out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, o4) : o4;
+                    so = 0;
+                    for (int i = 0; i < KD / 16; i++) so += s_part[1][i][v];
+                    so *= vec[SSM_QF + t];
+                    out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, so) : so;
                 }
                 __syncthreads();
             }
+            if (!first && c + 1 < chunks) values(c + 1, xs);
+            b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
+            b += __shfl_xor(b, 16);
+            b += __shfl_xor(b, 32);
+            if (l < 16) s_part[0][w8][l] = b;
+            __syncthreads();
+            b = 0;
+            for (int i = 0; i < 8; i++) b += s_part[0][i][v];
+            b = sqrtf(b) * 1.0001f;
+            pS = ssm_pow2(b);
+            put_S(8192.0f * ssm_inv2(pS));
         }
-#pragma unroll
-        for (int b = 0; b < KB; b++) *(f32x4 *)(s_S + v * LS + 16 * (KB * w + b) + 4 * (l / 16)) = S[b];
         __syncthreads();
     };
-    Ops o0, o1;
-    load(0, o0);
-    __syncthreads();
     for (int c = 0; c < chunks; c += 2) {
-        if (c + 1 < chunks) load(c + 1, o1);
+        load(min(c + 1, chunks - 1), o1);
+        if (c) load_x(min(c + 1, chunks - 1), xs);
         chunk(c, o0);
         if (c + 1 == chunks) break;
-        if (c + 2 < chunks) load(c + 2, o0);
+        load(min(c + 2, chunks - 1), o0);
+        load_x(min(c + 2, chunks - 1), xs);
         chunk(c + 1, o1);
     }
-#pragma unroll
-    for (int b = 0; b < KB; b++) *(f32x4 *)(state + 16 * (KB * w + b)) = S[b];
+    if (holds) *(f32x4 *)state = S;
     /* the inputs of the last positions: these value channels, and by one workgroup of a key head its own */
     for (int i = max(0, q.n - taps); i < q.n; i++) {
         float *to = A.s.conv + ((size_t)r * taps + ((unsigned)q.pos + i) % taps) * A.channels;
         const float *from = a.x + (size_t)(q.f0 + i) * a.x_row;
         if (tid < 16) to[2 * nk + v0 + tid] = from[2 * nk + v0 + tid];
         if (vb == 0 && h % A.rep == 0)
-            for (int j = tid; j < 2 * KD; j += SSM_T) {
+            for (int j = tid; j < 2 * KD; j += 2 * SSM_T) {
                 const int ch = j < KD ? kh * KD + j : nk + kh * KD + j - KD;
                 to[ch] = from[ch];
             }
@@ -685,7 +801,7 @@ extern "C" size_t roaster_ssm_ws_bytes(int rows, int most, const RoasterSsmState
     if (!ssm_state_ok(s) || rows < 0 || rows > (1 << 18) || most < 1 || (rows && most > rows)) return 0;
     if (most < SSM_CHUNK_MIN) return 16;
     const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads };
-    return (size_t)ssm_max_chunks(rows, s) * w.chunk_floats() * sizeof(float);
+    return (size_t)ssm_max_chunks(rows, s) * w.chunk_bytes();
 }
 
 extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *s)
@@ -732,13 +848,13 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
     SsmArgs A = { *p, *s, s->v_heads / s->k_heads, (int)ch };
     A.a.b = b;
     if (p->most >= SSM_CHUNK_MIN) {
-        const SsmWs W = { (float *)p->ws, s->k_dim, s->k_heads, s->v_heads };
+        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads };
         const int chunks = ssm_max_chunks(p->rows, s), groups = (A.rep + SSM_HG - 1) / SSM_HG, blocks = s->v_dim / 16;
 #define CHUNK(KD, D)                                                                                                          \
     do {                                                                                                                    \
         hipLaunchKernelGGL((ssm_prep_kernel<KD, D>), dim3(chunks, s->k_heads * groups), dim3(SSM_T), 0, rt().stream, A, W,    \
                            groups);                                                                                          \
-        hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, n), dim3(SSM_T), 0, rt().stream, A, W, blocks,        \
+        hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, n), dim3(2 * SSM_T), 0, rt().stream, A, W, blocks,    \
                            chunks, err);                                                                                    \
     } while (0)
         if (s->k_dim == 128) { if (delta) CHUNK(128, true); else CHUNK(128, false); }
