@@ -17,6 +17,7 @@
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4_a16 __attribute__((ext_vector_type(4)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 static inline size_t i8_rows(int rows) { return ((size_t)rows + 31) & ~(size_t)31; }
@@ -91,86 +92,119 @@ struct I8Args {
 
 __device__ __forceinline__ i32x4 i8_ld(const void *p) { return *(const GAS i32x4 *)p; }
 
-/* Up to 32 tokens: a workgroup takes 32 channels, its waves a part of the columns each and join in LDS
- * (integers, so in any order).  Weights go from memory straight into the products, tokens too (from the L2).
+/* Up to 32 tokens: a workgroup takes 16 channels, its waves a part of the columns each and join in LDS
+ * (integers, so in any order).  Weights go from memory straight into v_mfma_i32_16x16x64_i8 (lane l: row l%16, columns
+ * 16*(l/16) ..; results 4*(l/16) + i, i = 0..3, of token l%16), tokens too, from the L2; eight steps' loads are issued together.
  * Padded columns of the weights are zeros, so any byte of the token may stand there. */
+template <int TT>
 __global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a)
 {
-    __shared__ int s_sum[32 * 32];                     /* [token][channel] */
-    const int tid = threadIdx.x, l = tid % 64, w = tid / 64, W = blockDim.x / 64;
-    for (int i = tid; i < 1024; i += blockDim.x) s_sum[i] = 0;
-    const int k0 = a.k32 * w / W, k1 = a.k32 * (w + 1) / W;
-    const int8_t *wp = a.w + ((size_t)blockIdx.x * a.k32 + k0) * 1024 + 16 * l;
-    const int8_t *xp = a.x + min(l % 32, a.T - 1) * a.x_row;
-    i32x16 acc = {};
-    int k = k0;
-    for (; k + 8 <= k1; k += 8, wp += 8192) {
-        i32x4 A[8], B[8];
+    __shared__ int s_sum[TT * 16 * 16];                /* [token][channel] */
+    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), W = blockDim.x / 64;
+    const int k0 = a.k32 / 2 * w / W, k1 = a.k32 / 2 * (w + 1) / W, n16 = a.n16;
+    const int8_t *wp = a.w + (size_t)(blockIdx.x / 2) * a.k32 * 1024 + blockIdx.x % 2 * 256;
+    const unsigned off = l / 16 * 512 + l % 16 * 16;
+    const int8_t *xp[TT];
 #pragma unroll
-        for (int i = 0; i < 8; i++) A[i] = i8_ld(wp + 1024 * i);
+    for (int t = 0; t < TT; t++) xp[t] = a.x + min(16 * t + l % 16, a.T - 1) * a.x_row;
+    const int tok = tid / 16, ch = blockIdx.x * 16 + tid % 16;
+    const float ws = a.ws[min(ch, a.N - 1)];
+    float xs[TT];                                      /* of the first 256 threads' tokens tok + 16 t */
 #pragma unroll
-        for (int i = 0; i < 8; i++) B[i] = i8_ld(xp + 16 * min(2 * (k + i) + l / 32, a.n16 - 1));
+    for (int t = 0; t < TT; t++) xs[t] = a.xs[min(tok + 16 * t, a.T - 1)];
+    for (int i = tid; i < TT * 256; i += blockDim.x) s_sum[i] = 0;
+    i32x4 acc[TT] = {};
+    for (int k = k0; k < k1; k += 8) {
+        i32x4 A[8], B[TT][8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(A[i], B[i], acc, 0, 0, 0);
+        for (int i = 0; i < 8; i++) A[i] = *(const i32x4 *)(wp + (size_t)min(k + i, k1 - 1) * 2048 + off);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int t = 0; t < TT; t++) B[t][i] = i8_ld(xp[t] + 16 * min(4 * (k + i) + l / 16, n16 - 1));
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (k + i < k1) {
+#pragma unroll
+                for (int t = 0; t < TT; t++) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[i], B[t][i], acc[t], 0, 0, 0);
+            }
     }
-    for (; k < k1; k++, wp += 1024)
-        acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(i8_ld(wp), i8_ld(xp + 16 * min(2 * k + l / 32, a.n16 - 1)), acc, 0, 0, 0);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; i++) atomicAdd(&s_sum[(l % 32) * 32 + 8 * (i / 4) + 4 * (l / 32) + i % 4], acc[i]);
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) atomicAdd(&s_sum[(16 * t + l % 16) * 16 + 4 * (l / 16) + i], acc[t][i]);
     __syncthreads();
-    for (int i = tid; i < 32 * a.T; i += blockDim.x) {
-        const int t = i / 32, c = blockIdx.x * 32 + i % 32;
-        if (c < a.N) a.y[t * a.y_row + c] = (float)s_sum[i] * (a.xs[t] * a.ws[c]);
-    }
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+        if (tid < 256 && tok + 16 * t < a.T && ch < a.N) a.y[(tok + 16 * t) * a.y_row + ch] = (float)s_sum[tid + 256 * t] * (xs[t] * ws);
 }
 
 __device__ __forceinline__ void i8_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }   /* loads stay in flight */
 
-/* More tokens: a workgroup's tile is 32 TB tokens by 128 CB channels, a wave's all its tokens by 32 CB
- * channels.  So no two waves read the same weights, which go from the L2 straight into registers, and only
- * the tokens pass through LDS, 64 columns at a time, doubly buffered; both are loaded two such steps ahead.  Pieces of
- * 16 bytes of a token are exchanged by (token / 2) % 4, so that eight lanes' reads fall on different banks. */
-template <int TB, int CB>
+/* Four outputs of a token from channel ch on; STREAM: past the caches. */
+template <bool STREAM>
+__device__ __forceinline__ void i8_put(const I8Args &a, int tok, int ch, f32x4_a16 v)
+{
+    if (tok >= a.T) return;
+    float *y = a.y + tok * a.y_row + ch;
+    if (ch + 4 <= a.N) {
+        if (STREAM) __builtin_nontemporal_store((f32x4_a4)v, (f32x4_a4 *)y);
+        else *(f32x4_a4 *)y = v;
+    } else
+        for (int k = 0; k < 4; k++)
+            if (ch + k < a.N) y[k] = v[k];
+}
+
+/* More tokens: a workgroup's tile is 32 TB tokens by 128 CB channels, a wave's all its tokens by 32 CB channels.  So no
+ * two waves read the same weights, which go from the L2 straight into registers, and only the tokens pass through LDS, a
+ * step of U times 64 columns at a time, doubly buffered; both are loaded two steps ahead.  Pieces of 16 bytes of a token
+ * are exchanged by (token / 2) % 4, so that eight lanes' reads fall on different banks.  Outputs of the larger tiles are
+ * not kept in the caches (2048 tokens of 12288 x 2048: 62 us, kept 72). */
+template <int TB, int CB, int U>
 __global__ __launch_bounds__(I8_T, 2) void i8_tile_kernel(I8Args a, int tiles, int per, int tblocks)
 {
-    constexpr int TM = 32 * TB, XL = (TM * 4 + I8_T - 1) / I8_T;
-    __shared__ __attribute__((aligned(16))) int8_t s_x[2][TM * 64];
+    constexpr int TM = 32 * TB, XN = TM * 4 * U, XL = (XN + I8_T - 1) / I8_T;
+    constexpr int LY = 32 * CB + 4, YB = 4 * 32 * LY * 4, XB = 2 * U * TM * 64;      /* outputs of a wave's 32 tokens; buffers */
+    __shared__ __attribute__((aligned(16))) int8_t s_lds[XB > YB ? XB : YB];
     /* workgroup b runs on XCD b % 8: each has a run of tiles, tokens' blocks of one channel block in turn */
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= tiles) return;
-    const int tid = threadIdx.x, l = tid % 64, w = tid / 64;
-    const int t0 = id % tblocks * TM, c0 = id / tblocks * (128 * CB) + 32 * CB * w;
-    const int steps = a.k32 / 2;
+    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int t0 = id % tblocks * TM, c0 = id / tblocks * (128 * CB) + 32 * CB * w, all = a.k32 / 2, steps = (all + U - 1) / U;
+    int8_t *const s_x[2] = { s_lds, s_lds + U * TM * 64 };
     const int8_t *wp[CB];
     for (int c = 0; c < CB; c++) {
         const int cb = min(c0 / 32 + c, (a.N + 31) / 32 - 1);
-        wp[c] = a.w + (size_t)cb * a.k32 * 1024 + 16 * l;
+        wp[c] = a.w + (size_t)cb * a.k32 * 1024;
     }
     const int8_t *xp[XL];
     int xc[XL], xd[XL];
     for (int i = 0; i < XL; i++) {
-        const int q = min(tid + i * I8_T, TM * 4 - 1), t = q / 4;
+        const int q = min(tid + i * I8_T, XN - 1), t = q % (TM * 4) / 4, u = q / (TM * 4);
         xp[i] = a.x + min(t0 + t, a.T - 1) * a.x_row;
-        xc[i] = q % 4;
-        xd[i] = t * 64 + ((q % 4 ^ (t >> 1 & 3)) << 4);
+        xc[i] = 4 * u + q % 4;
+        xd[i] = (u * TM + t) * 64 + ((q % 4 ^ (t >> 1 & 3)) << 4);
     }
-    i32x4 W[2][2 * CB], X[2][XL];
-    auto load_w = [&](int s, i32x4 (&r)[2 * CB]) {
-        s = min(s, steps - 1);
+    i32x4 W[2][2 * CB * U], X[2][XL];
+    auto load_w = [&](int s, i32x4 (&r)[2 * CB * U]) {
 #pragma unroll
-        for (int c = 0; c < CB; c++)
+        for (int u = 0; u < U; u++) {
+            const size_t at = (size_t)min(s * U + u, all - 1) * 2048;
 #pragma unroll
-            for (int h = 0; h < 2; h++) r[2 * c + h] = i8_ld(wp[c] + (size_t)s * 2048 + 1024 * h);
+            for (int c = 0; c < CB; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) r[(2 * u + h) * CB + c] = *(const i32x4 *)(wp[c] + at + 1024 * h + 16u * l);
+        }
     };
     auto load_x = [&](int s, i32x4 (&r)[XL]) {
 #pragma unroll
-        for (int i = 0; i < XL; i++) r[i] = i8_ld(xp[i] + 16 * min(4 * s + xc[i], a.n16 - 1));
+        for (int i = 0; i < XL; i++) r[i] = i8_ld(xp[i] + 16 * min(4 * s * U + xc[i], a.n16 - 1));
     };
     auto store_x = [&](int b, const i32x4 (&r)[XL]) {
 #pragma unroll
         for (int i = 0; i < XL; i++)
-            if (TM * 4 % I8_T == 0 || tid + i * I8_T < TM * 4) *(i32x4 *)(s_x[b] + xd[i]) = r[i];
+            if (XN % I8_T == 0 || tid + i * I8_T < XN) *(i32x4 *)(s_x[b] + xd[i]) = r[i];
     };
     i32x16 acc[CB][TB];
     for (int c = 0; c < CB; c++)
@@ -179,13 +213,18 @@ __global__ __launch_bounds__(I8_T, 2) void i8_tile_kernel(I8Args a, int tiles, i
         store_x(b ^ 1, X[b ^ 1]);                       /* step s + 1, whose buffer no wave reads any more */
         load_x(s + 2, X[b]);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int u = 0; u < U; u++)
+            if (U <= 2 || s * U + u < all) {            /* columns are padded to 128: a step of 256 may be short */
 #pragma unroll
-            for (int t = 0; t < TB; t++) {
-                const int tok = 32 * t + l % 32, c16 = 2 * h + l / 32;
-                const i32x4 B = *(const i32x4 *)(s_x[b] + tok * 64 + ((c16 ^ (tok >> 1 & 3)) << 4));
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int c = 0; c < CB; c++) acc[c][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(W[b][2 * c + h], B, acc[c][t], 0, 0, 0);
+                    for (int t = 0; t < TB; t++) {
+                        const int tok = 32 * t + l % 32, c16 = 2 * h + l / 32;
+                        const i32x4 B = *(const i32x4 *)(s_x[b] + (u * TM + tok) * 64 + ((c16 ^ (tok >> 1 & 3)) << 4));
+#pragma unroll
+                        for (int c = 0; c < CB; c++)
+                            acc[c][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(W[b][(2 * u + h) * CB + c], B, acc[c][t], 0, 0, 0);
+                    }
             }
         load_w(s + 2, W[b]);
         i8_barrier();
@@ -196,27 +235,39 @@ __global__ __launch_bounds__(I8_T, 2) void i8_tile_kernel(I8Args a, int tiles, i
     load_w(1, W[1]);
     store_x(0, X[0]);
     i8_barrier();
-    for (int s = 0; s < steps; s += 2) {                /* an even number */
+    int s = 0;
+    for (; s + 2 <= steps; s += 2) {
         step(s, 0);
         step(s + 1, 1);
     }
+    if (s < steps) step(s, 0);
+    /* through the wave's own LDS, so that a store's lanes hold whole rows of 32 CB channels (the products leave
+     * four channels of 32 tokens); the barrier at the loop's end freed the tokens' buffers */
+    float xs[TB], ws[CB][16];
+#pragma unroll
+    for (int t = 0; t < TB; t++) xs[t] = a.xs[min(t0 + 32 * t + l % 32, a.T - 1)];
+#pragma unroll
     for (int c = 0; c < CB; c++)
-        for (int t = 0; t < TB; t++) {
-            const int tok = t0 + 32 * t + l % 32;
-            if (tok >= a.T) continue;
-            const float xs = a.xs[tok];
-            float *y = a.y + tok * a.y_row;
+#pragma unroll
+        for (int i = 0; i < 16; i++) ws[c][i] = a.ws[min(c0 + 32 * c + 8 * (i / 4) + 4 * (l / 32) + i % 4, a.N - 1)];
+    float *out = (float *)s_lds + w * 32 * LY;
+    for (int t = 0; t < TB; t++) {
+#pragma unroll
+        for (int c = 0; c < CB; c++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int ch = c0 + 32 * c + 8 * j + 4 * (l / 32);
-                f32x4_a4 v;
-                for (int i = 0; i < 4; i++) v[i] = (float)acc[c][t][4 * j + i] * (xs * a.ws[min(ch + i, a.N - 1)]);
-                if (ch + 4 <= a.N) *(f32x4_a4 *)(y + ch) = v;
-                else
-                    for (int i = 0; i < 4; i++)
-                        if (ch + i < a.N) y[ch + i] = v[i];
+                f32x4_a16 v;
+                for (int i = 0; i < 4; i++) v[i] = (float)acc[c][t][4 * j + i] * (xs[t] * ws[c][4 * j + i]);
+                *(f32x4_a16 *)(out + l % 32 * LY + 32 * c + 8 * j + 4 * (l / 32)) = v;
             }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 4 * CB; i++) {
+            const int row = l / (8 * CB) + i * (8 / CB), ch = 4 * (l % (8 * CB)), tok = t0 + 32 * t + row;
+            i8_put<(TB > 1)>(a, tok, c0 + ch, *(const f32x4_a16 *)(out + row * LY + ch));
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 }
 
 /* ---- entry points --------------------------------------------------------------- */
@@ -281,19 +332,27 @@ extern "C" int roaster_matmul_i8(const RoasterMatmulI8 *p, const RoasterI8 *w)
     I8Args a = { (const int8_t *)w->data, p->x, w->scale, p->x_scale, p->y, p->x_row, p->y_row, p->rows, w->rows, w->cols / 16,
                  (int)(i8_cols(w->cols) / 32) };
     if (T <= 32) {
-        const int waves = N <= 8192 ? 16 : 4;
-        hipLaunchKernelGGL(i8_few_kernel, dim3((N + 31) / 32), dim3(64 * waves), 0, rt().stream, a);
+        /* four waves to 16 channels (8 tokens, 12288 x 2048: 6.0 us, with eight 7.4, sixteen 14.6), eight for long
+         * columns (one token, 256 x 16384: 6.1 us, with four 7.2) */
+        const int waves = K <= 8192 ? 4 : 8;
+        if (T <= 16) hipLaunchKernelGGL(i8_few_kernel<1>, dim3((N + 15) / 16), dim3(64 * waves), 0, rt().stream, a);
+        else hipLaunchKernelGGL(i8_few_kernel<2>, dim3((N + 15) / 16), dim3(64 * waves), 0, rt().stream, a);
     } else {
         auto tiles = [&](int tb, int cb) { return ((T + 32 * tb - 1) / (32 * tb)) * ((N + 128 * cb - 1) / (128 * cb)); };
-#define TILE(TB, CB)                                                                                                       \
+#define TILE(TB, CB, U)                                                                                                    \
     do {                                                                                                                   \
         const int n = (int)tiles(TB, CB), per = (n + 7) / 8;                                                               \
-        hipLaunchKernelGGL((i8_tile_kernel<TB, CB>), dim3(8 * per), dim3(I8_T), 0, rt().stream, a, n, per,                 \
+        hipLaunchKernelGGL((i8_tile_kernel<TB, CB, U>), dim3(8 * per), dim3(I8_T), 0, rt().stream, a, n, per,       \
                            (int)((T + 32 * TB - 1) / (32 * TB)));                                                          \
     } while (0)
-        if (tiles(4, 2) >= 384) TILE(4, 2);
-        else if (tiles(4, 1) >= 192) TILE(4, 1);
-        else TILE(2, 1);
+        /* The largest tiles read least from the L2, which bounds the others (8 .. 9 TB/s), but need enough of them:
+         * us with 4 x 2 / 2 x 1 / 1 x 1, and how many there are:
+         *   12288 x 2048: 2048 tokens 61 / 74 / 119 (768), 1200 37 / 46 / 65 (480), 700 31 / 30 / 40 (288 / 1056)
+         *   8192 x 2048:  100 tokens 21 / 9.5 / 8.0 (.. / 256), 200 22 / 9.9 / 11.7 (.. / 448)
+         * 4 x 1 and 2 x 2, and two or four groups of waves that share the columns, never came first by more than a tenth. */
+        if (tiles(4, 2) >= 384) TILE(4, 2, 1);
+        else if (tiles(1, 1) <= 256) TILE(1, 1, 4);
+        else TILE(2, 1, 2);
 #undef TILE
     }
     return rt_check(hipGetLastError(), "matmul_i8 launch") ? ROASTER_EDEVICE : 0;
