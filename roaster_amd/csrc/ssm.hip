@@ -219,28 +219,30 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
 #define SSM_C 64                 /* tokens of a chunk */
 #define SSM_HG 2                 /* value heads of a workgroup of ssm_prep_kernel */
 #define SSM_UP 256.0f            /* Q, K, T and D o Q K^T as operands */
+/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; each value element's
+ * largest |v| (infinite where one is infinite or NaN); the largest gain, and 1 where the chunk has to go token by token. */
+enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_TOP = 384, SSM_MOST = 512, SSM_BAD = 513,
+       SSM_VEC = 576 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
 /* Workspace, in bytes: of a chunk and key head the operands of Q and K (tokens as rows) and K^T, of a chunk and value
- * head those of T and D o Q K^T and the vectors below.  An operand of 16 rows by 32 columns is a kilobyte
- * of high and one of low parts in lane order. */
+ * head those of T and D o Q K^T, V in f32 as the products leave such a matrix (blocks of 16 elements, then of 16 tokens), and
+ * the vectors below.  An operand of 16 rows by 32 columns is a kilobyte of high and one of low parts in lane order. */
 struct SsmWs {
     char *p;
-    int kd, kh, vh;
+    int kd, kh, vh, vd;
 
     __host__ __device__ size_t key_bytes() const { return 3 * (size_t)SSM_C * kd * 4; }
-    __host__ __device__ size_t head_bytes() const { return 2 * SSM_C * SSM_C * 4 + 7 * SSM_C * 4; }
+    __host__ __device__ size_t head_bytes() const { return 2 * SSM_C * SSM_C * 4 + (size_t)SSM_C * vd * 4 + SSM_VEC * 4; }
     __host__ __device__ size_t chunk_bytes() const { return kh * key_bytes() + vh * head_bytes(); }
     __device__ char *key(int c, int h) const { return p + c * chunk_bytes() + h * key_bytes(); }
     __device__ char *head(int c, int h) const { return p + c * chunk_bytes() + kh * key_bytes() + h * head_bytes(); }
-    __device__ float *vec(int c, int h) const { return (float *)(head(c, h) + 2 * SSM_C * SSM_C * 4); }
+    __device__ static float *values(char *head) { return (float *)(head + 2 * SSM_C * SSM_C * 4); }
+    __device__ float *vec(char *head) const { return values(head) + SSM_C * vd; }
 };
-/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; then the largest
- * gain, and 1 where the chunk has to go token by token. */
-enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_MOST = 384, SSM_BAD = 385 };
 
 /* Chunks of request r, 0 for one that is idle or left out. */
 __device__ __forceinline__ int ssm_chunks(const SsmArgs &A, int r)
@@ -333,63 +335,92 @@ __device__ __forceinline__ void ssm_mfma(const SsmOp &a, const SsmOp &b, f32x4 &
     d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, d, 0, 0, 0);
 }
 
+/* RG rows of a channel of the convolution, from row j0 of a chunk of `width` rows at x on (x[0]: row i0 of its request). */
+template <int RG>
+struct SsmConv {
+    SsmChannel cv;
+    float x[RG];
+
+    __device__ __forceinline__ void load(const SsmArgs &A, int r, int pos, int c, const float *rows, int i0, int j0, int width)
+    {
+        const size_t stride = A.a.x_row;
+        const float *at = rows + c;
+        cv.start(A, r, pos, c);
+#pragma unroll
+        for (int j = 0; j < 3; j++)                     /* at least RG rows before */
+            if (i0 + j0) cv.h[j] = at[(ptrdiff_t)min(j0 - 3 + j, width - 1) * (ptrdiff_t)stride];
+#pragma unroll
+        for (int i = 0; i < RG; i++) x[i] = at[(size_t)min(j0 + i, width - 1) * stride];
+    }
+};
+
 /* A chunk's tokens of one key head: convolution, norms, the products among tokens, and of SSM_HG of its value
- * heads the decays and T.  Waves 0 and 1 make a head's T each, by forward substitution with a column a lane,
- * waves 2 and 3 its D o Q K^T. */
+ * heads the values, the decays and T, whose 16 x 16 blocks on the diagonal one wave inverts by substitution, a column a lane,
+ * and joins by products in f32 (T_rc = - T_rr sum_k A_rk T_kc).  What bounds it: at 2048 tokens and 16 key heads
+ * two workgroups fill a CU and all run at once, so their chain of waits. */
 template <int KD, bool DELTA>
-__global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int groups)
+__global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs W, int groups)
 {
     constexpr int LD = KD + 4, LG = SSM_C + 4, KS = KD / 32, OPS = 4 * KS;           /* operands of Q, and of K */
-    constexpr int F0 = 2 * SSM_C * LD, F1 = (2 + SSM_HG) * SSM_C * LG;
+    constexpr int F0 = 2 * SSM_C * LD, F1 = (2 + SSM_HG) * SSM_C * LG, RQ = SSM_C * 2 * KD / (2 * SSM_T);
     __shared__ __attribute__((aligned(16))) float s_buf[F0 > F1 ? F0 : F1];
-    __shared__ double s_G[4][SSM_C];
-    __shared__ float s_rq[SSM_C], s_rk[SSM_C], s_qf[SSM_C], s_kf[SSM_C];
+    __shared__ double s_G[SSM_HG][SSM_C];
+    __shared__ float s_gain[SSM_HG][SSM_C], s_gl[SSM_HG][SSM_C], s_rq[SSM_C], s_rk[SSM_C], s_qf[SSM_C], s_kf[SSM_C];
     __shared__ int s_bad;
+    __shared__ unsigned s_top[SSM_HG * 128];
     const RoasterSsmScan &a = A.a;
-    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), taps = A.s.taps;
+    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), taps = A.s.taps, VD = A.s.v_dim;
     const int kh = blockIdx.y / groups, hg = blockIdx.y % groups, nk = A.s.k_heads * KD;
     int of;
     const int r = __builtin_amdgcn_readfirstlane(ssm_find(A, blockIdx.x, of));
     of = __builtin_amdgcn_readfirstlane(of);
     if (r < 0) return;
     const int f0 = a.first[r], n = a.first[r + 1] - f0, pos = a.row_pos[f0], i0 = of * SSM_C, width = min(SSM_C, n - i0);
+    const int heads = min(SSM_HG, A.rep - hg * SSM_HG), h0 = kh * A.rep + hg * SSM_HG;
+    const float *x = a.x + (size_t)(f0 + i0) * a.x_row;
     float *s_q = s_buf, *s_k = s_buf + SSM_C * LD;
     if (tid == 0) s_bad = 0;
+    if (tid < SSM_HG * 128) s_top[tid] = 0;
 
-    {   /* convolution: a channel a thread, all its rows (KD 64: half of them) in order */
-        constexpr int RG = SSM_C * 2 * KD / SSM_T;
-        const int ch = tid % (2 * KD), j0 = tid / (2 * KD) * RG, c = ch < KD ? kh * KD + ch : nk + kh * KD + ch - KD;
-        const float *x = a.x + (size_t)(f0 + i0) * a.x_row + c;
-        SsmChannel cv;
-        cv.start(A, r, pos, c);
-        if (i0 + j0) {                                  /* rows before: at least 32 */
-#pragma unroll
-            for (int j = 0; j < 3; j++) cv.h[j] = j0 - 3 + j < width ? x[((ptrdiff_t)j0 - 3 + j) * (ptrdiff_t)a.x_row] : 0.0f;
+    /* a channel a thread and RQ rows of it; then as many of a value channel */
+    const int ch = tid % (2 * KD), j0 = tid / (2 * KD) * RQ;
+    SsmConv<RQ> cq;
+    cq.load(A, r, pos, ch < KD ? kh * KD + ch : nk + kh * KD + ch - KD, x, i0, j0, width);
+    if (w < heads) {                                    /* a token a lane */
+        const bool in = l < width;
+        const size_t row = (size_t)(f0 + i0 + min(l, width - 1));
+        const int h = h0 + w;
+        const float dt = ssm_softplus(a.a[row * a.a_row + h] + (a.dt_bias ? a.dt_bias[h] : 0.0f));
+        const float gl = in ? a.a_coef[h] * dt : 0.0f;
+        double G = gl;
+        for (int o = 1; o < 64; o <<= 1) {
+            const double v = __shfl_up(G, o);
+            if (l >= o) G += v;
         }
+        s_G[w][l] = G;
+        s_gl[w][l] = gl;
+        s_gain[w][l] = !in ? 0.0f : DELTA ? ssm_sigmoid(a.b[row * a.b_row + h]) : dt;
+    }
+    {
         float *to = (ch < KD ? s_q + ch : s_k + ch - KD) + j0 * LD;
-        for (int j = 0; j < RG; j += 16) {
-            float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = x[(size_t)min(j0 + j + i, width - 1) * a.x_row];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float y = cv.next(v[i], taps);
-                to[(j + i) * LD] = j0 + j + i < width ? y : 0.0f;
-            }
+        for (int i = 0; i < RQ; i++) {
+            const float y = cq.cv.next(cq.x[i], taps);
+            to[i * LD] = j0 + i < width ? y : 0.0f;
         }
     }
     __syncthreads();
-    {   /* norms: four threads a row */
-        const int row = tid / 4;
+    {   /* norms: eight threads a row */
+        const int row = tid / 8;
         float sq = 0, sk = 0;
 #pragma unroll
-        for (int j = 0; j < KD / 16; j++) {
-            const float4 q = *(const float4 *)(s_q + row * LD + 4 * (tid % 4 + 4 * j)), k = *(const float4 *)(s_k + row * LD + 4 * (tid % 4 + 4 * j));
+        for (int j = 0; j < KD / 32; j++) {
+            const float4 q = *(const float4 *)(s_q + row * LD + 4 * (tid % 8 + 8 * j)), k = *(const float4 *)(s_k + row * LD + 4 * (tid % 8 + 8 * j));
             sq += q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
             sk += k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w;
         }
-        for (int o = 1; o < 4; o <<= 1) { sq += __shfl_xor(sq, o); sk += __shfl_xor(sk, o); }
-        if (tid % 4 == 0) {
+        for (int o = 1; o < 8; o <<= 1) { sq += __shfl_xor(sq, o); sk += __shfl_xor(sk, o); }
+        if (tid % 8 == 0) {
             const float pq = DELTA ? 1.0f : ssm_pow2(sqrtf(sq)), pk = DELTA ? 1.0f : ssm_pow2(sqrtf(sk));
             const float rq = DELTA ? 1.0f / sqrtf(sq + a.eps) : ssm_inv2(pq), rk = DELTA ? 1.0f / sqrtf(sk + a.eps) : ssm_inv2(pk);
             if (row < width && !(ssm_finite(sq) && ssm_finite(sk) && ssm_finite(rq) && ssm_finite(rk) && ssm_finite(a.scale * pq))) s_bad = 1;
@@ -400,18 +431,18 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
         }
     }
     __syncthreads();
-    SsmOp ops[OPS / 2];                                 /* of 2 OPS, wave w's: Q's first, then K's */
+    SsmOp ops[OPS / 4];                                 /* of 2 OPS, wave w's: Q's first, then K's */
     char *key = W.key(blockIdx.x, kh), *sop = (char *)s_buf;
 #pragma unroll
-    for (int f = 0; f < OPS / 2; f++) {
-        const int g = w * (OPS / 2) + f, row = g % OPS / KS * 16 + l % 16, col = g % KS * 32 + l / 16 * 8;
+    for (int f = 0; f < OPS / 4; f++) {
+        const int g = w * (OPS / 4) + f, row = g % OPS / KS * 16 + l % 16, col = g % KS * 32 + l / 16 * 8;
         const float *at = (g < OPS ? s_q : s_k) + row * LD + col, by = SSM_UP * (g < OPS ? s_rq : s_rk)[row];
         const float4 u = *(const float4 *)at, v = *(const float4 *)(at + 4);
         ops[f] = ssm_split({ u.x * by, u.y * by, u.z * by, u.w * by, v.x * by, v.y * by, v.z * by, v.w * by });
         if (hg == 0) ssm_st(key + g * 2048, l, ops[f]);
     }
     if (hg == 0)
-        for (int g = w; g < OPS; g += 4) {              /* K^T: 16 key elements by 32 tokens */
+        for (int g = w; g < OPS; g += 8) {              /* K^T: 16 key elements by 32 tokens */
             const int col = g / 2 * 16 + l % 16, row = g % 2 * 32 + l / 16 * 8;
             float v[8];
 #pragma unroll
@@ -420,118 +451,160 @@ __global__ __launch_bounds__(SSM_T) void ssm_prep_kernel(SsmArgs A, SsmWs W, int
         }
     __syncthreads();
 #pragma unroll
-    for (int f = 0; f < OPS / 2; f++) ssm_st(sop + (w * (OPS / 2) + f) * 2048, l, ops[f]);
+    for (int f = 0; f < OPS / 4; f++) ssm_st(sop + (w * (OPS / 4) + f) * 2048, l, ops[f]);
     __syncthreads();
-    /* products of tokens, lower blocks alone: wave w has rows 16 w of K K^T and rows 16 (3 - w) of Q K^T */
-    f32x4 kk[4] = {}, qk[4] = {}, kx[4] = {}, qx[4] = {};
-    const int wq = 3 - w;
+    /* products of tokens, lower blocks alone: waves 0 .. 3 have rows 16 w of Q K^T, waves 4 .. 7 of K K^T */
+    f32x4 kk[4] = {}, kx[4] = {};
+    const int m4 = w % 4;
+    const bool keys = w >= 4;
     auto op = [&](int g) { return SsmOp{ *(const h16x8 *)(sop + g * 2048 + 16 * l), *(const h16x8 *)(sop + g * 2048 + 1024 + 16 * l) }; };
-    for (int s = 0; s < KS; s++) {
-        const SsmOp ak = op(OPS + w * KS + s), aq = op(wq * KS + s);
+    if (DELTA || !keys)
+        for (int s = 0; s < KS; s++) {
+            const SsmOp u = op((keys ? OPS : 0) + m4 * KS + s);
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            if (b > w && b > wq) continue;
-            const SsmOp bk = op(OPS + b * KS + s);
-            if (DELTA && b <= w) ssm_mfma(ak, bk, kk[b], kx[b]);
-            if (b <= wq) ssm_mfma(aq, bk, qk[b], qx[b]);
+            for (int b = 0; b < 4; b++)
+                if (b <= m4) ssm_mfma(u, op(OPS + b * KS + s), kk[b], kx[b]);
         }
-    }
     __syncthreads();
-    float *s_kk = s_buf, *s_qk = s_buf + SSM_C * LG;
+    float *s_qk = s_buf, *s_kk = s_buf + SSM_C * LG;
 #pragma unroll
     for (int b = 0; b < 4; b++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (DELTA && b <= w) s_kk[(16 * w + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = (kk[b][i] + kx[b][i]) * (1 / (SSM_UP * SSM_UP));
-            if (b <= wq) s_qk[(16 * wq + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = (qk[b][i] + qx[b][i]) * (1 / SSM_UP);
-        }
+        for (int i = 0; i < 4; i++)
+            if ((DELTA || !keys) && b <= m4)
+                (keys ? s_kk : s_qk)[(16 * m4 + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = (kk[b][i] + kx[b][i]) * (keys ? 1 / (SSM_UP * SSM_UP) : 1 / SSM_UP);
     __syncthreads();
-    const int hh = hg * SSM_HG + w % SSM_HG, h = kh * A.rep + hh;
-    if (hh >= A.rep) return;
-    /* a token a lane */
-    const bool in = l < width;
-    const size_t row = (size_t)(f0 + i0 + l);
-    const float dt = in ? ssm_softplus(a.a[row * a.a_row + h] + (a.dt_bias ? a.dt_bias[h] : 0.0f)) : 0.0f;
-    const float gl = in ? a.a_coef[h] * dt : 0.0f;
-    const float gain = !in ? 0.0f : DELTA ? ssm_sigmoid(a.b[row * a.b_row + h]) : dt * s_kf[l];
-    double G = gl;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(G, o);
-        if (l >= o) G += v;
-    }
-    s_G[w][l] = G;
-    const double last = __shfl(G, 63);
-    char *out = W.head(blockIdx.x, h);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (w >= SSM_HG) {                                  /* D o Q K^T */
-        for (int m = 0; m < 4; m++)
-            for (int s = 0; s <= m / 2; s++) {
-                const int i = 16 * m + l % 16, j = 32 * s + 8 * (l / 16);
-                float v[8];
+    /* decays, four waves a head: row block w / 2 of D o Q K^T as an operand, and of A */
+    const int hh = w % SSM_HG, m = w / SSM_HG, h = h0 + hh;
+    float *s_A = s_buf + (2 + hh) * SSM_C * LG, *s_T = s_buf + hh * SSM_C * LG;    /* A; later T, with its columns as rows */
+    if (hh < heads) {
+        char *out = W.head(blockIdx.x, h);
+        const int i = 16 * m + l % 16;
+        const double Gi = s_G[hh][i];
+        const float beta = s_gain[hh][i];
+        for (int s = 0; s <= m / 2; s++) {
+            const int j = 32 * s + 8 * (l / 16);
+            float v[8], d[8];
 #pragma unroll
-                for (int c = 0; c < 8; c++) v[c] = j + c <= i ? s_qk[i * LG + j + c] * ssm_exp((float)(s_G[w][i] - s_G[w][j + c])) : 0.0f;
-                ssm_st(out + (8 + m * 2 + s) * 2048, l, ssm_split(v));
+            for (int c = 0; c < 8; c++) {
+                d[c] = j + c <= i ? ssm_exp((float)(Gi - s_G[hh][j + c])) : 0.0f;
+                v[c] = j + c <= i ? s_qk[i * LG + j + c] * d[c] : 0.0f;
             }
-        float *vec = W.vec(blockIdx.x, h), top = gain;
-        const float eg = ssm_exp((float)G), qf = s_qf[l];
-        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-        vec[SSM_EQ + l] = eg * qf;
-        vec[SSM_QF + l] = qf;
-        vec[SSM_EG + l] = eg;
-        vec[SSM_EC + l] = ssm_exp((float)(last - G));
-        vec[SSM_GAIN + l] = gain;
-        vec[SSM_GL + l] = gl;
-        const bool bad = __any(!ssm_finite(gl) || gl > 0.0f || !ssm_finite(gain)) || s_bad;
-        if (l == 0) {
-            vec[SSM_MOST] = top;
-            vec[SSM_BAD] = bad ? 1.0f : 0.0f;
+            ssm_st(out + (8 + m * 2 + s) * 2048, l, ssm_split(v));
+            if (DELTA) {
+#pragma unroll
+                for (int c = 0; c < 8; c++) v[c] = j + c < i ? beta * s_kk[i * LG + j + c] * d[c] : 0.0f;
+                *(f32x4 *)(s_A + i * LG + j) = (f32x4){ v[0], v[1], v[2], v[3] };
+                *(f32x4 *)(s_A + i * LG + j + 4) = (f32x4){ v[4], v[5], v[6], v[7] };
+            }
         }
-    } else if (DELTA) {
-        float *s_A = s_buf + (2 + w) * SSM_C * LG;
-        for (int m = 0; m < 4; m++)
-            for (int g = 0; g <= m; g++) {
-                const int i = 16 * m + l % 16, j = 16 * g + 4 * (l / 16);
-                const float4 p = *(const float4 *)(s_kk + i * LG + j);
-                const float v[4] = { p.x, p.y, p.z, p.w };
-                const float beta = __shfl(gain, i);
-                f32x4 d;
-#pragma unroll
-                for (int c = 0; c < 4; c++) d[c] = j + c < i ? beta * v[c] * ssm_exp((float)(s_G[w][i] - s_G[w][j + c])) : 0.0f;
-                *(f32x4 *)(s_A + i * LG + j) = d;
+        if (m == 0) {
+            float *vec = W.vec(out);
+            const double G = s_G[hh][l];
+            const float gl = s_gl[hh][l], eg = ssm_exp((float)G), qf = s_qf[l], gain = s_gain[hh][l] * (DELTA ? 1.0f : s_kf[l]);
+            float top = gain;
+            for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+            vec[SSM_EQ + l] = eg * qf;
+            vec[SSM_QF + l] = qf;
+            vec[SSM_EG + l] = eg;
+            vec[SSM_EC + l] = ssm_exp((float)(s_G[hh][SSM_C - 1] - G));
+            vec[SSM_GAIN + l] = gain;
+            vec[SSM_GL + l] = gl;
+            const bool bad = __any(!ssm_finite(gl) || gl > 0.0f || !ssm_finite(gain)) || s_bad;
+            if (l == 0) {
+                vec[SSM_MOST] = top;
+                vec[SSM_BAD] = bad ? 1.0f : 0.0f;
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        float x[SSM_C];
+        }
+    }
+    /* values: SSM_C * VD * heads of them, 32 rows (16 with 64 elements) a thread */
+    {
+        const int c = tid % (SSM_HG * VD), rows = SSM_C * SSM_HG * VD / (2 * SSM_T), g0 = tid / (SSM_HG * VD) * rows, vh = c / VD, e = c % VD;
+        if (vh < heads) {
+            float *to = W.values(W.head(blockIdx.x, h0 + vh)) + e / 16 * (SSM_C * 16) + e % 16 * 4;
+            unsigned top = 0;
+            for (int g = g0; g < g0 + rows; g += 16) {
+                SsmConv<16> cv;
+                cv.load(A, r, pos, 2 * nk + (h0 + vh) * VD + e, x, i0, g, width);
+                f32x4 V;
 #pragma unroll
-        for (int i = 0; i < SSM_C; i++) {
-            float s0 = i == l ? 1.0f : 0.0f, s1 = 0.0f;
+                for (int i = 0; i < 16; i++) {
+                    const float y = cv.cv.next(cv.x[i], taps);
+                    V[i % 4] = g + i < width ? y : 0.0f;
+                    top = max(top, __float_as_uint(V[i % 4]) & 0x7FFFFFFFu);
+                    if (i % 4 == 3) *(f32x4 *)(to + (g / 16 * 64 + i / 4 * 16) * 4) = V;
+                }
+            }
+            atomicMax(&s_top[vh * 128 + e], top);
+        }
+    }
+    __syncthreads();
+    if (tid < heads * VD) {
+        const unsigned top = s_top[tid / VD * 128 + tid % VD];
+        W.vec(W.head(blockIdx.x, h0 + tid / VD))[SSM_TOP + tid % VD] = __uint_as_float(min(top, 0x7F800000u));
+    }
+    if (!DELTA || w >= heads) return;                   /* waves 0 and 1: a head's T each */
+    {
+        const int b = l / 16, c = l % 16;
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float s0 = i == c ? 1.0f : 0.0f, s1 = 0.0f;
 #pragma unroll
             for (int j = 0; j < i; j += 4) {
-                const f32x4 v = *(const f32x4 *)(s_A + i * LG + j);
+                const f32x4 v = *(const f32x4 *)(s_A + (16 * b + i) * LG + 16 * b + j);
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (j + c < i) {
-                        if (c & 1) s1 = fmaf(-v[c], x[j + c], s1);
-                        else s0 = fmaf(-v[c], x[j + c], s0);
+                for (int k = 0; k < 4; k++)
+                    if (j + k < i) {
+                        if (k & 1) s1 = fmaf(-v[k], y[j + k], s1);
+                        else s0 = fmaf(-v[k], y[j + k], s0);
                     }
             }
-            x[i] = s0 + s1;
+            y[i] = s0 + s1;
         }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *(f32x4 *)(s_T + l * LG + 16 * b + i) = (f32x4){ y[i], y[i + 1], y[i + 2], y[i + 3] };
+        /* rows of the inverted blocks over A's own, which are not needed any more */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int i = 0; i < SSM_C; i++) s_A[i * LG + l] = x[i] * (gain * SSM_UP);
+        for (int i = 0; i < 16; i++) s_A[(16 * b + i) * LG + 16 * b + c] = y[i];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int m = 0; m < 4; m++)
-            for (int s = 0; s <= m / 2; s++) {
-                const float *at = s_A + (16 * m + l % 16) * LG + 32 * s + 8 * (l / 16);
-                const float4 u = *(const float4 *)at, v = *(const float4 *)(at + 4);
-                ssm_st(out + (m * 2 + s) * 2048, l, ssm_split({ u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w }));
-            }
     }
+    /* v_mfma_f32_16x16x4_f32, its lanes' four columns of 16 being 4*(l/16) .. + 3: results are operands of the next product as they come */
+    auto mul = [&](const f32x4 &u, const f32x4 &v, f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(u[i], v[i], c, 0, 0, 0);
+        return c;
+    };
+#pragma unroll
+    for (int d = 1; d < 4; d++) {
+#pragma unroll
+        for (int b = 0; b + d < 4; b++) {
+            f32x4 s = {};
+            const int row = 16 * (b + d) + l % 16, at = 4 * (l / 16);
+#pragma unroll
+            for (int k = b; k < b + d; k++)
+                s = mul(*(const f32x4 *)(s_A + row * LG + 16 * k + at), *(const f32x4 *)(s_T + (16 * b + l % 16) * LG + 16 * k + at), s);
+            s = mul(*(const f32x4 *)(s_A + row * LG + 16 * (b + d) + at), -s, (f32x4){ 0, 0, 0, 0 });
+            *(f32x4 *)(s_T + (16 * b + l % 16) * LG + 16 * (b + d) + at) = s;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    char *out = W.head(blockIdx.x, h0 + w);
+    for (int t = 0; t < 4; t++)
+        for (int s = 0; s <= t / 2; s++) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+                const int i = 16 * t + l % 16, j = 32 * s + 8 * (l / 16) + c;
+                v[c] = j <= i ? s_T[j * LG + i] * (s_gain[w][j] * SSM_UP) : 0.0f;
+            }
+            ssm_st(out + (t * 2 + s) * 2048, l, ssm_split(v));
+        }
 }
 
 /* A request's chunks in order, for 16 value elements of one head (v = l%16), with two groups of four waves: the first goes
- * from S to W, the second makes the outputs and the next chunk's values; token rows 16 (w % 4) .. each, and each
- * wave has 16 key elements of S.  S stays in registers as the products leave it (key elements 16 w + 4 (l/16) + i) and
+ * from S to W, the second makes the outputs; token rows 16 (w % 4) .. each, and each wave has 16 key elements of S.  S stays in registers as the products leave it (key elements 16 w + 4 (l/16) + i) and
  * in LDS as they take it.  Operands of the next chunk are loaded while this one is worked on, without conditions, so that
  * waits count those under way exactly. */
 template <int KD, bool DELTA>
@@ -539,8 +612,8 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
 {
     constexpr int KS = KD / 32, OPS = 4 * KS, LS = KD + 8, LT = SSM_C + 8, LV = SSM_C + 4;
     __shared__ __attribute__((aligned(16))) _Float16 s_S[2][16 * LS], s_R[2][16 * LT], s_W[2][16 * LT], s_We[2][16 * LT];
-    __shared__ __attribute__((aligned(16))) float s_V[2][16 * LV];
-    __shared__ float s_top[2][16][4], s_part[2][8][16];
+    __shared__ __attribute__((aligned(16))) float s_V[16 * LV];
+    __shared__ float s_part[2][8][16];
     const RoasterSsmScan &a = A.a;
     const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;    /* so that operands' addresses are scalar */
     const int taps = A.s.taps, VD = A.s.v_dim, VH = A.s.v_heads;
@@ -561,29 +634,21 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         for (int t = tid; t < q.n * 16; t += 2 * SSM_T) a.out[(size_t)(q.f0 + t / 16) * a.out_row + v0 + t % 16] = __uint_as_float(0x7FC00000u);
         return;
     }
-    const int v = l % 16, t4 = 16 * w + 4 * (l / 16), cv = 2 * nk + v0 + v;
+    const int v = l % 16, t4 = 16 * w + 4 * (l / 16);
     float *state = A.s.state + ((size_t)r * VH * VD + v0 + v) * KD + 16 * w8 + 4 * (l / 16);
     f32x4 S = {};
     if (holds && q.pos) S = *(const f32x4 *)state;
-    SsmChannel conv;                                    /* its history is that of the request's first row */
-    conv.start(A, r, q.pos, cv);
     const float skip = a.skip ? a.skip[h] : 0.0f;
-    const float *x = a.x + (size_t)q.f0 * a.x_row + cv;
 
     struct Ops {
         SsmOp one[KS], two[2], kt[2];                   /* DELTA's first group: K and T; else Q and D o Q K^T; K^T */
         f32x4 f, g;                                     /* exp(G) and exp(G_63 - G) (STATE: and gain), or the outputs' factors */
-        f32x4 gain;
-        float last, most, bad;
-    };
-    auto load_x = [&](int c, float (&xs)[7]) {
-#pragma unroll
-        for (int j = 0; j < 7; j++)                      /* rows before the first and behind the last are not used */
-            xs[j] = x[(size_t)min(max(c * SSM_C + t4 - 3 + j, 0), q.n - 1) * a.x_row];
+        f32x4 V, gain;
+        float last, most, bad, top;
     };
     auto load = [&](int c, Ops &o) {
-        const char *key = W.key(base + c, kh), *head = W.head(base + c, h);
-        const float *vec = W.vec(base + c, h);
+        char *key = W.key(base + c, kh), *head = W.head(base + c, h);
+        const float *vec = W.vec(head);
 #pragma unroll
         for (int s = 0; s < KS; s++) o.one[s] = ssm_ld(key + ((DELTA && first ? OPS : 0) + w * KS + s) * 2048, l);
         o.f = *(const f32x4 *)(vec + (first ? SSM_EG : SSM_EQ) + t4);
@@ -592,35 +657,13 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         o.last = vec[SSM_EG + SSM_C - 1];
         o.most = vec[SSM_MOST];
         o.bad = vec[SSM_BAD];
+        o.top = vec[SSM_TOP + vb * 16 + v];
+        o.V = *(const f32x4 *)(W.values(head) + vb * (SSM_C * 16) + (w * 64 + l) * 4);
 #pragma unroll
         for (int s = 0; s < 2; s++) {                    /* tokens 32 .. have no part in rows below */
             o.two[s] = ssm_ld(head + ((DELTA && first ? 0 : 8) + w * 2 + min(s, w / 2)) * 2048, l);
             o.kt[s] = ssm_ld(key + (2 * OPS + (holds ? w8 : 0) * 2 + s) * 2048, l);
         }
-    };
-    /* values of chunk c to LDS, and the largest of each element */
-    auto values = [&](int c, const float (&xs)[7]) {
-        float xx[7];
-#pragma unroll
-        for (int j = 0; j < 7; j++) xx[j] = xs[j];
-        if (c == 0 && t4 == 0) {
-#pragma unroll
-            for (int j = 0; j < 3; j++) xx[j] = conv.h[j];
-        }
-        f32x4 V;
-        float top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            SsmChannel cc = conv;
-            cc.h[0] = xx[i]; cc.h[1] = xx[i + 1]; cc.h[2] = xx[i + 2];
-            const float y = cc.next(xx[i + 3], taps);
-            V[i] = c * SSM_C + t4 + i < q.n ? y : 0.0f;
-            /* NaN and infinities stay: the largest tells whether all are finite */
-            top = ssm_finite(V[i]) ? fmaxf(top, fabsf(V[i])) : INFINITY;
-        }
-        for (int o = 16; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-        *(f32x4 *)(s_V[c & 1] + v * LV + t4) = V;
-        if (l < 16) s_top[c & 1][v][w] = top;
     };
     auto op = [&](const _Float16 *p, int ld, int s) {
         const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
@@ -631,11 +674,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     };
 
     Ops o0, o1;
-    float xs[7];
-    load_x(0, xs);
     load(0, o0);
-    if (!first) values(0, xs);
-    load_x(min(1, chunks - 1), xs);
     /* the norm of the element's row of S */
     float b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
     b += __shfl_xor(b, 16);
@@ -650,8 +689,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     __syncthreads();
 
     auto chunk = [&](int c, const Ops &o) {
-        const f32x4 tops = *(const f32x4 *)s_top[c & 1][v];
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const float top = o.top;
         /* the wave's lanes have all 16 elements, with the same bounds in every wave */
         const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
         const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
@@ -665,7 +703,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             for (int s = 0; s < KS; s++)
                 if (DELTA || !first) ssm_mfma(o.one[s], op(s_S[0], LS, s), X, Y);
             X = (X + Y) * (pS * (1 / (8192.0f * SSM_UP)));
-            const f32x4 V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
+            const f32x4 V = o.V;
             if (DELTA) {
                 if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
                 __syncthreads();
@@ -681,7 +719,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 } else w4 = o.gain * V;
                 ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
                 ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
-            } else if (c + 1 < chunks) values(c + 1, xs);
+            }
             __syncthreads();
             const float back = pW * (1 / (8192.0f * SSM_UP));
             if (holds) {
@@ -706,9 +744,11 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         } else {
             /* token by token, so that an infinite or NaN input does not reach those before it */
             const char *key = W.key(base + c, kh);
-            const float *vec = W.vec(base + c, h);
+            const float *vec = W.vec(W.head(base + c, h));
+            if (first) *(f32x4 *)(s_V + v * LV + t4) = o.V;
+            __syncthreads();
             for (int t = 0; t < min(SSM_C, q.n - c * SSM_C); t++) {
-                const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[c & 1][v * LV + t];
+                const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[v * LV + t];
                 f32x4 kf = {}, qf = {};
                 if (holds) {
                     const int k = 16 * w8 + 4 * (l / 16);
@@ -744,7 +784,6 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 }
                 __syncthreads();
             }
-            if (!first && c + 1 < chunks) values(c + 1, xs);
             b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
             b += __shfl_xor(b, 16);
             b += __shfl_xor(b, 32);
@@ -760,11 +799,9 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     };
     for (int c = 0; c < chunks; c += 2) {
         load(min(c + 1, chunks - 1), o1);
-        if (c) load_x(min(c + 1, chunks - 1), xs);
         chunk(c, o0);
         if (c + 1 == chunks) break;
         load(min(c + 2, chunks - 1), o0);
-        load_x(min(c + 2, chunks - 1), xs);
         chunk(c + 1, o1);
     }
     if (holds) *(f32x4 *)state = S;
@@ -800,7 +837,7 @@ extern "C" size_t roaster_ssm_ws_bytes(int rows, int most, const RoasterSsmState
 {
     if (!ssm_state_ok(s) || rows < 0 || rows > (1 << 18) || most < 1 || (rows && most > rows)) return 0;
     if (most < SSM_CHUNK_MIN) return 16;
-    const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads };
+    const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads, s->v_dim };
     return (size_t)ssm_max_chunks(rows, s) * w.chunk_bytes();
 }
 
@@ -848,11 +885,11 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
     SsmArgs A = { *p, *s, s->v_heads / s->k_heads, (int)ch };
     A.a.b = b;
     if (p->most >= SSM_CHUNK_MIN) {
-        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads };
+        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads, s->v_dim };
         const int chunks = ssm_max_chunks(p->rows, s), groups = (A.rep + SSM_HG - 1) / SSM_HG, blocks = s->v_dim / 16;
 #define CHUNK(KD, D)                                                                                                          \
     do {                                                                                                                    \
-        hipLaunchKernelGGL((ssm_prep_kernel<KD, D>), dim3(chunks, s->k_heads * groups), dim3(SSM_T), 0, rt().stream, A, W,    \
+        hipLaunchKernelGGL((ssm_prep_kernel<KD, D>), dim3(chunks, s->k_heads * groups), dim3(2 * SSM_T), 0, rt().stream, A, W, \
                            groups);                                                                                          \
         hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, n), dim3(2 * SSM_T), 0, rt().stream, A, W, blocks,    \
                            chunks, err);                                                                                    \
