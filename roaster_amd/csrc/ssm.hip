@@ -43,13 +43,9 @@ __device__ __forceinline__ bool ssm_request(const SsmArgs &A, int r, int col, in
     return false;
 }
 
-/* e^x as 2^(x log2 e), the product's rounding made good: to about 2^-23 of it in 8 instructions. */
-__device__ __forceinline__ float ssm_exp(float x)
-{
-    const float t = x * 1.44269502f, p = __builtin_amdgcn_exp2f(t);              /* log2 e = 1.44269502 + 1.93e-8 */
-    const float d = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -t)) * 0.693147182f;
-    return fabsf(t) < 126.0f ? fmaf(p, d, p) : p;
-}
+/* e^x as 2^(x log2 e): off by 2^-23 and |x| 2^-24 of it, which is |x| e^x 2^-24 at most 2^-25 for the decays (x <= 0), and
+ * in a sigmoid at most 2^-25 too. */
+__device__ __forceinline__ float ssm_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 __device__ __forceinline__ float ssm_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ssm_exp(-x)); }
 __device__ __forceinline__ float ssm_silu(float x) { return x * ssm_sigmoid(x); }
 __device__ __forceinline__ float ssm_softplus(float x) { return fmaxf(x, 0.0f) + log1pf(ssm_exp(-fabsf(x))); }
@@ -299,9 +295,12 @@ __device__ __forceinline__ SsmOp ssm_split(const float (&v)[8])
 {
     SsmOp o;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        o.hi[i] = (_Float16)v[i];
+    for (int i = 0; i < 8; i += 2) {                    /* the high part cut off: two at a time; what is left is exact in f32 */
+        const auto h = __builtin_amdgcn_cvt_pkrtz(v[i], v[i + 1]);
+        o.hi[i] = (_Float16)h[0];
+        o.hi[i + 1] = (_Float16)h[1];
         o.lo[i] = (_Float16)(v[i] - (float)o.hi[i]);
+        o.lo[i + 1] = (_Float16)(v[i + 1] - (float)o.hi[i + 1]);
     }
     return o;
 }
@@ -309,10 +308,13 @@ __device__ __forceinline__ void ssm_split4(f32x4 v, float by, _Float16 *hi, _Flo
 {
     h16x4 h, r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float x = v[i] * by;
-        h[i] = (_Float16)x;
+    for (int i = 0; i < 4; i += 2) {
+        const float x = v[i] * by, y = v[i + 1] * by;
+        const auto p = __builtin_amdgcn_cvt_pkrtz(x, y);
+        h[i] = (_Float16)p[0];
+        h[i + 1] = (_Float16)p[1];
         r[i] = (_Float16)(x - (float)h[i]);
+        r[i + 1] = (_Float16)(y - (float)h[i + 1]);
     }
     *(h16x4 *)hi = h;
     *(h16x4 *)lo = r;
@@ -344,13 +346,12 @@ struct SsmConv {
     __device__ __forceinline__ void load(const SsmArgs &A, int r, int pos, int c, const float *rows, int i0, int j0, int width)
     {
         const size_t stride = A.a.x_row;
-        const float *at = rows + c;
         cv.start(A, r, pos, c);
 #pragma unroll
         for (int j = 0; j < 3; j++)                     /* at least RG rows before */
-            if (i0 + j0) cv.h[j] = at[(ptrdiff_t)min(j0 - 3 + j, width - 1) * (ptrdiff_t)stride];
+            if (i0 + j0) cv.h[j] = (rows + (ptrdiff_t)min(j0 - 3 + j, width - 1) * (ptrdiff_t)stride)[(unsigned)c];
 #pragma unroll
-        for (int i = 0; i < RG; i++) x[i] = at[(size_t)min(j0 + i, width - 1) * stride];
+        for (int i = 0; i < RG; i++) x[i] = (rows + (size_t)min(j0 + i, width - 1) * stride)[(unsigned)c];
     }
 };
 
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     if (tid < SSM_HG * 128) s_top[tid] = 0;
 
     /* a channel a thread and RQ rows of it; then as many of a value channel */
-    const int ch = tid % (2 * KD), j0 = tid / (2 * KD) * RQ;
+    const int ch = tid % (2 * KD), j0 = __builtin_amdgcn_readfirstlane(tid / (2 * KD) * RQ);
     SsmConv<RQ> cq;
     cq.load(A, r, pos, ch < KD ? kh * KD + ch : nk + kh * KD + ch - KD, x, i0, j0, width);
     if (w < heads) {                                    /* a token a lane */
@@ -519,7 +520,8 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     }
     /* values: SSM_C * VD * heads of them, 32 rows (16 with 64 elements) a thread */
     {
-        const int c = tid % (SSM_HG * VD), rows = SSM_C * SSM_HG * VD / (2 * SSM_T), g0 = tid / (SSM_HG * VD) * rows, vh = c / VD, e = c % VD;
+        const int c = tid % (SSM_HG * VD), rows = SSM_C * SSM_HG * VD / (2 * SSM_T), g0 = __builtin_amdgcn_readfirstlane(tid / (SSM_HG * VD) * rows);
+        const int vh = __builtin_amdgcn_readfirstlane(c / VD), e = c % VD;
         if (vh < heads) {
             float *to = W.values(W.head(blockIdx.x, h0 + vh)) + e / 16 * (SSM_C * 16) + e % 16 * 4;
             unsigned top = 0;
@@ -640,17 +642,15 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     if (holds && q.pos) S = *(const f32x4 *)state;
     const float skip = a.skip ? a.skip[h] : 0.0f;
 
-    struct Ops {
-        SsmOp one[KS], two[2], kt[2];                   /* DELTA's first group: K and T; else Q and D o Q K^T; K^T */
-        f32x4 f, g;                                     /* exp(G) and exp(G_63 - G) (STATE: and gain), or the outputs' factors */
+    SsmOp one[KS], two[2], kt[2];                       /* DELTA's first group: K and T; else Q and D o Q K^T; K^T */
+    struct Head {
+        f32x4 f, g;                                     /* exp(G) and exp(G_63 - G), or the outputs' factors */
         f32x4 V, gain;
         float last, most, bad, top;
     };
-    auto load = [&](int c, Ops &o) {
-        char *key = W.key(base + c, kh), *head = W.head(base + c, h);
+    auto load_head = [&](int c, Head &o) {
+        char *head = W.head(base + c, h);
         const float *vec = W.vec(head);
-#pragma unroll
-        for (int s = 0; s < KS; s++) o.one[s] = ssm_ld(key + ((DELTA && first ? OPS : 0) + w * KS + s) * 2048, l);
         o.f = *(const f32x4 *)(vec + (first ? SSM_EG : SSM_EQ) + t4);
         o.g = *(const f32x4 *)(vec + (first ? SSM_EC : SSM_QF) + t4);
         if (!DELTA) o.gain = *(const f32x4 *)(vec + SSM_GAIN + t4);
@@ -659,10 +659,18 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         o.bad = vec[SSM_BAD];
         o.top = vec[SSM_TOP + vb * 16 + v];
         o.V = *(const f32x4 *)(W.values(head) + vb * (SSM_C * 16) + (w * 64 + l) * 4);
+    };
+    auto load_one = [&](int c) {
+        const char *at = W.key(base + c, kh) + ((DELTA && first ? OPS : 0) + w * KS) * 2048;
+#pragma unroll
+        for (int s = 0; s < KS; s++) one[s] = ssm_ld(at + s * 2048, l);
+    };
+    auto load_two = [&](int c) {
+        const char *key = W.key(base + c, kh) + (2 * OPS + (holds ? w8 : 0) * 2) * 2048, *head = W.head(base + c, h) + (DELTA && first ? 0 : 8) * 2048;
 #pragma unroll
         for (int s = 0; s < 2; s++) {                    /* tokens 32 .. have no part in rows below */
-            o.two[s] = ssm_ld(head + ((DELTA && first ? 0 : 8) + w * 2 + min(s, w / 2)) * 2048, l);
-            o.kt[s] = ssm_ld(key + (2 * OPS + (holds ? w8 : 0) * 2 + s) * 2048, l);
+            two[s] = ssm_ld(head + (w * 2 + min(s, w / 2)) * 2048, l);
+            kt[s] = ssm_ld(key + s * 2048, l);
         }
     };
     auto op = [&](const _Float16 *p, int ld, int s) {
@@ -673,8 +681,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         if (holds) ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
     };
 
-    Ops o0, o1;
-    load(0, o0);
+    Head o, next;
+    load_head(0, o);
+    load_one(0);
+    load_two(0);
     /* the norm of the element's row of S */
     float b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
     b += __shfl_xor(b, 16);
@@ -688,7 +698,9 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     put_S(8192.0f * ssm_inv2(pS));
     __syncthreads();
 
-    auto chunk = [&](int c, const Ops &o) {
+    for (int c = 0; c < chunks; c++) {
+        const int c1 = min(c + 1, chunks - 1);
+        load_head(c1, next);
         const float top = o.top;
         /* the wave's lanes have all 16 elements, with the same bounds in every wave */
         const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
@@ -701,7 +713,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             f32x4 X = {}, Y = {};
 #pragma unroll
             for (int s = 0; s < KS; s++)
-                if (DELTA || !first) ssm_mfma(o.one[s], op(s_S[0], LS, s), X, Y);
+                if (DELTA || !first) ssm_mfma(one[s], op(s_S[0], LS, s), X, Y);
             X = (X + Y) * (pS * (1 / (8192.0f * SSM_UP)));
             const f32x4 V = o.V;
             if (DELTA) {
@@ -714,18 +726,19 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     f32x4 d = {};
 #pragma unroll
                     for (int s = 0; s < 2; s++)
-                        if (s <= w / 2) ssm_mfma(o.two[s], op(s_R[0], LT, s), w4, d);
+                        if (s <= w / 2) ssm_mfma(two[s], op(s_R[0], LT, s), w4, d);
                     w4 = (w4 + d) * (pR * (1 / (8192.0f * SSM_UP)));
                 } else w4 = o.gain * V;
                 ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
                 ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
-            }
+                load_one(c1);
+            } else load_one(c1);
             __syncthreads();
             const float back = pW * (1 / (8192.0f * SSM_UP));
             if (holds) {
                 f32x4 s4 = {}, d = {};
 #pragma unroll
-                for (int s = 0; s < 2; s++) ssm_mfma(o.kt[s], op(s_We[0], LT, s), s4, d);
+                for (int s = 0; s < 2; s++) ssm_mfma(kt[s], op(s_We[0], LT, s), s4, d);
                 S = S * last + (s4 + d) * back;
             }
             b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
@@ -735,12 +748,13 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 f32x4 O = {}, d = {};
 #pragma unroll
                 for (int s = 0; s < 2; s++)
-                    if (s <= w / 2) ssm_mfma(o.two[s], op(s_W[0], LT, s), O, d);
+                    if (s <= w / 2) ssm_mfma(two[s], op(s_W[0], LT, s), O, d);
                 O = o.f * X + o.g * ((O + d) * back);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (c * SSM_C + t4 + i < q.n) out[(size_t)(t4 + i) * a.out_row] = a.skip ? fmaf(skip, V[i], O[i]) : O[i];
             }
+            load_two(c1);
         } else {
             /* token by token, so that an infinite or NaN input does not reach those before it */
             const char *key = W.key(base + c, kh);
@@ -794,15 +808,11 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             b = sqrtf(b) * 1.0001f;
             pS = ssm_pow2(b);
             put_S(8192.0f * ssm_inv2(pS));
+            load_one(c1);
+            load_two(c1);
         }
+        o = next;
         __syncthreads();
-    };
-    for (int c = 0; c < chunks; c += 2) {
-        load(min(c + 1, chunks - 1), o1);
-        chunk(c, o0);
-        if (c + 1 == chunks) break;
-        load(min(c + 2, chunks - 1), o0);
-        chunk(c + 1, o1);
     }
     if (holds) *(f32x4 *)state = S;
     /* the inputs of the last positions: these value channels, and by one workgroup of a key head its own */
