@@ -329,13 +329,17 @@ __device__ __forceinline__ void ssm_st(char *at, int l, const SsmOp &o)
     *(h16x8 *)(at + 16 * l) = o.hi;
     *(h16x8 *)(at + 1024 + 16 * l) = o.lo;
 }
-/* c += hi hi, d += hi lo + lo hi: two chains */
-__device__ __forceinline__ void ssm_mfma(const SsmOp &a, const SsmOp &b, f32x4 &c, f32x4 &d)
-{
-    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, d, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
-    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, d, 0, 0, 0);
-}
+/* The three products of the parts, a chain each. */
+struct SsmSum {
+    f32x4 hh = {}, hl = {}, lh = {};
+    __device__ __forceinline__ void add(const SsmOp &a, const SsmOp &b)
+    {
+        lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, lh, 0, 0, 0);
+        hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, hh, 0, 0, 0);
+        hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, hl, 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x4 get() const { return hh + (hl + lh); }
+};
 
 /* RG rows of a channel of the convolution, from row j0 of a chunk of `width` rows at x on (x[0]: row i0 of its request). */
 template <int RG>
@@ -455,7 +459,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     for (int f = 0; f < OPS / 4; f++) ssm_st(sop + (w * (OPS / 4) + f) * 2048, l, ops[f]);
     __syncthreads();
     /* products of tokens, lower blocks alone: waves 0 .. 3 have rows 16 w of Q K^T, waves 4 .. 7 of K K^T */
-    f32x4 kk[4] = {}, kx[4] = {};
+    SsmSum kk[4];
     const int m4 = w % 4;
     const bool keys = w >= 4;
     auto op = [&](int g) { return SsmOp{ *(const h16x8 *)(sop + g * 2048 + 16 * l), *(const h16x8 *)(sop + g * 2048 + 1024 + 16 * l) }; };
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
             const SsmOp u = op((keys ? OPS : 0) + m4 * KS + s);
 #pragma unroll
             for (int b = 0; b < 4; b++)
-                if (b <= m4) ssm_mfma(u, op(OPS + b * KS + s), kk[b], kx[b]);
+                if (b <= m4) kk[b].add(u, op(OPS + b * KS + s));
         }
     __syncthreads();
     float *s_qk = s_buf, *s_kk = s_buf + SSM_C * LG;
@@ -473,7 +477,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if ((DELTA || !keys) && b <= m4)
-                (keys ? s_kk : s_qk)[(16 * m4 + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = (kk[b][i] + kx[b][i]) * (keys ? 1 / (SSM_UP * SSM_UP) : 1 / SSM_UP);
+                (keys ? s_kk : s_qk)[(16 * m4 + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = kk[b].get()[i] * (keys ? 1 / (SSM_UP * SSM_UP) : 1 / SSM_UP);
     __syncthreads();
     /* decays, four waves a head: row block w / 2 of D o Q K^T as an operand, and of A */
     const int hh = w % SSM_HG, m = w / SSM_HG, h = h0 + hh;
@@ -654,9 +658,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         o.f = *(const f32x4 *)(vec + (first ? SSM_EG : SSM_EQ) + t4);
         o.g = *(const f32x4 *)(vec + (first ? SSM_EC : SSM_QF) + t4);
         if (!DELTA) o.gain = *(const f32x4 *)(vec + SSM_GAIN + t4);
-        o.last = vec[SSM_EG + SSM_C - 1];
-        o.most = vec[SSM_MOST];
-        o.bad = vec[SSM_BAD];
+        const __attribute__((address_space(4))) float *same = (const __attribute__((address_space(4))) float *)vec;      /* scalar loads */
+        o.last = same[SSM_EG + SSM_C - 1];
+        o.most = same[SSM_MOST];
+        o.bad = same[SSM_BAD];
         o.top = vec[SSM_TOP + vb * 16 + v];
         o.V = *(const f32x4 *)(W.values(head) + vb * (SSM_C * 16) + (w * 64 + l) * 4);
     };
@@ -698,23 +703,26 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     put_S(8192.0f * ssm_inv2(pS));
     __syncthreads();
 
-    for (int c = 0; c < chunks; c++) {
+    float *out = a.out + (size_t)(q.f0 + t4) * a.out_row + v0 + v;               /* this lane's four tokens in turn */
+    if (first) __builtin_amdgcn_s_setprio(1);            /* the other group waits for it */
+    for (int c = 0; c < chunks; c++, out += SSM_C * a.out_row) {
         const int c1 = min(c + 1, chunks - 1);
         load_head(c1, next);
         const float top = o.top;
         /* the wave's lanes have all 16 elements, with the same bounds in every wave */
         const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
         const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
-        float *out = a.out + (size_t)(q.f0 + c * SSM_C) * a.out_row + v0 + v;
         const float last = o.last;
         if (!bad) {
             /* bounds: of R, of W, and of the next S */
             const float bR = top + b, bW = DELTA ? b + 65.0f * top : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
-            f32x4 X = {}, Y = {};
+            f32x4 X = {};
+            if (DELTA || !first) {
+                SsmSum sum;
 #pragma unroll
-            for (int s = 0; s < KS; s++)
-                if (DELTA || !first) ssm_mfma(one[s], op(s_S[0], LS, s), X, Y);
-            X = (X + Y) * (pS * (1 / (8192.0f * SSM_UP)));
+                for (int s = 0; s < KS; s++) sum.add(one[s], op(s_S[0], LS, s));
+                X = sum.get() * (pS * (1 / (8192.0f * SSM_UP)));
+            }
             const f32x4 V = o.V;
             if (DELTA) {
                 if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
@@ -723,11 +731,11 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             if (first) {
                 f32x4 w4 = {};
                 if (DELTA) {
-                    f32x4 d = {};
+                    SsmSum sum;
 #pragma unroll
                     for (int s = 0; s < 2; s++)
-                        if (s <= w / 2) ssm_mfma(two[s], op(s_R[0], LT, s), w4, d);
-                    w4 = (w4 + d) * (pR * (1 / (8192.0f * SSM_UP)));
+                        if (s <= w / 2) sum.add(two[s], op(s_R[0], LT, s));
+                    w4 = sum.get() * (pR * (1 / (8192.0f * SSM_UP)));
                 } else w4 = o.gain * V;
                 ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
                 ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
@@ -736,23 +744,29 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             __syncthreads();
             const float back = pW * (1 / (8192.0f * SSM_UP));
             if (holds) {
-                f32x4 s4 = {}, d = {};
+                SsmSum sum;
 #pragma unroll
-                for (int s = 0; s < 2; s++) ssm_mfma(kt[s], op(s_We[0], LT, s), s4, d);
-                S = S * last + (s4 + d) * back;
+                for (int s = 0; s < 2; s++) sum.add(kt[s], op(s_We[0], LT, s));
+                S = S * last + sum.get() * back;
             }
             b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
             pS = ssm_pow2(b);
             put_S(8192.0f * ssm_inv2(pS));
             if (!first) {
-                f32x4 O = {}, d = {};
+                SsmSum sum;
 #pragma unroll
                 for (int s = 0; s < 2; s++)
-                    if (s <= w / 2) ssm_mfma(two[s], op(s_W[0], LT, s), O, d);
-                O = o.f * X + o.g * ((O + d) * back);
+                    if (s <= w / 2) sum.add(two[s], op(s_W[0], LT, s));
+                f32x4 O = o.f * X + o.g * (sum.get() * back);
+                if (a.skip) O = O + skip * V;
+                if ((c + 1) * SSM_C <= q.n) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (c * SSM_C + t4 + i < q.n) out[(size_t)(t4 + i) * a.out_row] = a.skip ? fmaf(skip, V[i], O[i]) : O[i];
+                    for (int i = 0; i < 4; i++) out[i * a.out_row] = O[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (c * SSM_C + t4 + i < q.n) out[i * a.out_row] = O[i];
+                }
             }
             load_two(c1);
         } else {
@@ -794,7 +808,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     so = 0;
                     for (int i = 0; i < KD / 16; i++) so += s_part[1][i][v];
                     so *= vec[SSM_QF + t];
-                    out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, so) : so;
+                    out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, so) : so;     /* threads 0 .. 15: t4 = 0 */
                 }
                 __syncthreads();
             }
