@@ -8,16 +8,17 @@
 
 #define NORM_T 256
 
-/* A row is L lanes' with V times four elements each, all of it in registers between the
- * sum and the outputs: x, res and gate are read once.  Heads of 16 .. 256 elements lie in 4 .. 64
- * neighbouring lanes of one wave. */
-template <int L, int V>
+/* A row is a workgroup's, V times four elements a thread, all of it in registers between the sum and the
+ * outputs: x, res and gate are read once.  Heads of 16 .. 256 elements lie in 4 .. 64 neighbouring lanes of one wave.
+ * What bounds it: a launch up to some hundred rows (one row of 2048 3.5 us), then memory: 2048 rows of 32 heads of 128
+ * with a gate 18.9 us, 5.3 TB/s of a copy's 4.9.  STREAM: y past the caches (22.7 us without). */
+template <int V, bool STREAM>
 __global__ __launch_bounds__(NORM_T) void norm_kernel(RoasterNorm a)
 {
+    constexpr int L = NORM_T;
     __shared__ float s_sum[NORM_T / 64];
     __shared__ unsigned s_top[NORM_T / 64];
-    const int tid = threadIdx.x % L, row = blockIdx.x * (NORM_T / L) + threadIdx.x / L;
-    if (row >= a.rows) return;                          /* L = 64: a whole wave, and no barrier below */
+    const int tid = threadIdx.x, row = blockIdx.x;
     const float *x = a.x + row * a.x_row;
     float4 v[V], g[V];
 #pragma unroll
@@ -50,12 +51,10 @@ __global__ __launch_bounds__(NORM_T) void norm_kernel(RoasterNorm a)
 #pragma unroll
         for (int i = 0; i < V; i++) ss += v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
         for (int o = 1; o < 64; o <<= 1) ss += __shfl_xor(ss, o);
-        if (L > 64) {
-            if (tid % 64 == 0) s_sum[tid / 64] = ss;
-            __syncthreads();
-            ss = 0;
-            for (int w = 0; w < L / 64; w++) ss += s_sum[w];
-        }
+        if (tid % 64 == 0) s_sum[tid / 64] = ss;
+        __syncthreads();
+        ss = 0;
+        for (int w = 0; w < L / 64; w++) ss += s_sum[w];
         const float r = 1.0f / sqrtf(ss / a.cols + a.eps);
 #pragma unroll
         for (int i = 0; i < V; i++) inv[i] = r;
@@ -82,17 +81,19 @@ __global__ __launch_bounds__(NORM_T) void norm_kernel(RoasterNorm a)
             v[i].z *= g[i].z / (1.0f + expf(-g[i].z));
             v[i].w *= g[i].w / (1.0f + expf(-g[i].w));
         }
-        if (a.y) *(float4 *)(a.y + row * a.y_row + e) = v[i];
+        if (a.y) {
+            float *y = a.y + row * a.y_row + e;
+            if (STREAM) __builtin_nontemporal_store((gf32x4){ v[i].x, v[i].y, v[i].z, v[i].w }, (GAS gf32x4 *)y);
+            else *(float4 *)y = v[i];
+        }
         const float m[4] = { v[i].x, v[i].y, v[i].z, v[i].w };
         for (int j = 0; j < 4; j++) top = max(top, __float_as_uint(m[j]) & 0x7FFFFFFFu);
     }
     if (!a.q) return;
     for (int o = 1; o < 64; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-    if (L > 64) {
-        if (tid % 64 == 0) s_top[tid / 64] = top;
-        __syncthreads();
-        for (int w = 0; w < L / 64; w++) top = max(top, s_top[w]);
-    }
+    if (tid % 64 == 0) s_top[tid / 64] = top;
+    __syncthreads();
+    for (int w = 0; w < L / 64; w++) top = max(top, s_top[w]);
     const I8Scale s = i8_scale(top);
     if (tid == 0) a.q_scale[row] = s.scale;
 #pragma unroll
@@ -140,12 +141,17 @@ extern "C" int roaster_norm(const RoasterNorm *p)
     if (rt_init_locked()) return ROASTER_EDEVICE;
     const AttnDevice dev;
     const int v = (int)(cols / 4 + NORM_T - 1) / NORM_T;
-#define NORM(L, V) hipLaunchKernelGGL((norm_kernel<L, V>), dim3((rows + NORM_T / L - 1) / (NORM_T / L)), dim3(NORM_T), 0, rt().stream, *p)
-    if (v <= 1) NORM(256, 1);
-    else if (v <= 2) NORM(256, 2);
-    else if (v <= 4) NORM(256, 4);
-    else if (v <= 8) NORM(256, 8);
-    else NORM(256, 16);
+    /* An output that the L2s (32 MB) would not hold anyway goes past them; the residual, which the next norm reads, never
+     * does (2048 rows of 2048 into 8 bits 24.5 us with torch's conversion behind it, past the caches 24.8). */
+    const bool stream = p->y && 4 * rows * cols >= ((size_t)24 << 20);
+#define NORM2(V, S) hipLaunchKernelGGL((norm_kernel<V, S>), dim3(rows), dim3(NORM_T), 0, rt().stream, *p)
+#define NORM(V) do { if (stream) NORM2(V, true); else NORM2(V, false); } while (0)
+    if (v <= 1) NORM(1);
+    else if (v <= 2) NORM(2);
+    else if (v <= 4) NORM(4);
+    else if (v <= 8) NORM(8);
+    else NORM(16);
 #undef NORM
+#undef NORM2
     return rt_check(hipGetLastError(), "norm launch") ? ROASTER_EDEVICE : 0;
 }

@@ -80,6 +80,14 @@ struct SsmChannel {
     }
 };
 
+/* States past the caches: a step's other layers lie between two uses. */
+__device__ __forceinline__ float4 ssm_ldnt(const float *p)
+{
+    const gf32x4 v = __builtin_nontemporal_load((const GAS gf32x4 *)p);
+    return make_float4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void ssm_stnt(float *p, float4 v) { __builtin_nontemporal_store((gf32x4){ v.x, v.y, v.z, v.w }, (GAS gf32x4 *)p); }
+
 /* Token by token: a workgroup has one request's block of VB value elements of one head, its state in
  * registers (KD / 16 lanes a row, 16 elements each).  The queries' and keys' channels are convolved by every
  * workgroup of the head: 2 KD inputs next to VB * KD states.
@@ -110,7 +118,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_token_kernel(SsmArgs A, int blocks,
     for (int i = 0; i < NR; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            S[i][j] = q.pos ? gld_f4(state + (size_t)i * RP * KD + 4 * P * j) : make_float4(0, 0, 0, 0);
+            S[i][j] = q.pos ? ssm_ldnt(state + (size_t)i * RP * KD + 4 * P * j) : make_float4(0, 0, 0, 0);
     const float coef = a.a_coef[h], dtb = a.dt_bias ? a.dt_bias[h] : 0.0f, skip = a.skip ? a.skip[h] : 0.0f;
     if (ONE) {
         float *to = A.s.conv + ((size_t)r * taps + (unsigned)q.pos % taps) * A.channels;
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_token_kernel(SsmArgs A, int blocks,
 #pragma unroll
     for (int i = 0; i < NR; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) *(float4 *)(state + (size_t)i * RP * KD + 4 * P * j) = S[i][j];
+        for (int j = 0; j < 4; j++) ssm_stnt(state + (size_t)i * RP * KD + 4 * P * j, S[i][j]);
 }
 
 /* The inputs of each request's last positions into its entries of `conv`. */
@@ -851,8 +859,15 @@ static bool ssm_state_ok(const RoasterSsmState *s)
 
 static inline int ssm_channels(const RoasterSsmState *s) { return 2 * s->k_heads * s->k_dim + s->v_heads * s->v_dim; }
 
-/* From so many new tokens of a request on a call goes by chunks. */
+/* From so many new tokens of a request on a call goes by chunks (us by chunks / by tokens, 32 heads of 128 x 128: one request
+ * of 16 tokens 28.8 / 27.7, of 32 28.7 / 48; 16 requests of 16 tokens 139 / 74, of 32 137 / 131): fewer where a
+ * token's workgroups leave most of the GPU idle. */
+#define SSM_CHUNK_FEW 20
 #define SSM_CHUNK_MIN 32
+static inline bool ssm_by_chunks(int most, const RoasterSsmState *s)
+{
+    return most >= SSM_CHUNK_MIN || (most >= SSM_CHUNK_FEW && s->n_req * s->v_heads <= 256);
+}
 
 /* Chunks of a step at most: the last of each request may be short. */
 static inline int ssm_max_chunks(int rows, const RoasterSsmState *s) { return rows / SSM_C + (rows < s->n_req ? rows : s->n_req); }
@@ -860,7 +875,7 @@ static inline int ssm_max_chunks(int rows, const RoasterSsmState *s) { return ro
 extern "C" size_t roaster_ssm_ws_bytes(int rows, int most, const RoasterSsmState *s)
 {
     if (!ssm_state_ok(s) || rows < 0 || rows > (1 << 18) || most < 1 || (rows && most > rows)) return 0;
-    if (most < SSM_CHUNK_MIN) return 16;
+    if (most < SSM_CHUNK_FEW) return 16;
     const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads, s->v_dim };
     return (size_t)ssm_max_chunks(rows, s) * w.chunk_bytes();
 }
@@ -908,7 +923,7 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
     if (!err) return ROASTER_EDEVICE;
     SsmArgs A = { *p, *s, s->v_heads / s->k_heads, (int)ch };
     A.a.b = b;
-    if (p->most >= SSM_CHUNK_MIN) {
+    if (ssm_by_chunks(p->most, s)) {
         const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads, s->v_dim };
         const int chunks = ssm_max_chunks(p->rows, s), groups = (A.rep + SSM_HG - 1) / SSM_HG, blocks = s->v_dim / 16;
 #define CHUNK(KD, D)                                                                                                          \
@@ -929,8 +944,11 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
                        s->v_dim / VB, err)
 #define TOKEN2(KD, VB, D) do { if (one) TOKEN3(KD, VB, D, true); else TOKEN3(KD, VB, D, false); } while (0)
 #define TOKEN(KD, VB) do { if (delta) TOKEN2(KD, VB, true); else TOKEN2(KD, VB, false); } while (0)
-    if (s->k_dim == 128) TOKEN(128, 32);
-    else TOKEN(64, 64);
+    /* 32 value elements a workgroup while that fills the GPU no more than four times, else 64, for fewer reads of the
+     * queries' and keys' channels (32 / 64: 4 requests 7.1 / 7.1 us, 16 15.3 / 12.0, 64 53.5 / 46.0; one 5.4 / 5.8) */
+    if (s->k_dim == 64) TOKEN(64, 64);
+    else if (n * ov / 32 >= 1024) TOKEN(128, 64);
+    else TOKEN(128, 32);
 #undef TOKEN
 #undef TOKEN2
 #undef TOKEN3
