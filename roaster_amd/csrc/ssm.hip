@@ -232,14 +232,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
-/* Workspace, in bytes: of a chunk and key head the operands of Q and K (tokens as rows) and K^T, of a chunk and value
- * head those of T and D o Q K^T, V in f32 as the products leave such a matrix (blocks of 16 elements, then of 16 tokens), and
+/* Workspace, in bytes: of a chunk and key head the operands of Q and K (tokens as rows), of a chunk and value head those of T and D o Q K^T, V in f32 as the products leave such a matrix (blocks of 16 elements, then of 16 tokens), and
  * the vectors below.  An operand of 16 rows by 32 columns is a kilobyte of high and one of low parts in lane order. */
 struct SsmWs {
     char *p;
     int kd, kh, vh, vd;
 
-    __host__ __device__ size_t key_bytes() const { return 3 * (size_t)SSM_C * kd * 4; }
+    __host__ __device__ size_t key_bytes() const { return 2 * (size_t)SSM_C * kd * 4; }
     __host__ __device__ size_t head_bytes() const { return 2 * SSM_C * SSM_C * 4 + (size_t)SSM_C * vd * 4 + SSM_VEC * 4; }
     __host__ __device__ size_t chunk_bytes() const { return kh * key_bytes() + vh * head_bytes(); }
     __device__ char *key(int c, int h) const { return p + c * chunk_bytes() + h * key_bytes(); }
@@ -336,6 +335,11 @@ __device__ __forceinline__ void ssm_st(char *at, int l, const SsmOp &o)
 {
     *(h16x8 *)(at + 16 * l) = o.hi;
     *(h16x8 *)(at + 1024 + 16 * l) = o.lo;
+}
+__device__ __forceinline__ h16x4 ssm_lds_cols(const char *at)
+{
+    typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)at));
 }
 /* The three products of the parts, a chain each. */
 struct SsmSum {
@@ -454,14 +458,6 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
         ops[f] = ssm_split({ u.x * by, u.y * by, u.z * by, u.w * by, v.x * by, v.y * by, v.z * by, v.w * by });
         if (hg == 0) ssm_st(key + g * 2048, l, ops[f]);
     }
-    if (hg == 0)
-        for (int g = w; g < OPS; g += 8) {              /* K^T: 16 key elements by 32 tokens */
-            const int col = g / 2 * 16 + l % 16, row = g % 2 * 32 + l / 16 * 8;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = s_k[(row + i) * LD + col] * (SSM_UP * s_rk[row + i]);
-            ssm_st(key + (2 * OPS + g) * 2048, l, ssm_split(v));
-        }
     __syncthreads();
 #pragma unroll
     for (int f = 0; f < OPS / 4; f++) ssm_st(sop + (w * (OPS / 4) + f) * 2048, l, ops[f]);
@@ -627,6 +623,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     constexpr int KS = KD / 32, OPS = 4 * KS, LS = KD + 8, LT = SSM_C + 8, LV = SSM_C + 4;
     __shared__ __attribute__((aligned(16))) _Float16 s_S[2][16 * LS], s_R[2][16 * LT], s_W[2][16 * LT], s_We[2][16 * LT];
     __shared__ __attribute__((aligned(16))) float s_V[16 * LV];
+    __shared__ __attribute__((aligned(16))) char s_K[OPS * 2048];                /* K's operands as they are, read as K^T's */
     __shared__ float s_part[2][8][16];
     const RoasterSsmScan &a = A.a;
     const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;    /* so that operands' addresses are scalar */
@@ -654,7 +651,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     if (holds && q.pos) S = *(const f32x4 *)state;
     const float skip = a.skip ? a.skip[h] : 0.0f;
 
-    SsmOp one[KS], two[2], kt[2];                       /* DELTA's first group: K and T; else Q and D o Q K^T; K^T */
+    SsmOp one[KS], two[2];                              /* the first group's K and T, the second's Q and D o Q K^T */
     struct Head {
         f32x4 f, g;                                     /* exp(G) and exp(G_63 - G), or the outputs' factors */
         f32x4 V, gain;
@@ -674,17 +671,28 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         o.V = *(const f32x4 *)(W.values(head) + vb * (SSM_C * 16) + (w * 64 + l) * 4);
     };
     auto load_one = [&](int c) {
-        const char *at = W.key(base + c, kh) + ((DELTA && first ? OPS : 0) + w * KS) * 2048;
+        const char *at = W.key(base + c, kh) + ((first ? OPS : 0) + w * KS) * 2048;
 #pragma unroll
         for (int s = 0; s < KS; s++) one[s] = ssm_ld(at + s * 2048, l);
     };
     auto load_two = [&](int c) {
-        const char *key = W.key(base + c, kh) + (2 * OPS + (holds ? w8 : 0) * 2) * 2048, *head = W.head(base + c, h) + (DELTA && first ? 0 : 8) * 2048;
+        const char *head = W.head(base + c, h) + (DELTA && first ? 0 : 8) * 2048;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {                    /* tokens 32 .. have no part in rows below */
-            two[s] = ssm_ld(head + (w * 2 + min(s, w / 2)) * 2048, l);
-            kt[s] = ssm_ld(key + s * 2048, l);
+        for (int s = 0; s < 2; s++) two[s] = ssm_ld(head + (w * 2 + min(s, w / 2)) * 2048, l);      /* tokens 32 .. have no part in rows below */
+    };
+    /* This wave's 16 key elements of K^T, tokens 32 s ..: the transposing read takes 4 tokens of 16 elements from 16 lanes (lane
+     * 4 i + j: elements 4 j .. of token i) and gives lane c the four of element c. */
+    auto key_cols = [&](int s) {
+        const int j = l % 4, at = (l / 4 % 4 + 8 * (l / 16 % 2) + 16 * (w8 % 2 * 2 + j / 2)) * 16 + j % 2 * 8;
+        const char *base = s_K + ((2 * s + l / 32) * KS + w8 / 2) * 2048 + at;
+        SsmOp o;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const h16x4 hi = ssm_lds_cols(base + 64 * i), lo = ssm_lds_cols(base + 1024 + 64 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) { o.hi[4 * i + e] = hi[e]; o.lo[4 * i + e] = lo[e]; }
         }
+        return o;
     };
     auto op = [&](const _Float16 *p, int ld, int s) {
         const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
@@ -731,6 +739,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 for (int s = 0; s < KS; s++) sum.add(one[s], op(s_S[0], LS, s));
                 X = sum.get() * (pS * (1 / (8192.0f * SSM_UP)));
             }
+            if (first) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) ssm_st(s_K + (w * KS + s) * 2048, l, one[s]);
+            }
             const f32x4 V = o.V;
             if (DELTA) {
                 if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
@@ -754,7 +766,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             if (holds) {
                 SsmSum sum;
 #pragma unroll
-                for (int s = 0; s < 2; s++) sum.add(kt[s], op(s_We[0], LT, s));
+                for (int s = 0; s < 2; s++) sum.add(key_cols(s), op(s_We[0], LT, s));
                 S = S * last + sum.get() * back;
             }
             b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
