@@ -223,28 +223,27 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
 #define SSM_C 64                 /* tokens of a chunk */
 #define SSM_HG 2                 /* value heads of a workgroup of ssm_prep_kernel */
 #define SSM_UP 256.0f            /* Q, K, T and D o Q K^T as operands */
-/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; each value element's
- * largest |v| (infinite where one is infinite or NaN); the largest gain, and 1 where the chunk has to go token by token. */
-enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_TOP = 384, SSM_MOST = 512, SSM_BAD = 513,
-       SSM_VEC = 576 };
+/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; then the largest gain,
+ * and 1 where the chunk has to go token by token. */
+enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_MOST = 384, SSM_BAD = 385, SSM_VEC = 448 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
-/* Workspace, in bytes: of a chunk and key head the operands of Q and K (tokens as rows), of a chunk and value head those of T and D o Q K^T, V in f32 as the products leave such a matrix (blocks of 16 elements, then of 16 tokens), and
- * the vectors below.  An operand of 16 rows by 32 columns is a kilobyte of high and one of low parts in lane order. */
+/* Workspace, in bytes: of a chunk and key head the operands of Q and K (tokens as rows), of a chunk and value head those of
+ * T and D o Q K^T, and the vectors below.  An operand of 16 rows by 32 columns is a kilobyte of high and one of low
+ * parts in lane order.  (K^T comes from K's operands, values from x: with both here too 2048 tokens took 138 us.) */
 struct SsmWs {
     char *p;
-    int kd, kh, vh, vd;
+    int kd, kh, vh;
 
     __host__ __device__ size_t key_bytes() const { return 2 * (size_t)SSM_C * kd * 4; }
-    __host__ __device__ size_t head_bytes() const { return 2 * SSM_C * SSM_C * 4 + (size_t)SSM_C * vd * 4 + SSM_VEC * 4; }
+    __host__ __device__ size_t head_bytes() const { return 2 * SSM_C * SSM_C * 4 + SSM_VEC * 4; }
     __host__ __device__ size_t chunk_bytes() const { return kh * key_bytes() + vh * head_bytes(); }
     __device__ char *key(int c, int h) const { return p + c * chunk_bytes() + h * key_bytes(); }
     __device__ char *head(int c, int h) const { return p + c * chunk_bytes() + kh * key_bytes() + h * head_bytes(); }
-    __device__ static float *values(char *head) { return (float *)(head + 2 * SSM_C * SSM_C * 4); }
-    __device__ float *vec(char *head) const { return values(head) + SSM_C * vd; }
+    __device__ static float *vec(char *head) { return (float *)(head + 2 * SSM_C * SSM_C * 4); }
 };
 
 /* Chunks of request r, 0 for one that is idle or left out. */
@@ -372,7 +371,7 @@ struct SsmConv {
 };
 
 /* A chunk's tokens of one key head: convolution, norms, the products among tokens, and of SSM_HG of its value
- * heads the values, the decays and T, whose 16 x 16 blocks on the diagonal one wave inverts by substitution, a column a lane,
+ * heads the decays and T, whose 16 x 16 blocks on the diagonal one wave inverts by substitution, a column a lane,
  * and joins by products in f32 (T_rc = - T_rr sum_k A_rk T_kc).  What bounds it: at 2048 tokens and 16 key heads
  * two workgroups fill a CU and all run at once, so their chain of waits. */
 template <int KD, bool DELTA>
@@ -384,9 +383,8 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     __shared__ double s_G[SSM_HG][SSM_C];
     __shared__ float s_gain[SSM_HG][SSM_C], s_gl[SSM_HG][SSM_C], s_rq[SSM_C], s_rk[SSM_C], s_qf[SSM_C], s_kf[SSM_C];
     __shared__ int s_bad;
-    __shared__ unsigned s_top[SSM_HG * 128];
     const RoasterSsmScan &a = A.a;
-    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), taps = A.s.taps, VD = A.s.v_dim;
+    const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), taps = A.s.taps;
     const int kh = blockIdx.y / groups, hg = blockIdx.y % groups, nk = A.s.k_heads * KD;
     int of;
     const int r = __builtin_amdgcn_readfirstlane(ssm_find(A, blockIdx.x, of));
@@ -397,9 +395,8 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     const float *x = a.x + (size_t)(f0 + i0) * a.x_row;
     float *s_q = s_buf, *s_k = s_buf + SSM_C * LD;
     if (tid == 0) s_bad = 0;
-    if (tid < SSM_HG * 128) s_top[tid] = 0;
 
-    /* a channel a thread and RQ rows of it; then as many of a value channel */
+    /* a channel a thread and RQ rows of it */
     const int ch = tid % (2 * KD), j0 = __builtin_amdgcn_readfirstlane(tid / (2 * KD) * RQ);
     SsmConv<RQ> cq;
     cq.load(A, r, pos, ch < KD ? kh * KD + ch : nk + kh * KD + ch - KD, x, i0, j0, width);
@@ -526,33 +523,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
             }
         }
     }
-    /* values: SSM_C * VD * heads of them, 32 rows (16 with 64 elements) a thread */
-    {
-        const int c = tid % (SSM_HG * VD), rows = SSM_C * SSM_HG * VD / (2 * SSM_T), g0 = __builtin_amdgcn_readfirstlane(tid / (SSM_HG * VD) * rows);
-        const int vh = __builtin_amdgcn_readfirstlane(c / VD), e = c % VD;
-        if (vh < heads) {
-            float *to = W.values(W.head(blockIdx.x, h0 + vh)) + e / 16 * (SSM_C * 16) + e % 16 * 4;
-            unsigned top = 0;
-            for (int g = g0; g < g0 + rows; g += 16) {
-                SsmConv<16> cv;
-                cv.load(A, r, pos, 2 * nk + (h0 + vh) * VD + e, x, i0, g, width);
-                f32x4 V;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float y = cv.cv.next(cv.x[i], taps);
-                    V[i % 4] = g + i < width ? y : 0.0f;
-                    top = max(top, __float_as_uint(V[i % 4]) & 0x7FFFFFFFu);
-                    if (i % 4 == 3) *(f32x4 *)(to + (g / 16 * 64 + i / 4 * 16) * 4) = V;
-                }
-            }
-            atomicMax(&s_top[vh * 128 + e], top);
-        }
-    }
     __syncthreads();
-    if (tid < heads * VD) {
-        const unsigned top = s_top[tid / VD * 128 + tid % VD];
-        W.vec(W.head(blockIdx.x, h0 + tid / VD))[SSM_TOP + tid % VD] = __uint_as_float(min(top, 0x7F800000u));
-    }
     if (!DELTA || w >= heads) return;                   /* waves 0 and 1: a head's T each */
     {
         const int b = l / 16, c = l % 16;
@@ -614,7 +585,8 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
 }
 
 /* A request's chunks in order, for 16 value elements of one head (v = l%16), with two groups of four waves: the first goes
- * from S to W, the second makes the outputs; token rows 16 (w % 4) .. each, and each wave has 16 key elements of S.  S stays in registers as the products leave it (key elements 16 w + 4 (l/16) + i) and
+ * from S to W, the second makes the outputs and the next chunk's values; token rows 16 (w % 4) .. each, and each wave has 16
+ * key elements of S.  S stays in registers as the products leave it (key elements 16 w + 4 (l/16) + i) and
  * in LDS as they take it.  Operands of the next chunk are loaded while this one is worked on, without conditions, so that
  * waits count those under way exactly. */
 template <int KD, bool DELTA>
@@ -622,7 +594,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
 {
     constexpr int KS = KD / 32, OPS = 4 * KS, LS = KD + 8, LT = SSM_C + 8, LV = SSM_C + 4;
     __shared__ __attribute__((aligned(16))) _Float16 s_S[2][16 * LS], s_R[2][16 * LT], s_W[2][16 * LT], s_We[2][16 * LT];
-    __shared__ __attribute__((aligned(16))) float s_V[16 * LV];
+    __shared__ __attribute__((aligned(16))) float s_V[2][16 * LV], s_top[2][16][4];
     __shared__ __attribute__((aligned(16))) char s_K[OPS * 2048];                /* K's operands as they are, read as K^T's */
     __shared__ float s_part[2][8][16];
     const RoasterSsmScan &a = A.a;
@@ -650,12 +622,15 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     f32x4 S = {};
     if (holds && q.pos) S = *(const f32x4 *)state;
     const float skip = a.skip ? a.skip[h] : 0.0f;
+    SsmChannel conv;                                    /* its history is that of the request's first row */
+    conv.start(A, r, q.pos, 2 * nk + v0 + v);
+    const float *x0 = a.x + (size_t)q.f0 * a.x_row + 2 * nk + v0 + v, *x4 = x0 + 4 * (l / 16) * a.x_row;
 
     SsmOp one[KS], two[2];                              /* the first group's K and T, the second's Q and D o Q K^T */
     struct Head {
         f32x4 f, g;                                     /* exp(G) and exp(G_63 - G), or the outputs' factors */
-        f32x4 V, gain;
-        float last, most, bad, top;
+        f32x4 gain;
+        float last, most, bad;
     };
     auto load_head = [&](int c, Head &o) {
         char *head = W.head(base + c, h);
@@ -667,8 +642,6 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         o.last = same[SSM_EG + SSM_C - 1];
         o.most = same[SSM_MOST];
         o.bad = same[SSM_BAD];
-        o.top = vec[SSM_TOP + vb * 16 + v];
-        o.V = *(const f32x4 *)(W.values(head) + vb * (SSM_C * 16) + (w * 64 + l) * 4);
     };
     auto load_one = [&](int c) {
         const char *at = W.key(base + c, kh) + ((first ? OPS : 0) + w * KS) * 2048;
@@ -694,6 +667,41 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         }
         return o;
     };
+    /* the inputs of this lane's four tokens of chunk c and the three before */
+    auto load_x = [&](int c, float (&xs)[7]) {
+        const int i0 = c * SSM_C + 16 * w - 3;
+        if (i0 >= 0 && i0 + 19 <= q.n) {
+#pragma unroll
+            for (int j = 0; j < 7; j++) xs[j] = x4[(size_t)(i0 + j) * a.x_row];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 7; j++)                  /* rows before the first and behind the last are not used */
+                xs[j] = x0[(size_t)min(max(i0 + 4 * (l / 16) + j, 0), q.n - 1) * a.x_row];
+        }
+    };
+    /* their values to LDS, and the largest of each element: infinite where one is infinite or NaN */
+    auto values = [&](int c, const float (&xs)[7]) {
+        float xx[7];
+#pragma unroll
+        for (int j = 0; j < 7; j++) xx[j] = xs[j];
+        if (c == 0 && t4 == 0) {
+#pragma unroll
+            for (int j = 0; j < 3; j++) xx[j] = conv.h[j];
+        }
+        f32x4 V;
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            SsmChannel cc = conv;
+            cc.h[0] = xx[i]; cc.h[1] = xx[i + 1]; cc.h[2] = xx[i + 2];
+            const float y = cc.next(xx[i + 3], taps);
+            V[i] = c * SSM_C + t4 + i < q.n ? y : 0.0f;
+            top = max(top, __float_as_uint(V[i]) & 0x7FFFFFFFu);
+        }
+        for (int o = 16; o < 64; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+        *(f32x4 *)(s_V[c & 1] + v * LV + t4) = V;
+        if (l < 16) s_top[c & 1][v][w] = __uint_as_float(min(top, 0x7F800000u));
+    };
     auto op = [&](const _Float16 *p, int ld, int s) {
         const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
         return SsmOp{ *(const h16x8 *)at, *(const h16x8 *)(at + 16 * ld) };
@@ -703,7 +711,13 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     };
 
     Head o, next;
+    float xs[7];
     load_head(0, o);
+    if (!first) {
+        load_x(0, xs);
+        values(0, xs);
+        load_x(min(1, chunks - 1), xs);
+    }
     load_one(0);
     load_two(0);
     /* the norm of the element's row of S */
@@ -724,7 +738,8 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     for (int c = 0; c < chunks; c++, out += SSM_C * a.out_row) {
         const int c1 = min(c + 1, chunks - 1);
         load_head(c1, next);
-        const float top = o.top;
+        const f32x4 tops = *(const f32x4 *)s_top[c & 1][v], V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         /* the wave's lanes have all 16 elements, with the same bounds in every wave */
         const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
         const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
@@ -743,7 +758,6 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
 #pragma unroll
                 for (int s = 0; s < KS; s++) ssm_st(s_K + (w * KS + s) * 2048, l, one[s]);
             }
-            const f32x4 V = o.V;
             if (DELTA) {
                 if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
                 __syncthreads();
@@ -760,7 +774,11 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
                 ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
                 load_one(c1);
-            } else load_one(c1);
+            } else {
+                if (c + 1 < chunks) values(c + 1, xs);
+                load_x(min(c + 2, chunks - 1), xs);      /* before the loads that both groups make, for the waits' sake */
+                load_one(c1);
+            }
             __syncthreads();
             const float back = pW * (1 / (8192.0f * SSM_UP));
             if (holds) {
@@ -793,10 +811,8 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             /* token by token, so that an infinite or NaN input does not reach those before it */
             const char *key = W.key(base + c, kh);
             const float *vec = W.vec(W.head(base + c, h));
-            if (first) *(f32x4 *)(s_V + v * LV + t4) = o.V;
-            __syncthreads();
             for (int t = 0; t < min(SSM_C, q.n - c * SSM_C); t++) {
-                const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[v * LV + t];
+                const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[c & 1][v * LV + t];
                 f32x4 kf = {}, qf = {};
                 if (holds) {
                     const int k = 16 * w8 + 4 * (l / 16);
@@ -842,6 +858,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             b = sqrtf(b) * 1.0001f;
             pS = ssm_pow2(b);
             put_S(8192.0f * ssm_inv2(pS));
+            if (!first) {
+                if (c + 1 < chunks) values(c + 1, xs);
+                load_x(min(c + 2, chunks - 1), xs);
+            }
             load_one(c1);
             load_two(c1);
         }
@@ -888,7 +908,7 @@ extern "C" size_t roaster_ssm_ws_bytes(int rows, int most, const RoasterSsmState
 {
     if (!ssm_state_ok(s) || rows < 0 || rows > (1 << 18) || most < 1 || (rows && most > rows)) return 0;
     if (most < SSM_CHUNK_FEW) return 16;
-    const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads, s->v_dim };
+    const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads };
     return (size_t)ssm_max_chunks(rows, s) * w.chunk_bytes();
 }
 
@@ -936,7 +956,7 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
     SsmArgs A = { *p, *s, s->v_heads / s->k_heads, (int)ch };
     A.a.b = b;
     if (ssm_by_chunks(p->most, s)) {
-        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads, s->v_dim };
+        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads };
         const int chunks = ssm_max_chunks(p->rows, s), groups = (A.rep + SSM_HG - 1) / SSM_HG, blocks = s->v_dim / 16;
 #define CHUNK(KD, D)                                                                                                          \
     do {                                                                                                                    \
