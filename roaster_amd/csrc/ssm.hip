@@ -11,6 +11,8 @@
 #include "mixer.h"
 #include "qdot.h"
 
+#include <type_traits>
+
 #define SSM_T 256
 
 struct SsmArgs {
@@ -600,7 +602,6 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     const RoasterSsmScan &a = A.a;
     const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;    /* so that operands' addresses are scalar */
     const int taps = A.s.taps, VD = A.s.v_dim, VH = A.s.v_heads;
-    const bool first = w8 < 4, holds = w8 < KD / 16;
     /* with a multiple of 8 heads, those of one key head and their blocks on one XCD (workgroup b runs on b % 8) */
     int h = blockIdx.x / blocks, vb = blockIdx.x % blocks;
     if (VH % 8 == 0) {
@@ -618,257 +619,275 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         return;
     }
     const int v = l % 16, t4 = 16 * w + 4 * (l / 16);
-    float *state = A.s.state + ((size_t)r * VH * VD + v0 + v) * KD + 16 * w8 + 4 * (l / 16);
-    f32x4 S = {};
-    if (holds && q.pos) S = *(const f32x4 *)state;
-    const float skip = a.skip ? a.skip[h] : 0.0f;
-    SsmChannel conv;                                    /* its history is that of the request's first row */
-    conv.start(A, r, q.pos, 2 * nk + v0 + v);
-    const float *x0 = a.x + (size_t)q.f0 * a.x_row + 2 * nk + v0 + v, *x4 = x0 + 4 * (l / 16) * a.x_row;
+    /* a loop for each group, so that its waits count its own loads */
+    auto run = [&](auto group) {
+        constexpr bool first = decltype(group)::value, holds = KD == 128 || first;
+        float *state = A.s.state + ((size_t)r * VH * VD + v0 + v) * KD + 16 * w8 + 4 * (l / 16);
+        f32x4 S = {};
+        if (holds && q.pos) S = *(const f32x4 *)state;
+        const float skip = a.skip ? a.skip[h] : 0.0f;
+        SsmChannel conv = {};                               /* the second group's; its history is that of the request's first row */
+        if (!first) conv.start(A, r, q.pos, 2 * nk + v0 + v);
+        const float *x0 = a.x + (size_t)q.f0 * a.x_row + 2 * nk + v0 + v, *x4 = x0 + 4 * (l / 16) * a.x_row;
 
-    SsmOp one[KS], two[2];                              /* the first group's K and T, the second's Q and D o Q K^T */
-    struct Head {
-        f32x4 f, g;                                     /* exp(G) and exp(G_63 - G), or the outputs' factors */
-        f32x4 gain;
-        float last, most, bad;
-    };
-    auto load_head = [&](int c, Head &o) {
-        char *head = W.head(base + c, h);
-        const float *vec = W.vec(head);
-        o.f = *(const f32x4 *)(vec + (first ? SSM_EG : SSM_EQ) + t4);
-        o.g = *(const f32x4 *)(vec + (first ? SSM_EC : SSM_QF) + t4);
-        if (!DELTA) o.gain = *(const f32x4 *)(vec + SSM_GAIN + t4);
-        const __attribute__((address_space(4))) float *same = (const __attribute__((address_space(4))) float *)vec;      /* scalar loads */
-        o.last = same[SSM_EG + SSM_C - 1];
-        o.most = same[SSM_MOST];
-        o.bad = same[SSM_BAD];
-    };
-    auto load_one = [&](int c) {
-        const char *at = W.key(base + c, kh) + ((first ? OPS : 0) + w * KS) * 2048;
+        SsmOp one[KS], two[2];                              /* the first group's K and T, the second's Q and D o Q K^T */
+        struct Head {
+            f32x4 f, g;                                     /* exp(G) and exp(G_63 - G), or the outputs' factors */
+            f32x4 gain;
+            float last, most, bad;
+        };
+        auto load_head = [&](int c, Head &o) {
+            char *head = W.head(base + c, h);
+            const float *vec = W.vec(head);
+            o.f = *(const f32x4 *)(vec + (first ? SSM_EG : SSM_EQ) + t4);
+            o.g = *(const f32x4 *)(vec + (first ? SSM_EC : SSM_QF) + t4);
+            if (!DELTA) o.gain = *(const f32x4 *)(vec + SSM_GAIN + t4);
+            const __attribute__((address_space(4))) float *same = (const __attribute__((address_space(4))) float *)vec;      /* scalar loads */
+            o.last = same[SSM_EG + SSM_C - 1];
+            o.most = same[SSM_MOST];
+            o.bad = same[SSM_BAD];
+        };
+        auto load_one = [&](int c) {
+            const char *at = W.key(base + c, kh) + ((first ? OPS : 0) + w * KS) * 2048;
 #pragma unroll
-        for (int s = 0; s < KS; s++) one[s] = ssm_ld(at + s * 2048, l);
-    };
-    auto load_two = [&](int c) {
-        const char *head = W.head(base + c, h) + (DELTA && first ? 0 : 8) * 2048;
+            for (int s = 0; s < KS; s++) one[s] = ssm_ld(at + s * 2048, l);
+        };
+        auto load_two = [&](int c) {
+            const char *head = W.head(base + c, h) + (DELTA && first ? 0 : 8) * 2048;
 #pragma unroll
-        for (int s = 0; s < 2; s++) two[s] = ssm_ld(head + (w * 2 + min(s, w / 2)) * 2048, l);      /* tokens 32 .. have no part in rows below */
-    };
-    /* This wave's 16 key elements of K^T, tokens 32 s ..: the transposing read takes 4 tokens of 16 elements from 16 lanes (lane
-     * 4 i + j: elements 4 j .. of token i) and gives lane c the four of element c. */
-    auto key_cols = [&](int s) {
-        const int j = l % 4, at = (l / 4 % 4 + 8 * (l / 16 % 2) + 16 * (w8 % 2 * 2 + j / 2)) * 16 + j % 2 * 8;
-        const char *base = s_K + ((2 * s + l / 32) * KS + w8 / 2) * 2048 + at;
-        SsmOp o;
+            for (int s = 0; s < 2; s++) two[s] = ssm_ld(head + (w * 2 + min(s, w / 2)) * 2048, l);      /* tokens 32 .. have no part in rows below */
+        };
+        /* This wave's 16 key elements of K^T, tokens 32 s ..: the transposing read takes 4 tokens of 16 elements from 16 lanes (lane
+         * 4 i + j: elements 4 j .. of token i) and gives lane c the four of element c. */
+        auto key_cols = [&](int s) {
+            const int j = l % 4, at = (l / 4 % 4 + 8 * (l / 16 % 2) + 16 * (w8 % 2 * 2 + j / 2)) * 16 + j % 2 * 8;
+            const char *base = s_K + ((2 * s + l / 32) * KS + w8 / 2) * 2048 + at;
+            SsmOp o;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const h16x4 hi = ssm_lds_cols(base + 64 * i), lo = ssm_lds_cols(base + 1024 + 64 * i);
+            for (int i = 0; i < 2; i++) {
+                const h16x4 hi = ssm_lds_cols(base + 64 * i), lo = ssm_lds_cols(base + 1024 + 64 * i);
 #pragma unroll
-            for (int e = 0; e < 4; e++) { o.hi[4 * i + e] = hi[e]; o.lo[4 * i + e] = lo[e]; }
-        }
-        return o;
-    };
-    /* the inputs of this lane's four tokens of chunk c and the three before */
-    auto load_x = [&](int c, float (&xs)[7]) {
-        const int i0 = c * SSM_C + 16 * w - 3;
-        if (i0 >= 0 && i0 + 19 <= q.n) {
+                for (int e = 0; e < 4; e++) { o.hi[4 * i + e] = hi[e]; o.lo[4 * i + e] = lo[e]; }
+            }
+            return o;
+        };
+        /* the inputs of this lane's four tokens of chunk c and the three before */
+        auto load_x = [&](int c, float (&xs)[7]) {
+            const int i0 = c * SSM_C + 16 * w - 3;
+            if (i0 >= 0 && i0 + 19 <= q.n) {
 #pragma unroll
-            for (int j = 0; j < 7; j++) xs[j] = x4[(size_t)(i0 + j) * a.x_row];
-        } else {
+                for (int j = 0; j < 7; j++) xs[j] = x4[(size_t)(i0 + j) * a.x_row];
+            } else {
 #pragma unroll
-            for (int j = 0; j < 7; j++)                  /* rows before the first and behind the last are not used */
-                xs[j] = x0[(size_t)min(max(i0 + 4 * (l / 16) + j, 0), q.n - 1) * a.x_row];
-        }
-    };
-    /* their values to LDS, and the largest of each element: infinite where one is infinite or NaN */
-    auto values = [&](int c, const float (&xs)[7]) {
-        float xx[7];
+                for (int j = 0; j < 7; j++)                  /* rows before the first and behind the last are not used */
+                    xs[j] = x0[(size_t)min(max(i0 + 4 * (l / 16) + j, 0), q.n - 1) * a.x_row];
+            }
+        };
+        /* their values to LDS, and the largest of each element: infinite where one is infinite or NaN */
+        auto values = [&](int c, const float (&xs)[7]) {
+            float xx[7];
 #pragma unroll
-        for (int j = 0; j < 7; j++) xx[j] = xs[j];
-        if (c == 0 && t4 == 0) {
+            for (int j = 0; j < 7; j++) xx[j] = xs[j];
+            if (c == 0 && t4 == 0) {
 #pragma unroll
-            for (int j = 0; j < 3; j++) xx[j] = conv.h[j];
-        }
-        f32x4 V;
-        unsigned top = 0;
+                for (int j = 0; j < 3; j++) xx[j] = conv.h[j];
+            }
+            f32x4 V;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            SsmChannel cc = conv;
-            cc.h[0] = xx[i]; cc.h[1] = xx[i + 1]; cc.h[2] = xx[i + 2];
-            const float y = cc.next(xx[i + 3], taps);
-            V[i] = c * SSM_C + t4 + i < q.n ? y : 0.0f;
-            top = max(top, __float_as_uint(V[i]) & 0x7FFFFFFFu);
-        }
-        for (int o = 16; o < 64; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-        *(f32x4 *)(s_V[c & 1] + v * LV + t4) = V;
-        if (l < 16) s_top[c & 1][v][w] = __uint_as_float(min(top, 0x7F800000u));
-    };
-    auto op = [&](const _Float16 *p, int ld, int s) {
-        const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
-        return SsmOp{ *(const h16x8 *)at, *(const h16x8 *)(at + 16 * ld) };
-    };
-    auto put_S = [&](float by) {
-        if (holds) ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
-    };
+            for (int i = 0; i < 4; i++) V[i] = fmaf(conv.w[3], xx[i + 3], fmaf(conv.w[2], xx[i + 2], conv.bias));
+            if (taps > 2) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) V[i] = fmaf(conv.w[1], xx[i + 1], V[i]);
+            }
+            if (taps > 3) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) V[i] = fmaf(conv.w[0], xx[i], V[i]);
+            }
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                V[i] = c * SSM_C + t4 + i < q.n ? ssm_silu(V[i]) : 0.0f;
+                top = max(top, __float_as_uint(V[i]) & 0x7FFFFFFFu);
+            }
+            const auto far = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max(far[0], far[1]);
+            const auto near = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = max(near[0], near[1]);
+            *(f32x4 *)(s_V[c & 1] + v * LV + t4) = V;
+            if (l < 16) s_top[c & 1][v][w] = __uint_as_float(min(top, 0x7F800000u));
+        };
+        auto op = [&](const _Float16 *p, int ld, int s) {
+            const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
+            return SsmOp{ *(const h16x8 *)at, *(const h16x8 *)(at + 16 * ld) };
+        };
+        auto put_S = [&](float by) {
+            if (holds) ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
+        };
 
-    Head o, next;
-    float xs[7];
-    load_head(0, o);
-    if (!first) {
-        load_x(0, xs);
-        values(0, xs);
-        load_x(min(1, chunks - 1), xs);
-    }
-    load_one(0);
-    load_two(0);
-    /* the norm of the element's row of S */
-    float b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
-    b += __shfl_xor(b, 16);
-    b += __shfl_xor(b, 32);
-    if (l < 16) s_part[0][w8][l] = b;
-    __syncthreads();
-    b = 0;
-    for (int i = 0; i < 8; i++) b += s_part[0][i][v];
-    b = sqrtf(b) * 1.0001f;
-    float pS = ssm_pow2(b);                              /* |S| < 2 pS; as an operand times 2^13 / pS, so below 2^14 */
-    put_S(8192.0f * ssm_inv2(pS));
-    __syncthreads();
+        Head o, next;
+        float xs[7];
+        load_head(0, o);
+        if (!first) {
+            load_x(0, xs);
+            values(0, xs);
+            load_x(min(1, chunks - 1), xs);
+        }
+        load_one(0);
+        load_two(0);
+        /* the norm of the element's row of S */
+        float b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
+        b += __shfl_xor(b, 16);
+        b += __shfl_xor(b, 32);
+        if (l < 16) s_part[0][w8][l] = b;
+        __syncthreads();
+        b = 0;
+        for (int i = 0; i < 8; i++) b += s_part[0][i][v];
+        b = sqrtf(b) * 1.0001f;
+        float pS = ssm_pow2(b);                              /* |S| < 2 pS; as an operand times 2^13 / pS, so below 2^14 */
+        put_S(8192.0f * ssm_inv2(pS));
+        __syncthreads();
 
-    float *out = a.out + (size_t)(q.f0 + t4) * a.out_row + v0 + v;               /* this lane's four tokens in turn */
-    if (first) __builtin_amdgcn_s_setprio(1);            /* the other group waits for it */
-    for (int c = 0; c < chunks; c++, out += SSM_C * a.out_row) {
-        const int c1 = min(c + 1, chunks - 1);
-        load_head(c1, next);
-        const f32x4 tops = *(const f32x4 *)s_top[c & 1][v], V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        /* the wave's lanes have all 16 elements, with the same bounds in every wave */
-        const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
-        const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
-        const float last = o.last;
-        if (!bad) {
-            /* bounds: of R, of W, and of the next S */
-            const float bR = top + b, bW = DELTA ? b + 65.0f * top : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
-            f32x4 X = {};
-            if (DELTA || !first) {
-                SsmSum sum;
+        float *out = a.out + (size_t)(q.f0 + t4) * a.out_row + v0 + v;               /* this lane's four tokens in turn */
+        if (first) __builtin_amdgcn_s_setprio(1);            /* the other group waits for it */
+        for (int c = 0; c < chunks; c++, out += SSM_C * a.out_row) {
+            const int c1 = min(c + 1, chunks - 1);
+            const f32x4 tops = *(const f32x4 *)s_top[c & 1][v], V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            /* the wave's lanes have all 16 elements, with the same bounds in every wave */
+            const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
+            const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
+            const float last = o.last;
+            if (!bad) {
+                /* bounds: of R, of W, and of the next S */
+                const float bR = top + b, bW = DELTA ? b + 65.0f * top : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
+                f32x4 X = {};
+                if (DELTA || !first) {
+                    SsmSum sum;
 #pragma unroll
-                for (int s = 0; s < KS; s++) sum.add(one[s], op(s_S[0], LS, s));
-                X = sum.get() * (pS * (1 / (8192.0f * SSM_UP)));
-            }
-            if (first) {
+                    for (int s = 0; s < KS; s++) sum.add(one[s], op(s_S[0], LS, s));
+                    X = sum.get() * (pS * (1 / (8192.0f * SSM_UP)));
+                }
+                if (first) {
 #pragma unroll
-                for (int s = 0; s < KS; s++) ssm_st(s_K + (w * KS + s) * 2048, l, one[s]);
-            }
-            if (DELTA) {
-                if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
-                __syncthreads();
-            }
-            if (first) {
-                f32x4 w4 = {};
+                    for (int s = 0; s < KS; s++) ssm_st(s_K + (w * KS + s) * 2048, l, one[s]);
+                }
                 if (DELTA) {
+                    if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
+                    __syncthreads();
+                }
+                if (first) {
+                    f32x4 w4 = {};
+                    if (DELTA) {
+                        SsmSum sum;
+#pragma unroll
+                        for (int s = 0; s < 2; s++)
+                            if (s <= w / 2) sum.add(two[s], op(s_R[0], LT, s));
+                        w4 = sum.get() * (pR * (1 / (8192.0f * SSM_UP)));
+                    } else w4 = o.gain * V;
+                    ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
+                    ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
+                    load_head(c1, next);
+                    load_one(c1);
+                } else {
+                    if (c + 1 < chunks) values(c + 1, xs);
+                    load_x(min(c + 2, chunks - 1), xs);
+                    load_head(c1, next);
+                    load_one(c1);
+                }
+                __syncthreads();
+                const float back = pW * (1 / (8192.0f * SSM_UP));
+                if (holds) {
+                    SsmSum sum;
+#pragma unroll
+                    for (int s = 0; s < 2; s++) sum.add(key_cols(s), op(s_We[0], LT, s));
+                    S = S * last + sum.get() * back;
+                }
+                b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
+                pS = ssm_pow2(b);
+                put_S(8192.0f * ssm_inv2(pS));
+                if (!first) {
                     SsmSum sum;
 #pragma unroll
                     for (int s = 0; s < 2; s++)
-                        if (s <= w / 2) sum.add(two[s], op(s_R[0], LT, s));
-                    w4 = sum.get() * (pR * (1 / (8192.0f * SSM_UP)));
-                } else w4 = o.gain * V;
-                ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
-                ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
-                load_one(c1);
-            } else {
-                if (c + 1 < chunks) values(c + 1, xs);
-                load_x(min(c + 2, chunks - 1), xs);      /* before the loads that both groups make, for the waits' sake */
-                load_one(c1);
-            }
-            __syncthreads();
-            const float back = pW * (1 / (8192.0f * SSM_UP));
-            if (holds) {
-                SsmSum sum;
+                        if (s <= w / 2) sum.add(two[s], op(s_W[0], LT, s));
+                    f32x4 O = o.f * X + o.g * (sum.get() * back);
+                    if (a.skip) O = O + skip * V;
+                    if ((c + 1) * SSM_C <= q.n) {
 #pragma unroll
-                for (int s = 0; s < 2; s++) sum.add(key_cols(s), op(s_We[0], LT, s));
-                S = S * last + sum.get() * back;
-            }
-            b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
-            pS = ssm_pow2(b);
-            put_S(8192.0f * ssm_inv2(pS));
-            if (!first) {
-                SsmSum sum;
+                        for (int i = 0; i < 4; i++) out[i * a.out_row] = O[i];
+                    } else {
 #pragma unroll
-                for (int s = 0; s < 2; s++)
-                    if (s <= w / 2) sum.add(two[s], op(s_W[0], LT, s));
-                f32x4 O = o.f * X + o.g * (sum.get() * back);
-                if (a.skip) O = O + skip * V;
-                if ((c + 1) * SSM_C <= q.n) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) out[i * a.out_row] = O[i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (c * SSM_C + t4 + i < q.n) out[i * a.out_row] = O[i];
-                }
-            }
-            load_two(c1);
-        } else {
-            /* token by token, so that an infinite or NaN input does not reach those before it */
-            const char *key = W.key(base + c, kh);
-            const float *vec = W.vec(W.head(base + c, h));
-            for (int t = 0; t < min(SSM_C, q.n - c * SSM_C); t++) {
-                const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[c & 1][v * LV + t];
-                f32x4 kf = {}, qf = {};
-                if (holds) {
-                    const int k = 16 * w8 + 4 * (l / 16);
-                    const char *at = key + (t / 16 * KS + k / 32) * 2048 + (t % 16 + 16 * (k % 32 / 8)) * 16 + k % 8 * 2;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        qf[i] = ((float)((const _Float16 *)at)[i] + (float)((const _Float16 *)(at + 1024))[i]) * (1 / SSM_UP);
-                        kf[i] = ((float)((const _Float16 *)(at + OPS * 2048))[i] + (float)((const _Float16 *)(at + OPS * 2048 + 1024))[i]) * (1 / SSM_UP);
+                        for (int i = 0; i < 4; i++)
+                            if (c * SSM_C + t4 + i < q.n) out[i * a.out_row] = O[i];
                     }
                 }
-                float wt = gain * val;
-                if (DELTA) {
-                    float sk = S[0] * kf[0] + S[1] * kf[1] + S[2] * kf[2] + S[3] * kf[3];
-                    sk += __shfl_xor(sk, 16);
-                    sk += __shfl_xor(sk, 32);
-                    if (l < 16) s_part[0][w8][l] = sk;
+                load_two(c1);
+            } else {
+                /* token by token, so that an infinite or NaN input does not reach those before it */
+                const char *key = W.key(base + c, kh);
+                const float *vec = W.vec(W.head(base + c, h));
+                for (int t = 0; t < min(SSM_C, q.n - c * SSM_C); t++) {
+                    const float decay = ssm_exp(vec[SSM_GL + t]), gain = vec[SSM_GAIN + t], val = s_V[c & 1][v * LV + t];
+                    f32x4 kf = {}, qf = {};
+                    if (holds) {
+                        const int k = 16 * w8 + 4 * (l / 16);
+                        const char *at = key + (t / 16 * KS + k / 32) * 2048 + (t % 16 + 16 * (k % 32 / 8)) * 16 + k % 8 * 2;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            qf[i] = ((float)((const _Float16 *)at)[i] + (float)((const _Float16 *)(at + 1024))[i]) * (1 / SSM_UP);
+                            kf[i] = ((float)((const _Float16 *)(at + OPS * 2048))[i] + (float)((const _Float16 *)(at + OPS * 2048 + 1024))[i]) * (1 / SSM_UP);
+                        }
+                    }
+                    float wt = gain * val;
+                    if (DELTA) {
+                        float sk = S[0] * kf[0] + S[1] * kf[1] + S[2] * kf[2] + S[3] * kf[3];
+                        sk += __shfl_xor(sk, 16);
+                        sk += __shfl_xor(sk, 32);
+                        if (l < 16) s_part[0][w8][l] = sk;
+                        __syncthreads();
+                        sk = 0;
+                        for (int i = 0; i < KD / 16; i++) sk += s_part[0][i][v];
+                        wt = gain * (val - decay * sk);
+                    }
+                    S = decay * S + wt * kf;
+                    float so = S[0] * qf[0] + S[1] * qf[1] + S[2] * qf[2] + S[3] * qf[3];
+                    so += __shfl_xor(so, 16);
+                    so += __shfl_xor(so, 32);
+                    if (l < 16) s_part[1][w8][l] = so;
                     __syncthreads();
-                    sk = 0;
-                    for (int i = 0; i < KD / 16; i++) sk += s_part[0][i][v];
-                    wt = gain * (val - decay * sk);
+                    if (tid < 16) {
+                        so = 0;
+                        for (int i = 0; i < KD / 16; i++) so += s_part[1][i][v];
+                        so *= vec[SSM_QF + t];
+                        out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, so) : so;     /* threads 0 .. 15: t4 = 0 */
+                    }
+                    __syncthreads();
                 }
-                S = decay * S + wt * kf;
-                float so = S[0] * qf[0] + S[1] * qf[1] + S[2] * qf[2] + S[3] * qf[3];
-                so += __shfl_xor(so, 16);
-                so += __shfl_xor(so, 32);
-                if (l < 16) s_part[1][w8][l] = so;
+                b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
+                b += __shfl_xor(b, 16);
+                b += __shfl_xor(b, 32);
+                if (l < 16) s_part[0][w8][l] = b;
                 __syncthreads();
-                if (tid < 16) {
-                    so = 0;
-                    for (int i = 0; i < KD / 16; i++) so += s_part[1][i][v];
-                    so *= vec[SSM_QF + t];
-                    out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, so) : so;     /* threads 0 .. 15: t4 = 0 */
+                b = 0;
+                for (int i = 0; i < 8; i++) b += s_part[0][i][v];
+                b = sqrtf(b) * 1.0001f;
+                pS = ssm_pow2(b);
+                put_S(8192.0f * ssm_inv2(pS));
+                if (!first) {
+                    if (c + 1 < chunks) values(c + 1, xs);
+                    load_x(min(c + 2, chunks - 1), xs);
                 }
-                __syncthreads();
+                load_head(c1, next);
+                load_one(c1);
+                load_two(c1);
             }
-            b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
-            b += __shfl_xor(b, 16);
-            b += __shfl_xor(b, 32);
-            if (l < 16) s_part[0][w8][l] = b;
+            o = next;
             __syncthreads();
-            b = 0;
-            for (int i = 0; i < 8; i++) b += s_part[0][i][v];
-            b = sqrtf(b) * 1.0001f;
-            pS = ssm_pow2(b);
-            put_S(8192.0f * ssm_inv2(pS));
-            if (!first) {
-                if (c + 1 < chunks) values(c + 1, xs);
-                load_x(min(c + 2, chunks - 1), xs);
-            }
-            load_one(c1);
-            load_two(c1);
         }
-        o = next;
-        __syncthreads();
-    }
-    if (holds) *(f32x4 *)state = S;
+        if (holds) *(f32x4 *)state = S;
+    };
+    if (w8 < 4) run(std::true_type());
+    else run(std::false_type());
     /* the inputs of the last positions: these value channels, and by one workgroup of a key head its own */
     for (int i = max(0, q.n - taps); i < q.n; i++) {
         float *to = A.s.conv + ((size_t)r * taps + ((unsigned)q.pos + i) % taps) * A.channels;
