@@ -771,6 +771,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
 #pragma unroll
                     for (int s = 0; s < KS; s++) ssm_st(s_K + (w * KS + s) * 2048, l, one[s]);
                 }
+                if (first) load_one(c1);
                 if (DELTA) {
                     if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
                     __syncthreads();
@@ -786,13 +787,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     } else w4 = o.gain * V;
                     ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
                     ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
-                    load_head(c1, next);
-                    load_one(c1);
                 } else {
+                    load_one(c1);
                     if (c + 1 < chunks) values(c + 1, xs);
                     load_x(min(c + 2, chunks - 1), xs);
-                    load_head(c1, next);
-                    load_one(c1);
                 }
                 __syncthreads();
                 const float back = pW * (1 / (8192.0f * SSM_UP));
@@ -814,7 +812,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     if (a.skip) O = O + skip * V;
                     if ((c + 1) * SSM_C <= q.n) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) out[i * a.out_row] = O[i];
+                        for (int i = 0; i < 4; i++) __builtin_nontemporal_store(O[i], out + i * a.out_row);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -822,6 +820,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     }
                 }
                 load_two(c1);
+                load_head(c1, next);
             } else {
                 /* token by token, so that an infinite or NaN input does not reach those before it */
                 const char *key = W.key(base + c, kh);
