@@ -215,8 +215,8 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
  * hi hi + hi lo + lo hi, since f32 MFMAs have a sixteenth of the rate:
  *   A[m][k]: lane l holds m = l%16, k = 8*(l/16) + i, i = 0..7     (B[k][n] likewise)
  *   D[m][n]: lane l holds m = 4*(l/16) + i, n = l%16, i = 0..3
- * Q and K are unit vectors (STATE: powers of two make them such to a factor of two, K's going into dt and Q's into
- * the output), so they, D o Q K^T and T are at most 4 in size and enter times 2^8.  S, R and W enter
+ * Q and K are unit vectors (STATE: powers of two bring their largest element to 1/16 .. 1/8, their norms so below 1.5, K's
+ * going into dt and Q's into the output), so they, D o Q K^T and T are at most 4 in size and enter times 2^8.  S, R and W enter
  * times a power of two for each value element, from bounds that need no look at them: the norm of an element's
  * row of S is at most b and grows by the sum of gain |v| |k| alone, |R| <= |v| + b, |w| <= |v| + |S|.  fp16's
  * range below the bound (2^-38 of it) leaves 22 bits where the bound is 2^15 too large.  That takes decays
@@ -290,12 +290,14 @@ __device__ __forceinline__ int ssm_base(const SsmArgs &A, int r)
 }
 
 __device__ __forceinline__ bool ssm_finite(float x) { return fabsf(x) < INFINITY; }
-/* 2^e of a finite x, 2^e <= |x| < 2^(e + 1), within 2^-100 .. 2^123; 1 for others. */
-__device__ __forceinline__ float ssm_pow2(float x)
+/* 2^e of a finite x, 2^e <= |x| < 2^(e + 1), e within lo - 127 .. hi - 127; 1 for others. */
+__device__ __forceinline__ float ssm_pow2(float x, int lo = 27, int hi = 250)
 {
     const int e = (int)(__float_as_uint(x) >> 23 & 255);
-    return e == 255 ? 1.0f : __uint_as_float((unsigned)min(max(e, 27), 250) << 23);
+    return e == 255 ? 1.0f : __uint_as_float((unsigned)min(max(e, lo), hi) << 23);
 }
+/* The larger of top and |x|, NaN being larger than all. */
+__device__ __forceinline__ float ssm_top(float top, float x) { return __uint_as_float(max(__float_as_uint(top), __float_as_uint(x) & 0x7FFFFFFFu)); }
 __device__ __forceinline__ float ssm_inv2(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }   /* 1 / 2^e */
 
 struct SsmOp { h16x8 hi, lo; };                         /* one lane's of an operand */
@@ -432,14 +434,26 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
 #pragma unroll
         for (int j = 0; j < KD / 32; j++) {
             const float4 q = *(const float4 *)(s_q + row * LD + 4 * (tid % 8 + 8 * j)), k = *(const float4 *)(s_k + row * LD + 4 * (tid % 8 + 8 * j));
-            sq += q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
-            sk += k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w;
+            if (DELTA) {
+                sq += q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
+                sk += k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w;
+            } else {                                    /* the largest, NaN being larger than all */
+                sq = ssm_top(ssm_top(ssm_top(ssm_top(sq, q.x), q.y), q.z), q.w);
+                sk = ssm_top(ssm_top(ssm_top(ssm_top(sk, k.x), k.y), k.z), k.w);
+            }
         }
-        for (int o = 1; o < 8; o <<= 1) { sq += __shfl_xor(sq, o); sk += __shfl_xor(sk, o); }
+        for (int o = 1; o < 8; o <<= 1) {
+            const float oq = __shfl_xor(sq, o), ok = __shfl_xor(sk, o);
+            sq = DELTA ? sq + oq : ssm_top(sq, oq);
+            sk = DELTA ? sk + ok : ssm_top(sk, ok);
+        }
         if (tid % 8 == 0) {
-            const float pq = DELTA ? 1.0f : ssm_pow2(sqrtf(sq)), pk = DELTA ? 1.0f : ssm_pow2(sqrtf(sk));
+            /* not from sums of squares, which leave f32's range where the vectors do not */
+            const float pq = DELTA ? 1.0f : 16.0f * ssm_pow2(sq, 8, 249), pk = DELTA ? 1.0f : 16.0f * ssm_pow2(sk, 8, 249);
             const float rq = DELTA ? 1.0f / sqrtf(sq + a.eps) : ssm_inv2(pq), rk = DELTA ? 1.0f / sqrtf(sk + a.eps) : ssm_inv2(pk);
-            if (row < width && !(ssm_finite(sq) && ssm_finite(sk) && ssm_finite(rq) && ssm_finite(rk) && ssm_finite(a.scale * pq))) s_bad = 1;
+            /* without eps a sum of squares near f32's smallest makes no unit vector */
+            const bool fine = sq < 0x1p120f && sk < 0x1p120f && (!DELTA || (rq < 0x1p60f && rk < 0x1p60f)) && ssm_finite(a.scale * pq);
+            if (row < width && !fine) s_bad = 1;
             s_rq[row] = row < width ? rq : 0.0f;
             s_rk[row] = row < width ? rk : 0.0f;
             s_qf[row] = a.scale * pq;
@@ -724,6 +738,27 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             if (holds) ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
         };
 
+        /* The norm of the element's row of S, no less; squares of small states would leave f32's range. */
+        auto row_norm = [&] {
+            const f32x4 U = S * 0x1p64f;
+            float one = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3], up = U[0] * U[0] + U[1] * U[1] + U[2] * U[2] + U[3] * U[3];
+            one += __shfl_xor(one, 16);
+            up += __shfl_xor(up, 16);
+            one += __shfl_xor(one, 32);
+            up += __shfl_xor(up, 32);
+            if (l < 16) {
+                s_part[0][w8][l] = one;
+                s_part[1][w8][l] = up;
+            }
+            __syncthreads();
+            one = up = 0;
+            for (int i = 0; i < 8; i++) {
+                one += s_part[0][i][v];
+                up += s_part[1][i][v];
+            }
+            return (one >= 0x1p-60f ? sqrtf(one) : sqrtf(up) * 0x1p-64f) * 1.0001f;
+        };
+
         Head o, next;
         float xs[7];
         load_head(0, o);
@@ -734,15 +769,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         }
         load_one(0);
         load_two(0);
-        /* the norm of the element's row of S */
-        float b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
-        b += __shfl_xor(b, 16);
-        b += __shfl_xor(b, 32);
-        if (l < 16) s_part[0][w8][l] = b;
-        __syncthreads();
-        b = 0;
-        for (int i = 0; i < 8; i++) b += s_part[0][i][v];
-        b = sqrtf(b) * 1.0001f;
+        float b = row_norm();
         float pS = ssm_pow2(b);                              /* |S| < 2 pS; as an operand times 2^13 / pS, so below 2^14 */
         put_S(8192.0f * ssm_inv2(pS));
         __syncthreads();
@@ -862,14 +889,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     }
                     __syncthreads();
                 }
-                b = S[0] * S[0] + S[1] * S[1] + S[2] * S[2] + S[3] * S[3];
-                b += __shfl_xor(b, 16);
-                b += __shfl_xor(b, 32);
-                if (l < 16) s_part[0][w8][l] = b;
-                __syncthreads();
-                b = 0;
-                for (int i = 0; i < 8; i++) b += s_part[0][i][v];
-                b = sqrtf(b) * 1.0001f;
+                b = row_norm();
                 pS = ssm_pow2(b);
                 put_S(8192.0f * ssm_inv2(pS));
                 if (!first) {

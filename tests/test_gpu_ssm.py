@@ -4,7 +4,7 @@ import pytest
 
 import roaster_amd as R
 from attn_util import sync
-from gpu_util import log
+from gpu_util import Dev, log
 from mixer_util import Scan, ScanCall, check_scan, scan_oracle
 
 pytestmark = pytest.mark.gpu
@@ -160,3 +160,88 @@ def test_many_requests_mostly_idle():
     new[5], new[1999] = 70, 40
     s = Scan(rng, new, pos, DELTA, 1, 1, 64, 64)
     check_scan(run(s), scan_oracle(s))
+
+
+@pytest.mark.parametrize("qs,ks,scale", [(1, 1e22, 0.5), (1e22, 1, 0.5), (1e-24, 1, 1e22), (1, 1e-24, 1e22), (1e-24, 1e22, 3.0), (1e-30, 1e-30, 1e37)])
+@pytest.mark.parametrize("new", [[2, 1], [70, 33]])
+def test_vectors_whose_squares_leave_the_range(new, qs, ks, scale):
+    """Without unit vectors only the vectors themselves have to be within f32's range."""
+    s = Scan(np.random.default_rng(21), new, [0, 4], STATE, 1, 2, 128, 64, bias=False, skip=False, scale=scale)
+    s.conv_w[:128] *= np.float32(qs)
+    s.conv_w[128:256] *= np.float32(ks)
+    s.state[1] *= np.float32(ks)
+    out, conv, state = run(s)
+    o, c, st, oe, se = scan_oracle(s)
+    assert np.array_equal(conv.astype(np.float64), c)
+    assert np.all(np.abs(out - o) <= oe)
+    assert np.all(np.linalg.norm((state - st) / ks, axis=3) <= se / ks + 1e-9)       # that of -ks 1e-9: f32's least normal value
+
+
+@pytest.mark.parametrize("new,at", [([2, 1], 1), ([70, 30], 5)])
+def test_without_eps_a_zero_vector_is_nan_from_its_row_on(new, at):
+    s = Scan(np.random.default_rng(22), new, [0, 4], DELTA, 2, 4, 128, 128, taps=2, bias=False)
+    s.eps = 0.0
+    want = scan_oracle(s)
+    s.x[at - 1:at + 1, 256:384] = 0                         # key head 0's keys: value heads 0 and 1
+    out, conv, state = run(s)
+    bad = np.zeros(out.shape, bool)
+    bad[at:new[0], :2] = True
+    assert np.isnan(out[bad]).all() and np.isnan(state[0, :2]).all()
+    ok = ~bad
+    ok[at - 1] = False                                      # whose own key is another now
+    assert np.all(np.abs(out - want[0])[ok] <= want[3][ok] + 1e-30)
+    assert np.all(np.linalg.norm(state[1] - want[2][1], axis=2) <= want[4][1] + 1e-30)
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+@pytest.mark.parametrize("new", [[3, 1], [100, 40]])
+def test_decays_above_one(mode, new):
+    s = Scan(np.random.default_rng(23), new, [0, 4], mode, 2, 4, 64, 128)
+    s.a_coef = np.array([0.02, -0.5, 0.05, 0.0], np.float32)
+    log(check_scan(run(s), scan_oracle(s)))
+
+
+@pytest.mark.parametrize("noise", [0.0, 0.05])
+def test_the_same_key_again_and_again(noise):
+    """Gains of nearly one and hardly any decay: the solution takes back what the token before added."""
+    s = Scan(np.random.default_rng(24), [200, 64], [0, 4], DELTA, 1, 2, 128, 64)
+    keys = slice(128, 256)
+    s.x[:, keys] = s.x[0, keys] + np.float32(noise) * s.x[:, keys]
+    s.a[:], s.b[:] = -12, 8
+    s.a_coef[:], s.dt_bias[:] = -0.1, 0
+    log(check_scan(run(s), scan_oracle(s)))
+
+
+@pytest.mark.parametrize("most", [19, 20, 31, 32])
+@pytest.mark.parametrize("n", [1, 70])
+def test_both_ways_about_their_limits(most, n):
+    s = Scan(np.random.default_rng(most + n), [most] + [2] * (n - 1), [3] * n, DELTA, 2, 4, 128, 128)
+    log(check_scan(run(s), scan_oracle(s)))
+
+
+@pytest.mark.parametrize("new", [[2, 1], [70, 33]])
+def test_a_wider_output(new):
+    s = Scan(np.random.default_rng(26), new, [1, 0], DELTA, 1, 3, 64, 64, pad=2)
+    c = ScanCall(s, out_row=3 * 64 + 12)
+    c.out = Dev(np.full((s.rows, 3 * 64 + 12), 77, np.float32))
+    c.a.out = c.out.p
+    R.check(c.call(), "scan")
+    sync()
+    out, conv, state = c.got()
+    assert np.all(out[:, 192:] == 77)
+    check_scan((np.ascontiguousarray(out[:, :192]).reshape(s.rows, 3, 64), conv, state), scan_oracle(s))
+
+
+def test_requests_that_share_rows():
+    """More tokens than rows: a request whose chunks have no place left is reported and its state stays as it was."""
+    s = Scan(np.random.default_rng(27), [640, 0, 0, 0], [2, 0, 0, 0], DELTA, 1, 1, 64, 64)
+    want = scan_oracle(s)
+    s.first = np.array([0, 640, 0, 640, 640], np.int32)
+    c = ScanCall(s)
+    R.check(c.call(), "scan")
+    assert R.lib().roaster_sync() == R.EINVAL and "left out" in R.last_error()
+    out, conv, state = c.got()
+    for r in (1, 2, 3):
+        assert np.array_equal(state[r], s.state[r]) and np.array_equal(conv[r], s.conv[r])
+    assert np.array_equal(conv[0].astype(np.float64), want[1][0])
+    assert np.all(np.linalg.norm(state[0] - want[2][0], axis=2) <= want[4][0])
