@@ -375,8 +375,8 @@ struct SsmConv {
 };
 
 /* A chunk's tokens of one key head: convolution, norms, the products among tokens, and of SSM_HG of its value
- * heads the decays and T, whose 16 x 16 blocks on the diagonal one wave inverts by substitution, a column a lane,
- * and joins by products in f32 (T_rc = - T_rr sum_k A_rk T_kc).  What bounds it: at 2048 tokens and 16 key heads
+ * heads the decays and T, whose 16 x 16 blocks on the diagonal are inverted by substitution, a column a lane,
+ * and joined by products in f32 (T_rc = - T_rr sum_k A_rk T_kc), a wave having a block c of columns.  What bounds it: at 2048 tokens and 16 key heads
  * two workgroups fill a CU and all run at once, so their chain of waits. */
 template <int KD, bool DELTA>
 __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs W, int groups)
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     __syncthreads();
     /* decays, four waves a head: row block w / 2 of D o Q K^T as an operand, and of A */
     const int hh = w % SSM_HG, m = w / SSM_HG, h = h0 + hh;
-    float *s_A = s_buf + (2 + hh) * SSM_C * LG, *s_T = s_buf + hh * SSM_C * LG;    /* A; later T, with its columns as rows */
+    float *const s_A = s_buf + (2 + hh) * SSM_C * LG, *const s_T = s_buf + hh * SSM_C * LG;    /* A; later T, with its columns as rows */
     if (hh < heads) {
         char *out = W.head(blockIdx.x, h);
         const int i = 16 * m + l % 16;
@@ -540,16 +540,17 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
         }
     }
     __syncthreads();
-    if (!DELTA || w >= heads) return;                   /* waves 0 and 1: a head's T each */
-    {
-        const int b = l / 16, c = l % 16;
+    if (!DELTA) return;
+    /* T by blocks of 16 columns, one to a wave */
+    if (hh < heads) {                                   /* the block on the diagonal, a column a lane, four times over */
+        const int c = l % 16;
         float y[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             float s0 = i == c ? 1.0f : 0.0f, s1 = 0.0f;
 #pragma unroll
             for (int j = 0; j < i; j += 4) {
-                const f32x4 v = *(const f32x4 *)(s_A + (16 * b + i) * LG + 16 * b + j);
+                const f32x4 v = *(const f32x4 *)(s_A + (16 * m + i) * LG + 16 * m + j);
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                     if (j + k < i) {
@@ -559,44 +560,45 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
             }
             y[i] = s0 + s1;
         }
+        if (l < 16) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) *(f32x4 *)(s_T + l * LG + 16 * b + i) = (f32x4){ y[i], y[i + 1], y[i + 2], y[i + 3] };
-        /* rows of the inverted blocks over A's own, which are not needed any more */
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int i = 0; i < 16; i += 4) *(f32x4 *)(s_T + (16 * m + c) * LG + 16 * m + i) = (f32x4){ y[i], y[i + 1], y[i + 2], y[i + 3] };
+            /* its rows over A's own, which are not needed any more */
 #pragma unroll
-        for (int i = 0; i < 16; i++) s_A[(16 * b + i) * LG + 16 * b + c] = y[i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    /* v_mfma_f32_16x16x4_f32, its lanes' four columns of 16 being 4*(l/16) .. + 3: results are operands of the next product as they come */
-    auto mul = [&](const f32x4 &u, const f32x4 &v, f32x4 c) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(u[i], v[i], c, 0, 0, 0);
-        return c;
-    };
-#pragma unroll
-    for (int d = 1; d < 4; d++) {
-#pragma unroll
-        for (int b = 0; b + d < 4; b++) {
-            f32x4 s = {};
-            const int row = 16 * (b + d) + l % 16, at = 4 * (l / 16);
-#pragma unroll
-            for (int k = b; k < b + d; k++)
-                s = mul(*(const f32x4 *)(s_A + row * LG + 16 * k + at), *(const f32x4 *)(s_T + (16 * b + l % 16) * LG + 16 * k + at), s);
-            s = mul(*(const f32x4 *)(s_A + row * LG + 16 * (b + d) + at), -s, (f32x4){ 0, 0, 0, 0 });
-            *(f32x4 *)(s_T + (16 * b + l % 16) * LG + 16 * (b + d) + at) = s;
+            for (int i = 0; i < 16; i++) s_A[(16 * m + i) * LG + 16 * m + c] = y[i];
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    char *out = W.head(blockIdx.x, h0 + w);
-    for (int t = 0; t < 4; t++)
-        for (int s = 0; s <= t / 2; s++) {
+    __syncthreads();
+    if (hh < heads) {
+        /* v_mfma_f32_16x16x4_f32, its lanes' four columns of 16 being 4*(l/16) .. + 3: results are operands of the next product as they come */
+        auto mul = [&](const f32x4 &u, const f32x4 &v, f32x4 c) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(u[i], v[i], c, 0, 0, 0);
+            return c;
+        };
+        const int at = 4 * (l / 16);
+        f32x4 T[4];                                     /* T_kb, k = 0 .. */
+        for (int k = 0; k < 4; k++) T[k] = (f32x4){};
+        T[0] = *(const f32x4 *)(s_T + (16 * m + l % 16) * LG + 16 * m + at);
+#pragma unroll
+        for (int d = 1; d < 4; d++)                     /* block row m + d */
+            if (m + d < 4) {
+                f32x4 s = {};
+                const float *A = s_A + (16 * (m + d) + l % 16) * LG + 16 * m + at;
+#pragma unroll
+                for (int k = 0; k < d; k++) s = mul(*(const f32x4 *)(A + 16 * k), T[k], s);
+                T[d] = mul(*(const f32x4 *)(A + 16 * d), -s, (f32x4){ 0, 0, 0, 0 });
+                *(f32x4 *)(s_T + (16 * m + l % 16) * LG + 16 * (m + d) + at) = T[d];
+            }
+    }
+    __syncthreads();
+    if (hh < heads)
+        for (int s = 0; s <= m / 2; s++) {
+            const int i = 16 * m + l % 16, j = 32 * s + 8 * (l / 16);
             float v[8];
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-                const int i = 16 * t + l % 16, j = 32 * s + 8 * (l / 16) + c;
-                v[c] = j <= i ? s_T[j * LG + i] * (s_gain[w][j] * SSM_UP) : 0.0f;
-            }
-            ssm_st(out + (t * 2 + s) * 2048, l, ssm_split(v));
+            for (int c = 0; c < 8; c++) v[c] = j + c <= i ? s_T[(j + c) * LG + i] * (s_gain[hh][j + c] * SSM_UP) : 0.0f;
+            ssm_st(W.head(blockIdx.x, h0 + hh) + (m * 2 + s) * 2048, l, ssm_split(v));
         }
 }
 
