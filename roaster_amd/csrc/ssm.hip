@@ -11,6 +11,7 @@
 #include "mixer.h"
 #include "qdot.h"
 
+#include <climits>
 #include <type_traits>
 
 #define SSM_T 256
@@ -19,10 +20,19 @@ struct SsmArgs {
     RoasterSsmScan a;
     RoasterSsmState s;
     int rep, channels;           /* value heads to a key head; channels of a row */
+    int lim;                     /* requests of so many rows and more go by chunks */
 };
 
 /* A request's rows and first position. */
 struct SsmReq { int f0, n, pos; };
+
+/* Rows f0 .. f1 - 1 left out: NaN in `width` elements from `col` on, and a report. */
+__device__ __forceinline__ void ssm_leave(const SsmArgs &A, int f0, int f1, int col, int width, int *err)
+{
+    if (threadIdx.x == 0) atomicOr(err, ATTN_ERR_SCAN);
+    for (int t = max(f0, 0); t < min(f1, A.a.rows); t++)
+        for (int i = threadIdx.x; i < width; i += blockDim.x) A.a.out[t * A.a.out_row + col + i] = __uint_as_float(0x7FC00000u);
+}
 
 /* Whether request r has rows to work on; a bad one's are filled with NaN (`width` elements from `col` on). */
 __device__ __forceinline__ bool ssm_request(const SsmArgs &A, int r, int col, int width, SsmReq &q, int *err)
@@ -37,11 +47,7 @@ __device__ __forceinline__ bool ssm_request(const SsmArgs &A, int r, int col, in
         q.pos = a.row_pos[f0];
         if (q.pos >= 0) return true;
     }
-    if (err) {
-        if (threadIdx.x == 0) atomicOr(err, ATTN_ERR_SCAN);
-        for (int t = max(f0, 0); t < min(f1, a.rows); t++)
-            for (int i = threadIdx.x; i < width; i += blockDim.x) a.out[t * a.out_row + col + i] = __uint_as_float(0x7FC00000u);
-    }
+    if (err) ssm_leave(A, f0, f1, col, width, err);
     return false;
 }
 
@@ -104,7 +110,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_token_kernel(SsmArgs A, int blocks,
     const int tid = threadIdx.x, r = blockIdx.y, h = blockIdx.x / blocks, v0 = blockIdx.x % blocks * VB;
     const int VD = A.s.v_dim, taps = A.s.taps, nk = A.s.k_heads * KD, kh = h / A.rep;
     SsmReq q;
-    if (!ssm_request(A, r, h * VD + v0, VB, q, err)) return;
+    if (!ssm_request(A, r, h * VD + v0, VB, q, err) || q.n >= A.lim) return;
     const bool qk = tid < 2 * KD, val = tid < VB;
     const int cq = tid < KD ? kh * KD + tid : nk + kh * KD + tid - KD, cv = 2 * nk + h * VD + v0 + tid;
     const float *x = a.x + (size_t)q.f0 * a.x_row;
@@ -191,15 +197,21 @@ __global__ __launch_bounds__(SSM_T) void ssm_token_kernel(SsmArgs A, int blocks,
         for (int j = 0; j < 4; j++) ssm_stnt(state + (size_t)i * RP * KD + 4 * P * j, S[i][j]);
 }
 
-/* The inputs of each request's last positions into its entries of `conv`. */
-__global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
+/* The inputs of a request's last positions into its entries of `conv`, four channels; of requests that go token by token. */
+__device__ __forceinline__ void ssm_conv_put(const SsmArgs &A, int r, int c)
 {
     SsmReq q;
-    const int r = blockIdx.y, c = 4 * (blockIdx.x * SSM_T + threadIdx.x), taps = A.s.taps;
-    if (!ssm_request(A, r, 0, 0, q, nullptr) || c >= A.channels) return;
+    const int taps = A.s.taps;
+    if (!ssm_request(A, r, 0, 0, q, nullptr) || q.n >= A.lim) return;
     for (int t = max(0, q.n - taps); t < q.n; t++)
         *(float4 *)(A.s.conv + ((size_t)r * taps + ((unsigned)q.pos + t) % taps) * A.channels + c) =
             gld_f4(A.a.x + (size_t)(q.f0 + t) * A.a.x_row + c);
+}
+
+__global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
+{
+    const int c = 4 * (blockIdx.x * SSM_T + threadIdx.x);
+    if (c < A.channels) ssm_conv_put(A, blockIdx.y, c);
 }
 
 /* ---- prompts: 64 tokens at a time -------------------------------------------------
@@ -248,12 +260,12 @@ struct SsmWs {
     __device__ static float *vec(char *head) { return (float *)(head + 2 * SSM_C * SSM_C * 4); }
 };
 
-/* Chunks of request r, 0 for one that is idle or left out. */
+/* Chunks of request r, 0 for one that is idle, left out or short. */
 __device__ __forceinline__ int ssm_chunks(const SsmArgs &A, int r)
 {
     if (r >= A.s.n_req) return 0;
     const int f0 = A.a.first[r], f1 = A.a.first[r + 1];
-    if (f0 < 0 || f1 <= f0 || f1 > A.a.rows || f1 - f0 > A.a.most || A.a.row_pos[f0] < 0) return 0;
+    if (f0 < 0 || f1 <= f0 || f1 > A.a.rows || f1 - f0 > A.a.most || f1 - f0 < A.lim || A.a.row_pos[f0] < 0) return 0;
     return (f1 - f0 + SSM_C - 1) / SSM_C;
 }
 
@@ -280,13 +292,23 @@ __device__ __forceinline__ int ssm_find(const SsmArgs &A, int c, int &of)
     return -1;
 }
 
-/* Chunks of the requests before r. */
-__device__ __forceinline__ int ssm_base(const SsmArgs &A, int r)
+/* The request that is number j of those with chunks, and the chunks of those before it; likewise. */
+__device__ __forceinline__ int ssm_nth(const SsmArgs &A, int j, int &base)
 {
-    int base = 0;
-    for (int r0 = threadIdx.x % 64; r0 < r; r0 += 64) base += ssm_chunks(A, r0);
-    for (int o = 1; o < 64; o <<= 1) base += __shfl_xor(base, o);
-    return base;
+    const int l = threadIdx.x % 64;
+    base = 0;
+    for (int r0 = 0; r0 < A.s.n_req; r0 += 64) {
+        const int n = ssm_chunks(A, r0 + l);
+        const unsigned long long some = __ballot(n > 0);
+        const unsigned long long hit = __ballot(n > 0 && __popcll(some & ((1ull << l) - 1)) == j);
+        const int at = hit ? __ffsll(hit) - 1 : 64;
+        int sum = l < at ? n : 0;
+        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+        base += sum;
+        if (hit) return r0 + at;
+        j -= __popcll(some);
+    }
+    return -1;
 }
 
 __device__ __forceinline__ bool ssm_finite(float x) { return fabsf(x) < INFINITY; }
@@ -625,13 +647,27 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         h = blockIdx.x % 8 * (VH / 8) + j / blocks;
         vb = j % blocks;
     }
-    const int r = blockIdx.y, kh = h / A.rep, nk = A.s.k_heads * KD, v0 = h * VD + vb * 16;
+    const int kh = h / A.rep, nk = A.s.k_heads * KD, v0 = h * VD + vb * 16;
+    int r = 0, base = 0;
+    if (A.s.n_req > 1) {
+        if (blockIdx.y == gridDim.y - 1) {              /* the short requests' `conv`, which ssm_token_kernel in front of this has read */
+            const int pieces = A.channels / 4;
+            for (int i = blockIdx.x * 2 * SSM_T + tid; i < A.s.n_req * pieces; i += gridDim.x * 2 * SSM_T)
+                ssm_conv_put(A, i / pieces, 4 * (i % pieces));
+            /* more long requests than rows would hold, so that some share them */
+            if (blockIdx.x == 0)
+                for (int j = gridDim.y - 1; (r = ssm_nth(A, j, base)) >= 0; j++) ssm_leave(A, A.a.first[r], A.a.first[r + 1], 0, VH * VD, err);
+            return;
+        }
+        r = __builtin_amdgcn_readfirstlane(ssm_nth(A, blockIdx.y, base));
+        base = __builtin_amdgcn_readfirstlane(base);
+        if (r < 0) return;
+    }
     SsmReq q;
     if (!ssm_request(A, r, v0, 16, q, err)) return;
-    const int base = __builtin_amdgcn_readfirstlane(ssm_base(A, r)), chunks = (q.n + SSM_C - 1) / SSM_C;
+    const int chunks = (q.n + SSM_C - 1) / SSM_C;
     if (base + chunks > max_chunks) {                   /* requests that share rows, so that `first` is none of a plan */
-        if (tid == 0) atomicOr(err, ATTN_ERR_SCAN);
-        for (int t = tid; t < q.n * 16; t += 2 * SSM_T) a.out[(size_t)(q.f0 + t / 16) * a.out_row + v0 + t % 16] = __uint_as_float(0x7FC00000u);
+        ssm_leave(A, q.f0, q.f0 + q.n, v0, 16, err);
         return;
     }
     const int v = l % 16, t4 = 16 * w + 4 * (l / 16);
@@ -931,23 +967,29 @@ static bool ssm_state_ok(const RoasterSsmState *s)
 
 static inline int ssm_channels(const RoasterSsmState *s) { return 2 * s->k_heads * s->k_dim + s->v_heads * s->v_dim; }
 
-/* From so many new tokens of a request on a call goes by chunks (us by chunks / by tokens, 32 heads of 128 x 128: one request
- * of 16 tokens 28.8 / 27.7, of 32 28.7 / 48; 16 requests of 16 tokens 139 / 74, of 32 137 / 131): fewer where a
- * token's workgroups leave most of the GPU idle. */
-#define SSM_CHUNK_FEW 20
-#define SSM_CHUNK_MIN 32
-static inline bool ssm_by_chunks(int most, const RoasterSsmState *s)
+/* Of a call with long requests those of fewer tokens go token by token, in a kernel in front (63 requests of one token and one of
+ * 256: 99 us, all by chunks 487; 15 and one of 256 58 / 134; with 32 here 89 and 54, but 30, 300, 700, 60 and 40 tokens 132
+ * instead of 96). */
+#define SSM_SHORT 24
+/* A call goes by chunks if a request may have so many new tokens, us by chunks / by tokens with 32 heads of 128 x 128: one
+ * request of 12 tokens 24 / 22, of 16 24 / 28; 4 of 20 47 / 41, of 24 47 / 47; 8 of 32 73 / 73; 16 of 32 138 / 131; 32 of 32
+ * 263 / 206.  A token's chain of waits is long where its workgroups leave most of the GPU idle, and chunks of few tokens do the
+ * work of 64 where it is full. */
+static inline int ssm_limit(const RoasterSsmState *s)
 {
-    return most >= SSM_CHUNK_MIN || (most >= SSM_CHUNK_FEW && s->n_req * s->v_heads <= 256);
+    const int blocks = s->n_req * s->v_heads;
+    if (s->n_req == 1 && blocks <= 64) return 16;
+    return blocks <= 128 ? SSM_SHORT : blocks <= 256 ? 32 : 40;
 }
 
-/* Chunks of a step at most: the last of each request may be short. */
-static inline int ssm_max_chunks(int rows, const RoasterSsmState *s) { return rows / SSM_C + (rows < s->n_req ? rows : s->n_req); }
+/* Chunks of a step at most: the last of each long request may be short. */
+static inline int ssm_max_long(int rows, const RoasterSsmState *s) { return s->n_req == 1 ? 1 : min(s->n_req, rows / SSM_SHORT); }
+static inline int ssm_max_chunks(int rows, const RoasterSsmState *s) { return rows / SSM_C + ssm_max_long(rows, s); }
 
 extern "C" size_t roaster_ssm_ws_bytes(int rows, int most, const RoasterSsmState *s)
 {
     if (!ssm_state_ok(s) || rows < 0 || rows > (1 << 18) || most < 1 || (rows && most > rows)) return 0;
-    if (most < SSM_CHUNK_FEW) return 16;
+    if (most < ssm_limit(s)) return 16;
     const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads };
     return (size_t)ssm_max_chunks(rows, s) * w.chunk_bytes();
 }
@@ -993,23 +1035,9 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
     const AttnDevice dev;
     int *err = rt_attn_err();
     if (!err) return ROASTER_EDEVICE;
-    SsmArgs A = { *p, *s, s->v_heads / s->k_heads, (int)ch };
+    const bool chunked = p->most >= ssm_limit(s);
+    SsmArgs A = { *p, *s, s->v_heads / s->k_heads, (int)ch, !chunked ? INT_MAX : n == 1 ? 1 : SSM_SHORT };
     A.a.b = b;
-    if (ssm_by_chunks(p->most, s)) {
-        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads };
-        const int chunks = ssm_max_chunks(p->rows, s), groups = (A.rep + SSM_HG - 1) / SSM_HG, blocks = s->v_dim / 16;
-#define CHUNK(KD, D)                                                                                                          \
-    do {                                                                                                                    \
-        hipLaunchKernelGGL((ssm_prep_kernel<KD, D>), dim3(chunks, s->k_heads * groups), dim3(2 * SSM_T), 0, rt().stream, A, W, \
-                           groups);                                                                                          \
-        hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, n), dim3(2 * SSM_T), 0, rt().stream, A, W, blocks,    \
-                           chunks, err);                                                                                    \
-    } while (0)
-        if (s->k_dim == 128) { if (delta) CHUNK(128, true); else CHUNK(128, false); }
-        else { if (delta) CHUNK(64, true); else CHUNK(64, false); }
-#undef CHUNK
-        return rt_check(hipGetLastError(), "ssm_chunk launch") ? ROASTER_EDEVICE : 0;
-    }
     const bool one = p->most == 1;
 #define TOKEN3(KD, VB, D, O)                                                                                              \
     hipLaunchKernelGGL((ssm_token_kernel<KD, VB, D, O>), dim3(vh * (s->v_dim / VB), n), dim3(SSM_T), 0, rt().stream, A,    \
@@ -1018,13 +1046,30 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
 #define TOKEN(KD, VB) do { if (delta) TOKEN2(KD, VB, true); else TOKEN2(KD, VB, false); } while (0)
     /* 32 value elements a workgroup while that fills the GPU no more than four times, else 64, for fewer reads of the
      * queries' and keys' channels (32 / 64: 4 requests 7.1 / 7.1 us, 16 15.3 / 12.0, 64 53.5 / 46.0; one 5.4 / 5.8) */
-    if (s->k_dim == 64) TOKEN(64, 64);
-    else if (n * ov / 32 >= 1024) TOKEN(128, 64);
-    else TOKEN(128, 32);
+    if (!chunked || n > 1) {
+        if (s->k_dim == 64) TOKEN(64, 64);
+        else if (n * ov / 32 >= 1024) TOKEN(128, 64);
+        else TOKEN(128, 32);
+    }
 #undef TOKEN
 #undef TOKEN2
 #undef TOKEN3
     if (rt_check(hipGetLastError(), "ssm_token launch")) return ROASTER_EDEVICE;
+    if (chunked) {
+        const SsmWs W = { (char *)p->ws, s->k_dim, s->k_heads, s->v_heads };
+        const int chunks = ssm_max_chunks(p->rows, s), groups = (A.rep + SSM_HG - 1) / SSM_HG, blocks = s->v_dim / 16;
+#define CHUNK(KD, D)                                                                                                          \
+    do {                                                                                                                    \
+        hipLaunchKernelGGL((ssm_prep_kernel<KD, D>), dim3(chunks, s->k_heads * groups), dim3(2 * SSM_T), 0, rt().stream, A, W, \
+                           groups);                                                                                          \
+        hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, ssm_max_long(p->rows, s) + (n > 1)), dim3(2 * SSM_T), 0, rt().stream, A, W, blocks,    \
+                           chunks, err);                                                                                    \
+    } while (0)
+        if (s->k_dim == 128) { if (delta) CHUNK(128, true); else CHUNK(128, false); }
+        else { if (delta) CHUNK(64, true); else CHUNK(64, false); }
+#undef CHUNK
+        return rt_check(hipGetLastError(), "ssm_chunk launch") ? ROASTER_EDEVICE : 0;
+    }
     if (!one) {
         hipLaunchKernelGGL(ssm_conv_kernel, dim3((ch / 4 + SSM_T - 1) / SSM_T, n), dim3(SSM_T), 0, rt().stream, A);
         if (rt_check(hipGetLastError(), "ssm_conv launch")) return ROASTER_EDEVICE;

@@ -212,10 +212,20 @@ def test_the_same_key_again_and_again(noise):
     log(check_scan(run(s), scan_oracle(s)))
 
 
-@pytest.mark.parametrize("most", [19, 20, 31, 32])
-@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("most", [15, 16, 23, 24, 31, 32, 39, 40])
+@pytest.mark.parametrize("n", [1, 2, 40, 70])
 def test_both_ways_about_their_limits(most, n):
     s = Scan(np.random.default_rng(most + n), [most] + [2] * (n - 1), [3] * n, DELTA, 2, 4, 128, 128)
+    log(check_scan(run(s), scan_oracle(s)))
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+@pytest.mark.parametrize("kd,vd", [(128, 64), (64, 128)])
+@pytest.mark.parametrize("new", [[1] * 20 + [90] + [1] * 60 + [0, 200], [64, 1, 0, 23, 24, 25, 2, 65], [0, 1, 100], [1] * 130 + [30]])
+def test_prompts_among_single_tokens(mode, kd, vd, new):
+    rng = np.random.default_rng(len(new) + kd)
+    pos = rng.integers(0, 5, len(new)).tolist()
+    s = Scan(rng, new, pos, mode, 2, 2, kd, vd, pad=3)
     log(check_scan(run(s), scan_oracle(s)))
 
 
@@ -232,16 +242,19 @@ def test_a_wider_output(new):
     check_scan((np.ascontiguousarray(out[:, :192]).reshape(s.rows, 3, 64), conv, state), scan_oracle(s))
 
 
-def test_requests_that_share_rows():
+@pytest.mark.parametrize("n", [4, 60])
+def test_requests_that_share_rows(n):
     """More tokens than rows: a request whose chunks have no place left is reported and its state stays as it was."""
-    s = Scan(np.random.default_rng(27), [640, 0, 0, 0], [2, 0, 0, 0], DELTA, 1, 1, 64, 64)
+    s = Scan(np.random.default_rng(27), [640] + [0] * (n - 1), [2] + [0] * (n - 1), DELTA, 1, 1, 64, 64)
     want = scan_oracle(s)
-    s.first = np.array([0, 640, 0, 640, 640], np.int32)
+    s.first = np.array([0, 640, 0, 640, 640] if n == 4 else [0, 640] + [0, 640] * 29 + [0], np.int32)
     c = ScanCall(s)
     R.check(c.call(), "scan")
     assert R.lib().roaster_sync() == R.EINVAL and "left out" in R.last_error()
     out, conv, state = c.got()
-    for r in (1, 2, 3):
+    # chunks of 64 rows, and one for each request that may have 24 rows of its own: of 14 chunks requests of ten find place once, of
+    # 36 three times (every second one: those between are out of range)
+    for r in [1, 2, 3] if n == 4 else [1, 3, 5] + list(range(6, n)):
         assert np.array_equal(state[r], s.state[r]) and np.array_equal(conv[r], s.conv[r])
     assert np.array_equal(conv[0].astype(np.float64), want[1][0])
     assert np.all(np.linalg.norm(state[0] - want[2][0], axis=2) <= want[4][0])
