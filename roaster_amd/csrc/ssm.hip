@@ -378,21 +378,62 @@ struct SsmSum {
     __device__ __forceinline__ f32x4 get() const { return hh + (hl + lh); }
 };
 
-/* RG rows of a channel of the convolution, from row j0 of a chunk of `width` rows at x on (x[0]: row i0 of its request). */
+/* Four channels of the convolution over RG rows, from row j0 of a chunk of `width` rows at x on (x[0]: row i0 of its request). */
 template <int RG>
-struct SsmConv {
-    SsmChannel cv;
-    float x[RG];
+struct SsmConv4 {
+    float4 w[4], bias, x[RG + 3];                       /* the last three are the rows before */
 
     __device__ __forceinline__ void load(const SsmArgs &A, int r, int pos, int c, const float *rows, int i0, int j0, int width)
     {
         const size_t stride = A.a.x_row;
-        cv.start(A, r, pos, c);
+        const int taps = A.s.taps;
 #pragma unroll
-        for (int j = 0; j < 3; j++)                     /* at least RG rows before */
-            if (i0 + j0) cv.h[j] = (rows + (ptrdiff_t)min(j0 - 3 + j, width - 1) * (ptrdiff_t)stride)[(unsigned)c];
+        for (int i = 0; i < RG; i++) x[i] = gld_f4(rows + (size_t)min(j0 + i, width - 1) * stride + (unsigned)c);
+        const float *hist = A.s.conv + (size_t)r * taps * A.channels + c;
 #pragma unroll
-        for (int i = 0; i < RG; i++) x[i] = (rows + (size_t)min(j0 + i, width - 1) * stride)[(unsigned)c];
+        for (int j = 0; j < 3; j++) {
+            const int back = 3 - j;                     /* positions behind the first of them; a request's rows are RG or more apart */
+            if (i0 + j0) x[RG + j] = gld_f4(rows + (ptrdiff_t)min(j0 - back, width - 1) * (ptrdiff_t)stride + (unsigned)c);
+            else x[RG + j] = back < taps && pos >= back ? gld_f4(hist + (size_t)((unsigned)(pos - back) % taps) * A.channels) : make_float4(0, 0, 0, 0);
+        }
+        bias = make_float4(0, 0, 0, 0);
+        if (A.a.conv_b) bias = make_float4(A.a.conv_b[c], A.a.conv_b[c + 1], A.a.conv_b[c + 2], A.a.conv_b[c + 3]);
+        const float *at = A.a.conv_w + (size_t)c * taps;          /* 4 * taps in a row */
+        const float4 zero = make_float4(0, 0, 0, 0), f0 = gld_f4(at), f1 = gld_f4(at + 4);
+        if (taps == 2) {
+            w[0] = w[1] = zero;
+            w[2] = make_float4(f0.x, f0.z, f1.x, f1.z);
+            w[3] = make_float4(f0.y, f0.w, f1.y, f1.w);
+            return;
+        }
+        const float4 f2 = gld_f4(at + 8);
+        if (taps == 3) {
+            w[0] = zero;
+            w[1] = make_float4(f0.x, f0.w, f1.z, f2.y);
+            w[2] = make_float4(f0.y, f1.x, f1.w, f2.z);
+            w[3] = make_float4(f0.z, f1.y, f2.x, f2.w);
+            return;
+        }
+        const float4 f3 = gld_f4(at + 12);
+        w[0] = make_float4(f0.x, f1.x, f2.x, f3.x);
+        w[1] = make_float4(f0.y, f1.y, f2.y, f3.y);
+        w[2] = make_float4(f0.z, f1.z, f2.z, f3.z);
+        w[3] = make_float4(f0.w, f1.w, f2.w, f3.w);
+    }
+    __device__ __forceinline__ static float4 mad(float4 u, float4 v, float4 c)
+    {
+        return make_float4(fmaf(u.x, v.x, c.x), fmaf(u.y, v.y, c.y), fmaf(u.z, v.z, c.z), fmaf(u.w, v.w, c.w));
+    }
+    /* row i; inputs of unused taps are not touched, since they may be infinite or NaN */
+    __device__ __forceinline__ float4 row(int i, int taps) const
+    {
+        auto in = [&](int k) { return k < 0 ? x[RG + 3 + k] : x[k]; };
+        float4 c = bias;
+        if (taps > 3) c = mad(w[0], in(i - 3), c);
+        if (taps > 2) c = mad(w[1], in(i - 2), c);
+        c = mad(w[2], in(i - 1), c);
+        c = mad(w[3], in(i), c);
+        return make_float4(ssm_silu(c.x), ssm_silu(c.y), ssm_silu(c.z), ssm_silu(c.w));
     }
 };
 
@@ -404,7 +445,7 @@ template <int KD, bool DELTA>
 __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs W, int groups)
 {
     constexpr int LD = KD + 4, LG = SSM_C + 4, KS = KD / 32, OPS = 4 * KS;           /* operands of Q, and of K */
-    constexpr int F0 = 2 * SSM_C * LD, F1 = (2 + SSM_HG) * SSM_C * LG, RQ = SSM_C * 2 * KD / (2 * SSM_T);
+    constexpr int F0 = 2 * SSM_C * LD, F1 = (2 + SSM_HG) * SSM_C * LG, RQ = SSM_C * (KD / 2) / (2 * SSM_T);
     __shared__ __attribute__((aligned(16))) float s_buf[F0 > F1 ? F0 : F1];
     __shared__ double s_G[SSM_HG][SSM_C];
     __shared__ float s_gain[SSM_HG][SSM_C], s_gl[SSM_HG][SSM_C], s_rq[SSM_C], s_rk[SSM_C], s_qf[SSM_C], s_kf[SSM_C];
@@ -422,9 +463,9 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
     float *s_q = s_buf, *s_k = s_buf + SSM_C * LD;
     if (tid == 0) s_bad = 0;
 
-    /* a channel a thread and RQ rows of it */
-    const int ch = tid % (2 * KD), j0 = __builtin_amdgcn_readfirstlane(tid / (2 * KD) * RQ);
-    SsmConv<RQ> cq;
+    /* four channels a thread and RQ rows of them */
+    const int ch = 4 * (tid % (KD / 2)), j0 = (KD == 128 ? w : tid / (KD / 2)) * RQ;
+    SsmConv4<RQ> cq;
     cq.load(A, r, pos, ch < KD ? kh * KD + ch : nk + kh * KD + ch - KD, x, i0, j0, width);
     if (w < heads) {                                    /* a token a lane */
         const bool in = l < width;
@@ -445,8 +486,8 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
         float *to = (ch < KD ? s_q + ch : s_k + ch - KD) + j0 * LD;
 #pragma unroll
         for (int i = 0; i < RQ; i++) {
-            const float y = cq.cv.next(cq.x[i], taps);
-            to[i * LD] = j0 + i < width ? y : 0.0f;
+            const float4 y = cq.row(i, taps);
+            *(float4 *)(to + i * LD) = j0 + i < width ? y : make_float4(0, 0, 0, 0);
         }
     }
     __syncthreads();
