@@ -674,7 +674,7 @@ template <int KD, bool DELTA>
 __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmWs W, int blocks, int max_chunks, int *err)
 {
     constexpr int KS = KD / 32, OPS = 4 * KS, LS = KD + 8, LT = SSM_C + 8, LV = SSM_C + 4;
-    __shared__ __attribute__((aligned(16))) _Float16 s_S[2][16 * LS], s_R[2][16 * LT], s_W[2][16 * LT], s_We[2][16 * LT];
+    __shared__ __attribute__((aligned(16))) _Float16 s_S[2][16 * LS], s_R[2][16 * LT], s_W[2][2][16 * LT], s_We[2][16 * LT];
     __shared__ __attribute__((aligned(16))) float s_V[2][16 * LV], s_top[2][16][4];
     __shared__ __attribute__((aligned(16))) char s_K[OPS * 2048];                /* K's operands as they are, read as K^T's */
     __shared__ float s_part[2][8][16];
@@ -847,15 +847,35 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             load_x(min(1, chunks - 1), xs);
         }
         load_one(0);
-        load_two(0);
+        if (first) load_two(0);
         float b = row_norm();
         float pS = ssm_pow2(b);                              /* |S| < 2 pS; as an operand times 2^13 / pS, so below 2^14 */
         put_S(8192.0f * ssm_inv2(pS));
         __syncthreads();
 
         float *out = a.out + (size_t)(q.f0 + t4) * a.out_row + v0 + v;               /* this lane's four tokens in turn */
+        /* A chunk's outputs are finished while the first group works on the next W: what does not need W, and the factors of D W */
+        f32x4 part = {}, by = {};
+        bool open = false;
+        auto close = [&](int c, int n) {
+            SsmSum sum;
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+                if (s <= w / 2) sum.add(two[s], op(s_W[c & 1][0], LT, s));
+            const f32x4 O = part + by * sum.get();
+            float *at = out + (ptrdiff_t)c * SSM_C * (ptrdiff_t)a.out_row;
+            if (n >= SSM_C) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) __builtin_nontemporal_store(O[i], at + i * a.out_row);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (t4 + i < n) at[i * a.out_row] = O[i];
+            }
+            open = false;
+        };
         if (first) __builtin_amdgcn_s_setprio(1);            /* the other group waits for it */
-        for (int c = 0; c < chunks; c++, out += SSM_C * a.out_row) {
+        for (int c = 0; c < chunks; c++) {
             const int c1 = min(c + 1, chunks - 1);
             const f32x4 tops = *(const f32x4 *)s_top[c & 1][v], V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -866,6 +886,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             if (!bad) {
                 /* bounds: of R, of W, and of the next S */
                 const float bR = top + b, bW = DELTA ? b + 65.0f * top : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
+                const float back = pW * (1 / (8192.0f * SSM_UP));
                 f32x4 X = {};
                 if (DELTA || !first) {
                     SsmSum sum;
@@ -877,7 +898,8 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
 #pragma unroll
                     for (int s = 0; s < KS; s++) ssm_st(s_K + (w * KS + s) * 2048, l, one[s]);
                 }
-                if (first) load_one(c1);
+                load_one(c1);
+                if (!first && c + 1 < chunks) values(c + 1, xs);
                 if (DELTA) {
                     if (first) ssm_split4(V - o.f * X, 8192.0f * ssm_inv2(pR), s_R[0] + v * LT + t4, s_R[1] + v * LT + t4);
                     __syncthreads();
@@ -891,15 +913,18 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                             if (s <= w / 2) sum.add(two[s], op(s_R[0], LT, s));
                         w4 = sum.get() * (pR * (1 / (8192.0f * SSM_UP)));
                     } else w4 = o.gain * V;
-                    ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[0] + v * LT + t4, s_W[1] + v * LT + t4);
+                    ssm_split4(w4, 8192.0f * ssm_inv2(pW), s_W[c & 1][0] + v * LT + t4, s_W[c & 1][1] + v * LT + t4);
                     ssm_split4(o.g * w4, 8192.0f * ssm_inv2(pW), s_We[0] + v * LT + t4, s_We[1] + v * LT + t4);
                 } else {
-                    load_one(c1);
-                    if (c + 1 < chunks) values(c + 1, xs);
                     load_x(min(c + 2, chunks - 1), xs);
+                    if (open) close(c - 1, SSM_C);
+                    load_two(c);
+                    part = o.f * X;
+                    if (a.skip) part = part + skip * V;
+                    by = o.g * back;
+                    open = true;
                 }
                 __syncthreads();
-                const float back = pW * (1 / (8192.0f * SSM_UP));
                 if (holds) {
                     SsmSum sum;
 #pragma unroll
@@ -909,25 +934,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
                 pS = ssm_pow2(b);
                 put_S(8192.0f * ssm_inv2(pS));
-                if (!first) {
-                    SsmSum sum;
-#pragma unroll
-                    for (int s = 0; s < 2; s++)
-                        if (s <= w / 2) sum.add(two[s], op(s_W[0], LT, s));
-                    f32x4 O = o.f * X + o.g * (sum.get() * back);
-                    if (a.skip) O = O + skip * V;
-                    if ((c + 1) * SSM_C <= q.n) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) __builtin_nontemporal_store(O[i], out + i * a.out_row);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (c * SSM_C + t4 + i < q.n) out[i * a.out_row] = O[i];
-                    }
-                }
-                load_two(c1);
+                if (first) load_two(c1);
                 load_head(c1, next);
             } else {
+                if (!first && open) close(c - 1, SSM_C);
                 /* token by token, so that an infinite or NaN input does not reach those before it */
                 const char *key = W.key(base + c, kh);
                 const float *vec = W.vec(W.head(base + c, h));
@@ -964,7 +974,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                         so = 0;
                         for (int i = 0; i < KD / 16; i++) so += s_part[1][i][v];
                         so *= vec[SSM_QF + t];
-                        out[(size_t)t * a.out_row] = a.skip ? fmaf(skip, val, so) : so;     /* threads 0 .. 15: t4 = 0 */
+                        out[(size_t)(c * SSM_C + t) * a.out_row] = a.skip ? fmaf(skip, val, so) : so;     /* threads 0 .. 15: t4 = 0 */
                     }
                     __syncthreads();
                 }
@@ -977,11 +987,12 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 }
                 load_head(c1, next);
                 load_one(c1);
-                load_two(c1);
+                if (first) load_two(c1);
             }
             o = next;
             __syncthreads();
         }
+        if (!first && open) close(chunks - 1, q.n - (chunks - 1) * SSM_C);
         if (holds) *(f32x4 *)state = S;
     };
     if (w8 < 4) run(std::true_type());
