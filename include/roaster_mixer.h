@@ -36,8 +36,8 @@ extern "C" {
  *   q = y * 127 / max|y|, rounded to nearest even, and q_scale = max|y| / 127
  * A row whose largest |y| is below 2^-119 has scale and values 0; a row with an
  * infinite or NaN y has scale NaN and values 0.  Sums are in f32.  A row's results
- * are the same whatever the other rows, except that how its sum is ordered goes by
- * rows and cols.  y may be x (with the same stride); nothing else may overlap.
+ * are the same whatever the other rows.  A row whose squares pass f32's range gives
+ * zeros.  y may be x (with the same stride); nothing else may overlap.
  * rows = 0 does nothing. */
 typedef struct {
     int rows;                 /* 0 .. 2^20 */
@@ -87,8 +87,8 @@ int roaster_i8_pack(const void *W, int from, const RoasterI8 *to);
 
 /* y[t][r] = x_scale[t] * scale[r] * sum_c x[t][c] * value[r][c]
  * for rows tokens x of 8-bit values (roaster_norm's q and q_scale).  The sums are exact
- * (32-bit integers); the product with the two scales, which are multiplied first, is rounded as f32.  An infinite or NaN
- * scale reaches its row or channel alone.  Outputs must not overlap inputs.  rows = 0 does
+ * (32-bit integers); the product with the two scales, which are multiplied first, is rounded as
+ * f32.  An infinite or NaN scale reaches its row or channel alone.  Outputs must not overlap inputs.  rows = 0 does
  * nothing. */
 typedef struct {
     int rows;                 /* 0 .. 2^20 */
@@ -127,12 +127,17 @@ typedef struct {
  *   STATE:  S = d S + dt v k^T
  *   out = scale * S q  (+ skip * v)
  * Rows from first[n_req] on stay as they were, and so do the states of requests without new
- * tokens.  States, sums and decays are in f32 (sums of a_coef * dt in 64 bits).  Infinite or NaN
- * inputs reach their request's rows from their own on, and its states, and no other's.  a_coef * dt must be
- * finite.  A request whose rows are not within 0 .. rows, whose position is negative or that
- * has more than `most` new tokens is left out, its rows NaN where they are within 0 .. rows and its states as they
- * were, and reported by roaster_sync (ROASTER_EINVAL).  What kernels run goes by rows, most
- * and n_req; last bits of a row depend on them, and are the same for the same call.
+ * tokens.  States, sums and decays are in f32 (sums of a_coef * dt in 64 bits).  Of requests of many
+ * tokens 64 are taken at a time; beside f32's own errors theirs are up to 2^-32 of the largest |v|
+ * and row of S among them.  With eps = 0 queries and keys whose sum of squares is 0 in f32 give NaN.
+ * Infinite or NaN inputs reach their request's rows from their own on, and its states, and no
+ * other's.  a_coef * dt must be finite; where it is positive a prompt goes token by token.
+ * A request whose rows are not within 0 .. rows, whose position is negative or that has more than
+ * `most` new tokens is left out, its rows NaN where they are within 0 .. rows and its states as they
+ * were, and reported by roaster_sync (ROASTER_EINVAL).  Requests' rows must not overlap (those of a
+ * plan never do): rows that several claim are any of theirs, and what does not fit the workspace is
+ * left out like this.  What kernels run goes by rows, most, n_req and v_heads and by each request's
+ * own number of tokens; last bits of a row depend on them, and are the same for the same call.
  * rows = 0 does nothing. */
 typedef struct {
     int rows;                 /* 0 .. 262144 */

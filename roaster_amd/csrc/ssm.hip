@@ -100,7 +100,10 @@ __device__ __forceinline__ void ssm_stnt(float *p, float4 v) { __builtin_nontemp
  * registers (KD / 16 lanes a row, 16 elements each).  The queries' and keys' channels are convolved by every
  * workgroup of the head: 2 KD inputs next to VB * KD states.
  * ONE: no request has more than one row, so the entry of `conv` that it fills is none that it reads, and the workgroup writes
- * it; else ssm_conv_kernel does behind this kernel. */
+ * it; else ssm_conv_kernel or ssm_chunk_kernel does behind this kernel.
+ * What bounds it: with one request of 32 heads of 128 x 128 (5.3 us) a launch and the chain position, inputs, sums, state,
+ * with 58 of them (42 us) memory, 254 MB at 6.0 TB/s.  Of several tokens each costs 1.3 us, the chain of the exchange in LDS,
+ * the two dot products and their sums over lanes. */
 template <int KD, int VB, bool DELTA, bool ONE>
 __global__ __launch_bounds__(SSM_T) void ssm_token_kernel(SsmArgs A, int blocks, int *err)
 {
@@ -439,8 +442,9 @@ struct SsmConv4 {
 
 /* A chunk's tokens of one key head: convolution, norms, the products among tokens, and of SSM_HG of its value
  * heads the decays and T, whose 16 x 16 blocks on the diagonal are inverted by substitution, a column a lane,
- * and joined by products in f32 (T_rc = - T_rr sum_k A_rk T_kc), a wave having a block c of columns.  What bounds it: at 2048 tokens and 16 key heads
- * two workgroups fill a CU and all run at once, so their chain of waits. */
+ * and joined by products in f32 (T_rc = - T_rr sum_k A_rk T_kc), a wave having a block c of columns.  What bounds it: of 29 us for 2048 tokens
+ * and 16 key heads (two workgroups a CU, all at once) about 9 are its 94 MB beyond what one workgroup alone needs, 20 us: inputs
+ * 6, the solve 5, decays 4, outputs 3, products and silu 2 each, a chain of waits with few waves to fill them. */
 template <int KD, bool DELTA>
 __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs W, int groups)
 {
@@ -557,7 +561,8 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if ((DELTA || !keys) && b <= m4)
-                (keys ? s_kk : s_qk)[(16 * m4 + 4 * (l / 16) + i) * LG + 16 * b + l % 16] = kk[b].get()[i] * (keys ? 1 / (SSM_UP * SSM_UP) : 1 / SSM_UP);
+                (keys ? s_kk : s_qk)[(16 * m4 + 4 * (l / 16) + i) * LG + 16 * b + l % 16] =
+                    kk[b].get()[i] * (keys ? 1 / (SSM_UP * SSM_UP) : 1 / SSM_UP);
     __syncthreads();
     /* decays, four waves a head: row block w / 2 of D o Q K^T as an operand, and of A */
     const int hh = w % SSM_HG, m = w / SSM_HG, h = h0 + hh;
@@ -669,7 +674,11 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
  * from S to W, the second makes the outputs and the next chunk's values; token rows 16 (w % 4) .. each, and each wave has 16
  * key elements of S.  S stays in registers as the products leave it (key elements 16 w + 4 (l/16) + i) and
  * in LDS as they take it.  Operands of the next chunk are loaded while this one is worked on, without conditions, so that
- * waits count those under way exactly. */
+ * waits count those under way exactly.  The second group is a step behind: it makes the next chunk's values before the first
+ * barrier and finishes the last chunk's outputs before the second, so that neither barrier waits for it (82 -> 77 us).
+ * What bounds it: 2048 tokens of 32 heads of 128 x 128 take 77 us, 32 chunks of 2.4 us one after another (2.0 if nothing
+ * comes from memory): K S, T R and K^T W wait for each other, with a split into parts, LDS and a barrier between, and LDS
+ * passes 200 KB a chunk, some 1600 cycles of 128 bytes.  Two workgroups a CU would need 128 registers a wave, which spills (prompt 99 -> 211 us). */
 template <int KD, bool DELTA>
 __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmWs W, int blocks, int max_chunks, int *err)
 {
@@ -679,7 +688,8 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     __shared__ __attribute__((aligned(16))) char s_K[OPS * 2048];                /* K's operands as they are, read as K^T's */
     __shared__ float s_part[2][8][16];
     const RoasterSsmScan &a = A.a;
-    const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;    /* so that operands' addresses are scalar */
+    /* the wave's number from the first lane, so that operands' addresses are scalar */
+    const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;
     const int taps = A.s.taps, VD = A.s.v_dim, VH = A.s.v_heads;
     /* with a multiple of 8 heads, those of one key head and their blocks on one XCD (workgroup b runs on b % 8) */
     int h = blockIdx.x / blocks, vb = blockIdx.x % blocks;
@@ -879,13 +889,14 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             const int c1 = min(c + 1, chunks - 1);
             const f32x4 tops = *(const f32x4 *)s_top[c & 1][v], V = *(const f32x4 *)(s_V[c & 1] + v * LV + t4);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            /* the wave's lanes have all 16 elements, with the same bounds in every wave */
-            const float all = b + 128.0f * fmaxf(1.0f, o.most) * top;
+            /* the wave's lanes have all 16 elements.  Both groups have to come to the same bounds, bit by bit, so their roundings are
+             * written out and not left to the compiler */
+            const float all = fmaf(128.0f * fmaxf(1.0f, o.most), top, b);
             const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
             const float last = o.last;
             if (!bad) {
                 /* bounds: of R, of W, and of the next S */
-                const float bR = top + b, bW = DELTA ? b + 65.0f * top : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
+                const float bR = top + b, bW = DELTA ? fmaf(65.0f, top, b) : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
                 const float back = pW * (1 / (8192.0f * SSM_UP));
                 f32x4 X = {};
                 if (DELTA || !first) {
@@ -931,7 +942,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     for (int s = 0; s < 2; s++) sum.add(key_cols(s), op(s_We[0], LT, s));
                     S = S * last + sum.get() * back;
                 }
-                b = last * b + 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top);
+                b = fmaf(last, b, 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top));
                 pS = ssm_pow2(b);
                 put_S(8192.0f * ssm_inv2(pS));
                 if (first) load_two(c1);
@@ -949,8 +960,9 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                         const char *at = key + (t / 16 * KS + k / 32) * 2048 + (t % 16 + 16 * (k % 32 / 8)) * 16 + k % 8 * 2;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            qf[i] = ((float)((const _Float16 *)at)[i] + (float)((const _Float16 *)(at + 1024))[i]) * (1 / SSM_UP);
-                            kf[i] = ((float)((const _Float16 *)(at + OPS * 2048))[i] + (float)((const _Float16 *)(at + OPS * 2048 + 1024))[i]) * (1 / SSM_UP);
+                            const _Float16 *aq = (const _Float16 *)at + i, *ak = (const _Float16 *)(at + OPS * 2048) + i;
+                            qf[i] = ((float)aq[0] + (float)aq[512]) * (1 / SSM_UP);
+                            kf[i] = ((float)ak[0] + (float)ak[512]) * (1 / SSM_UP);
                         }
                     }
                     float wt = gain * val;
@@ -1019,14 +1031,14 @@ static bool ssm_state_ok(const RoasterSsmState *s)
 
 static inline int ssm_channels(const RoasterSsmState *s) { return 2 * s->k_heads * s->k_dim + s->v_heads * s->v_dim; }
 
-/* Of a call with long requests those of fewer tokens go token by token, in a kernel in front (63 requests of one token and one of
- * 256: 99 us, all by chunks 487; 15 and one of 256 58 / 134; with 32 here 89 and 54, but 30, 300, 700, 60 and 40 tokens 132
- * instead of 96). */
+/* Of a call with long requests those of fewer tokens go token by token, in a kernel in front, us with 24 / 32 / 2 here and 32
+ * heads of 128 x 128: 63 requests of one token and one of 256 100 / 91 / 146, 15 of four and one of 128 62 / 60 / 143; of 30, 300,
+ * 700, 60 and 40 tokens 93 / 131 / 93.  (All by chunks, single tokens too, 487, 136 and 92.) */
 #define SSM_SHORT 24
-/* A call goes by chunks if a request may have so many new tokens, us by chunks / by tokens with 32 heads of 128 x 128: one
- * request of 12 tokens 24 / 22, of 16 24 / 28; 4 of 20 47 / 41, of 24 47 / 47; 8 of 32 73 / 73; 16 of 32 138 / 131; 32 of 32
- * 263 / 206.  A token's chain of waits is long where its workgroups leave most of the GPU idle, and chunks of few tokens do the
- * work of 64 where it is full. */
+/* A call goes by chunks if a request may have so many new tokens, us by chunks / by tokens: one request of 12 tokens 23 / 22,
+ * of 16 23 / 28; 4 of 20 49 / 42, of 24 50 / 48; 8 of 32 78 / 73; 16 of 32 144 / 131; 32 of 24 279 / 160, of 32 277 / 207.  A
+ * token's chain of waits is long where its workgroups leave most of the GPU idle, and chunks of few tokens do the work of 64
+ * where it is full. */
 static inline int ssm_limit(const RoasterSsmState *s)
 {
     const int blocks = s->n_req * s->v_heads;
@@ -1096,8 +1108,8 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
                        s->v_dim / VB, err)
 #define TOKEN2(KD, VB, D) do { if (one) TOKEN3(KD, VB, D, true); else TOKEN3(KD, VB, D, false); } while (0)
 #define TOKEN(KD, VB) do { if (delta) TOKEN2(KD, VB, true); else TOKEN2(KD, VB, false); } while (0)
-    /* 32 value elements a workgroup while that fills the GPU no more than four times, else 64, for fewer reads of the
-     * queries' and keys' channels (32 / 64: 4 requests 7.1 / 7.1 us, 16 15.3 / 12.0, 64 53.5 / 46.0; one 5.4 / 5.8) */
+    /* 32 value elements a workgroup while that fills the GPU no more than four times, else 64, for fewer reads of the queries' and
+     * keys' channels (32 / 64: one request 5.6 / 6.2 us, 4 7.1 / 7.1, 8 8.5 / 8.4, 16 15.4 / 12.4, 64 52.8 / 46.1) */
     if (!chunked || n > 1) {
         if (s->k_dim == 64) TOKEN(64, 64);
         else if (n * ov / 32 >= 1024) TOKEN(128, 64);
@@ -1114,8 +1126,8 @@ extern "C" int roaster_ssm_scan(const RoasterSsmScan *p, const RoasterSsmState *
     do {                                                                                                                    \
         hipLaunchKernelGGL((ssm_prep_kernel<KD, D>), dim3(chunks, s->k_heads * groups), dim3(2 * SSM_T), 0, rt().stream, A, W, \
                            groups);                                                                                          \
-        hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, ssm_max_long(p->rows, s) + (n > 1)), dim3(2 * SSM_T), 0, rt().stream, A, W, blocks,    \
-                           chunks, err);                                                                                    \
+        hipLaunchKernelGGL((ssm_chunk_kernel<KD, D>), dim3(vh * blocks, ssm_max_long(p->rows, s) + (n > 1)), dim3(2 * SSM_T), 0,    \
+                           rt().stream, A, W, blocks, chunks, err);                                                          \
     } while (0)
         if (s->k_dim == 128) { if (delta) CHUNK(128, true); else CHUNK(128, false); }
         else { if (delta) CHUNK(64, true); else CHUNK(64, false); }
