@@ -92,7 +92,7 @@ struct I8Args {
 
 __device__ __forceinline__ i32x4 i8_ld(const void *p) { return *(const GAS i32x4 *)p; }
 
-/* Up to 32 tokens: a workgroup takes 16 channels, its waves a part of the columns each and join in LDS
+/* Few results: a workgroup takes 16 channels of up to 32 tokens, its waves a part of the columns each and join in LDS
  * (integers, so in any order).  Weights go from memory straight into v_mfma_i32_16x16x64_i8 (lane l: row l%16, columns
  * 16*(l/16) ..; results 4*(l/16) + i, i = 0..3, of token l%16), tokens too, from the L2; eight steps' loads are issued together.
  * Padded columns of the weights are zeros, so any byte of the token may stand there.
@@ -103,13 +103,13 @@ __global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a)
 {
     __shared__ int s_sum[TT * 16 * 16];                /* [token][channel] */
     const int tid = threadIdx.x, l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), W = blockDim.x / 64;
-    const int k0 = a.k32 / 2 * w / W, k1 = a.k32 / 2 * (w + 1) / W, n16 = a.n16;
+    const int k0 = a.k32 / 2 * w / W, k1 = a.k32 / 2 * (w + 1) / W, n16 = a.n16, t0 = 16 * TT * blockIdx.y;
     const int8_t *wp = a.w + (size_t)(blockIdx.x / 2) * a.k32 * 1024 + blockIdx.x % 2 * 256;
     const unsigned off = l / 16 * 512 + l % 16 * 16;
     const int8_t *xp[TT];
 #pragma unroll
-    for (int t = 0; t < TT; t++) xp[t] = a.x + min(16 * t + l % 16, a.T - 1) * a.x_row;
-    const int tok = tid / 16, ch = blockIdx.x * 16 + tid % 16;
+    for (int t = 0; t < TT; t++) xp[t] = a.x + min(t0 + 16 * t + l % 16, a.T - 1) * a.x_row;
+    const int tok = t0 + tid / 16, ch = blockIdx.x * 16 + tid % 16;
     const float ws = a.ws[min(ch, a.N - 1)];
     float xs[TT];                                      /* of the first 256 threads' tokens tok + 16 t */
 #pragma unroll
@@ -337,12 +337,16 @@ extern "C" int roaster_matmul_i8(const RoasterMatmulI8 *p, const RoasterI8 *w)
     const AttnDevice dev;
     I8Args a = { (const int8_t *)w->data, p->x, w->scale, p->x_scale, p->y, p->x_row, p->y_row, p->rows, w->rows, w->cols / 16,
                  (int)(i8_cols(w->cols) / 32) };
-    if (T <= 32) {
+    /* Up to 256 workgroups of 32 tokens by 16 channels go by those, whose columns four waves share, and not by tiles, which have
+     * a longer chain of steps (33 tokens, 2048 x 2048 4.6 us, by tiles 6.8; 64 of 2048 x 4096 7.1 / 10.5; 256 of 512 x 2048 4.6 /
+     * 6.8, of 300 x 512 4.5 / 4.4); with more of them a CU has two in turn (333 of 512 x 2048 6.6 / 6.8, of 1111 x 2064 9.7 / 7.5) */
+    const size_t blocks = ((T + 31) / 32) * ((N + 15) / 16);
+    if (T <= 32 || blocks <= 256) {
         /* four waves to 16 channels (8 tokens, 12288 x 2048: 6.0 us, with eight 7.4, sixteen 14.6), eight for long
          * columns (one token, 256 x 16384: 6.1 us, with four 7.2) */
         const int waves = K <= 8192 ? 4 : 8;
         if (T <= 16) hipLaunchKernelGGL(i8_few_kernel<1>, dim3((N + 15) / 16), dim3(64 * waves), 0, rt().stream, a);
-        else hipLaunchKernelGGL(i8_few_kernel<2>, dim3((N + 15) / 16), dim3(64 * waves), 0, rt().stream, a);
+        else hipLaunchKernelGGL(i8_few_kernel<2>, dim3((N + 15) / 16, (T + 31) / 32), dim3(64 * waves), 0, rt().stream, a);
     } else {
         auto tiles = [&](int tb, int cb) { return ((T + 32 * tb - 1) / (32 * tb)) * ((N + 128 * cb - 1) / (128 * cb)); };
 #define TILE(TB, CB, U)                                                                                                    \
