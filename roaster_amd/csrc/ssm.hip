@@ -240,9 +240,9 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
 #define SSM_C 64                 /* tokens of a chunk */
 #define SSM_HG 2                 /* value heads of a workgroup of ssm_prep_kernel */
 #define SSM_UP 256.0f            /* Q, K, T and D o Q K^T as operands */
-/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; then the largest gain,
- * and 1 where the chunk has to go token by token. */
-enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_MOST = 384, SSM_BAD = 385, SSM_VEC = 448 };
+/* A token's: exp(G) * qf, qf (scale, and Q's power of two), exp(G), exp(G_63 - G), gain, a_coef dt; then 1 where the chunk has
+ * to go token by token. */
+enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_BAD = 384, SSM_VEC = 448 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
@@ -592,8 +592,6 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
             float *vec = W.vec(out);
             const double G = s_G[hh][l];
             const float gl = s_gl[hh][l], eg = ssm_exp((float)G), qf = s_qf[l], gain = s_gain[hh][l] * (DELTA ? 1.0f : s_kf[l]);
-            float top = gain;
-            for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
             vec[SSM_EQ + l] = eg * qf;
             vec[SSM_QF + l] = qf;
             vec[SSM_EG + l] = eg;
@@ -601,10 +599,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
             vec[SSM_GAIN + l] = gain;
             vec[SSM_GL + l] = gl;
             const bool bad = __any(!ssm_finite(gl) || gl > 0.0f || !ssm_finite(gain)) || s_bad;
-            if (l == 0) {
-                vec[SSM_MOST] = top;
-                vec[SSM_BAD] = bad ? 1.0f : 0.0f;
-            }
+            if (l == 0) vec[SSM_BAD] = bad ? 1.0f : 0.0f;
         }
     }
     __syncthreads();
@@ -737,7 +732,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         struct Head {
             f32x4 f, g;                                     /* exp(G) and exp(G_63 - G), or the outputs' factors */
             f32x4 gain;
-            float last, most, bad;
+            float last, bad;
         };
         auto load_head = [&](int c, Head &o) {
             char *head = W.head(base + c, h);
@@ -747,7 +742,6 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             if (!DELTA) o.gain = *(const f32x4 *)(vec + SSM_GAIN + t4);
             const __attribute__((address_space(4))) float *same = (const __attribute__((address_space(4))) float *)vec;      /* scalar loads */
             o.last = same[SSM_EG + SSM_C - 1];
-            o.most = same[SSM_MOST];
             o.bad = same[SSM_BAD];
         };
         auto load_one = [&](int c) {
@@ -774,8 +768,10 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             }
             return o;
         };
-        /* the inputs of this lane's four tokens of chunk c and the three before */
+        /* the inputs of this lane's four tokens of chunk c and the three before; STATE: their gains, for the largest gain |v| */
+        f32x4 gains = {};
         auto load_x = [&](int c, float (&xs)[7]) {
+            if (!DELTA) gains = *(const f32x4 *)(W.vec(W.head(base + c, h)) + SSM_GAIN + t4);
             const int i0 = c * SSM_C + 16 * w - 3;
             if (i0 >= 0 && i0 + 19 <= q.n) {
 #pragma unroll
@@ -786,7 +782,8 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     xs[j] = x0[(size_t)min(max(i0 + 4 * (l / 16) + j, 0), q.n - 1) * a.x_row];
             }
         };
-        /* their values to LDS, and the largest of each element: infinite where one is infinite or NaN */
+        /* their values to LDS, and the largest of each element (STATE: of a token's gain times its value, since the largest of both
+         * can be those of different tokens): infinite where one is infinite or NaN */
         auto values = [&](int c, const float (&xs)[7]) {
             float xx[7];
 #pragma unroll
@@ -810,7 +807,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 V[i] = c * SSM_C + t4 + i < q.n ? ssm_silu(V[i]) : 0.0f;
-                top = max(top, __float_as_uint(V[i]) & 0x7FFFFFFFu);
+                top = max(top, __float_as_uint(DELTA ? V[i] : gains[i] * V[i]) & 0x7FFFFFFFu);
             }
             const auto far = __builtin_amdgcn_permlane32_swap(top, top, false, false);
             top = max(far[0], far[1]);
@@ -891,12 +888,12 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             /* the wave's lanes have all 16 elements.  Both groups have to come to the same bounds, bit by bit, so their roundings are
              * written out and not left to the compiler */
-            const float all = fmaf(128.0f * fmaxf(1.0f, o.most), top, b);
+            const float all = fmaf(128.0f, top, b);
             const bool bad = __any(o.bad != 0.0f || !(all < 0x1p120f));
             const float last = o.last;
             if (!bad) {
                 /* bounds: of R, of W, and of the next S */
-                const float bR = top + b, bW = DELTA ? fmaf(65.0f, top, b) : o.most * top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
+                const float bR = top + b, bW = DELTA ? fmaf(65.0f, top, b) : top, pR = ssm_pow2(bR), pW = ssm_pow2(bW);
                 const float back = pW * (1 / (8192.0f * SSM_UP));
                 f32x4 X = {};
                 if (DELTA || !first) {
@@ -942,7 +939,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     for (int s = 0; s < 2; s++) sum.add(key_cols(s), op(s_We[0], LT, s));
                     S = S * last + sum.get() * back;
                 }
-                b = fmaf(last, b, 64.0f * 1.0001f * (DELTA ? top : 2.0f * o.most * top));
+                b = fmaf(last, b, (DELTA ? 1.0f : 1.5f) * 64.0f * 1.0001f * top);
                 pS = ssm_pow2(b);
                 put_S(8192.0f * ssm_inv2(pS));
                 if (first) load_two(c1);
