@@ -232,9 +232,11 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
  *   D[m][n]: lane l holds m = 4*(l/16) + i, n = l%16, i = 0..3
  * Q and K are unit vectors (STATE: powers of two bring their largest element to 1/16 .. 1/8, their norms so below 1.5, K's
  * going into dt and Q's into the output), so they, D o Q K^T and T are at most 4 in size and enter times 2^8.  S, R and W enter
- * times a power of two for each value element, from bounds that need no look at them: the norm of an element's
- * row of S is at most b and grows by the sum of gain |v| |k| alone, |R| <= |v| + b, |w| <= |v| + |S|.  fp16's
- * range below the bound (2^-38 of it) leaves 22 bits where the bound is 2^15 too large.  That takes decays
+ * times a power of two for each value element, from bounds that no product waits for: the norm of an element's
+ * row of S is at most b, which a chunk makes of the norm before it (summed while the chunk runs: a bound carried from the
+ * request's first chunk on keeps what the correction takes out of S again) and the sum of gain |v| |k|; |R| <= |v| + b, |w| <= |v| + |S|.
+ * fp16's range below the bound (2^-38 of it) leaves 22 bits where the bound is 2^15 too large; the bounds are at most
+ * 130 times the largest |v| and row of S among the chunk's and the 64 tokens before.  That takes decays
  * of at most 1: a chunk with a positive a_coef dt, or with an infinite or NaN input, goes token by token.
  * Tokens behind a request's last are zeros with gain 0 and the decay of the last. */
 #define SSM_C 64                 /* tokens of a chunk */
@@ -682,6 +684,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
     __shared__ __attribute__((aligned(16))) float s_V[2][16 * LV], s_top[2][16][4];
     __shared__ __attribute__((aligned(16))) char s_K[OPS * 2048];                /* K's operands as they are, read as K^T's */
     __shared__ float s_part[2][8][16];
+    __shared__ __attribute__((aligned(16))) float s_norm[2][16][8];              /* squares of an element's row of S, a wave's part each; of even and of odd chunks */
     const RoasterSsmScan &a = A.a;
     /* the wave's number from the first lane, so that operands' addresses are scalar */
     const int tid = threadIdx.x, l = tid % 64, w8 = __builtin_amdgcn_readfirstlane(tid / 64), w = w8 % 4;
@@ -820,8 +823,26 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
             const _Float16 *at = p + v * ld + 32 * s + 8 * (l / 16);
             return SsmOp{ *(const h16x8 *)at, *(const h16x8 *)(at + 16 * ld) };
         };
-        auto put_S = [&](float by) {
-            if (holds) ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
+        /* chunk c's S as an operand, and the sum of its squares as such */
+        auto put_S = [&](int c, float by) {
+            if (!holds) return;
+            ssm_split4(S, by, s_S[0] + v * LS + 16 * w8 + 4 * (l / 16), s_S[1] + v * LS + 16 * w8 + 4 * (l / 16));
+            const f32x4 U = S * by;
+            float sum = U[0] * U[0] + U[1] * U[1] + U[2] * U[2] + U[3] * U[3];
+            const auto far = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+            sum = __uint_as_float(far[0]) + __uint_as_float(far[1]);
+            const auto near = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+            sum = __uint_as_float(near[0]) + __uint_as_float(near[1]);
+            if (l < 16) s_norm[c & 1][l][w8] = sum;
+        };
+        /* The norm of the element's row of the S that put_S had with 8192 / p, no less (squares below f32's range are less than 2^-56
+         * p together); p's own bound may be far above it.  Roundings are written out, see below.  It is read where it is used, while
+         * other waves put the next chunk's: read at the chunk's beginning, which would spare the second buffer, it holds up the loads
+         * under way (2048 tokens 109 us instead of 99). */
+        auto norm_S = [&](int c, float p) {
+            f32x4 sum = *(const f32x4 *)s_norm[c & 1][v];
+            if (KD == 128) sum += *(const f32x4 *)(s_norm[c & 1][v] + 4);
+            return fmaf(__builtin_amdgcn_sqrtf((sum[0] + sum[1]) + (sum[2] + sum[3])), p * (1.0001f / 8192.0f), p * 0x1p-56f);
         };
 
         /* The norm of the element's row of S, no less; squares of small states would leave f32's range. */
@@ -857,7 +878,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
         if (first) load_two(0);
         float b = row_norm();
         float pS = ssm_pow2(b);                              /* |S| < 2 pS; as an operand times 2^13 / pS, so below 2^14 */
-        put_S(8192.0f * ssm_inv2(pS));
+        put_S(0, 8192.0f * ssm_inv2(pS));
         __syncthreads();
 
         float *out = a.out + (size_t)(q.f0 + t4) * a.out_row + v0 + v;               /* this lane's four tokens in turn */
@@ -939,9 +960,9 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                     for (int s = 0; s < 2; s++) sum.add(key_cols(s), op(s_We[0], LT, s));
                     S = S * last + sum.get() * back;
                 }
-                b = fmaf(last, b, (DELTA ? 1.0f : 1.5f) * 64.0f * 1.0001f * top);
+                b = fmaf(last, fminf(b, norm_S(c, pS)), (DELTA ? 1.0f : 1.5f) * 64.0f * 1.0001f * top);
                 pS = ssm_pow2(b);
-                put_S(8192.0f * ssm_inv2(pS));
+                put_S(c + 1, 8192.0f * ssm_inv2(pS));
                 if (first) load_two(c1);
                 load_head(c1, next);
             } else {
@@ -989,7 +1010,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 }
                 b = row_norm();
                 pS = ssm_pow2(b);
-                put_S(8192.0f * ssm_inv2(pS));
+                put_S(c + 1, 8192.0f * ssm_inv2(pS));
                 if (!first) {
                     if (c + 1 < chunks) values(c + 1, xs);
                     load_x(min(c + 2, chunks - 1), xs);

@@ -87,6 +87,20 @@ def slow(rng, n, mode, coef=-2e-4, **kw):
     return s
 
 
+@pytest.mark.parametrize("coef", [-2e-4, 0.0])
+@pytest.mark.parametrize("early,by", [(1, 1e6), (64, 1e5)])
+def test_large_values_at_the_beginning(early, by, coef):
+    """Keys of one direction after the other, so that the correction takes the large values out of the state within a thousand
+    tokens; those behind have the precision of their own values."""
+    s = slow(np.random.default_rng(31), 4096, DELTA, coef, taps=2, bias=False)
+    s.x[:early, 256:] *= np.float32(by)
+    s.conv_w[:, 0], s.conv_w[:, 1] = 0, 1
+    s.x[:, 128:256] = 0.1 * s.x[:, 128:256] - 8
+    s.x[np.arange(4096), 128 + np.arange(4096) % 128] += 16
+    s.b[:] = 2 + 0.1 * s.b
+    compare(s, [(0, 256), (3072, 4096)])
+
+
 @pytest.mark.parametrize("early,by", [(1, 1e6), (64, 1e5)])
 def test_large_values_that_decay(early, by):
     """Without the correction: e^-0.01 a token."""
