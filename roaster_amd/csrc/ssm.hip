@@ -479,7 +479,9 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
         const int h = h0 + w;
         const float dt = ssm_softplus(a.a[row * a.a_row + h] + (a.dt_bias ? a.dt_bias[h] : 0.0f));
         const float gl = in ? a.a_coef[h] * dt : 0.0f;
-        double G = gl;
+        /* e^-256 is 0 in f32 as is all below it, and a sum that holds such a token alone would lose the decays behind it: of 64
+         * tokens no more than 2^14, so that their differences keep 38 bits behind the point */
+        double G = fmaxf(gl, -256.0f);
         for (int o = 1; o < 64; o <<= 1) {
             const double v = __shfl_up(G, o);
             if (l >= o) G += v;

@@ -1,6 +1,6 @@
 """How near roaster_ssm_scan's prompts, taken 64 tokens at a time, come to the recurrence in 64 bits
 where a bound of the state could leave the state behind: long prompts without decay, values far above
-the ones that follow, steps and values that peak at different tokens.
+the ones that follow, steps and values that peak at different tokens, decays that wipe a state out.
 
 Each is held to the plain recurrence in f32 on the same inputs: the error over a span of tokens is at most
 eight of its errors (operands of 22 bits to f32's 24, whose products leave out up to another 2^-20) and
@@ -12,7 +12,7 @@ import pytest
 import roaster_amd as R
 from attn_util import sync
 from gpu_util import log
-from mixer_util import Scan, ScanCall, sigmoid
+from mixer_util import Scan, ScanCall, check_scan, scan_oracle, sigmoid
 
 pytestmark = pytest.mark.gpu
 DELTA, STATE = R.SCAN_DELTA, R.SCAN_STATE
@@ -123,3 +123,22 @@ def test_steps_and_values_that_peak_at_different_tokens(coef):
     s.x[::2, 256:] *= np.float32(0.01)
     s.x[1::2, 256:] *= np.float32(1e4)
     compare(s, [(0, 64), (1024, 2048)])
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+@pytest.mark.parametrize("a", [300.0, 1e13, 1e17, 1e20, 1e36])
+def test_a_token_that_wipes_the_state_out(mode, a):
+    """A step of 1e13 and more leaves nothing of the state before it; the tokens behind it decay as ever.  STATE: without a
+    value of its own, which such a step would put far above all others."""
+    s = Scan(np.random.default_rng(35), [100, 40], [0, 4], mode, 2, 4, 64, 64, taps=2, bias=False, dt_bias=False)
+    s.a[:], s.a_coef[:] = 0.1 * s.a - 2, -0.8                # e^-0.1 a token
+    for at in (9, 10, 70, 108):
+        s.a[at] = np.float32(a)
+        if mode == STATE:
+            s.x[at - 1:at + 1, 2 * 2 * 64:] = 0
+    call = ScanCall(s)
+    R.check(call.call(), "scan")
+    sync()
+    with np.errstate(over="ignore"):
+        want = scan_oracle(s)
+    log(check_scan(call.got(), want))
