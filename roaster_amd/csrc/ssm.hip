@@ -247,6 +247,7 @@ __global__ __launch_bounds__(SSM_T) void ssm_conv_kernel(SsmArgs A)
 enum { SSM_EQ = 0, SSM_QF = 64, SSM_EG = 128, SSM_EC = 192, SSM_GAIN = 256, SSM_GL = 320, SSM_BAD = 384, SSM_VEC = 448 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
@@ -327,17 +328,25 @@ __device__ __forceinline__ float ssm_pow2(float x, int lo = 27, int hi = 250)
 __device__ __forceinline__ float ssm_top(float top, float x) { return __uint_as_float(max(__float_as_uint(top), __float_as_uint(x) & 0x7FFFFFFFu)); }
 __device__ __forceinline__ float ssm_inv2(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }   /* 1 / 2^e */
 
+/* Rounded to nearest, so that the low parts are as often negative and no larger than half a step of the high ones: the
+ * product of two of them, which is left out, is at most 2^-22 of the whole and on average nothing.  (Cut off, which is as fast, it is
+ * up to 2^-20 and always of the whole's sign.) */
+__device__ __forceinline__ h16x2 ssm_half2(float x, float y)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector((f32x2){ x, y }, h16x2);
+}
 struct SsmOp { h16x8 hi, lo; };                         /* one lane's of an operand */
 __device__ __forceinline__ SsmOp ssm_split(const float (&v)[8])
 {
     SsmOp o;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {                    /* the high part cut off: two at a time; what is left is exact in f32 */
-        const auto h = __builtin_amdgcn_cvt_pkrtz(v[i], v[i + 1]);
-        o.hi[i] = (_Float16)h[0];
-        o.hi[i + 1] = (_Float16)h[1];
-        o.lo[i] = (_Float16)(v[i] - (float)o.hi[i]);
-        o.lo[i + 1] = (_Float16)(v[i + 1] - (float)o.hi[i + 1]);
+    for (int i = 0; i < 8; i += 2) {                    /* two at a time; what the high part leaves is exact in f32 */
+        const h16x2 h = ssm_half2(v[i], v[i + 1]), r = ssm_half2(v[i] - (float)h[0], v[i + 1] - (float)h[1]);
+        o.hi[i] = h[0];
+        o.hi[i + 1] = h[1];
+        o.lo[i] = r[0];
+        o.lo[i + 1] = r[1];
     }
     return o;
 }
@@ -347,11 +356,11 @@ __device__ __forceinline__ void ssm_split4(f32x4 v, float by, _Float16 *hi, _Flo
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
         const float x = v[i] * by, y = v[i + 1] * by;
-        const auto p = __builtin_amdgcn_cvt_pkrtz(x, y);
-        h[i] = (_Float16)p[0];
-        h[i + 1] = (_Float16)p[1];
-        r[i] = (_Float16)(x - (float)h[i]);
-        r[i + 1] = (_Float16)(y - (float)h[i + 1]);
+        const h16x2 p = ssm_half2(x, y), q = ssm_half2(x - (float)p[0], y - (float)p[1]);
+        h[i] = p[0];
+        h[i + 1] = p[1];
+        r[i] = q[0];
+        r[i + 1] = q[1];
     }
     *(h16x4 *)hi = h;
     *(h16x4 *)lo = r;

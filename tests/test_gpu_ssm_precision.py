@@ -3,7 +3,7 @@ where a bound of the state could leave the state behind: long prompts without de
 the ones that follow, steps and values that peak at different tokens, decays that wipe a state out.
 
 Each is held to the plain recurrence in f32 on the same inputs: the error over a span of tokens is at most
-eight of its errors (operands of 22 bits to f32's 24, whose products leave out up to another 2^-20) and
+eight of its errors (operands of 22 bits to f32's 24, whose products leave out up to another 2^-22) and
 FINE times the largest |v| and row of the state in the span.  FINE: an operand's lowest bit is 2^-30 of those,
 and a row's error sums up to 128 elements' or 64 tokens', which do not all point one way: 16 of them."""
 import numpy as np
@@ -142,3 +142,20 @@ def test_a_token_that_wipes_the_state_out(mode, a):
     with np.errstate(over="ignore"):
         want = scan_oracle(s)
     log(check_scan(call.got(), want))
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
+def test_roundings_do_not_lean_to_one_side(mode):
+    """What the products of operands in two parts leave out must not have the product's sign: the errors' mean along the outputs.
+    The part of it that f32 itself has is that of constants (log2 e is off by 2^-26 of itself, in exponentials of about -2 .. 2)
+    and of the reciprocal's last bit: below 2^-24 together; what is left of a million roundings that go either way is far
+    below.  With high parts cut off a single product leans by (2^-11 * 0.7)^2, 2^-23, and outputs come through three in a row."""
+    s = Scan(np.random.default_rng(36), [2048], [0], mode, 1, 4, 128, 128, skip=False)
+    call = ScanCall(s)
+    R.check(call.call(), "scan")
+    sync()
+    out = call.got()[0].astype(np.float64)
+    o, _, _ = recurrence(s, np.float64)
+    lean = ((out - o) * o).sum(axis=(0, 2)) / (o * o).sum(axis=(0, 2))
+    log("errors along the outputs:", lean, "all of them:", np.linalg.norm(out - o) / np.linalg.norm(o))
+    assert np.all(np.abs(lean) <= 2.0 ** -23)
