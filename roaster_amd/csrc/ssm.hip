@@ -1082,7 +1082,7 @@ static inline int ssm_max_chunks(int rows, const RoasterSsmState *s) { return ro
 extern "C" size_t roaster_ssm_ws_bytes(int rows, int most, const RoasterSsmState *s)
 {
     if (!ssm_state_ok(s) || rows < 0 || rows > (1 << 18) || most < 1 || (rows && most > rows)) return 0;
-    if (most < ssm_limit(s)) return 16;
+    if (!rows || most < ssm_limit(s)) return 16;
     const SsmWs w = { NULL, s->k_dim, s->k_heads, s->v_heads };
     return (size_t)ssm_max_chunks(rows, s) * w.chunk_bytes();
 }

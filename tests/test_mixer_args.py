@@ -154,3 +154,10 @@ def test_workspace_is_checked_and_grows():
 def test_bytes_of_weights():
     assert R.lib().roaster_i8_bytes(1, 16) == 32 * 128 and R.lib().roaster_i8_bytes(33, 144) == 64 * 256
     assert R.lib().roaster_i8_bytes(1 << 20, 65536) == 1 << 36
+
+
+@pytest.mark.parametrize("most", [1, 16, 64, 4096])
+@pytest.mark.parametrize("n_req", [1, 8, 2048])
+def test_a_workspace_for_no_rows(n_req, most):
+    """A step without rows is a good one, whatever `most`: 0 bytes would say that its arguments are bad."""
+    assert R.lib().roaster_ssm_ws_bytes(0, most, C.byref(state(n_req=n_req))) > 0
