@@ -130,7 +130,8 @@ typedef struct {
  * tokens.  States, sums and decays are in f32 (sums of a_coef * dt in 64 bits).  Of requests of many
  * tokens 64 are taken at a time, by products whose operands have 22 bits and none below 2^-30 of the largest
  * |v| (STATE: |dt v| |k|) and row of S among them and the 64 tokens before: within eight times the error of the
- * same steps in f32 and 2^-26 of those.  With eps = 0 queries and keys whose sum of squares is 0 in f32 give NaN.
+ * same steps in f32 and 2^-26 of those.  A query or key whose sum of squares passes f32's range is a zero vector (DELTA);
+ * with eps = 0 those whose sum is 0 in f32 give NaN.
  * Infinite or NaN inputs reach their request's rows from their own on, and its states, and no
  * other's.  a_coef * dt must be finite; where it is positive a prompt goes token by token.
  * A request whose rows are not within 0 .. rows, whose position is negative or that has more than

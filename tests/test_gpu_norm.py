@@ -131,3 +131,25 @@ def test_odd_values(D, group):
     R.check(n.call(), "norm")
     sync()
     assert not n.q.get().any() and not n.scale.get().any() and np.all(n.y.get() == 2.0 ** -125)
+
+
+@pytest.mark.parametrize("D,group", [(256, 256), (512, 64)])
+def test_rows_whose_squares_pass_the_range_are_zeros(D, group):
+    """The residual is added all the same; other rows, and a row's other heads, come out as without it."""
+    rng = np.random.default_rng(D + 1)
+    x, r = (rng.standard_normal((4, D)).astype(np.float32) for _ in range(2))
+    x[1, :group] = np.float32(3e19)
+    n = Norm(x, group, r, q=True)
+    R.check(n.call(), "norm")
+    sync()
+    v = x + r
+    assert np.array_equal(n.d["res"].get(), v)
+    y, k, s = n.y.get(), n.q.get(), n.scale.get()
+    fine = np.ones((4, D), bool)
+    fine[1, :group] = False
+    with np.errstate(over="ignore"):
+        want = norm_oracle(v, group, None, None, EPS)
+    near(y[fine], want[fine])
+    assert not y[~fine].any() and not k[~fine].any()
+    kk, ss = eights(y)
+    assert np.array_equal(k, kk) and np.array_equal(s, ss)

@@ -159,3 +159,23 @@ def test_roundings_do_not_lean_to_one_side(mode):
     lean = ((out - o) * o).sum(axis=(0, 2)) / (o * o).sum(axis=(0, 2))
     log("errors along the outputs:", lean, "all of them:", np.linalg.norm(out - o) / np.linalg.norm(o))
     assert np.all(np.abs(lean) <= 2.0 ** -23)
+
+
+@pytest.mark.parametrize("new", [[2, 1], [70, 33]])
+def test_vectors_whose_squares_pass_the_range_are_zeros(new):
+    """Key head 0's keys of one row and key head 1's queries of another are above 1e19: as if they were zeros, in both kernels."""
+    s = Scan(np.random.default_rng(37), new, [0, 4], DELTA, 2, 4, 128, 128, taps=2, bias=False)
+    s.conv_w[:512, 0], s.conv_w[:512, 1] = 0, 1
+    rows = (new[0] - 1, new[0])
+    parts = (slice(256, 384), slice(128, 256))
+    for row, part in zip(rows, parts):
+        s.x[row, part] = 0                                 # silu(0) = 0
+    want = scan_oracle(s)
+    for row, part in zip(rows, parts):
+        s.x[row, part] = np.float32(3e19)
+    call = ScanCall(s)
+    R.check(call.call(), "scan")
+    sync()
+    out, conv, state = call.got()
+    assert np.all(np.abs(out - want[0]) <= want[3] + 1e-30)
+    assert np.all(np.linalg.norm(state - want[2], axis=3) <= want[4] + 1e-30)
