@@ -43,7 +43,8 @@ __device__ __forceinline__ float q6k_weight(const uint8_t *blk, int i)
     return f16_bits_to_f32(gld_u16(blk + 208)) * sc * (float)((lo | hi << 4) - 32);
 }
 
-/* One workgroup a row of the padded matrix; 16 columns a thread at a time. */
+/* One workgroup a row of the padded matrix; 16 columns a thread at a time.  Once a matrix, so left simple: 12288 x 2048 from
+ * f32 40 us, Q4_K 80, Q6_K 46, int8 23; 2048 x 4096 from Q4_K 31. */
 template <int FROM>
 __global__ __launch_bounds__(I8_T) void i8_pack_kernel(const uint8_t *W, RoasterI8 to, int padded)
 {
@@ -97,7 +98,7 @@ __device__ __forceinline__ i32x4 i8_ld(const void *p) { return *(const GAS i32x4
  * 16*(l/16) ..; results 4*(l/16) + i, i = 0..3, of token l%16), tokens too, from the L2; eight steps' loads are issued together.
  * Padded columns of the weights are zeros, so any byte of the token may stand there.
  * What bounds it: a launch and one chain of loads for a small matrix (2048 x 4096 3.8 us), memory for a large one (12288 x 2048
- * 5.9 us, 4.3 TB/s all in all, of which a launch is 2 us). */
+ * 6.1 us, 4.2 TB/s all in all, of which a launch is 2 us). */
 template <int TT>
 __global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a)
 {
@@ -162,9 +163,11 @@ __device__ __forceinline__ void i8_put(const I8Args &a, int tok, int ch, f32x4_a
  * two waves read the same weights, which go from the L2 straight into registers, and only the tokens pass through LDS, a
  * step of U times 64 columns at a time, doubly buffered; both are loaded two steps ahead.  Pieces of 16 bytes of a token
  * are exchanged by (token / 2) % 4, so that eight lanes' reads fall on different banks.  Outputs of the larger tiles are
- * not kept in the caches (2048 tokens of 12288 x 2048: 62 us, kept 72).
- * What bounds it: 2048 tokens of 12288 x 2048 run at 1750 TOPS (59 us; the library's product of 8192^3 at 2105), 100 MB of
- * outputs among them; 256 tokens (12.4 us) are 384 tiles for 256 CUs, each with its first loads and its outputs at the ends. */
+ * not kept in the caches, whatever their size: 2048 tokens of 12288 x 2048 by themselves 60 us, kept 70, 256 tokens 14.6 / 15.1,
+ * 200 of 8192 x 2048 9.9 / 10.4; with the scan and the norm that read them behind it, a whole recurrent layer, 2048 tokens
+ * 247 / 249, 256 tokens 76 / 76.
+ * What bounds it: 2048 tokens of 12288 x 2048 run at 1720 TOPS (60 us; the library's product of 8192^3 at 2105), 100 MB of
+ * outputs among them; 256 tokens (12 .. 14.6 us) are 384 tiles for 256 CUs, each with its first loads and its outputs at the ends. */
 template <int TB, int CB, int U>
 __global__ __launch_bounds__(I8_T, 2) void i8_tile_kernel(I8Args a, int tiles, int per, int tblocks)
 {
@@ -338,11 +341,11 @@ extern "C" int roaster_matmul_i8(const RoasterMatmulI8 *p, const RoasterI8 *w)
     I8Args a = { (const int8_t *)w->data, p->x, w->scale, p->x_scale, p->y, p->x_row, p->y_row, p->rows, w->rows, w->cols / 16,
                  (int)(i8_cols(w->cols) / 32) };
     /* Up to 256 workgroups of 32 tokens by 16 channels go by those, whose columns four waves share, and not by tiles, which have
-     * a longer chain of steps (33 tokens, 2048 x 2048 4.6 us, by tiles 6.8; 64 of 2048 x 4096 7.1 / 10.5; 256 of 512 x 2048 4.6 /
-     * 6.8, of 300 x 512 4.5 / 4.4); with more of them a CU has two in turn (333 of 512 x 2048 6.6 / 6.8, of 1111 x 2064 9.7 / 7.5) */
+     * a longer chain of steps (33 tokens, 2048 x 2048 5.0 us, by tiles 6.7; 64 of 2048 x 4096 7.1 / 10.3; 256 of 512 x 2048 5.0 /
+     * 6.8, of 300 x 512 4.5 / 4.4); with more of them a CU has two in turn (333 of 512 x 2048 6.6 / 6.8, of 1111 x 2064 9.9 / 7.4) */
     const size_t blocks = ((T + 31) / 32) * ((N + 15) / 16);
     if (T <= 32 || blocks <= 256) {
-        /* four waves to 16 channels (8 tokens, 12288 x 2048: 6.0 us, with eight 7.4, sixteen 14.6), eight for long
+        /* four waves to 16 channels (8 tokens, 12288 x 2048: 6.1 us, with eight 7.4, sixteen 14.6), eight for long
          * columns (one token, 256 x 16384: 6.1 us, with four 7.2) */
         const int waves = K <= 8192 ? 4 : 8;
         if (T <= 16) hipLaunchKernelGGL(i8_few_kernel<1>, dim3((N + 15) / 16), dim3(64 * waves), 0, rt().stream, a);
@@ -357,8 +360,8 @@ extern "C" int roaster_matmul_i8(const RoasterMatmulI8 *p, const RoasterI8 *w)
     } while (0)
         /* The largest tiles read least from the L2, which bounds the others (8 .. 9 TB/s), but need enough of them:
          * us with 4 x 2 / 2 x 1 / 1 x 1, and how many there are:
-         *   12288 x 2048: 2048 tokens 61 / 74 / 119 (768), 1200 37 / 46 / 65 (480), 700 31 / 30 / 40 (288 / 1056)
-         *   8192 x 2048:  100 tokens 21 / 9.5 / 8.0 (.. / 256), 200 22 / 9.9 / 11.7 (.. / 448)
+         *   12288 x 2048: 2048 tokens 60 / 75 / 116 (768), 1200 37 / 44 / 62 (480), 700 31 / 29 / 39 (288 / 1056)
+         *   8192 x 2048:  100 tokens 19 / 9.5 / 7.8 (.. / 256), 200 19 / 10.1 / 11.3 (.. / 448)
          * 4 x 1 and 2 x 2, and two or four groups of waves that share the columns, never came first by more than a tenth. */
         if (tiles(4, 2) >= 384) TILE(4, 2, 1);
         else if (tiles(1, 1) <= 256) TILE(1, 1, 4);

@@ -10,8 +10,9 @@
 
 /* A row is a workgroup's, V times four elements a thread, all of it in registers between the sum and the
  * outputs: x, res and gate are read once.  Heads of 16 .. 256 elements lie in 4 .. 64 neighbouring lanes of one wave.
- * What bounds it: a launch up to some hundred rows (one row of 2048 3.5 us), then memory: 2048 rows of 32 heads of 128
- * with a gate 18.1 us, 5.6 TB/s of a copy's 4.9.  STREAM: y past the caches (22.7 us without). */
+ * What bounds it: a launch up to some hundred rows (one row of 2048 3.7 us a call, 2.5 of them the kernel), then memory: 2048
+ * rows of 32 heads of 128 with a gate 18.1 us, 5.6 TB/s, where a copy past the caches makes 6.0 .. 6.3.  STREAM: y past the
+ * caches (22.7 us without). */
 template <int V, bool STREAM>
 __global__ __launch_bounds__(NORM_T) void norm_kernel(RoasterNorm a)
 {

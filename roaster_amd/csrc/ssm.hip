@@ -101,7 +101,7 @@ __device__ __forceinline__ void ssm_stnt(float *p, float4 v) { __builtin_nontemp
  * workgroup of the head: 2 KD inputs next to VB * KD states.
  * ONE: no request has more than one row, so the entry of `conv` that it fills is none that it reads, and the workgroup writes
  * it; else ssm_conv_kernel or ssm_chunk_kernel does behind this kernel.
- * What bounds it: with one request of 32 heads of 128 x 128 (5.3 us) a launch and the chain position, inputs, sums, state,
+ * What bounds it: with one request of 32 heads of 128 x 128 (5.0 .. 5.6 us) a launch and the chain position, inputs, sums, state,
  * with 58 of them (42 us) memory, 254 MB at 6.0 TB/s.  Of several tokens each costs 1.3 us, the chain of the exchange in LDS,
  * the two dot products and their sums over lanes. */
 template <int KD, int VB, bool DELTA, bool ONE>
@@ -453,7 +453,7 @@ struct SsmConv4 {
 
 /* A chunk's tokens of one key head: convolution, norms, the products among tokens, and of SSM_HG of its value
  * heads the decays and T, whose 16 x 16 blocks on the diagonal are inverted by substitution, a column a lane,
- * and joined by products in f32 (T_rc = - T_rr sum_k A_rk T_kc), a wave having a block c of columns.  What bounds it: of 29 us for 2048 tokens
+ * and joined by products in f32 (T_rc = - T_rr sum_k A_rk T_kc), a wave having a block c of columns.  What bounds it: of 30 us for 2048 tokens
  * and 16 key heads (two workgroups a CU, all at once) about 9 are its 94 MB beyond what one workgroup alone needs, 20 us: inputs
  * 6, the solve 5, decays 4, outputs 3, products and silu 2 each, a chain of waits with few waves to fill them. */
 template <int KD, bool DELTA>
@@ -684,7 +684,7 @@ __global__ __launch_bounds__(2 * SSM_T, 4) void ssm_prep_kernel(SsmArgs A, SsmWs
  * in LDS as they take it.  Operands of the next chunk are loaded while this one is worked on, without conditions, so that
  * waits count those under way exactly.  The second group is a step behind: it makes the next chunk's values before the first
  * barrier and finishes the last chunk's outputs before the second, so that neither barrier waits for it (82 -> 77 us).
- * What bounds it: 2048 tokens of 32 heads of 128 x 128 take 77 us, 32 chunks of 2.4 us one after another (2.0 if nothing
+ * What bounds it: 2048 tokens of 32 heads of 128 x 128 take 78 us, 32 chunks of 2.4 us one after another (2.0 if nothing
  * comes from memory): K S, T R and K^T W wait for each other, with a split into parts, LDS and a barrier between, and LDS
  * passes 200 KB a chunk, some 1600 cycles of 128 bytes.  Two workgroups a CU would need 128 registers a wave, which spills (prompt 99 -> 211 us). */
 template <int KD, bool DELTA>
@@ -978,7 +978,7 @@ __global__ __launch_bounds__(2 * SSM_T, 2) void ssm_chunk_kernel(SsmArgs A, SsmW
                 load_head(c1, next);
             } else {
                 if (!first && open) close(c - 1, SSM_C);
-                /* token by token, so that an infinite or NaN input does not reach those before it */
+                /* token by token in f32 (q and k from their operands), so that an infinite or NaN input does not reach those before it */
                 const char *key = W.key(base + c, kh);
                 const float *vec = W.vec(W.head(base + c, h));
                 for (int t = 0; t < min(SSM_C, q.n - c * SSM_C); t++) {
@@ -1067,7 +1067,10 @@ static inline int ssm_channels(const RoasterSsmState *s) { return 2 * s->k_heads
 /* A call goes by chunks if a request may have so many new tokens, us by chunks / by tokens: one request of 12 tokens 23 / 22,
  * of 16 23 / 28; 4 of 20 49 / 42, of 24 50 / 48; 8 of 32 78 / 73; 16 of 32 144 / 131; 32 of 24 279 / 160, of 32 277 / 207.  A
  * token's chain of waits is long where its workgroups leave most of the GPU idle, and chunks of few tokens do the work of 64
- * where it is full. */
+ * where it is full.  That is with 32 heads of 128 x 128; the lines hold within a seventh for the others: 64 x 64 (keys x values)
+ * one request of 12 20 / 22, 4 of 20 31 / 34, of 24 31 / 39, 8 of 28 46 / 45, of 32 46 / 50, 16 of 32 72 / 61, of 40 73 / 74, 32 of 40
+ * 127 / 98; 64 x 128 one of 16 26 / 28, 4 of 24 43 / 40, 8 of 32 68 / 60, 16 of 40 120 / 98; 128 x 64 one of 12 23 / 23, 4 of 20 37 / 34,
+ * of 24 36 / 40, 8 of 28 52 / 54, 16 of 40 88 / 88, 32 of 40 157 / 159. */
 static inline int ssm_limit(const RoasterSsmState *s)
 {
     const int blocks = s->n_req * s->v_heads;
