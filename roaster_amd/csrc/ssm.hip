@@ -40,11 +40,9 @@ __device__ __forceinline__ bool ssm_request(const SsmArgs &A, int r, int col, in
     const RoasterSsmScan &a = A.a;
     const int f0 = a.first[r], f1 = a.first[r + 1];
     if (f0 == f1) return false;
-    q.f0 = f0;
-    q.n = f1 - f0;
-    q.pos = -1;
+    /* differences only of numbers that are known to be rows: of others they can leave an int's range */
     if (f0 >= 0 && f1 > f0 && f1 <= a.rows && f1 - f0 <= a.most) {
-        q.pos = a.row_pos[f0];
+        q = { f0, f1 - f0, a.row_pos[f0] };
         if (q.pos >= 0) return true;
     }
     if (err) ssm_leave(A, f0, f1, col, width, err);

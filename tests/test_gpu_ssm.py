@@ -258,3 +258,18 @@ def test_requests_that_share_rows(n):
         assert np.array_equal(state[r], s.state[r]) and np.array_equal(conv[r], s.conv[r])
     assert np.array_equal(conv[0].astype(np.float64), want[1][0])
     assert np.all(np.linalg.norm(state[0] - want[2][0], axis=2) <= want[4][0])
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_rows_at_the_ends_of_an_int(n):
+    """Differences of such rows do not fit an int: 2^31 - 1 to -2^31 would be one row."""
+    s = Scan(np.random.default_rng(28), [n, 0, 0, 0], [3, 1, 2, 4], DELTA, 2, 2, 64, 64, pad=3)
+    want = scan_oracle(s)
+    s.first = np.array([0, n, 2 ** 31 - 1, -2 ** 31, 0], np.int64).astype(np.int32)
+    c = ScanCall(s)
+    R.check(c.call(), "scan")
+    assert R.lib().roaster_sync() == R.EINVAL and "left out" in R.last_error()
+    out, conv, state = c.got()
+    assert np.all(np.abs(out[:n] - want[0][:n]) <= want[3][:n] + 1e-30) and np.isnan(out[n:]).all()
+    assert np.array_equal(conv.astype(np.float64), want[1]) and np.array_equal(state[1:], s.state[1:])
+    assert np.all(np.linalg.norm(state[0] - want[2][0], axis=2) <= want[4][0] + 1e-30)
