@@ -110,6 +110,16 @@ def test_large_values_that_decay(early, by):
 
 
 @pytest.mark.parametrize("mode", [DELTA, STATE])
+@pytest.mark.parametrize("at", [64, 100, 127])
+def test_a_large_value_in_the_middle(mode, at):
+    """It takes bits from the 64 tokens that it is taken with and from the next 64, from none before them."""
+    s = slow(np.random.default_rng(38), 256, mode, -2e-4, taps=2, bias=False)
+    s.conv_w[256:, 0], s.conv_w[256:, 1] = 0, 1
+    s.x[at, 256:] *= np.float32(1e6)
+    compare(s, [(0, 64), (64, at), (at, 128), (128, 192)] if at > 64 else [(0, 64), (64, 128), (128, 192)])
+
+
+@pytest.mark.parametrize("mode", [DELTA, STATE])
 def test_a_long_prompt_without_decay(mode):
     compare(slow(np.random.default_rng(33), 20000, mode, 0.0), [(0, 64), (19000, 20000)])
 
