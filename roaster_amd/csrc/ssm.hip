@@ -1065,15 +1065,16 @@ static inline int ssm_channels(const RoasterSsmState *s) { return 2 * s->k_heads
 /* A call goes by chunks if a request may have so many new tokens, us by chunks / by tokens: one request of 12 tokens 23 / 22,
  * of 16 23 / 28; 4 of 20 49 / 42, of 24 50 / 48; 8 of 32 78 / 73; 16 of 32 144 / 131; 32 of 24 279 / 160, of 32 277 / 207.  A
  * token's chain of waits is long where its workgroups leave most of the GPU idle, and chunks of few tokens do the work of 64
- * where it is full.  That is with 32 heads of 128 x 128; the lines hold within a seventh for the others: 64 x 64 (keys x values)
- * one request of 12 20 / 22, 4 of 20 31 / 34, of 24 31 / 39, 8 of 28 46 / 45, of 32 46 / 50, 16 of 32 72 / 61, of 40 73 / 74, 32 of 40
- * 127 / 98; 64 x 128 one of 16 26 / 28, 4 of 24 43 / 40, 8 of 32 68 / 60, 16 of 40 120 / 98; 128 x 64 one of 12 23 / 23, 4 of 20 37 / 34,
- * of 24 36 / 40, 8 of 28 52 / 54, 16 of 40 88 / 88, 32 of 40 157 / 159. */
+ * where it is full.  That is with 32 heads of 128 x 128; the lines hold within an eighth for the others: 64 x 64 (keys x values)
+ * one request of 12 20 / 22, 4 of 20 31 / 34, of 24 31 / 39, 8 of 28 46 / 45, of 32 46 / 50; 64 x 128 one of 16 26 / 28, 4 of 24 43 /
+ * 40, 8 of 32 68 / 60; 128 x 64 one of 12 23 / 23, 4 of 20 37 / 34, of 24 36 / 40, 8 of 28 52 / 54, 16 of 40 88 / 88, 32 of 40 157 / 159.
+ * But where it is full, tokens of 64 keys are shorter: 64 x 64 16 requests of 40 73 / 74, of 48 73 / 87, 32 of 40 127 / 98, of 48 124 /
+ * 115; 64 x 128 16 of 40 120 / 98, of 48 119 / 115, 32 of 40 224 / 178, of 48 227 / 211. */
 static inline int ssm_limit(const RoasterSsmState *s)
 {
     const int blocks = s->n_req * s->v_heads;
     if (s->n_req == 1 && blocks <= 64) return 16;
-    return blocks <= 128 ? SSM_SHORT : blocks <= 256 ? 32 : 40;
+    return blocks <= 128 ? SSM_SHORT : blocks <= 256 ? 32 : s->k_dim == 64 ? 48 : 40;
 }
 
 /* Chunks of a step at most: the last of each long request may be short. */

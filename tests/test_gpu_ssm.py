@@ -273,3 +273,10 @@ def test_rows_at_the_ends_of_an_int(n):
     assert np.all(np.abs(out[:n] - want[0][:n]) <= want[3][:n] + 1e-30) and np.isnan(out[n:]).all()
     assert np.array_equal(conv.astype(np.float64), want[1]) and np.array_equal(state[1:], s.state[1:])
     assert np.all(np.linalg.norm(state[0] - want[2][0], axis=2) <= want[4][0] + 1e-30)
+
+
+@pytest.mark.parametrize("most", [39, 40, 47, 48])
+@pytest.mark.parametrize("n,vh", [(70, 4), (33, 8)])
+def test_both_ways_about_their_limits_with_64_keys(most, n, vh):
+    s = Scan(np.random.default_rng(most + n), [most] + [2] * (n - 1), [3] * n, DELTA, 2, vh, 64, 64)
+    log(check_scan(run(s), scan_oracle(s)))
