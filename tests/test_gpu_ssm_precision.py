@@ -98,7 +98,7 @@ def test_large_values_at_the_beginning(early, by, coef):
     s.x[:, 128:256] = 0.1 * s.x[:, 128:256] - 8
     s.x[np.arange(4096), 128 + np.arange(4096) % 128] += 16
     s.b[:] = 2 + 0.1 * s.b
-    compare(s, [(0, 256), (3072, 4096)])
+    compare(s, [(0, 256), (3200, 4096)])
 
 
 @pytest.mark.parametrize("early,by", [(1, 1e6), (64, 1e5)])
@@ -106,7 +106,7 @@ def test_large_values_that_decay(early, by):
     """Without the correction: e^-0.01 a token."""
     s = slow(np.random.default_rng(32), 4096, STATE, -0.2)
     s.x[:early, 256:] *= np.float32(by)
-    compare(s, [(0, 256), (3072, 4096)])
+    compare(s, [(0, 256), (3200, 4096)])
 
 
 @pytest.mark.parametrize("mode", [DELTA, STATE])
